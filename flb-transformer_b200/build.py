@@ -33,6 +33,10 @@ CU_SOURCES = [
     "wavefront_prims.cu",
     "wavefront_grid.cu",
     "flb_block.cu",
+    "c_abi_ops.cu",
+    "layer_norm_fwd.cu",
+    "layer_norm_bwd.cu",
+    "kept8.cu",
     "microbench.cu",
     "umma_selftest.cu",
 ]

@@ -1,0 +1,387 @@
+// LayerNorm backward. With h the normalised row (from x and the forward's mean and 1/sigma, or from its
+// 8-bit kept form), gw = dy w:
+//
+//   dx = (gw - mean(gw) - h mean(gw h)) / sigma,   dw = sum over rows of dy h,   db = sum over rows of dy
+//
+// Bound by memory: dy and h are read once, dx is written once. A warp (D <= 1024) or block walks over rows
+// a fixed distance apart, the next rows on their way to shared memory meanwhile, and adds up dw and db of
+// the columns that its threads own in float32 registers. A block's sums go to its own row of a
+// workspace, which a second kernel adds up in a fixed order: no atomics, the same bits every time. With
+// one block a group (few rows) the block writes dw and db itself.
+#include "rows.cuh"
+
+namespace flb {
+
+using namespace rows;
+
+namespace {
+
+struct BwdArgs {
+  const void* x;
+  int64_t ldx;
+  const int8_t* codes;  // the kept form of h instead of x and mean
+  const uint8_t* exps;
+  const float *mean, *rstd;
+  const void* w;
+  bool w32;
+  const void* dy;
+  void* dx;
+  void *dw, *db;  // final gradients (one block a group), w's type
+  float* part;    // [G][blocks][2][D] otherwise; null with both dw and db null
+  int64_t R;
+  int D;
+};
+
+template <typename T> __device__ __forceinline__ void store_param(void* p, bool f32, int64_t i, float v) {
+  if (!p) return;
+  if (f32) reinterpret_cast<float*>(p)[i] = v; else st(reinterpret_cast<T*>(p) + i, v);
+}
+
+// Copies of the rows ahead, in shared memory. A thread copies, and later reads, only its own elements, so
+// its own wait for its copies is all the synchronisation there is. 16-bit rows that do not start on 16
+// bytes have no such copies (the smallest is 4 bytes): they are loaded when their turn comes.
+template <typename T, bool VEC> constexpr bool kCopies = VEC || sizeof(T) == 4;
+
+__device__ __forceinline__ uint32_t shared_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool there) {
+  // with no source bytes the destination is filled with zeros
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(there ? BYTES : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// One chunk's eight elements of this thread: slots [word group][thread], so that a warp's accesses are contiguous
+template <typename T, bool VEC>
+__device__ __forceinline__ void copy8(uint8_t* slot, const T* row, int base, int lane, int D) {
+  const uint32_t at = shared_addr(slot);
+  if constexpr (VEC) {
+    const int p = base + lane * 8;
+    const uint8_t* src = reinterpret_cast<const uint8_t*>(row + (p < D ? p : 0));
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+      copy_async<16>(at + (i * blockDim.x + threadIdx.x) * 16, src + 16 * i, p < D);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int p = base + j * 32 + lane;
+      copy_async<4>(at + (j * blockDim.x + threadIdx.x) * 4, row + (p < D ? p : 0), p < D);
+    }
+  }
+}
+template <typename T, bool VEC> __device__ __forceinline__ void copied8(const uint8_t* slot, float (&v)[8]) {
+  if constexpr (VEC) {
+    Raw8<T> r;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+      const uint4 u = reinterpret_cast<const uint4*>(slot)[i * blockDim.x + threadIdx.x];
+      r.w[4 * i] = u.x, r.w[4 * i + 1] = u.y, r.w[4 * i + 2] = u.z, r.w[4 * i + 3] = u.w;
+    }
+    to_float<T>(r, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = reinterpret_cast<const float*>(slot)[j * blockDim.x + threadIdx.x];
+  }
+}
+
+// Rows held at a time: three with 16-bit elements, two with float32; in the widest form, whose block is a
+// whole SM's, two and one.
+template <typename T, bool WIDE> constexpr int kStages = (sizeof(T) == 4 ? 2 : 3) - (WIDE ? 1 : 0);
+constexpr int kWarps = 4;  // of a block whose warps have a row each
+// such blocks on an SM: by the ring with float32, by the sums' registers with four chunks a thread
+template <typename T, int CH> constexpr int kBlocksPerSm = sizeof(T) == 4 || CH == 4 ? 3 : 4;
+
+// Bytes a thread's chunk takes in the ring
+template <typename T, bool VEC, bool KEPT> constexpr int chunk_bytes() {
+  const int elems = kCopies<T, VEC> ? 8 * (int)sizeof(T) : 0;
+  return KEPT ? elems + (VEC ? 8 : 0) : 2 * elems;
+}
+
+// MODE 0: a warp a row (D <= 1024), 1: a block a row (D <= 8192), 2: a block of up to 1024 threads (D <= 16384)
+template <typename T, bool VEC, int MODE, int CH, bool KEPT>
+__global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 1024, MODE == 0 ? kBlocksPerSm<T, CH> : 1)
+    ln_bwd_kernel(const BwdArgs a) {
+  constexpr bool WARP = MODE == 0;
+  constexpr int S = kStages<T, MODE == 2>, CB = chunk_bytes<T, VEC, KEPT>();
+  constexpr bool COPY_DY = kCopies<T, VEC>, COPY_X = !KEPT && COPY_DY, COPY_CODES = KEPT && VEC;
+  extern __shared__ __align__(16) uint8_t ring[];  // [S][CH][x or codes | dy][threads]; at the end [2][D] floats
+  __shared__ float slot[WARP ? 1 : 2][2][32];
+  let_successor_start();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t group = blockIdx.y;
+  const int D = a.D;
+  const int first = WARP ? 0 : warp * 256, step = WARP ? 256 : (int)blockDim.x * 8;
+  const int64_t stride = WARP ? (int64_t)gridDim.x * kWarps : gridDim.x;
+  const int64_t row0 = WARP ? (int64_t)blockIdx.x * kWarps + warp : blockIdx.x;
+  const float inv_d = 1.f / D;
+  auto part_of = [&](int stage, int c, bool dy) {
+    return ring + ((size_t)(stage * CH + c) * CB + (dy ? (KEPT ? (COPY_CODES ? 8 : 0) : 8 * (int)sizeof(T)) : 0)) * blockDim.x;
+  };
+  auto dy_row = [&](int64_t r) { return reinterpret_cast<const T*>(a.dy) + (group * a.R + r) * D; };
+  auto x_row = [&](int64_t r) { return reinterpret_cast<const T*>(a.x) + (group * a.R + r) * a.ldx; };
+  auto code_row = [&](int64_t r) { return a.codes + (group * a.R + r) * code_pitch(D); };
+  auto issue = [&](int64_t r, int stage) {
+    if (r < a.R) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int base = first + c * step;
+        if constexpr (COPY_DY) copy8<T, VEC>(part_of(stage, c, true), dy_row(r), base, lane, D);
+        if constexpr (COPY_X) copy8<T, VEC>(part_of(stage, c, false), x_row(r), base, lane, D);
+        if constexpr (COPY_CODES) {
+          const int p = base + lane * 8;
+          copy_async<8>(shared_addr(part_of(stage, c, false)) + threadIdx.x * 8, code_row(r) + (p < D ? p : 0), p < D);
+        }
+      }
+    }
+    copies_commit();
+  };
+
+  float dw[CH][8], db[CH][8];
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dw[c][j] = db[c][j] = 0.f;
+
+  // what is not copied: the row's statistics, its blocks' exponents, and the rows without copies
+  float mean = 0.f, rstd = 0.f;
+  uint32_t exps[CH];
+  auto fetch_small = [&](int64_t r) {
+    const int64_t rr = group * a.R + r;
+    if constexpr (!KEPT) mean = __ldg(a.mean + rr);
+    rstd = __ldg(a.rstd + rr);
+    if constexpr (KEPT) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) exps[c] = load_exps<VEC>(a.exps + rr * blocks_of(D), first + c * step, lane, D);
+    }
+  };
+
+#pragma unroll
+  for (int k = 0; k < S - 1; ++k) issue(row0 + k * stride, k);
+  if (row0 < a.R) fetch_small(row0);
+  int stage = 0, turn = 0;
+  for (int64_t row = row0; row < a.R; row += stride) {
+    issue(row + (S - 1) * stride, stage == 0 ? S - 1 : stage - 1);  // where the row before this one was
+    const float m = mean, rs = rstd;
+    Kept8 rk[CH];
+    Raw8<T> rx[CH], rdy[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int base = first + c * step;
+      if constexpr (KEPT) rk[c].e = exps[c];
+      if constexpr (KEPT && !COPY_CODES) rk[c].c = load_codes<VEC>(code_row(row), base, lane, D);
+      if constexpr (!KEPT && !COPY_X) load_raw<T, VEC>(rx[c], x_row(row), base, lane, D);
+      if constexpr (!COPY_DY) load_raw<T, VEC>(rdy[c], dy_row(row), base, lane, D);
+    }
+    if (row + stride < a.R) fetch_small(row + stride);
+    copies_wait<S - 1>();
+    // h and gw = dy w of chunk c; read again after the sums, which costs less than the registers to hold them
+    auto values = [&](int c, float (&h)[8], float (&dy)[8], float (&gw)[8]) {
+      const int base = first + c * step;
+      if constexpr (COPY_DY) copied8<T, VEC>(part_of(stage, c, true), dy); else to_float<T>(rdy[c], dy);
+      if constexpr (KEPT) {
+        Kept8 k = rk[c];
+        if constexpr (COPY_CODES) k.c = reinterpret_cast<const uint2*>(part_of(stage, c, false))[threadIdx.x];
+        kept_to_float<VEC>(k, h);
+      } else {
+        if constexpr (COPY_X) copied8<T, VEC>(part_of(stage, c, false), h); else to_float<T>(rx[c], h);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[j] = (h[j] - m) * rs;
+      }
+      if (a.w) {
+        if (a.w32) load8<float, VEC>(gw, reinterpret_cast<const float*>(a.w) + group * D, base, lane, D);
+        else load8<T, VEC>(gw, reinterpret_cast<const T*>(a.w) + group * D, base, lane, D);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) gw[j] *= dy[j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) gw[j] = dy[j];
+      }
+    };
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      float h[8], dy[8], gw[8];
+      values(c, h, dy, gw);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {  // dy is zero beyond D
+        dw[c][j] = fmaf(dy[j], h[j], dw[c][j]);
+        db[c][j] += dy[j];
+        s1 += gw[j];
+        s2 = fmaf(gw[j], h[j], s2);
+      }
+    }
+    s1 = warp_sum(s1);
+    s2 = warp_sum(s2);
+    if constexpr (!WARP) {
+      // the slots alternate: a warp that is a row ahead writes the other pair, and is not two ahead
+      // before every warp has passed the barrier of the row between, after reading this one's
+      if (lane == 0) slot[turn][0][warp] = s1, slot[turn][1][warp] = s2;
+      __syncthreads();
+      const int n = blockDim.x >> 5;
+      s1 = warp_sum(lane < n ? slot[turn][0][lane] : 0.f);
+      s2 = warp_sum(lane < n ? slot[turn][1][lane] : 0.f);
+      turn ^= 1;
+    }
+    s1 *= inv_d;
+    s2 *= inv_d;
+    T* dx = reinterpret_cast<T*>(a.dx) + (group * a.R + row) * D;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      float h[8], dy[8], gw[8];
+      values(c, h, dy, gw);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) gw[j] = rs * (gw[j] - s1 - h[j] * s2);
+      store8<T, VEC>(dx, gw, first + c * step, lane, D);
+    }
+    stage = stage + 1 == S ? 0 : stage + 1;
+  }
+
+  if (!a.dw && !a.db) return;  // uniform over the grid
+  const bool alone = gridDim.x == 1;
+  float* pw = a.part + (group * gridDim.x + blockIdx.x) * 2 * D;
+  auto out = [&](int p, float vw, float vb) {
+    if (alone) {
+      store_param<T>(a.dw, a.w32, group * D + p, vw);
+      store_param<T>(a.db, a.w32, group * D + p, vb);
+    } else {
+      pw[p] = vw;
+      pw[D + p] = vb;
+    }
+  };
+  if constexpr (WARP) {
+    copies_wait<0>();  // every copy into the ring has landed before it is used for the sums
+    float* sm = reinterpret_cast<float*>(ring);
+    for (int t = 0; t < kWarps; ++t) {  // the warps' sums in order
+      __syncthreads();
+      if (warp != t) continue;
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int p = Chunk<VEC>::at(first + c * step, lane, j);
+          if (p < D) {
+            sm[p] = (t ? sm[p] : 0.f) + dw[c][j];
+            sm[D + p] = (t ? sm[D + p] : 0.f) + db[c][j];
+          }
+        }
+    }
+    __syncthreads();
+    for (int p = threadIdx.x; p < D; p += blockDim.x) out(p, sm[p], sm[D + p]);
+  } else {
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int p = Chunk<VEC>::at(first + c * step, lane, j);
+        if (p < D) out(p, dw[c][j], db[c][j]);
+      }
+  }
+}
+
+// dw and db from the blocks' sums: 32 columns a block, a warp for every 32nd workspace row.
+template <typename T>
+__global__ void __launch_bounds__(1024) ln_sum_kernel(const float* __restrict__ part, void* dw, void* db, bool w32,
+                                                      int blocks, int D) {
+  __shared__ float s[32][33];
+  wait_predecessor();
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int col = blockIdx.x * 32 + tx, which = blockIdx.z;
+  const int64_t group = blockIdx.y;
+  float v = 0.f;
+  if (col < D) {
+    const float* p = part + (group * blocks * 2 + which) * D + col;
+#pragma unroll 4
+    for (int i = ty; i < blocks; i += 32) v += __ldg(p + (int64_t)i * 2 * D);
+  }
+  s[ty][tx] = v;
+  __syncthreads();
+  v = warp_sum(s[tx][ty]);  // the 32 sums of column ty
+  const int out = blockIdx.x * 32 + ty;
+  if (tx == 0 && out < D) store_param<T>(which ? db : dw, w32, group * D + out, v);
+}
+
+// Threads a row, and blocks a group: enough to fill the SMs (kBlocksPerSm, or 512 threads on each), but at least two rows a warp or block, and one block where that leaves it
+// four rows a warp at most.
+struct BwdShape {
+  int mode, threads;
+  int64_t blocks;
+};
+BwdShape bwd_shape(int64_t G, int64_t R, int64_t D, int dtype) {
+  BwdShape p;
+  p.mode = D <= 1024 ? 0 : D <= 8192 ? 1 : 2;
+  p.threads = p.mode == 0 ? 32 * kWarps : 32 * (int)((D + 511) / 512);
+  const int64_t at_once = p.mode == 0 ? kWarps : 1;
+  const int per_sm = p.mode == 0 ? (dtype == FLB_F32 || D > 768 ? 3 : 4) : std::max(1, 512 / p.threads);
+  const int64_t room = std::max<int64_t>(1, (int64_t)num_sms() * per_sm / G);
+  p.blocks = R <= 4 * at_once ? 1 : std::min<int64_t>(room, (R + 2 * at_once - 1) / (2 * at_once));
+  return p;
+}
+
+template <typename T, bool VEC, int MODE, int CH, bool KEPT>
+int launch_mode(const BwdArgs& a, const BwdShape& p, int64_t G, cudaStream_t s) {
+  auto k = ln_bwd_kernel<T, VEC, MODE, CH, KEPT>;
+  const size_t ring = (size_t)kStages<T, MODE == 2> * CH * chunk_bytes<T, VEC, KEPT>() * p.threads;
+  const size_t smem = std::max(ring, MODE == 0 ? (size_t)2 * a.D * sizeof(float) : (size_t)0);
+  const int st = ensure_dyn_smem(reinterpret_cast<const void*>(k), (int)smem, "layer_norm_bwd shared memory");
+  if (st != FLB_OK) return st;
+  k<<<dim3((unsigned)p.blocks, (unsigned)G), p.threads, smem, s>>>(a);
+  return FLB_OK;
+}
+
+template <typename T, bool VEC, bool KEPT>
+int launch_bwd(const BwdArgs& a, int64_t G, int dtype, cudaStream_t s) {
+  const int D = a.D;
+  const BwdShape p = bwd_shape(G, a.R, D, dtype);
+  int st;
+  if (p.mode == 0) {
+    switch ((D + 255) / 256) {
+      case 1: st = launch_mode<T, VEC, 0, 1, KEPT>(a, p, G, s); break;
+      case 2: st = launch_mode<T, VEC, 0, 2, KEPT>(a, p, G, s); break;
+      case 3: st = launch_mode<T, VEC, 0, 3, KEPT>(a, p, G, s); break;
+      default: st = launch_mode<T, VEC, 0, 4, KEPT>(a, p, G, s); break;
+    }
+  } else if (p.mode == 1) {
+    st = launch_mode<T, VEC, 1, 2, KEPT>(a, p, G, s);
+  } else {
+    st = launch_mode<T, VEC, 2, 2, KEPT>(a, p, G, s);
+  }
+  if (st != FLB_OK) return st;
+  count_launches(1);
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess && p.blocks > 1 && (a.dw || a.db)) {
+    e = launch_dependent(ln_sum_kernel<T>, dim3((unsigned)((D + 31) / 32), (unsigned)G, 2), dim3(1024), 0, s,
+                         (const float*)a.part, a.dw, a.db, a.w32, (int)p.blocks, D);
+    count_launches(1);
+  }
+  return check_cuda(e, "layer_norm_bwd launch");
+}
+
+bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+template <typename T> int dispatch_bwd(const BwdArgs& a, int64_t G, int dtype, cudaStream_t s) {
+  const bool vec = a.D % 8 == 0 && on16(a.x) && a.ldx * sizeof(T) % 16 == 0 && on16(a.codes) && on16(a.w) && on16(a.dy) && on16(a.dx);
+  if (a.codes) return vec ? launch_bwd<T, true, true>(a, G, dtype, s) : launch_bwd<T, false, true>(a, G, dtype, s);
+  return vec ? launch_bwd<T, true, false>(a, G, dtype, s) : launch_bwd<T, false, false>(a, G, dtype, s);
+}
+
+}  // namespace
+
+size_t layer_norm_bwd_workspace_bytes(int64_t G, int64_t R, int64_t D, int dtype) {
+  const BwdShape p = bwd_shape(G, R, D, dtype);
+  return p.blocks > 1 ? (size_t)G * p.blocks * 2 * D * sizeof(float) : 0;
+}
+
+int layer_norm_bwd(const void* x, int64_t ldx, const int8_t* codes, const uint8_t* exps, const float* mean,
+                   const float* rstd, const void* w, int wdtype, const void* dy, void* dx, void* dw, void* db, int64_t G,
+                   int64_t R, int64_t D, int dtype, void* ws, cudaStream_t s) {
+  const BwdArgs a{x, ldx, codes, exps, mean, rstd, w, wdtype == FLB_F32, dy, dx, dw, db, reinterpret_cast<float*>(ws), R, (int)D};
+  switch (dtype) {
+    case FLB_F32: return dispatch_bwd<float>(a, G, dtype, s);
+    case FLB_F16: return dispatch_bwd<__half>(a, G, dtype, s);
+    default: return dispatch_bwd<__nv_bfloat16>(a, G, dtype, s);
+  }
+}
+
+}  // namespace flb

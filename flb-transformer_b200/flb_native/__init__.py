@@ -86,6 +86,17 @@ PROTOTYPES = {
     "flb_grid_band_bwd": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                  _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _sz, _i32,
                                  _vp]),
+    "flb_code_pitch": (_i64, [_i64]),
+    "flb_kept_blocks": (_i64, [_i64]),
+    "flb_layer_norm_fwd": (_i32, [_vp, _i64, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i64,
+                                  _i64, _i32, ctypes.c_float, _vp]),
+    "flb_layer_norm_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32]),
+    "flb_layer_norm_bwd": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i64,
+                                  _i64, _i64, _i32, _vp, _sz, _vp]),
+    "flb_pack8": (_i32, [_vp, _vp, _vp, _i64, _i64, _i32, _vp]),
+    "flb_unpack8": (_i32, [_vp, _vp, _vp, _i64, _i64, _i32, _vp]),
+    "flb_gate_fwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _vp]),
+    "flb_gate_bwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _vp]),
     "flb_microbench": (_i32, [_i32, _vp, _dblp]),
     "flb_selftest_umma": (_i32, [_i32, _i32, _vp, _vp, _vp, _vp, _vp]),
 }

@@ -390,6 +390,52 @@ int flb_grid_fwd_drop_flag_test(const void* x, int x_layout, const void* W_l, co
                                 int64_t drop_col, uint32_t spin_limit, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * LayerNorm and activations kept in 8 bits (no reference counterpart: the reference uses
+ * torch's LayerNorm and keeps activations in their own type).
+ * Rows are G groups of R rows of D elements, group after group; each group has a weight and bias
+ * of its own ([G, D], of dtype wdtype: float32 or the rows' dtype; either may be NULL). x has a row
+ * pitch of ldx elements; every other row array is contiguous. D <= 32768 (backward: 16384).
+ *
+ * The kept form of rows [rows, D]: codes, int8 [rows, flb_code_pitch(D)], 16-byte aligned (bytes
+ * at and beyond D are not touched), and exps, uint8 [rows, flb_kept_blocks(D)], one per block of
+ * 128 elements of a row: element = code * 2^(exps - 127), exps the smallest of at least 1 for
+ * which the block's largest magnitude rounds to a code of at most 127. 255 marks a block that
+ * held an infinity or NaN; all of it comes back as NaN.
+ * ------------------------------------------------------------------------------------------ */
+int64_t flb_code_pitch(int64_t D);   /* D rounded up to a multiple of 16 */
+int64_t flb_kept_blocks(int64_t D);  /* ceil(D / 128) */
+
+/* y = h * w + b, h = (x - mean) / sqrt(var + eps). mean and rstd (float32 [G * R]; NULL: not
+ * wanted) are what flb_layer_norm_bwd reads; with codes and exps (both or neither) the kept form
+ * of h is written too, and the backward reads it in place of x and mean. */
+int flb_layer_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b, int wdtype, void* y,
+                       float* mean, float* rstd, int8_t* codes, uint8_t* exps, int64_t G, int64_t R,
+                       int64_t D, int dtype, float eps, void* stream);
+
+/* dx in dtype; dw and db ([G, D] in wdtype, OVERWRITTEN; both or neither NULL) are summed in a fixed
+ * order (the same bits every time). Either x and mean, or codes and exps. Workspace:
+ * flb_layer_norm_bwd_workspace_bytes(), 16-byte aligned, asked for on the same device. */
+size_t flb_layer_norm_bwd_workspace_bytes(int64_t G, int64_t R, int64_t D, int dtype);
+int flb_layer_norm_bwd(const void* x, int64_t ldx, const int8_t* codes, const uint8_t* exps,
+                       const float* mean, const float* rstd, const void* w, int wdtype, const void* dy,
+                       void* dx, void* dw, void* db, int64_t G, int64_t R, int64_t D, int dtype,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rows x [R, D] into their kept form, and back (out in any dtype; float16 saturates). */
+int flb_pack8(const void* x, int8_t* codes, uint8_t* exps, int64_t R, int64_t D, int dtype, void* stream);
+int flb_unpack8(const int8_t* codes, const uint8_t* exps, void* out, int64_t R, int64_t D, int dtype,
+                void* stream);
+
+/* y = x * sigmoid(z) over [R, D]. With cx, ex, cz, ez (all or none) the kept forms of x and z are
+ * written too; the backward reads them in place of x and z (which are then NULL):
+ * dx = dy * sigmoid(z), dz = dy * x * sigmoid(z) * sigmoid(-z). */
+int flb_gate_fwd(const void* x, const void* z, void* y, int8_t* cx, uint8_t* ex, int8_t* cz, uint8_t* ez,
+                 int64_t R, int64_t D, int dtype, void* stream);
+int flb_gate_bwd(const void* x, const void* z, const int8_t* cx, const uint8_t* ex, const int8_t* cz,
+                 const uint8_t* ez, const void* dy, void* dx, void* dz, int64_t R, int64_t D, int dtype,
+                 void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Measurement helpers (used by bench.py for the roofline denominators).
  * ------------------------------------------------------------------------------------------ */
 
