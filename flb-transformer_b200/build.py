@@ -4,6 +4,8 @@ Outputs (next to this file, git-ignored, shipped with the source tree):
   libflb_b200.so                      C-ABI library: every CUDA kernel, compiled for sm_100a only
   wavefront_backend.<abi>.so          pybind11 module with execute_forward / execute_backward,
                                       linked against libflb_b200.so
+  flb_ops.<abi>.so                    pybind11 module with the row operators' torch calls and autograd
+                                      functions, linked against libflb_b200.so
 
 Usage: python build.py [--force] [-j N]
 Objects go to _build/ (git-ignored). Rebuilds only what changed.
@@ -37,9 +39,11 @@ CU_SOURCES = [
     "layer_norm_fwd.cu",
     "layer_norm_bwd.cu",
     "kept8.cu",
+    "int8_linear.cu",
     "microbench.cu",
     "umma_selftest.cu",
 ]
+MODULES = ["wavefront_backend", "flb_ops"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
@@ -96,13 +100,14 @@ def build_library(force: bool = False, jobs: int = 8) -> str:
     return lib
 
 
-def build_backend(force: bool = False) -> str:
+def build_module(name: str, force: bool = False) -> str:
+    """The pybind11 module `name` from csrc/<name>.cpp, next to the library it is linked against."""
     import torch.utils.cpp_extension as ce  # deferred: torch import is slow
     import pybind11
 
     suffix = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
-    out = os.path.join(ROOT, "wavefront_backend" + suffix)
-    src = os.path.join(CSRC, "wavefront_backend.cpp")
+    out = os.path.join(ROOT, name + suffix)
+    src = os.path.join(CSRC, name + ".cpp")
     lib = os.path.join(ROOT, LIB_NAME)
     if not force and not _stale(out, [src, lib] + _headers()):
         return out
@@ -112,8 +117,10 @@ def build_backend(force: bool = False) -> str:
     import torch
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     cmd = ["g++", "-O3", "-std=c++17", "-shared", "-fPIC", src, "-o", out,
-           f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=wavefront_backend",
-           "-DTORCH_API_INCLUDE_EXTENSION_H"]
+           f"-D_GLIBCXX_USE_CXX11_ABI={abi}", f"-DTORCH_EXTENSION_NAME={name}",
+           "-DTORCH_API_INCLUDE_EXTENSION_H",
+           # gcc's false alarms about torch's inlined std::vector<bool>
+           "-Wno-array-bounds", "-Wno-stringop-overflow"]
     cmd += [f"-I{p}" for p in incs]
     cmd += [f"-L{p}" for p in libdirs] + [f"-L{ROOT}"]
     cmd += ["-lflb_b200", "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10_cuda",
@@ -125,7 +132,8 @@ def build_backend(force: bool = False) -> str:
 
 def build(force: bool = False, jobs: int = 8) -> None:
     build_library(force=force, jobs=jobs)
-    build_backend(force=force)
+    with ThreadPoolExecutor(max_workers=2) as ex:
+        list(ex.map(lambda name: build_module(name, force=force), MODULES))
 
 
 if __name__ == "__main__":

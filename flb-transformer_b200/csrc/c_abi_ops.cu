@@ -1,4 +1,5 @@
-// extern "C" boundary of the row operators: LayerNorm, the 8-bit kept form, the sigmoid gate.
+// extern "C" boundary of the row operators (LayerNorm, the 8-bit kept form, the sigmoid gate) and of the 8-bit
+// integer product.
 #include "common.cuh"
 #include "rows.cuh"
 
@@ -11,6 +12,14 @@ size_t layer_norm_bwd_workspace_bytes(int64_t G, int64_t R, int64_t D, int dtype
 int layer_norm_bwd(const void* x, int64_t ldx, const int8_t* codes, const uint8_t* exps, const float* mean,
                    const float* rstd, const void* w, int wdtype, const void* dy, void* dx, void* dw, void* db, int64_t G,
                    int64_t R, int64_t D, int dtype, void* ws, cudaStream_t s);
+int layer_norm_int8(const void* x, int64_t ldx, const void* w, const void* b, int wdtype, int8_t* codes, float* scale,
+                    int64_t G, int64_t R, int64_t D, int dtype, float eps, cudaStream_t s);
+int int8_rows(const void* x, int64_t ldx, int8_t* codes, float* scale, int64_t R, int64_t D, int dtype, uint32_t* zero,
+              int64_t n_zero, cudaStream_t s);
+size_t int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, bool quantise);
+int int8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, const float* x_scale, const int8_t* w_codes,
+                int64_t ldw, const float* w_scale, const void* bias, int bias_dtype, void* out, int64_t M, int64_t N,
+                int64_t K, int dtype, void* ws, int check_timeout, cudaStream_t s);
 int pack8(const void* x, int8_t* codes, uint8_t* exps, int64_t R, int64_t D, int dtype, cudaStream_t s);
 int unpack8(const int8_t* codes, const uint8_t* exps, void* out, int64_t R, int64_t D, int dtype, cudaStream_t s);
 int gate_fwd(const void* x, const void* z, void* y, int8_t* cx, uint8_t* ex, int8_t* cz, uint8_t* ez, int64_t R,
@@ -54,6 +63,17 @@ int check_rows(const char* what, int64_t R, int64_t D, int dtype) {
   if (R < 0 || D < 1) return fail(FLB_ERR_SHAPE, at + ": R >= 0 and D >= 1 required");
   if (D > INT32_MAX / 2) return fail(FLB_ERR_UNSUPPORTED, at + ": rows this wide are not supported");
   if (R > INT64_MAX / 8 / (D + 256)) return fail(FLB_ERR_SHAPE, at + ": too many rows");
+  return FLB_OK;
+}
+
+constexpr int64_t kWidestInt8 = 32768;  // a row's elements: 32768 * 127^2 < 2^31
+
+// The sizes of an 8-bit product: within what the grid, the tensor maps and 32-bit sums hold.
+int check_product(int64_t M, int64_t N, int64_t K) {
+  if (M < 0 || N < 0 || K < 1) return fail(FLB_ERR_SHAPE, "int8_linear: M, N >= 0 and K >= 1 required");
+  if (K > kWidestInt8) return fail(FLB_ERR_UNSUPPORTED, "int8_linear: rows wider than 32768 are not supported");
+  if (M > INT32_MAX - 1024 || N > INT32_MAX - 1024 || (M > 0 && N > ((int64_t)1 << 44) / M))
+    return fail(FLB_ERR_SHAPE, "int8_linear: too many rows");
   return FLB_OK;
 }
 
@@ -115,6 +135,59 @@ int flb_layer_norm_bwd(const void* x, int64_t ldx, const int8_t* codes, const ui
     return fail(FLB_ERR_WORKSPACE, "layer_norm_bwd: workspace smaller than flb_layer_norm_bwd_workspace_bytes()");
   if (off(workspace, 16)) return fail(FLB_ERR_ALIGN, "layer_norm_bwd: workspace must be 16-byte aligned");
   return layer_norm_bwd(x, ldx, codes, exps, mean, rstd, w, wdtype, dy, dx, dw, db, G, R, D, dtype, workspace, s);
+}
+
+int flb_layer_norm_int8(const void* x, int64_t ldx, const void* w, const void* b, int wdtype, int8_t* codes, float* scale,
+                        int64_t G, int64_t R, int64_t D, int dtype, float eps, void* stream) {
+  bool empty;
+  int st = check_norm("layer_norm_int8", w, b, wdtype, G, R, D, ldx, dtype, kWidestInt8, &empty);
+  if (st != FLB_OK || empty) return st;
+  if (!x || !codes || !scale) return fail(FLB_ERR_SHAPE, "layer_norm_int8: null x, codes or scale");
+  if (off(x, (size_t)dtype_size(dtype)) || off(codes, 16) || off(scale, 4))
+    return fail(FLB_ERR_ALIGN, "layer_norm_int8: codes must be 16-byte aligned, x and scale to their element size");
+  return layer_norm_int8(x, ldx, w, b, wdtype, codes, scale, G, R, D, dtype, eps, as_stream(stream));
+}
+
+int flb_int8_rows(const void* x, int64_t ldx, int8_t* codes, float* scale, int64_t R, int64_t D, int dtype, void* stream) {
+  bool empty;
+  int st = check_norm("int8_rows", nullptr, nullptr, dtype, 1, R, D, ldx, dtype, kWidestInt8, &empty);
+  if (st != FLB_OK || empty) return st;
+  if (!x || !codes || !scale) return fail(FLB_ERR_SHAPE, "int8_rows: null x, codes or scale");
+  if (off(x, (size_t)dtype_size(dtype)) || off(codes, 16) || off(scale, 4))
+    return fail(FLB_ERR_ALIGN, "int8_rows: codes must be 16-byte aligned, x and scale to their element size");
+  return int8_rows(x, ldx, codes, scale, R, D, dtype, nullptr, 0, as_stream(stream));
+}
+
+size_t flb_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int x_is_codes) {
+  if (check_product(M, N, K) != FLB_OK || M == 0 || N == 0) return 0;
+  return int8_linear_workspace_bytes(M, N, K, !x_is_codes);
+}
+
+int flb_int8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, const float* x_scale,
+                    const int8_t* w_codes, int64_t ldw, const float* w_scale, const void* bias, int bias_dtype, void* out,
+                    int64_t M, int64_t N, int64_t K, int dtype, void* workspace, size_t workspace_bytes, int check_timeout,
+                    void* stream) {
+  if (dtype_size(dtype) == 0) return fail(FLB_ERR_DTYPE, "int8_linear: dtype must be f32, f16 or bf16");
+  if (bias && bias_dtype != FLB_F32 && bias_dtype != dtype)
+    return fail(FLB_ERR_DTYPE, "int8_linear: the bias must be float32 or of the output's dtype");
+  int st = check_product(M, N, K);
+  if (st != FLB_OK) return st;
+  if (M == 0 || N == 0) return FLB_OK;
+  if (!x == !x_codes || !x_codes != !x_scale) return fail(FLB_ERR_SHAPE, "int8_linear: either x, or x_codes and x_scale");
+  if (!w_codes || !w_scale || !out) return fail(FLB_ERR_SHAPE, "int8_linear: null weight or out");
+  if (x ? ldx < 0 : ldc < K) return fail(FLB_ERR_SHAPE, "int8_linear: bad row pitch of x");
+  if (ldw < K) return fail(FLB_ERR_SHAPE, "int8_linear: bad row pitch of the weight");
+  if (off(w_codes, 16) || ldw % 16 || (x_codes && (off(x_codes, 16) || ldc % 16)))
+    return fail(FLB_ERR_ALIGN, "int8_linear: codes must start every row on 16 bytes");
+  const size_t es = (size_t)dtype_size(dtype);
+  if (off(x, es) || off(out, es) || off(w_scale, 4) || off(x_scale, 4) || off(bias, bias ? (size_t)dtype_size(bias_dtype) : 1))
+    return fail(FLB_ERR_ALIGN, "int8_linear: pointers must be aligned to their element size");
+  const size_t need = int8_linear_workspace_bytes(M, N, K, x != nullptr);
+  if (!workspace || workspace_bytes < need)
+    return fail(FLB_ERR_WORKSPACE, "int8_linear: workspace smaller than flb_int8_linear_workspace_bytes()");
+  if (off(workspace, 256)) return fail(FLB_ERR_ALIGN, "int8_linear: workspace must be 256-byte aligned");
+  return int8_linear(x, ldx, x_codes, ldc, x_scale, w_codes, ldw, w_scale, bias, bias_dtype, out, M, N, K, dtype, workspace,
+                     check_timeout, as_stream(stream));
 }
 
 int flb_pack8(const void* x, int8_t* codes, uint8_t* exps, int64_t R, int64_t D, int dtype, void* stream) {

@@ -31,6 +31,8 @@ struct RowArgs {
   int64_t rows, rows_per_group;
   int D;
   float eps;
+  uint32_t* zero;  // words that a kernel after this one counts in
+  int64_t n_zero;
 };
 
 // `fill` where there is no such vector
@@ -51,6 +53,11 @@ template <typename T, bool VEC, bool WARP, int CH, bool NORM, int OUT>
 __global__ void __launch_bounds__(WARP ? 256 : 1024) row_fwd_kernel(const RowArgs a) {
   __shared__ float slot[WARP ? 1 : 3][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if constexpr (!NORM) {
+    let_successor_start();
+    if (blockIdx.x == 0)
+      for (int64_t i = threadIdx.x; i < a.n_zero; i += blockDim.x) a.zero[i] = 0;
+  }
   const int64_t row = WARP ? (int64_t)blockIdx.x * (blockDim.x >> 5) + warp : blockIdx.x;
   if (row >= a.rows) return;
   const int D = a.D;
@@ -163,18 +170,19 @@ template <bool NORM, int OUT> int dispatch_rows(const RowArgs& a, int dtype, cud
 int layer_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b, int wdtype, void* y, float* mean,
                    float* rstd, int8_t* codes, uint8_t* exps, int64_t G, int64_t R, int64_t D, int dtype, float eps,
                    cudaStream_t s) {
-  const RowArgs a{x, ldx, w, b, wdtype == FLB_F32, y, mean, rstd, codes, exps, nullptr, G * R, R, (int)D, eps};
+  const RowArgs a{x, ldx, w, b, wdtype == FLB_F32, y, mean, rstd, codes, exps, nullptr, G * R, R, (int)D, eps, nullptr, 0};
   return codes ? dispatch_rows<true, OUT_KEPT>(a, dtype, s) : dispatch_rows<true, OUT_Y>(a, dtype, s);
 }
 
 int layer_norm_int8(const void* x, int64_t ldx, const void* w, const void* b, int wdtype, int8_t* codes, float* scale,
                     int64_t G, int64_t R, int64_t D, int dtype, float eps, cudaStream_t s) {
-  const RowArgs a{x, ldx, w, b, wdtype == FLB_F32, nullptr, nullptr, nullptr, codes, nullptr, scale, G * R, R, (int)D, eps};
+  const RowArgs a{x, ldx, w, b, wdtype == FLB_F32, nullptr, nullptr, nullptr, codes, nullptr, scale, G * R, R, (int)D, eps, nullptr, 0};
   return dispatch_rows<true, OUT_INT8>(a, dtype, s);
 }
 
-int int8_rows(const void* x, int64_t ldx, int8_t* codes, float* scale, int64_t R, int64_t D, int dtype, cudaStream_t s) {
-  const RowArgs a{x, ldx, nullptr, nullptr, false, nullptr, nullptr, nullptr, codes, nullptr, scale, R, R, (int)D, 0.f};
+int int8_rows(const void* x, int64_t ldx, int8_t* codes, float* scale, int64_t R, int64_t D, int dtype, uint32_t* zero,
+              int64_t n_zero, cudaStream_t s) {
+  const RowArgs a{x, ldx, nullptr, nullptr, false, nullptr, nullptr, nullptr, codes, nullptr, scale, R, R, (int)D, 0.f, zero, n_zero};
   return dispatch_rows<false, OUT_INT8>(a, dtype, s);
 }
 

@@ -97,6 +97,12 @@ PROTOTYPES = {
     "flb_unpack8": (_i32, [_vp, _vp, _vp, _i64, _i64, _i32, _vp]),
     "flb_gate_fwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _vp]),
     "flb_gate_bwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _vp]),
+    "flb_int8_rows": (_i32, [_vp, _i64, _vp, _vp, _i64, _i64, _i32, _vp]),
+    "flb_layer_norm_int8": (_i32, [_vp, _i64, _vp, _vp, _i32, _vp, _vp, _i64, _i64, _i64, _i32,
+                                   ctypes.c_float, _vp]),
+    "flb_int8_linear_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32]),
+    "flb_int8_linear": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i32, _vp, _i64, _i64,
+                               _i64, _i32, _vp, _sz, _i32, _vp]),
     "flb_microbench": (_i32, [_i32, _vp, _dblp]),
     "flb_selftest_umma": (_i32, [_i32, _i32, _vp, _vp, _vp, _vp, _vp]),
 }

@@ -3,7 +3,8 @@
  *   (1) fused additive attention  s[i,j] = sum_d w[d] * tanh(q[i,d] + k[j,d]) / sqrt(D),
  *       row softmax, out = P @ V, forward and backward;
  *   (2) the anti-diagonal wavefront engine (dependency gather, port scatter, gradient routing)
- *       and the persistent tanh grid-cell kernels.
+ *       and the persistent tanh grid-cell kernels;
+ * and of operators beside them: LayerNorm, activations kept in 8 bits, 8-bit integer products.
  *
  * Conventions shared by every entry point:
  *   - all pointers are DEVICE pointers unless stated otherwise; the library never allocates,
@@ -434,6 +435,31 @@ int flb_gate_fwd(const void* x, const void* z, void* y, int8_t* cx, uint8_t* ex,
 int flb_gate_bwd(const void* x, const void* z, const int8_t* cx, const uint8_t* ex, const int8_t* cz,
                  const uint8_t* ez, const void* dy, void* dx, void* dz, int64_t R, int64_t D, int dtype,
                  void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * 8-bit integer rows and their product (no reference counterpart).
+ * Rows x [R, D] (pitch ldx elements) in 8-bit integers: codes, int8 [R, flb_code_pitch(D)], 16-byte aligned
+ * (bytes at and beyond D are not touched), and scale, float32 [R]: with a the row's largest magnitude,
+ * code = round(x * (127 / a)), scale = a / 127, x = code * scale. A row with an infinity or NaN gets the
+ * scale NaN; one whose largest magnitude is below 2^-118 counts as zeros. D <= 32768.
+ * ------------------------------------------------------------------------------------------ */
+int flb_int8_rows(const void* x, int64_t ldx, int8_t* codes, float* scale, int64_t R, int64_t D, int dtype,
+                  void* stream);
+/* The rows of a LayerNorm's output (before its rounding to dtype); arguments as flb_layer_norm_fwd. */
+int flb_layer_norm_int8(const void* x, int64_t ldx, const void* w, const void* b, int wdtype, int8_t* codes,
+                        float* scale, int64_t G, int64_t R, int64_t D, int dtype, float eps, void* stream);
+
+/* out[m, n] = (sum_k X[m, k] W[n, k]) sx[m] sw[n] + bias[n], contiguous [M, N] in dtype, the sums in 32-bit
+ * integers. X: codes and scale (pitch ldc), or x [M, K] in dtype (pitch ldx elements), made into 8-bit rows
+ * on the way. W: codes [N, K] (pitch ldw >= K, a multiple of 16, 16-byte aligned) and scale [N]. bias: [N],
+ * float32 or dtype, or NULL. K <= 32768. Workspace: flb_int8_linear_workspace_bytes(), 256-byte
+ * aligned, asked for on the same device; calls that may overlap on the GPU need one each.
+ * check_timeout != 0: reads the kernel's error word back (synchronises `stream`). */
+size_t flb_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int x_is_codes);
+int flb_int8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, const float* x_scale,
+                    const int8_t* w_codes, int64_t ldw, const float* w_scale, const void* bias,
+                    int bias_dtype, void* out, int64_t M, int64_t N, int64_t K, int dtype, void* workspace,
+                    size_t workspace_bytes, int check_timeout, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Measurement helpers (used by bench.py for the roofline denominators).

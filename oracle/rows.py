@@ -115,3 +115,23 @@ def gate_backward(x, z, dy, dtype, keep8=False):
     dz = dy * x * torch.sigmoid(z) * torch.sigmoid(-z)
     return ((dx, (half_step(dtype) + rel + U) * dx.abs() + floor_of(dtype)),
             (dz, (half_step(dtype) + 2 * rel + 3 * U) * dz.abs() + floor_of(dtype)))
+
+
+def int8_rows(x):
+    """(codes as float64, scale float32) by the definition's own float32 steps, which IEEE arithmetic fixes."""
+    x = x.float()
+    a = x.abs().amax(-1, keepdim=True) if x.shape[-1] else x.new_zeros((*x.shape[:-1], 1))
+    bad = ~torch.isfinite(x).all(-1, keepdim=True)
+    small = a < 2.0 ** -118
+    f = torch.where(bad | small, torch.zeros_like(a), torch.tensor(127.0) / a)
+    codes = torch.round(torch.where(f == 0, torch.zeros_like(x), x) * f)
+    return codes.double(), torch.where(bad, torch.full_like(a, math.nan), a / 127)[..., 0]
+
+
+def int8_product(codes, scale, w_codes, w_scale, bias, dtype):
+    """The product of integer rows and its bound: the integer sum's rounding to float32, two products and
+    the addition, then the type's."""
+    prod = (codes.double() @ w_codes.double().t()) * scale.double()[..., None] * w_scale.double()
+    b = torch.zeros(w_codes.shape[0], dtype=torch.float64) if bias is None else bias.double()
+    out = prod + b
+    return out, half_step(dtype) * out.abs() + 4 * U * prod.abs() + 2 * U * out.abs() + floor_of(dtype)

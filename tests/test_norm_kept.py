@@ -88,7 +88,7 @@ def test_kept_arguments():
 
 def test_rows_of_views():
     """Which views the kernels take as they are, and which are copied."""
-    from kernels._rows import as_rows
+    from flb_ops import rows_of as as_rows
     t = torch.arange(5 * 8 * 12.).reshape(5, 8, 12)
     for v, pitch, same in ((t, 12, True), (t[:, :, 2:6], 12, True), (t[:, ::2, :4], 24, True), (t[:, :3], None, False),
                            (t.transpose(0, 1), None, False), (t[:1, :1, :5], 5, None), (t[..., ::2], 6, False), (t[2:3, :, 1:4], 12, True)):
