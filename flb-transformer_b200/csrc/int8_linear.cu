@@ -6,7 +6,7 @@
 // consecutive channels of one token, so its stores are contiguous without a transpose.
 //
 // One block a SM, persistent over units of work: a unit is a tile, or with few tiles a part of the
-// tile's K range. Warp 0 loads by TMA into a ring, warp 1 issues the MMAs, warps 2-5 read TMEM (two accumulators, so
+// tile's K range. Warp 0 loads by TMA into a ring, warp 1 issues the MMAs, warps 2-9 read TMEM (two accumulators, so
 // that a tile's epilogue runs beside the next one's MMAs). Parts of a tile leave integer sums in the
 // workspace; the block that counts itself last adds them up: integers, the same in any order.
 //
@@ -25,7 +25,8 @@ namespace {
 constexpr int kChannels = 128;   // a tile's weight rows
 constexpr int kStep = 128;       // bytes of K a stage
 constexpr int kRing = 198 * 1024;
-constexpr int kGemmThreads = 192;
+constexpr int kEpilogue = 256;   // threads that read TMEM and store
+constexpr int kGemmThreads = 64 + kEpilogue;
 constexpr uint32_t kWaitLimit = 4000000u;  // polls, each of which the hardware may hold for a while
 
 template <int NT> constexpr int stage_bytes() { return (kChannels + NT) * kStep; }
@@ -59,40 +60,51 @@ __device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t a_desc, uint64
       : "memory");
 }
 
-__device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ void load_cols(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
+__device__ __forceinline__ void load_cols(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
 
-// One channel's values of 32 tokens from token t0 on: scaled, with the bias, stored.
-template <typename T>
-__device__ __forceinline__ void store_tokens(const Int8Args& a, const int32_t (&acc)[32], const float* sx, float sw, float bias,
+__device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+// One channel's values of CW tokens from token t0 on: scaled, with the bias, stored. FULL: the tile is
+// inside the output.
+template <typename T, int CW, bool FULL>
+__device__ __forceinline__ void store_tokens(const Int8Args& a, const uint32_t (&acc)[CW], const float* sx, float sw, float bias,
                                              int64_t t0, int64_t channel) {
   T* out = reinterpret_cast<T*>(a.out);
   const int lane = threadIdx.x & 31;
-  float v[32];
+  float v[CW];
 #pragma unroll
-  for (int j = 0; j < 32; j += 4) {
+  for (int j = 0; j < CW; j += 4) {
     const float4 s = *reinterpret_cast<const float4*>(sx + j);
-    v[j] = fmaf(__int2float_rn(acc[j]) * s.x, sw, bias);
-    v[j + 1] = fmaf(__int2float_rn(acc[j + 1]) * s.y, sw, bias);
-    v[j + 2] = fmaf(__int2float_rn(acc[j + 2]) * s.z, sw, bias);
-    v[j + 3] = fmaf(__int2float_rn(acc[j + 3]) * s.w, sw, bias);
+    v[j] = fmaf(__int2float_rn((int)acc[j]) * s.x, sw, bias);
+    v[j + 1] = fmaf(__int2float_rn((int)acc[j + 1]) * s.y, sw, bias);
+    v[j + 2] = fmaf(__int2float_rn((int)acc[j + 2]) * s.z, sw, bias);
+    v[j + 3] = fmaf(__int2float_rn((int)acc[j + 3]) * s.w, sw, bias);
   }
   if (sizeof(T) == 2 && a.pairs) {
     // two channels a store: an even lane takes both channels of an even token, its neighbour of the odd one
-    const int64_t c = channel & ~(int64_t)1;
-    const bool odd = lane & 1;
+    const int odd = lane & 1;
+    const int64_t c = channel - odd;
+    T* p = out + (t0 + odd) * a.N + c;
+    const bool in = FULL || c < a.N;
+    const int left = FULL ? CW : (int)min((int64_t)CW, a.M - t0 - odd);  // tokens from this lane's first on
 #pragma unroll
-    for (int j = 0; j < 32; j += 2) {
+    for (int j = 0; j < CW; j += 2) {
       const float other = __shfl_xor_sync(0xffffffffu, odd ? v[j] : v[j + 1], 1);
-      const int64_t t = t0 + j + (odd ? 1 : 0);
       const float lo = odd ? other : v[j], hi = odd ? v[j + 1] : other;
       if constexpr (sizeof(T) == 2) {
-        if (t < a.M && c < a.N) *reinterpret_cast<uint32_t*>(out + t * a.N + c) = rows::pack2<T>(lo, hi);
+        if (FULL || (in && j < left)) *reinterpret_cast<uint32_t*>(p) = rows::pack2<T>(lo, hi);
       }
+      p += 2 * a.N;
     }
   } else {
+    T* p = out + t0 * a.N + channel;
+    const int left = FULL ? CW : channel < a.N ? (int)min((int64_t)CW, a.M - t0) : 0;
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (t0 + j < a.M && channel < a.N) st(out + (t0 + j) * a.N + channel, v[j]);
+    for (int j = 0; j < CW; ++j) {
+      if (FULL || j < left) st(p, v[j]);
+      p += a.N;
+    }
   }
 }
 
@@ -104,7 +116,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   extern __shared__ uint8_t dyn[];
   __shared__ __align__(8) uint64_t full[S], empty[S], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_base, last_flag;
-  __shared__ __align__(16) float scales[4][32];
+  __shared__ __align__(16) float scales[kEpilogue / 32][NT > 64 ? NT / 2 : 32];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -112,7 +124,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     tma_prefetch_desc(&tm_w);
     tma_prefetch_desc(&tm_x);
     for (int i = 0; i < S; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
-    for (int i = 0; i < 2; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], 128);
+    for (int i = 0; i < 2; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], kEpilogue);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -207,79 +219,83 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       if (!ok) atomicExch(a.error, 1u);
     }
   } else {
-    // each epilogue warp has the 32 TMEM lanes, here channels, of its number mod 4
-    const int q = warp & 3;
-    float* sx = scales[q];
+    // each epilogue warp has the 32 TMEM lanes, here channels, of its number mod 4, and half of the tokens
+    // (the first four warps all of 16)
+    constexpr int COLS = NT >= 32 ? NT / 2 : NT, CW = COLS < 32 ? COLS : 32, STEPS = COLS / CW;
+    const int q = warp & 3, first = (warp - 2) / 4 * COLS;
+    const bool has_cols = first < NT;
+    float* sx = scales[warp - 2];
     uint32_t local = 0, limit = kWaitLimit;
     wait_predecessor();
     for (int u = blockIdx.x; u < units; u += gridDim.x, ++local) {
       const uint32_t b = local & 1;
       const int tile = u / a.splits, split = u % a.splits;
-      const int64_t n0 = (int64_t)(tile % a.n_tiles) * kChannels, m0 = (int64_t)(tile / a.n_tiles) * NT;
+      const int64_t n0 = (int64_t)(tile % a.n_tiles) * kChannels, m0 = (int64_t)(tile / a.n_tiles) * NT + first;
       const int64_t channel = n0 + q * 32 + lane;
-      const bool there = channel < a.N;
+      const bool there = channel < a.N, full_tile = n0 + kChannels <= a.N && m0 + COLS <= a.M;
       const float sw = there ? __ldg(a.sw + channel) : 0.f;
       float bias = 0.f;
       if (a.bias && there)
         bias = a.bias32 ? __ldg(reinterpret_cast<const float*>(a.bias) + channel) : ld(reinterpret_cast<const T*>(a.bias) + channel);
+      __syncwarp();
+#pragma unroll
+      for (int c = 0; c < COLS; c += 32)
+        if (c + lane < COLS) sx[c + lane] = m0 + c + lane < a.M ? __ldg(a.sx + m0 + c + lane) : 0.f;
+      __syncwarp();
       if (!mbar_wait(&acc_full[b], (local >> 1) & 1, limit)) {
-        // carries on with what is there, so that the four warps meet at every barrier below
+        // carries on with what is there, so that the warps meet at every barrier below
         limit = 1;
         if (lane == 0) atomicExch(a.error, 1u);
       }
       tc_fence_after();
-      const uint32_t acc = tmem + b * NT + ((uint32_t)(q * 32) << 16);
-      constexpr int CW = NT < 32 ? NT : 32;  // columns at a time
-      int32_t* part = a.parts + ((int64_t)tile * a.splits + split) * NT * kChannels + q * 32 + lane;
-#pragma unroll 1
-      for (int c = 0; c < NT; c += CW) {
-        int32_t v[32];
-        if constexpr (CW == 32) {
-          tmem_ld32(acc + c, reinterpret_cast<uint32_t(&)[32]>(v));
-        } else {
-          uint32_t r[16];
-          tmem_ld16(acc + c, r);
+      const uint32_t acc = tmem + b * NT + first + ((uint32_t)(q * 32) << 16);
+      int32_t* part = a.parts + (((int64_t)tile * a.splits + split) * NT + first) * kChannels + q * 32 + lane;
+      if (has_cols) {
+        uint32_t v[2][CW];  // the next columns on their way from TMEM while these are stored
+        load_cols(acc, v[0]);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = (int32_t)r[j], v[16 + j] = 0;
-        }
-        tmem_wait_ld();
-        if (a.splits > 1) {
-          // tokens beyond M have no reader
+        for (int i = 0; i < STEPS; ++i) {
+          tmem_wait_ld();
+          if (i + 1 < STEPS) {
+            load_cols(acc + (i + 1) * CW, v[(i + 1) & 1]);
+          } else {
+            tc_fence_before();
+            mbar_arrive(&acc_empty[b]);
+          }
+          if (a.splits > 1) {
+            // tokens beyond M have no reader
 #pragma unroll
-          for (int j = 0; j < CW; ++j)
-            if (m0 + c + j < a.M) part[(c + j) * kChannels] = v[j];
-        } else {
-          __syncwarp();
-          sx[lane] = m0 + c + lane < a.M ? __ldg(a.sx + m0 + c + lane) : 0.f;
-          __syncwarp();
-          if (m0 + c < a.M) store_tokens<T>(a, v, sx, sw, bias, m0 + c, channel);
+            for (int j = 0; j < CW; ++j)
+              if (m0 + i * CW + j < a.M) part[(i * CW + j) * kChannels] = (int32_t)v[i & 1][j];
+          } else if (full_tile) {
+            store_tokens<T, CW, true>(a, v[i & 1], sx + i * CW, sw, bias, m0 + i * CW, channel);
+          } else if (m0 + i * CW < a.M) {
+            store_tokens<T, CW, false>(a, v[i & 1], sx + i * CW, sw, bias, m0 + i * CW, channel);
+          }
         }
+      } else {
+        mbar_arrive(&acc_empty[b]);
       }
-      tc_fence_before();
-      mbar_arrive(&acc_empty[b]);
       if (a.splits > 1) {
         __threadfence();
         epilogue_barrier();
         if (threadIdx.x == 64) last_flag = atomicAdd(a.counts + tile, 1u) == (uint32_t)a.splits - 1 ? 1u : 0u;
         epilogue_barrier();
-        if (last_flag) {
+        if (last_flag && has_cols) {
           __threadfence();
-          const int32_t* p0 = a.parts + (int64_t)tile * a.splits * NT * kChannels + q * 32 + lane;
+          const int32_t* p0 = a.parts + ((int64_t)tile * a.splits * NT + first) * kChannels + q * 32 + lane;
 #pragma unroll 1
-          for (int c = 0; c < NT && m0 + c < a.M; c += CW) {
-            int32_t v[32];
+          for (int c = 0; c < COLS && m0 + c < a.M; c += CW) {
+            uint32_t v[CW];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = 0;
+            for (int j = 0; j < CW; ++j) v[j] = 0;
 #pragma unroll 1
             for (int i = 0; i < a.splits; ++i) {
 #pragma unroll
               for (int j = 0; j < CW; ++j)
-                if (m0 + c + j < a.M) v[j] += __ldcg(p0 + ((int64_t)i * NT + c + j) * kChannels);
+                if (m0 + c + j < a.M) v[j] += (uint32_t)__ldcg(p0 + ((int64_t)i * NT + c + j) * kChannels);
             }
-            __syncwarp();
-            sx[lane] = lane < CW && m0 + c + lane < a.M ? __ldg(a.sx + m0 + c + lane) : 0.f;
-            __syncwarp();
-            store_tokens<T>(a, v, sx, sw, bias, m0 + c, channel);
+            store_tokens<T, CW, false>(a, v, sx + c, sw, bias, m0 + c, channel);
           }
         }
       }

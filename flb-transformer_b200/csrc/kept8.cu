@@ -5,7 +5,7 @@
 // Bound by memory: every element is read and written once. A warp takes 256 consecutive elements of a row at
 // a time, two blocks of the kept form, whose largest magnitudes are a reduction over 16 lanes (32 where rows
 // do not start on 16 bytes).
-#include <type_traits>
+#include <initializer_list>
 #include "rows.cuh"
 
 namespace flb {
@@ -35,60 +35,90 @@ template <typename T> __device__ __forceinline__ float2 gate_of(float z) {
 }
 
 // The warp's chunks, one after the other; the body gets the row, the chunk's first element and the lane.
-template <typename F> __device__ __forceinline__ void for_chunks(const KeptArgs& a, F&& body) {
+template <bool FLAT, typename F> __device__ __forceinline__ void for_chunks(const KeptArgs& a, F&& body) {
   const int lane = threadIdx.x & 31;
   const int64_t n = (int64_t)gridDim.x * (kThreads / 32);
   for (int64_t i = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); i < a.chunks; i += n) {
-    const int64_t row = a.per_row == 1 ? i : a.chunks <= 0xffffffffll ? (uint32_t)i / (uint32_t)a.per_row : i / a.per_row;
-    body(row, (int)(i - row * a.per_row) * 256, lane);
+    if constexpr (FLAT) {
+      body(i, 0, lane);
+    } else {
+      const int64_t row = a.chunks <= 0xffffffffll ? (uint32_t)i / (uint32_t)a.per_row : i / a.per_row;
+      body(row, (int)(i - row * a.per_row) * 256, lane);
+    }
   }
 }
 
-template <typename T, bool VEC> __global__ void __launch_bounds__(kThreads) pack_kernel(const KeptArgs a) {
-  const int D = a.D;
-  for_chunks(a, [&](int64_t row, int base, int lane) {
-    float v[8];
-    load8<T, VEC>(v, reinterpret_cast<const T*>(a.x) + row * D, base, lane, D);
-    keep8<VEC>(v, a.cx + row * code_pitch(D), a.ex + row * blocks_of(D), base, lane, D);
+template <typename T, bool VEC>
+__device__ __forceinline__ void keep_raw(const Raw8<T>& r, const F2 (&v)[4], int8_t* codes, uint8_t* exps, int64_t row, int base,
+                                         int lane, int D) {
+  uint32_t m[VEC ? 1 : 2];
+  max_bits<T, VEC>(r, m);
+  keep8<VEC>(v, m, codes + row * code_pitch(D), exps + row * blocks_of(D), base, lane, D);
+}
+
+// FORM 0: rows that start on 16 bytes, a multiple of 8 wide; 1: others; 2: FLAT
+template <int FORM> constexpr bool kVec = FORM != 1;
+
+template <typename T, int FORM> __global__ void __launch_bounds__(kThreads) pack_kernel(const KeptArgs a) {
+  constexpr bool VEC = kVec<FORM>;
+  const int D = FORM == 2 ? 256 : a.D;
+  for_chunks<FORM == 2>(a, [&](int64_t row, int base, int lane) {
+    Raw8<T> r;
+    F2 v[4];
+    load_raw<T, VEC>(r, reinterpret_cast<const T*>(a.x) + row * D, base, lane, D);
+    to_float<T>(r, v);
+    keep_raw<T, VEC>(r, v, a.cx, a.ex, row, base, lane, D);
   });
 }
 
-template <typename T, bool VEC> __global__ void __launch_bounds__(kThreads) unpack_kernel(const KeptArgs a) {
-  const int D = a.D;
-  for_chunks(a, [&](int64_t row, int base, int lane) {
-    float v[8];
+template <typename T, int FORM> __global__ void __launch_bounds__(kThreads) unpack_kernel(const KeptArgs a) {
+  constexpr bool VEC = kVec<FORM>;
+  const int D = FORM == 2 ? 256 : a.D;
+  for_chunks<FORM == 2>(a, [&](int64_t row, int base, int lane) {
+    F2 v[4];
     kept_to_float<VEC>(load_kept<VEC>(a.cx + row * code_pitch(D), a.ex + row * blocks_of(D), base, lane, D), v);
     if constexpr (std::is_same<T, __half>::value) {
       // a magnitude near the type's largest can be kept as 65536: back to the largest (a NaN stays one)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = fabsf(v[j]) > 65504.f ? copysignf(65504.f, v[j]) : v[j];
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = split(v[i]);
+        v[i] = f2(fabsf(f.x) > 65504.f ? copysignf(65504.f, f.x) : f.x, fabsf(f.y) > 65504.f ? copysignf(65504.f, f.y) : f.y);
+      }
     }
     store8<T, VEC>(reinterpret_cast<T*>(a.y) + row * D, v, base, lane, D);
   });
 }
 
-template <typename T, bool VEC, bool KEEP> __global__ void __launch_bounds__(kThreads) gate_fwd_kernel(const KeptArgs a) {
-  const int D = a.D;
-  for_chunks(a, [&](int64_t row, int base, int lane) {
-    float x[8], z[8];
-    load8<T, VEC>(x, reinterpret_cast<const T*>(a.x) + row * D, base, lane, D);
-    load8<T, VEC>(z, reinterpret_cast<const T*>(a.z) + row * D, base, lane, D);
+template <typename T, int FORM, bool KEEP> __global__ void __launch_bounds__(kThreads) gate_fwd_kernel(const KeptArgs a) {
+  constexpr bool VEC = kVec<FORM>;
+  const int D = FORM == 2 ? 256 : a.D;
+  for_chunks<FORM == 2>(a, [&](int64_t row, int base, int lane) {
+    Raw8<T> rx, rz;
+    F2 x[4], z[4];
+    load_raw<T, VEC>(rx, reinterpret_cast<const T*>(a.x) + row * D, base, lane, D);
+    load_raw<T, VEC>(rz, reinterpret_cast<const T*>(a.z) + row * D, base, lane, D);
+    to_float<T>(rx, x);
+    to_float<T>(rz, z);
     if constexpr (KEEP) {
-      keep8<VEC>(x, a.cx + row * code_pitch(D), a.ex + row * blocks_of(D), base, lane, D);
-      keep8<VEC>(z, a.cz + row * code_pitch(D), a.ez + row * blocks_of(D), base, lane, D);
+      keep_raw<T, VEC>(rx, x, a.cx, a.ex, row, base, lane, D);
+      keep_raw<T, VEC>(rz, z, a.cz, a.ez, row, base, lane, D);
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] *= gate_of<T>(z[j]).x;
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = split(z[i]);
+      x[i] = mul2(x[i], f2(gate_of<T>(f.x).x, gate_of<T>(f.y).x));
+    }
     store8<T, VEC>(reinterpret_cast<T*>(a.y) + row * D, x, base, lane, D);
   });
 }
 
 // x, z as in the forward, or their kept form; y takes dx, y2 takes dz
-template <typename T, bool VEC, bool KEEP>
+template <typename T, int FORM, bool KEEP>
 __global__ void __launch_bounds__(kThreads) gate_bwd_kernel(const KeptArgs a, const void* dy_) {
-  const int D = a.D;
-  for_chunks(a, [&](int64_t row, int base, int lane) {
-    float x[8], z[8], dy[8], dz[8];
+  constexpr bool VEC = kVec<FORM>;
+  const int D = FORM == 2 ? 256 : a.D;
+  for_chunks<FORM == 2>(a, [&](int64_t row, int base, int lane) {
+    F2 x[4], z[4], dy[4], dz[4];
     load8<T, VEC>(dy, reinterpret_cast<const T*>(dy_) + row * D, base, lane, D);
     if constexpr (KEEP) {
       const Kept8 kx = load_kept<VEC>(a.cx + row * code_pitch(D), a.ex + row * blocks_of(D), base, lane, D);
@@ -100,11 +130,11 @@ __global__ void __launch_bounds__(kThreads) gate_bwd_kernel(const KeptArgs a, co
       load8<T, VEC>(z, reinterpret_cast<const T*>(a.z) + row * D, base, lane, D);
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float2 g = gate_of<T>(z[j]);
-      const float dx = dy[j] * g.x;
-      dz[j] = dx * x[j] * g.y;
-      x[j] = dx;
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = split(z[i]), g = gate_of<T>(f.x), h = gate_of<T>(f.y);
+      const F2 dx = mul2(dy[i], f2(g.x, h.x));
+      dz[i] = mul2(mul2(dx, x[i]), f2(g.y, h.y));
+      x[i] = dx;
     }
     store8<T, VEC>(reinterpret_cast<T*>(a.y) + row * D, x, base, lane, D);
     store8<T, VEC>(reinterpret_cast<T*>(a.y2) + row * D, dz, base, lane, D);
@@ -119,38 +149,51 @@ unsigned grid_of(int64_t chunks) {
   return (unsigned)std::max<int64_t>(1, std::min<int64_t>((chunks + per - 1) / per, (int64_t)num_sms() * 16));
 }
 
-template <template <typename, bool> class Launch, typename... A>
-int by_type(int dtype, bool vec, const A&... args) {
+template <template <typename, int> class Launch, typename T, typename... A> void by_form(int form, const A&... args) {
+  if (form == 2) Launch<T, 2>::run(args...);
+  else if (form == 1) Launch<T, 1>::run(args...);
+  else Launch<T, 0>::run(args...);
+}
+template <template <typename, int> class Launch, typename... A> int by_type(int dtype, int form, const A&... args) {
   switch (dtype) {
-    case FLB_F32: vec ? Launch<float, true>::run(args...) : Launch<float, false>::run(args...); break;
-    case FLB_F16: vec ? Launch<__half, true>::run(args...) : Launch<__half, false>::run(args...); break;
-    default: vec ? Launch<__nv_bfloat16, true>::run(args...) : Launch<__nv_bfloat16, false>::run(args...); break;
+    case FLB_F32: by_form<Launch, float>(form, args...); break;
+    case FLB_F16: by_form<Launch, __half>(form, args...); break;
+    default: by_form<Launch, __nv_bfloat16>(form, args...); break;
   }
   count_launches(1);
   return check_cuda(cudaGetLastError(), "8-bit kept form launch");
 }
 
-template <typename T, bool VEC> struct Pack {
-  static void run(const KeptArgs& a, cudaStream_t s) { pack_kernel<T, VEC><<<grid_of(a.chunks), kThreads, 0, s>>>(a); }
+template <typename T, int FORM> struct Pack {
+  static void run(const KeptArgs& a, cudaStream_t s) { pack_kernel<T, FORM><<<grid_of(a.chunks), kThreads, 0, s>>>(a); }
 };
-template <typename T, bool VEC> struct Unpack {
-  static void run(const KeptArgs& a, cudaStream_t s) { unpack_kernel<T, VEC><<<grid_of(a.chunks), kThreads, 0, s>>>(a); }
+template <typename T, int FORM> struct Unpack {
+  static void run(const KeptArgs& a, cudaStream_t s) { unpack_kernel<T, FORM><<<grid_of(a.chunks), kThreads, 0, s>>>(a); }
 };
-template <typename T, bool VEC> struct GateFwd {
+template <typename T, int FORM> struct GateFwd {
   static void run(const KeptArgs& a, cudaStream_t s) {
-    if (a.cx) gate_fwd_kernel<T, VEC, true><<<grid_of(a.chunks), kThreads, 0, s>>>(a);
-    else gate_fwd_kernel<T, VEC, false><<<grid_of(a.chunks), kThreads, 0, s>>>(a);
+    if (a.cx) gate_fwd_kernel<T, FORM, true><<<grid_of(a.chunks), kThreads, 0, s>>>(a);
+    else gate_fwd_kernel<T, FORM, false><<<grid_of(a.chunks), kThreads, 0, s>>>(a);
   }
 };
-template <typename T, bool VEC> struct GateBwd {
+template <typename T, int FORM> struct GateBwd {
   static void run(const KeptArgs& a, const void* dy, cudaStream_t s) {
-    if (a.cx) gate_bwd_kernel<T, VEC, true><<<grid_of(a.chunks), kThreads, 0, s>>>(a, dy);
-    else gate_bwd_kernel<T, VEC, false><<<grid_of(a.chunks), kThreads, 0, s>>>(a, dy);
+    if (a.cx) gate_bwd_kernel<T, FORM, true><<<grid_of(a.chunks), kThreads, 0, s>>>(a, dy);
+    else gate_bwd_kernel<T, FORM, false><<<grid_of(a.chunks), kThreads, 0, s>>>(a, dy);
   }
 };
 
-KeptArgs kept_args(int64_t R, int64_t D) {
+// The chunks of [R, D], and the form that every pointer and the width allow
+KeptArgs kept_args(int64_t R, int64_t D, std::initializer_list<const void*> pointers, int* form) {
   KeptArgs a = {};
+  *form = D % 8 == 0 ? 0 : 1;
+  for (const void* p : pointers)
+    if (!on16(p)) *form = 1;
+  if (*form == 0 && D % kBlock == 0 && R * D % 256 == 0) {
+    *form = 2;
+    R = R * D / 256;
+    D = 256;
+  }
   a.per_row = (D + 255) / 256;
   a.chunks = R * a.per_row;
   a.D = (int)D;
@@ -160,32 +203,35 @@ KeptArgs kept_args(int64_t R, int64_t D) {
 }  // namespace
 
 int pack8(const void* x, int8_t* codes, uint8_t* exps, int64_t R, int64_t D, int dtype, cudaStream_t s) {
-  KeptArgs a = kept_args(R, D);
+  int form;
+  KeptArgs a = kept_args(R, D, {x, codes}, &form);
   a.x = x, a.cx = codes, a.ex = exps;
-  return by_type<Pack>(dtype, D % 8 == 0 && on16(x) && on16(codes), a, s);
+  return by_type<Pack>(dtype, form, a, s);
 }
 
 int unpack8(const int8_t* codes, const uint8_t* exps, void* out, int64_t R, int64_t D, int dtype, cudaStream_t s) {
-  KeptArgs a = kept_args(R, D);
+  int form;
+  KeptArgs a = kept_args(R, D, {codes, out}, &form);
   a.cx = const_cast<int8_t*>(codes), a.ex = const_cast<uint8_t*>(exps), a.y = out;
-  return by_type<Unpack>(dtype, D % 8 == 0 && on16(out) && on16(codes), a, s);
+  return by_type<Unpack>(dtype, form, a, s);
 }
 
 int gate_fwd(const void* x, const void* z, void* y, int8_t* cx, uint8_t* ex, int8_t* cz, uint8_t* ez, int64_t R,
              int64_t D, int dtype, cudaStream_t s) {
-  KeptArgs a = kept_args(R, D);
+  int form;
+  KeptArgs a = kept_args(R, D, {x, z, y, cx, cz}, &form);
   a.x = x, a.z = z, a.y = y, a.cx = cx, a.ex = ex, a.cz = cz, a.ez = ez;
-  return by_type<GateFwd>(dtype, D % 8 == 0 && on16(x) && on16(z) && on16(y) && on16(cx) && on16(cz), a, s);
+  return by_type<GateFwd>(dtype, form, a, s);
 }
 
 int gate_bwd(const void* x, const void* z, const int8_t* cx, const uint8_t* ex, const int8_t* cz, const uint8_t* ez,
              const void* dy, void* dx, void* dz, int64_t R, int64_t D, int dtype, cudaStream_t s) {
-  KeptArgs a = kept_args(R, D);
+  int form;
+  KeptArgs a = kept_args(R, D, {x, z, cx, cz, dy, dx, dz}, &form);
   a.x = x, a.z = z, a.y = dx, a.y2 = dz;
   a.cx = const_cast<int8_t*>(cx), a.ex = const_cast<uint8_t*>(ex);
   a.cz = const_cast<int8_t*>(cz), a.ez = const_cast<uint8_t*>(ez);
-  return by_type<GateBwd>(dtype, D % 8 == 0 && on16(x) && on16(z) && on16(cx) && on16(cz) && on16(dy) && on16(dx) && on16(dz),
-                          a, dy, s);
+  return by_type<GateBwd>(dtype, form, a, dy, s);
 }
 
 }  // namespace flb

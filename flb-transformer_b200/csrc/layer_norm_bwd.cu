@@ -71,19 +71,19 @@ __device__ __forceinline__ void copy8(uint8_t* slot, const T* row, int base, int
     }
   }
 }
-template <typename T, bool VEC> __device__ __forceinline__ void copied8(const uint8_t* slot, float (&v)[8]) {
+template <typename T, bool VEC> __device__ __forceinline__ void copied8(const uint8_t* slot, F2 (&v)[4]) {
+  Raw8<T> r;
   if constexpr (VEC) {
-    Raw8<T> r;
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
       const uint4 u = reinterpret_cast<const uint4*>(slot)[i * blockDim.x + threadIdx.x];
       r.w[4 * i] = u.x, r.w[4 * i + 1] = u.y, r.w[4 * i + 2] = u.z, r.w[4 * i + 3] = u.w;
     }
-    to_float<T>(r, v);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = reinterpret_cast<const float*>(slot)[j * blockDim.x + threadIdx.x];
+    for (int j = 0; j < 8; ++j) r.w[j % (sizeof(T) * 2)] = reinterpret_cast<const uint32_t*>(slot)[j * blockDim.x + threadIdx.x];
   }
+  to_float<T>(r, v);
 }
 
 // Rows held at a time: three with 16-bit elements, two with float32; in the widest form, whose block is a
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
   constexpr int S = kStages<T, MODE == 2>, CB = chunk_bytes<T, VEC, KEPT>();
   constexpr bool COPY_DY = kCopies<T, VEC>, COPY_X = !KEPT && COPY_DY, COPY_CODES = KEPT && VEC;
   extern __shared__ __align__(16) uint8_t ring[];  // [S][CH][x or codes | dy][threads]; at the end [2][D] floats
-  __shared__ float slot[WARP ? 1 : 2][2][32];
+  __shared__ float2 slot[WARP ? 1 : 2][32];
   let_successor_start();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t group = blockIdx.y;
@@ -138,11 +138,11 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
     copies_commit();
   };
 
-  float dw[CH][8], db[CH][8];
+  F2 dw[CH][4], db[CH][4];
 #pragma unroll
   for (int c = 0; c < CH; ++c)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) dw[c][j] = db[c][j] = 0.f;
+    for (int i = 0; i < 4; ++i) dw[c][i] = db[c][i] = f2(0.f);
 
   // what is not copied: the row's statistics, its blocks' exponents, and the rows without copies
   float mean = 0.f, rstd = 0.f;
@@ -176,64 +176,69 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
     }
     if (row + stride < a.R) fetch_small(row + stride);
     copies_wait<S - 1>();
-    // h and gw = dy w of chunk c; read again after the sums, which costs less than the registers to hold them
-    auto values = [&](int c, float (&h)[8], float (&dy)[8], float (&gw)[8]) {
+    // chunk c of x (or the kept h), dy and the weight; read again after the sums, which costs less than the
+    // registers to hold them
+    auto values = [&](int c, F2 (&x)[4], F2 (&dy)[4], F2 (&w)[4]) {
       const int base = first + c * step;
       if constexpr (COPY_DY) copied8<T, VEC>(part_of(stage, c, true), dy); else to_float<T>(rdy[c], dy);
       if constexpr (KEPT) {
         Kept8 k = rk[c];
         if constexpr (COPY_CODES) k.c = reinterpret_cast<const uint2*>(part_of(stage, c, false))[threadIdx.x];
-        kept_to_float<VEC>(k, h);
+        kept_to_float<VEC>(k, x);
       } else {
-        if constexpr (COPY_X) copied8<T, VEC>(part_of(stage, c, false), h); else to_float<T>(rx[c], h);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) h[j] = (h[j] - m) * rs;
+        if constexpr (COPY_X) copied8<T, VEC>(part_of(stage, c, false), x); else to_float<T>(rx[c], x);
       }
-      if (a.w) {
-        if (a.w32) load8<float, VEC>(gw, reinterpret_cast<const float*>(a.w) + group * D, base, lane, D);
-        else load8<T, VEC>(gw, reinterpret_cast<const T*>(a.w) + group * D, base, lane, D);
+      if (!a.w) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) gw[j] *= dy[j];
+        for (int i = 0; i < 4; ++i) w[i] = f2(1.f);
+      } else if (a.w32) {
+        load8<float, VEC>(w, reinterpret_cast<const float*>(a.w) + group * D, base, lane, D);
       } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) gw[j] = dy[j];
+        load8<T, VEC>(w, reinterpret_cast<const T*>(a.w) + group * D, base, lane, D);
       }
     };
-    float s1 = 0.f, s2 = 0.f;
+    // h = x h1 + h0
+    const float h1 = KEPT ? 1.f : rs, h0 = KEPT ? 0.f : -m * rs;
+    F2 t1 = f2(0.f), t2 = f2(0.f);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      float h[8], dy[8], gw[8];
-      values(c, h, dy, gw);
+      F2 x[4], dy[4], w[4];
+      values(c, x, dy, w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {  // dy is zero beyond D
-        dw[c][j] = fmaf(dy[j], h[j], dw[c][j]);
-        db[c][j] += dy[j];
-        s1 += gw[j];
-        s2 = fmaf(gw[j], h[j], s2);
+      for (int i = 0; i < 4; ++i) {  // dy is zero beyond D
+        const F2 h = KEPT ? x[i] : fma2(x[i], f2(h1), f2(h0)), gw = mul2(dy[i], w[i]);
+        dw[c][i] = fma2(dy[i], h, dw[c][i]);
+        db[c][i] = add2(db[c][i], dy[i]);
+        t1 = add2(t1, gw);
+        t2 = fma2(gw, h, t2);
       }
     }
-    s1 = warp_sum(s1);
-    s2 = warp_sum(s2);
+    float s1 = warp_sum(sum2(t1)), s2 = warp_sum(sum2(t2));
     if constexpr (!WARP) {
-      // the slots alternate: a warp that is a row ahead writes the other pair, and is not two ahead
+      // the slots alternate: a warp that is a row ahead writes the other ones, and is not two ahead
       // before every warp has passed the barrier of the row between, after reading this one's
-      if (lane == 0) slot[turn][0][warp] = s1, slot[turn][1][warp] = s2;
+      if (lane == 0) slot[turn][warp] = make_float2(s1, s2);
       __syncthreads();
-      const int n = blockDim.x >> 5;
-      s1 = warp_sum(lane < n ? slot[turn][0][lane] : 0.f);
-      s2 = warp_sum(lane < n ? slot[turn][1][lane] : 0.f);
+      s1 = s2 = 0.f;
+      for (int i = 0; i < (int)(blockDim.x >> 5); ++i) {
+        const float2 t = slot[turn][i];
+        s1 += t.x;
+        s2 += t.y;
+      }
       turn ^= 1;
     }
+    // dx = rs (dy w - s1 - h s2) = rs w dy + x c1 + c0
     s1 *= inv_d;
     s2 *= inv_d;
+    const float c1 = -rs * s2 * h1, c0 = -rs * fmaf(s2, h0, s1);
     T* dx = reinterpret_cast<T*>(a.dx) + (group * a.R + row) * D;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      float h[8], dy[8], gw[8];
-      values(c, h, dy, gw);
+      F2 x[4], dy[4], w[4];
+      values(c, x, dy, w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) gw[j] = rs * (gw[j] - s1 - h[j] * s2);
-      store8<T, VEC>(dx, gw, first + c * step, lane, D);
+      for (int i = 0; i < 4; ++i) x[i] = fma2(mul2(f2(rs), w[i]), dy[i], fma2(x[i], f2(c1), f2(c0)));
+      store8<T, VEC>(dx, x, first + c * step, lane, D);
     }
     stage = stage + 1 == S ? 0 : stage + 1;
   }
@@ -257,26 +262,34 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
       __syncthreads();
       if (warp != t) continue;
 #pragma unroll
-      for (int c = 0; c < CH; ++c)
+      for (int c = 0; c < CH; ++c) {
+        float vw[8], vb[8];
+        to_scalars(dw[c], vw);
+        to_scalars(db[c], vb);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int p = Chunk<VEC>::at(first + c * step, lane, j);
           if (p < D) {
-            sm[p] = (t ? sm[p] : 0.f) + dw[c][j];
-            sm[D + p] = (t ? sm[D + p] : 0.f) + db[c][j];
+            sm[p] = (t ? sm[p] : 0.f) + vw[j];
+            sm[D + p] = (t ? sm[D + p] : 0.f) + vb[j];
           }
         }
+      }
     }
     __syncthreads();
     for (int p = threadIdx.x; p < D; p += blockDim.x) out(p, sm[p], sm[D + p]);
   } else {
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+    for (int c = 0; c < CH; ++c) {
+      float vw[8], vb[8];
+      to_scalars(dw[c], vw);
+      to_scalars(db[c], vb);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int p = Chunk<VEC>::at(first + c * step, lane, j);
-        if (p < D) out(p, dw[c][j], db[c][j]);
+        if (p < D) out(p, vw[j], vb[j]);
       }
+    }
   }
 }
 
@@ -292,7 +305,7 @@ __global__ void __launch_bounds__(1024) ln_sum_kernel(const float* __restrict__ 
   float v = 0.f;
   if (col < D) {
     const float* p = part + (group * blocks * 2 + which) * D + col;
-#pragma unroll 4
+#pragma unroll 8
     for (int i = ty; i < blocks; i += 32) v += __ldg(p + (int64_t)i * 2 * D);
   }
   s[ty][tx] = v;

@@ -6,8 +6,8 @@
 //
 // Bound by memory: a row is read and written once. It stays in registers between its statistics and its
 // output, so the variance is the second moment about the mean itself, not a difference of large sums. A
-// warp takes a row of up to 1024 elements and needs no barrier; wider rows get a block each, 16 elements a
-// thread (32 beyond 16384). The weight and bias are re-read for every row: they stay in L1.
+// warp takes a row of up to 1024 elements and needs no barrier; wider rows get a block each, 32 elements a
+// thread. The weight and bias are re-read for every row: they stay in L1.
 #include "rows.cuh"
 
 namespace flb {
@@ -37,15 +37,25 @@ struct RowArgs {
 
 // `fill` where there is no such vector
 template <typename T, bool VEC>
-__device__ __forceinline__ void load_param(float (&v)[8], const void* p, bool f32, float fill, int64_t off, int base,
+__device__ __forceinline__ void load_param(F2 (&v)[4], const void* p, bool f32, float fill, int64_t off, int base,
                                            int lane, int D) {
   if (!p) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = fill;
+    for (int i = 0; i < 4; ++i) v[i] = f2(fill);
   } else if (f32) {
     load8<float, VEC>(v, reinterpret_cast<const float*>(p) + off, base, lane, D);
   } else {
     load8<T, VEC>(v, reinterpret_cast<const T*>(p) + off, base, lane, D);
+  }
+}
+
+// Zeros in the place of a chunk's elements at or beyond D
+template <bool VEC> __device__ __forceinline__ void zero_beyond(F2 (&v)[4], int base, int lane, int D) {
+  if (Chunk<VEC>::has(base, lane, 7, D)) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 r = split(v[i]);
+    v[i] = f2(Chunk<VEC>::has(base, lane, 2 * i, D) ? r.x : 0.f, Chunk<VEC>::has(base, lane, 2 * i + 1, D) ? r.y : 0.f);
   }
 }
 
@@ -64,55 +74,88 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) row_fwd_kernel(const RowArg
   // chunk c of this warp starts at first + c * step
   const int first = WARP ? 0 : warp * 256, step = WARP ? 256 : (int)blockDim.x * 8;
   const T* x = reinterpret_cast<const T*>(a.x) + row * a.ldx;
-  float v[CH][8];
+  Raw8<T> raw[CH];  // as loaded: fewer registers for 16-bit rows, so more rows in flight
 #pragma unroll
-  for (int c = 0; c < CH; ++c) load8<T, VEC>(v[c], x, first + c * step, lane, D);
-
+  for (int c = 0; c < CH; ++c) load_raw<T, VEC>(raw[c], x, first + c * step, lane, D);
+  float mean = 0.f, rstd = 1.f;
   if constexpr (NORM) {
-    float s = 0.f;
+    F2 s = f2(0.f);
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+    for (int c = 0; c < CH; ++c) {
+      F2 v[4];
+      to_float<T>(raw[c], v);
+      s = add2(s, add2(add2(v[0], v[1]), add2(v[2], v[3])));
+    }
+    mean = row_sum<WARP>(sum2(s), slot[0]) / D;
+    s = f2(0.f);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s += v[c][j];
-    const float mean = row_sum<WARP>(s, slot[0]) / D;
-    s = 0.f;
+    for (int c = 0; c < CH; ++c) {
+      F2 v[4];
+      to_float<T>(raw[c], v);
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+      for (int i = 0; i < 4; ++i) v[i] = add2(v[i], f2(-mean));
+      zero_beyond<VEC>(v, first + c * step, lane, D);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[c][j] = Chunk<VEC>::at(first + c * step, lane, j) < D ? v[c][j] - mean : 0.f;
-        s = fmaf(v[c][j], v[c][j], s);
-      }
-    const float rstd = 1.f / sqrtf(row_sum<WARP>(s, slot[WARP ? 0 : 1]) / D + a.eps);
+      for (int i = 0; i < 4; ++i) s = fma2(v[i], v[i], s);
+    }
+    rstd = 1.f / sqrtf(row_sum<WARP>(sum2(s), slot[WARP ? 0 : 1]) / D + a.eps);
     if (threadIdx.x == 0 || (WARP && lane == 0)) {
       if (a.mean) a.mean[row] = mean;
       if (a.rstd) a.rstd[row] = rstd;
     }
-    const int64_t group = row / a.rows_per_group;
+  }
+  const int64_t param = NORM && a.rows_per_group != a.rows ? row / a.rows_per_group * D : 0;
+  // the normalised chunk, then with the weight and bias (beyond the row: anything)
+  auto normalised = [&](int c, F2 (&v)[4]) {
+    to_float<T>(raw[c], v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = mul2(add2(v[i], f2(-mean)), f2(rstd));
+  };
+  auto affine = [&](int c, F2 (&v)[4]) {
+    F2 w[4], b[4];
+    load_param<T, VEC>(w, a.w, a.w32, 1.f, param, first + c * step, lane, D);
+    load_param<T, VEC>(b, a.b, a.w32, 0.f, param, first + c * step, lane, D);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = fma2(v[i], w[i], b[i]);
+  };
+  if constexpr (OUT != OUT_INT8) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int base = first + c * step;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[c][j] *= rstd;
+      F2 v[4];
+      normalised(c, v);
       if constexpr (OUT == OUT_KEPT) {
-        if (base < D)
-          keep8<VEC>(v[c], a.codes + row * code_pitch(D), a.exps + row * blocks_of(D), base, lane, D);
+        if (base < D) {
+          zero_beyond<VEC>(v, base, lane, D);
+          // a row with an infinity or NaN has NaN throughout, so a block's values are all NaN or none
+          uint32_t m[VEC ? 1 : 2];
+          max_bits<VEC>(v, m);
+          keep8<VEC>(v, m, a.codes + row * code_pitch(D), a.exps + row * blocks_of(D), base, lane, D);
+        }
       }
-      float w[8], b[8];
-      load_param<T, VEC>(w, a.w, a.w32, 1.f, group * D, base, lane, D);
-      load_param<T, VEC>(b, a.b, a.w32, 0.f, group * D, base, lane, D);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[c][j] = fmaf(v[c][j], w[j], b[j]);
-      if constexpr (OUT != OUT_INT8) store8<T, VEC>(reinterpret_cast<T*>(a.y) + row * D, v[c], base, lane, D);
+      affine(c, v);
+      store8<T, VEC>(reinterpret_cast<T*>(a.y) + row * D, v, base, lane, D);
     }
-  }
-  if constexpr (OUT == OUT_INT8) {
+  } else {
     uint32_t m = 0;
+    F2 v[NORM ? CH : 1][4];
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+    for (int c = 0; c < CH; ++c) {
+      if constexpr (NORM) {
+        normalised(c, v[c]);
+        affine(c, v[c]);
+        zero_beyond<VEC>(v[c], first + c * step, lane, D);
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (Chunk<VEC>::at(first + c * step, lane, j) < D) m = max(m, abs_bits(v[c][j]));
+        for (int i = 0; i < 4; ++i) {
+          const float2 r = split(v[c][i]);
+          m = __vimax3_u32(m, abs_bits(r.x), abs_bits(r.y));
+        }
+      } else {
+        uint32_t h[1];
+        max_bits<T, true>(raw[c], h);
+        m = max(m, h[0]);
+      }
+    }
     m = row_max<WARP>(m, reinterpret_cast<uint32_t*>(slot[WARP ? 0 : 2]));
     // An infinity or NaN in the row makes its scale, and so all that is computed with it, NaN. Below
     // 2^-118 the factor 127 / a would be infinite: such a row counts as zeros.
@@ -123,9 +166,14 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) row_fwd_kernel(const RowArg
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       uint32_t q[8];
-      // product and rounding apart, each rounded as written above
+      F2 u[4];
+      if constexpr (!NORM) to_float<T>(raw[c], u);
+      float t[8];
+      to_scalars(NORM ? v[NORM ? c : 0] : u, t);
+      // product and rounding apart, each rounded as written above (as a packed pair they come out as one
+      // multiply-add, with another code now and then)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) q[j] = code_of(f == 0.f ? 0.f : __fmul_rn(v[c][j], f));
+      for (int j = 0; j < 8; ++j) q[j] = f == 0.f ? 0u : code_of(__fmul_rn(t[j], f));
       store_codes<VEC>(a.codes + row * code_pitch(D), q, first + c * step, lane, D);
     }
   }
@@ -144,8 +192,6 @@ int launch_rows(const RowArgs& a, cudaStream_t s) {
       case 3: row_fwd_kernel<T, VEC, true, 3, NORM, OUT><<<grid, block, 0, s>>>(a); break;
       default: row_fwd_kernel<T, VEC, true, 4, NORM, OUT><<<grid, block, 0, s>>>(a); break;
     }
-  } else if (D <= 16384) {
-    row_fwd_kernel<T, VEC, false, 2, NORM, OUT><<<(unsigned)a.rows, 32 * ((D + 511) / 512), 0, s>>>(a);
   } else {
     row_fwd_kernel<T, VEC, false, 4, NORM, OUT><<<(unsigned)a.rows, 32 * ((D + 1023) / 1024), 0, s>>>(a);
   }

@@ -2,6 +2,7 @@
 // over a row, the 8-bit kept form and 8-bit integer codes, programmatic dependent launch.
 #pragma once
 #include <algorithm>
+#include <type_traits>
 #include "common.cuh"
 
 namespace flb {
@@ -13,11 +14,50 @@ namespace rows {
 // that a warp's scalar accesses are still one contiguous run each. Both ways a warp's chunk is two blocks
 // of 128 elements: lanes 0-15 and 16-31, or a lane's first four and last four.
 template <bool VEC> struct Chunk {
-  // element j of the chunk that starts at `base`
+  // element j of the chunk that starts at `base`, and whether the row of D elements has it (VEC: all eight or none)
+  static __device__ __forceinline__ bool has(int base, int lane, int j, int D) {
+    return VEC ? base + lane * 8 < D : base + j * 32 + lane < D;
+  }
   static __device__ __forceinline__ int at(int base, int lane, int j) {
     return VEC ? base + lane * 8 + j : base + j * 32 + lane;
   }
 };
+
+// Two float32 in one 64-bit register pair: Blackwell multiplies and adds both in one instruction, and the
+// row kernels are near the rate at which instructions can be issued.
+struct F2 {
+  unsigned long long u;
+};
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.u) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ F2 f2(float v) { return f2(v, v); }
+__device__ __forceinline__ float2 split(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.u));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.u) : "l"(a.u), "l"(b.u));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.u) : "l"(a.u), "l"(b.u));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.u) : "l"(a.u), "l"(b.u), "l"(c.u));
+  return r;
+}
+__device__ __forceinline__ float sum2(F2 a) {
+  const float2 v = split(a);
+  return v.x + v.y;
+}
 
 template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t u);
 template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
@@ -67,26 +107,34 @@ __device__ __forceinline__ void load_raw(Raw8<T>& r, const T* __restrict__ row, 
     }
   }
 }
-template <typename T> __device__ __forceinline__ void to_float(const Raw8<T>& r, float (&v)[8]) {
-  if constexpr (sizeof(T) == 4) {
+template <typename T> __device__ __forceinline__ void to_float(const Raw8<T>& r, F2 (&v)[4]) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r.w[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = unpack2<T>(r.w[j]);
-      v[2 * j] = f.x, v[2 * j + 1] = f.y;
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      v[i] = f2(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]));
+    } else {
+      const float2 f = unpack2<T>(r.w[i]);
+      v[i] = f2(f.x, f.y);
     }
   }
 }
+__device__ __forceinline__ void to_scalars(const F2 (&v)[4], float (&s)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = split(v[i]);
+    s[2 * i] = f.x, s[2 * i + 1] = f.y;
+  }
+}
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(float (&v)[8], const T* __restrict__ row, int base, int lane, int D) {
+__device__ __forceinline__ void load8(F2 (&v)[4], const T* __restrict__ row, int base, int lane, int D) {
   Raw8<T> r;
   load_raw<T, VEC>(r, row, base, lane, D);
   to_float<T>(r, v);
 }
 template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* __restrict__ row, const float (&v)[8], int base, int lane, int D) {
+__device__ __forceinline__ void store8(T* __restrict__ row, const F2 (&f)[4], int base, int lane, int D) {
+  float v[8];
+  to_scalars(f, v);
   if constexpr (VEC) {
     const int p = base + lane * 8;
     if (p >= D) return;
@@ -147,12 +195,13 @@ __device__ __forceinline__ uint2 load_codes(const int8_t* __restrict__ row, int 
   return r;
 }
 // A signed byte b as a float: 2^23 + (b + 128) has b + 128 in its low byte.
-__device__ __forceinline__ void codes_to_float(uint2 c, float (&v)[8]) {
-  const uint32_t lo = c.x ^ 0x80808080u, hi = c.y ^ 0x80808080u;
+__device__ __forceinline__ void codes_to_float(uint2 c, F2 (&v)[4]) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    v[j] = __uint_as_float(__byte_perm(lo, 0x4B000000u, 0x7540 | j)) - 8388736.f;
-    v[4 + j] = __uint_as_float(__byte_perm(hi, 0x4B000000u, 0x7540 | j)) - 8388736.f;
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t b = (i < 2 ? c.x : c.y) ^ 0x80808080u;
+    const int j = 2 * (i & 1);
+    v[i] = add2(f2(__uint_as_float(__byte_perm(b, 0x4B000000u, 0x7540 | j)), __uint_as_float(__byte_perm(b, 0x4B000000u, 0x7541 | j))),
+                f2(-8388736.f));
   }
 }
 
@@ -182,37 +231,75 @@ __device__ __forceinline__ float scale_of(uint32_t e) {  // 2^(e - 127), NaN for
 // or NaN, whose exponent field is 255, is above every number.
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-// Keeps a lane's eight elements (chunk at `base`): codes to `crow`, the two blocks' E to `erow`.
-// All 32 lanes take part; elements at or beyond D must be zero.
-template <bool VEC>
-__device__ __forceinline__ void keep8(const float (&v)[8], int8_t* __restrict__ crow, uint8_t* __restrict__ erow,
-                                      int base, int lane, int D) {
-  uint32_t q[8];
-  auto code = [](float x, uint32_t e) {
-    // 2^(127 - E) as (254 - E) in the exponent field. The largest E, 249, has 64 for a magnitude that
-    // its own type holds and 64 * 2^122 exceeds float32: 63 then. A bad block's codes are not read.
-    if (e >= 249u) x = fminf(fmaxf(x, -63.f * 5.316911983139664e36f), 63.f * 5.316911983139664e36f);
-    return code_of(x * __uint_as_float((254u - (e > 249u ? 249u : e)) << 23));
-  };
-  if constexpr (VEC) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[j]));
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const uint32_t e = block_exp(m);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) q[j] = code(v[j], e);
-    if ((lane & 15) == 0 && base + lane * 8 < D) erow[(base + lane * 8) / kBlock] = (uint8_t)e;
+// The largest magnitude's bits among a lane's eight elements (VEC), or its first four and last four. 16-bit
+// types: the packed halves' as 16-bit integers first, then as the float32 they are.
+template <typename T> __device__ __forceinline__ uint32_t float_bits(uint32_t h) {
+  if constexpr (std::is_same<T, __half>::value) return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
+  else return h << 16;
+}
+__device__ __forceinline__ uint32_t max2_u16(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t max_halves(uint32_t v) { return max(v & 0xffffu, v >> 16); }
+template <typename T, bool VEC> __device__ __forceinline__ void max_bits(const Raw8<T>& r, uint32_t (&m)[VEC ? 1 : 2]) {
+  if constexpr (sizeof(T) == 4) {
+    constexpr uint32_t k = 0x7fffffffu;
+    const uint32_t lo = max(__vimax3_u32(r.w[0] & k, r.w[1] & k, r.w[2] & k), r.w[3] & k);
+    const uint32_t hi = max(__vimax3_u32(r.w[4] & k, r.w[5] & k, r.w[6] & k), r.w[7] & k);
+    if constexpr (VEC) m[0] = max(lo, hi); else m[0] = lo, m[1] = hi;
   } else {
-    uint32_t m[2] = {0, 0}, e[2];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m[j / 4] = max(m[j / 4], abs_bits(v[j]));
+    constexpr uint32_t k = 0x7fff7fffu;
+    const uint32_t lo = max2_u16(r.w[0] & k, r.w[1] & k), hi = max2_u16(r.w[2] & k, r.w[3] & k);
+    if constexpr (VEC) m[0] = float_bits<T>(max_halves(max2_u16(lo, hi)));
+    else m[0] = float_bits<T>(max_halves(lo)), m[1] = float_bits<T>(max_halves(hi));
+  }
+}
+// The same of eight floats. fmaxf passes over a NaN unless all are: for values of which all or none are.
+template <bool VEC> __device__ __forceinline__ void max_bits(const F2 (&f)[4], uint32_t (&m)[VEC ? 1 : 2]) {
+  float v[8];
+  to_scalars(f, v);
+  const float lo = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+  const float hi = fmaxf(fmaxf(fabsf(v[4]), fabsf(v[5])), fmaxf(fabsf(v[6]), fabsf(v[7])));
+  if constexpr (VEC) m[0] = __float_as_uint(fmaxf(lo, hi)) & 0x7fffffffu;
+  else m[0] = __float_as_uint(lo) & 0x7fffffffu, m[1] = __float_as_uint(hi) & 0x7fffffffu;
+}
+
+// Keeps a lane's eight elements (chunk at `base`), whose largest magnitudes' bits are m: codes to `crow`,
+// the two blocks' E to `erow`. All 32 lanes take part; elements at or beyond D must be zero.
+template <bool VEC>
+__device__ __forceinline__ void keep8(const F2 (&v)[4], const uint32_t (&m)[VEC ? 1 : 2], int8_t* __restrict__ crow,
+                                      uint8_t* __restrict__ erow, int base, int lane, int D) {
+  uint32_t q[8], e[2];
+  if constexpr (VEC) {
+    e[0] = e[1] = block_exp(__reduce_max_sync(lane < 16 ? 0xffffu : 0xffff0000u, m[0]));
+    if ((lane & 15) == 0 && base + lane * 8 < D) erow[(base + lane * 8) / kBlock] = (uint8_t)e[0];
+  } else {
 #pragma unroll
     for (int h = 0; h < 2; ++h) e[h] = block_exp(__reduce_max_sync(0xffffffffu, m[h]));
-#pragma unroll
-    for (int j = 0; j < 8; ++j) q[j] = code(v[j], e[j / 4]);
     if (lane < 2 && base + lane * kBlock < D) erow[base / kBlock + lane] = (uint8_t)(lane ? e[1] : e[0]);
+  }
+  if (max(e[0], e[1]) < 249u) {
+    // the unit's inverse, 2^(127 - E), has 254 - E in the exponent field; the product with it is exact, so the sum's
+    // rounding is the only one
+    const float f[2] = {__uint_as_float((254u - e[0]) << 23), __uint_as_float((254u - e[1]) << 23)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 r = split(fma2(v[i], f2(f[VEC ? 0 : i / 2]), f2(kRound)));
+      q[2 * i] = __float_as_uint(r.x), q[2 * i + 1] = __float_as_uint(r.y);
+    }
+  } else {
+    // E = 249, the largest, has 64 for a magnitude that its own type holds and 64 * 2^122 exceeds float32: 63
+    // then. A bad block's codes are not read.
+    constexpr float top = 63.f * 5.316911983139664e36f;
+    float s[8];
+    to_scalars(v, s);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t ej = e[VEC ? 0 : j / 4];
+      q[j] = code_of(fminf(fmaxf(s[j], -top), top) * __uint_as_float((254u - (ej > 249u ? 249u : ej)) << 23));
+    }
   }
   store_codes<VEC>(crow, q, base, lane, D);
 }
@@ -233,11 +320,11 @@ __device__ __forceinline__ Kept8 load_kept(const int8_t* __restrict__ crow, cons
                                            int base, int lane, int D) {
   return Kept8{load_codes<VEC>(crow, base, lane, D), load_exps<VEC>(erow, base, lane, D)};
 }
-template <bool VEC> __device__ __forceinline__ void kept_to_float(const Kept8& k, float (&v)[8]) {
+template <bool VEC> __device__ __forceinline__ void kept_to_float(const Kept8& k, F2 (&v)[4]) {
   codes_to_float(k.c, v);
   const float s0 = scale_of(k.e & 0xffu), s1 = VEC ? s0 : scale_of(k.e >> 8);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] *= j < 4 ? s0 : s1;
+  for (int i = 0; i < 4; ++i) v[i] = mul2(v[i], f2(i < 2 ? s0 : s1));
 }
 
 // Where the codes of [.., D] rows lie: rows of this many bytes, and this many E bytes a row.
@@ -250,10 +337,11 @@ __host__ __device__ inline int64_t blocks_of(int64_t D) { return (D + kBlock - 1
 template <bool WARP> __device__ __forceinline__ float row_sum(float v, float* slot) {
   v = warp_sum(v);
   if constexpr (!WARP) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = blockDim.x >> 5;
-    if (lane == 0) slot[warp] = v;
+    const int n = blockDim.x >> 5;
+    if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = warp_sum(lane < n ? slot[lane] : 0.f);
+    v = slot[0];
+    for (int i = 1; i < n; ++i) v += slot[i];
   }
   return v;
 }

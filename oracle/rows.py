@@ -1,16 +1,16 @@
 """64-bit CPU definitions of the row operators (LayerNorm, the 8-bit kept form, the sigmoid gate, 8-bit
 integer rows), each with how far a float32 computation rounded once to the output's type may be from it.
 
-A rounding to type T is off by at most half a step, eps(T) / 2 of the value; u = 2^-24 for float32. The sums
-over a row add at most 32 terms in a thread and join 1024 threads in two trees of five levels: at most
-SUM = 42 roundings each, relative to the sum of magnitudes.
+A rounding to type T is off by at most half a step, eps(T) / 2 of the value; u = 2^-24 for float32. A sum over a
+row passes at most 8 roundings in a thread, or 16 where a warp has the row alone, one between the thread's
+two halves, 5 over the warp and 32 over a block's warps: at most SUM = 46, relative to the sum of magnitudes.
 """
 import math
 
 import torch
 
 U = 2.0 ** -24
-SUM = 42
+SUM = 46
 BLOCK = 128
 
 
