@@ -1,17 +1,21 @@
 // Product of 8-bit integer rows, each with a scale: out[m, n] = (sum_k X[m, k] W[n, k]) sx[m] sw[n] + bias[n].
 //
-// tcgen05.mma kind::i8, 32-bit integer accumulators in TMEM (exact for K <= 131072: K 127^2 < 2^31). The weight
-// rows are the M side of the instruction, 128 output channels a tile, and the tokens its N side, NT of 16 to
-// 256: a decoding step of few tokens wastes little of a tile, and in the epilogue a warp's lanes are
-// consecutive channels of one token, so its stores are contiguous without a transpose.
+// tcgen05.mma kind::i8, 32-bit integer accumulators in TMEM (exact for K <= 32768: K 127^2 < 2^31). One block
+// a SM, persistent over units of work. Warp 0 loads by TMA into a ring, warp 1 issues the MMAs, warps 2-9 read
+// TMEM (two accumulators, so that a tile's epilogue runs beside the next one's MMAs). Two kernels:
 //
-// One block a SM, persistent over units of work: a unit is a tile, or with few tiles a part of the
-// tile's K range. Warp 0 loads by TMA into a ring, warp 1 issues the MMAs, warps 2-9 read TMEM (two accumulators, so
-// that a tile's epilogue runs beside the next one's MMAs). Parts of a tile leave integer sums in the
-// workspace; the block that counts itself last adds them up: integers, the same in any order.
+// int8_few_kernel, for few tokens or tiles. The weight rows are the M side of the instruction, 128 output
+// channels a tile, and the tokens its N side, NT of 16 to 128: a decoding step wastes little of a tile.
+// With fewer tiles than SMs a unit is a part of a tile's K range; the parts leave integer sums in the
+// workspace, and the block that counts itself last adds them up: integers, the same in any order. Bound by
+// reading the weight, of which a ring of 11 stages (NT = 16) keeps 176 KB a SM in flight. Any N and alignment.
 //
-// Few tokens: bound by reading the weight, of which a ring of 11 stages keeps 176 KB a SM in flight. Many: by
-// the tensor cores and the operands' way from L2 (48 KB for 512 cycles of MMA at NT = 256).
+// int8_many_kernel, for tiles enough to fill the SMs. The tokens are the M side, 128 a tile, and 256 or 128
+// channels the N side: a thread of the epilogue has a token's consecutive channels, packs them and leaves
+// them in shared memory for a TMA store. (With the other orientation a thread has one channel of many
+// tokens; pairing them up by shuffles took three times the instructions and bound the kernel: 552 us
+// against XXX for 16384 x 768 x 32000.) Bound by the tensor cores, and by the output's way to memory for
+// small K.
 #include "rows.cuh"
 #include "sm100.cuh"
 #include "tma_host.cuh"
@@ -110,7 +114,7 @@ __device__ __forceinline__ void store_tokens(const Int8Args& a, const uint32_t (
 
 template <int NT, typename T>
 __global__ void __launch_bounds__(kGemmThreads, 1)
-    int8_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Int8Args a) {
+    int8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Int8Args a) {
   constexpr int S = stages<NT>();
   constexpr uint32_t kBytes = stage_bytes<NT>();
   extern __shared__ uint8_t dyn[];
@@ -309,22 +313,238 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   }
 }
 
-// Tokens a tile and parts of a tile's K range. Up to 128 tokens: one tile of tokens. More: the width whose
-// rounds of tiles over the SMs cost least, a tile's K step costing its operands' rows. Fewer tiles than SMs:
-// as many parts of K as fill them.
-struct GemmShape {
-  int nt, n_tiles, tiles, splits;
-};
-GemmShape gemm_shape(int64_t M, int64_t N, int64_t K) {
-  GemmShape g;
-  const int64_t sms = num_sms();
-  g.n_tiles = (int)((N + kChannels - 1) / kChannels);
-  g.nt = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-  if (M > 128) {
-    auto cost = [&](int nt) { return (((M + nt - 1) / nt * g.n_tiles + sms - 1) / sms) * (kChannels + nt); };
-    if (cost(256) <= cost(128)) g.nt = 256;
+// ---- many tokens ----------------------------------------------------------------------------------------
+
+constexpr int kTokens = 128;    // a tile's tokens
+constexpr int kStaged = 4096;   // bytes a warp hands to one TMA store: 32 tokens of 128 bytes
+constexpr int kGroup = 16;      // tiles of tokens that go through all channels together, so that few operand
+                                // tiles are in use at a time
+
+template <int NC> constexpr int many_stage_bytes() { return (kTokens + NC) * kStep; }
+template <int NC> constexpr int many_stages() { return NC == 256 ? 3 : 4; }
+// ring | two staged tiles a warp | a warp's channel scales and biases
+template <int NC> constexpr int many_smem() {
+  return many_stages<NC>() * many_stage_bytes<NC>() + kEpilogue / 32 * (2 * kStaged + NC / 2 * 8) + 1024;
+}
+
+__device__ __forceinline__ void tma_store_2d(const void* tmap, const void* src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(tmap), "r"(smem_u32(src)), "r"(c0),
+               "r"(c1)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+
+template <int NC, typename T>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+    int8_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
+                     const __grid_constant__ CUtensorMap tm_out, const Int8Args a) {
+  constexpr int S = many_stages<NC>();
+  constexpr uint32_t kBytes = many_stage_bytes<NC>();
+  extern __shared__ uint8_t dyn[];
+  __shared__ __align__(8) uint64_t full[S], empty[S], acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_base;
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tm_w);
+    tma_prefetch_desc(&tm_x);
+    tma_prefetch_desc(&tm_out);
+    for (int i = 0; i < S; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], kEpilogue);
+    fence_mbar_init();
   }
-  g.tiles = (int)((M + g.nt - 1) / g.nt * g.n_tiles);
+  if (warp == 1) {
+    tmem_alloc(&tmem_base, 2 * NC);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base;
+  const int m_tiles = a.tiles / a.n_tiles;
+  auto place = [&](int tile, int& m0, int& n0) {
+    const int g = tile / (kGroup * a.n_tiles), in = tile - g * kGroup * a.n_tiles;
+    const int rows = min(kGroup, m_tiles - g * kGroup);
+    m0 = (g * kGroup + in % rows) * kTokens;
+    n0 = in / rows * NC;
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      bool ok = true;
+      uint32_t it = 0;
+      wait_predecessor();
+      for (int tile = blockIdx.x; tile < a.tiles && ok; tile += gridDim.x) {
+        int m0, n0;
+        place(tile, m0, n0);
+        for (int k = 0; k < a.k_blocks; ++k, ++it) {
+          const int s = it % S;
+          if (it >= (uint32_t)S && !mbar_wait(&empty[s], ((it / S) & 1) ^ 1, kWaitLimit)) {
+            ok = false;
+            break;
+          }
+          uint8_t* st = ring + (size_t)s * kBytes;
+          mbar_arrive_expect_tx(&full[s], kBytes);
+          tma_load_2d(st, &tm_x, &full[s], k * kStep, m0);
+          tma_load_2d(st + kTokens * kStep, &tm_w, &full[s], k * kStep, n0);
+        }
+      }
+      if (!ok) {
+        atomicExch(a.error, 1u);
+        // the copies still in flight land before the block's shared memory is given up
+        for (uint32_t i = it > (uint32_t)S ? it - S : 0; i < it; ++i) mbar_wait(&full[i % S], (i / S) & 1, kWaitLimit);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_i8<NC>();
+      uint32_t it = 0, local = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < a.tiles && ok; tile += gridDim.x, ++local) {
+        const uint32_t b = local & 1;
+        if (local >= 2 && !mbar_wait(&acc_empty[b], ((local >> 1) & 1) ^ 1, kWaitLimit)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        for (int k = 0; k < a.k_blocks; ++k, ++it) {
+          const int s = it % S;
+          if (!mbar_wait(&full[s], (it / S) & 1, kWaitLimit)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t at = smem_u32(ring + (size_t)s * kBytes);
+          uint64_t da = make_smem_desc(at, 16, 1024, kSwizzle128B);
+          uint64_t db = make_smem_desc(at + kTokens * kStep, 16, 1024, kSwizzle128B);
+#pragma unroll
+          for (int i = 0; i < kStep / 32; ++i, da += 2, db += 2) umma_i8(tmem + b * NC, da, db, idesc, (k > 0 || i > 0) ? 1u : 0u);
+          umma_commit(&empty[s]);
+        }
+        if (ok) umma_commit(&acc_full[b]);
+      }
+      if (!ok) atomicExch(a.error, 1u);
+    }
+  } else {
+    // a warp has the 32 TMEM lanes, here tokens, of its number mod 4, and half of the channels
+    constexpr int COLS = NC / 2, STEPS = COLS / 32, kWords = 32 * (int)sizeof(T) / 16;  // 16-byte words a lane stages a step
+    const int q = warp & 3, first = (warp - 2) / 4 * COLS;
+    uint8_t* mine = ring + (size_t)S * kBytes + (size_t)(warp - 2) * (2 * kStaged);
+    float* sw = reinterpret_cast<float*>(ring + (size_t)S * kBytes + (size_t)(kEpilogue / 32) * (2 * kStaged)) + (warp - 2) * 2 * COLS;
+    float* sb = sw + COLS;
+    uint32_t local = 0, limit = kWaitLimit, stores = 0;
+    wait_predecessor();
+    for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ++local) {
+      const uint32_t b = local & 1;
+      int m0, n0;
+      place(tile, m0, n0);
+      n0 += first;
+      const int token = m0 + q * 32 + lane;
+      const float sx = token < a.M ? __ldg(a.sx + token) : 0.f;
+      __syncwarp();
+#pragma unroll
+      for (int c = 0; c < COLS; c += 32) {
+        const int64_t n = n0 + c + lane;
+        const bool there = n < a.N;
+        sw[c + lane] = there ? __ldg(a.sw + n) : 0.f;
+        float bias = 0.f;
+        if (a.bias && there) bias = a.bias32 ? __ldg(reinterpret_cast<const float*>(a.bias) + n) : ld(reinterpret_cast<const T*>(a.bias) + n);
+        sb[c + lane] = bias;
+      }
+      __syncwarp();
+      if (!mbar_wait(&acc_full[b], (local >> 1) & 1, limit)) {
+        limit = 1;  // carries on with what is there
+        if (lane == 0) atomicExch(a.error, 1u);
+      }
+      tc_fence_after();
+      const uint32_t acc = tmem + b * NC + first + ((uint32_t)(q * 32) << 16);
+      uint32_t v[2][32];
+      tmem_ld32(acc, v[0]);
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        tmem_wait_ld();
+        if (i + 1 < STEPS) {
+          tmem_ld32(acc + (i + 1) * 32, v[(i + 1) & 1]);
+        } else {
+          tc_fence_before();
+          mbar_arrive(&acc_empty[b]);
+        }
+        // the staged tile of 32 tokens x 128 bytes is full after one step of float32, two of 16-bit types
+        constexpr int kPer = 128 / (kWords * 16);
+        uint8_t* tile_at = mine + (stores & 1) * kStaged;
+        if (i % kPer == 0) {
+          // the store before the last one has read its bytes
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+          __syncwarp();
+        }
+        uint32_t w[kWords * 4];
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const float4 s = *reinterpret_cast<const float4*>(sw + i * 32 + j), t = *reinterpret_cast<const float4*>(sb + i * 32 + j);
+          const rows::F2 x = rows::f2(sx);
+          const rows::F2 lo = rows::fma2(rows::mul2(rows::f2(__int2float_rn((int)v[i & 1][j]), __int2float_rn((int)v[i & 1][j + 1])), x),
+                                         rows::f2(s.x, s.y), rows::f2(t.x, t.y));
+          const rows::F2 hi = rows::fma2(rows::mul2(rows::f2(__int2float_rn((int)v[i & 1][j + 2]), __int2float_rn((int)v[i & 1][j + 3])), x),
+                                         rows::f2(s.z, s.w), rows::f2(t.z, t.w));
+          const float2 p = rows::split(lo), r = rows::split(hi);
+          if constexpr (sizeof(T) == 4) {
+            w[j] = __float_as_uint(p.x), w[j + 1] = __float_as_uint(p.y), w[j + 2] = __float_as_uint(r.x), w[j + 3] = __float_as_uint(r.y);
+          } else {
+            w[j / 2] = rows::pack2<T>(p.x, p.y), w[j / 2 + 1] = rows::pack2<T>(r.x, r.y);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < kWords; ++j)
+          *reinterpret_cast<uint4*>(tile_at + sw128_offset(lane, (i % kPer) * kWords + j)) =
+              make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+        if (i % kPer == kPer - 1) {
+          fence_async_shared();
+          __syncwarp();
+          // a store that starts outside the output is left out; one that ends outside is cut there
+          if (lane == 0) {
+            const int c = n0 + (i / kPer) * kPer * 32;
+            if (c < a.N && m0 + q * 32 < a.M) tma_store_2d(&tm_out, tile_at, c, m0 + q * 32);
+            else asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+          ++stores;
+        }
+      }
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 2 * NC);
+  }
+}
+
+// Which kernel, its tile's other side (NT or NC), and parts of a tile's K range.
+struct GemmShape {
+  bool many;
+  int width, n_tiles, tiles, splits;
+};
+GemmShape gemm_shape(int64_t M, int64_t N, int64_t K, bool rows_on_16) {
+  GemmShape g;
+  const int64_t sms = num_sms(), m_tiles = (M + kTokens - 1) / kTokens;
+  auto tiles = [&](int nc) { return m_tiles * ((N + nc - 1) / nc); };
+  // The kernel for many tokens where its smaller tiles fill the SMs once over and its stores can be made; of its two
+  // widths the one whose rounds of tiles over the SMs cost least, a K step of a tile costing the rows it loads.
+  g.many = rows_on_16 && M > 64 && tiles(128) >= sms;
+  if (g.many) {
+    auto cost = [&](int nc) { return (tiles(nc) + sms - 1) / sms * (kTokens + nc); };
+    g.width = cost(256) <= cost(128) ? 256 : 128;
+    g.n_tiles = (int)((N + g.width - 1) / g.width);
+    g.tiles = (int)tiles(g.width);
+    g.splits = 1;
+    return g;
+  }
+  g.width = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+  g.n_tiles = (int)((N + kChannels - 1) / kChannels);
+  g.tiles = (int)((M + g.width - 1) / g.width * g.n_tiles);
+  // fewer tiles than SMs: as many parts of K as fill them
   const int64_t blocks = (K + kStep - 1) / kStep;
   g.splits = (int)std::max<int64_t>(1, std::min<int64_t>(blocks, sms / g.tiles));
   return g;
@@ -334,8 +554,7 @@ GemmShape gemm_shape(int64_t M, int64_t N, int64_t K) {
 struct GemmWs {
   size_t counts, codes, scale, parts, bytes;
 };
-GemmWs gemm_ws(int64_t M, int64_t N, int64_t K, bool quantise) {
-  const GemmShape g = gemm_shape(M, N, K);
+GemmWs gemm_ws(const GemmShape& g, int64_t M, int64_t K, bool quantise) {
   auto al = [](size_t x) { return (x + 255) & ~(size_t)255; };
   GemmWs w;
   w.counts = 4;
@@ -345,37 +564,51 @@ GemmWs gemm_ws(int64_t M, int64_t N, int64_t K, bool quantise) {
   w.scale = off;
   off += quantise ? al((size_t)M * 4) : 0;
   w.parts = off;
-  off += g.splits > 1 ? (size_t)g.tiles * g.splits * g.nt * kChannels * 4 : 0;
+  off += g.splits > 1 ? (size_t)g.tiles * g.splits * g.width * kChannels * 4 : 0;
   w.bytes = off;
   return w;
 }
 
-template <int NT, typename T>
-int launch_gemm(const CUtensorMap& tw, const CUtensorMap& tx, const Int8Args& a, bool after_rows, cudaStream_t s) {
-  auto k = int8_gemm_kernel<NT, T>;
-  const int smem = stages<NT>() * stage_bytes<NT>() + 1024;
+template <typename... K, typename... A>
+int launch(void (*k)(K...), int smem, const Int8Args& a, bool after_rows, cudaStream_t s, const A&... args) {
   int st = ensure_dyn_smem(reinterpret_cast<const void*>(k), smem, "int8_linear shared memory");
   if (st != FLB_OK) return st;
   const dim3 grid((unsigned)std::min<int64_t>((int64_t)a.tiles * a.splits, num_sms()));
   cudaError_t e;
   if (after_rows) {
-    e = launch_dependent(k, grid, dim3(kGemmThreads), smem, s, tw, tx, a);
+    e = launch_dependent(k, grid, dim3(kGemmThreads), smem, s, args..., a);
   } else {
-    k<<<grid, kGemmThreads, smem, s>>>(tw, tx, a);
+    k<<<grid, kGemmThreads, smem, s>>>(args..., a);
     e = cudaGetLastError();
   }
   count_launches(1);
   return check_cuda(e, "int8_linear launch");
 }
 
+template <int NT, typename T>
+int launch_few(const CUtensorMap& tw, const CUtensorMap& tx, const Int8Args& a, bool after_rows, cudaStream_t s) {
+  return launch(int8_few_kernel<NT, T>, stages<NT>() * stage_bytes<NT>() + 1024, a, after_rows, s, tw, tx);
+}
+
 template <typename T>
-int launch_gemm_t(int nt, const CUtensorMap& tw, const CUtensorMap& tx, const Int8Args& a, bool after_rows, cudaStream_t s) {
-  switch (nt) {
-    case 16: return launch_gemm<16, T>(tw, tx, a, after_rows, s);
-    case 32: return launch_gemm<32, T>(tw, tx, a, after_rows, s);
-    case 64: return launch_gemm<64, T>(tw, tx, a, after_rows, s);
-    case 128: return launch_gemm<128, T>(tw, tx, a, after_rows, s);
-    default: return launch_gemm<256, T>(tw, tx, a, after_rows, s);
+int launch_t(const GemmShape& g, const CUtensorMap& tw, const CUtensorMap& tx, const Int8Args& a, bool after_rows, cudaStream_t s) {
+  if (g.many) {
+    CUtensorMap to;
+    const uint64_t dims[2] = {(uint64_t)a.N, (uint64_t)a.M};
+    const uint64_t strides[1] = {(uint64_t)a.N * sizeof(T)};
+    const uint32_t box[2] = {128 / sizeof(T), 32};
+    const CUtensorMapDataType dt = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const int st = make_tmap(&to, a.out, dt, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (st != FLB_OK) return st;
+    if (g.width == 256) return launch(int8_many_kernel<256, T>, many_smem<256>(), a, after_rows, s, tw, tx, to);
+    return launch(int8_many_kernel<128, T>, many_smem<128>(), a, after_rows, s, tw, tx, to);
+  }
+  switch (g.width) {
+    case 16: return launch_few<16, T>(tw, tx, a, after_rows, s);
+    case 32: return launch_few<32, T>(tw, tx, a, after_rows, s);
+    case 64: return launch_few<64, T>(tw, tx, a, after_rows, s);
+    default: return launch_few<128, T>(tw, tx, a, after_rows, s);
   }
 }
 
@@ -391,13 +624,16 @@ int code_map(CUtensorMap* m, const int8_t* codes, int64_t rows, int64_t ld, int6
 int int8_rows(const void* x, int64_t ldx, int8_t* codes, float* scale, int64_t R, int64_t D, int dtype, uint32_t* zero,
               int64_t n_zero, cudaStream_t s);
 
-size_t int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, bool quantise) { return gemm_ws(M, N, K, quantise).bytes; }
+// For either kernel: which one runs also depends on where the output lies.
+size_t int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, bool quantise) {
+  return std::max(gemm_ws(gemm_shape(M, N, K, false), M, K, quantise).bytes, gemm_ws(gemm_shape(M, N, K, true), M, K, quantise).bytes);
+}
 
 int int8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, const float* x_scale, const int8_t* w_codes,
                 int64_t ldw, const float* w_scale, const void* bias, int bias_dtype, void* out, int64_t M, int64_t N,
                 int64_t K, int dtype, void* ws, int check_timeout, cudaStream_t s) {
-  const GemmShape g = gemm_shape(M, N, K);
-  const GemmWs l = gemm_ws(M, N, K, x != nullptr);
+  const GemmShape g = gemm_shape(M, N, K, N * dtype_size(dtype) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0);
+  const GemmWs l = gemm_ws(g, M, K, x != nullptr);
   uint8_t* p = reinterpret_cast<uint8_t*>(ws);
   const int64_t n_zero = 1 + (g.splits > 1 ? g.tiles : 0);
   int st;
@@ -411,16 +647,16 @@ int int8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, 
     return st;
   }
   CUtensorMap tw, tx;
-  if ((st = code_map(&tw, w_codes, N, ldw, K, kChannels)) != FLB_OK) return st;
-  if ((st = code_map(&tx, x_codes, M, ldc, K, g.nt)) != FLB_OK) return st;
+  if ((st = code_map(&tw, w_codes, N, ldw, K, g.many ? g.width : kChannels)) != FLB_OK) return st;
+  if ((st = code_map(&tx, x_codes, M, ldc, K, g.many ? kTokens : g.width)) != FLB_OK) return st;
   const Int8Args a{x_scale, w_scale, bias, bias_dtype == FLB_F32, out, M, N,
                    N % 2 == 0 && reinterpret_cast<uintptr_t>(out) % 4 == 0, (int)((K + kStep - 1) / kStep), g.n_tiles, g.tiles,
                    g.splits, reinterpret_cast<int32_t*>(p + l.parts), reinterpret_cast<uint32_t*>(p + l.counts),
                    reinterpret_cast<uint32_t*>(p)};
   switch (dtype) {
-    case FLB_F32: st = launch_gemm_t<float>(g.nt, tw, tx, a, x != nullptr, s); break;
-    case FLB_F16: st = launch_gemm_t<__half>(g.nt, tw, tx, a, x != nullptr, s); break;
-    default: st = launch_gemm_t<__nv_bfloat16>(g.nt, tw, tx, a, x != nullptr, s); break;
+    case FLB_F32: st = launch_t<float>(g, tw, tx, a, x != nullptr, s); break;
+    case FLB_F16: st = launch_t<__half>(g, tw, tx, a, x != nullptr, s); break;
+    default: st = launch_t<__nv_bfloat16>(g, tw, tx, a, x != nullptr, s); break;
   }
   if (st != FLB_OK || !check_timeout) return st;
   uint32_t err = 0;
