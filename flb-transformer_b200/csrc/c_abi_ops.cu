@@ -8,7 +8,7 @@ namespace flb {
 int layer_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b, int wdtype, void* y, float* mean,
                    float* rstd, int8_t* codes, uint8_t* exps, int64_t G, int64_t R, int64_t D, int dtype, float eps,
                    cudaStream_t s);
-size_t layer_norm_bwd_workspace_bytes(int64_t G, int64_t R, int64_t D, int dtype);
+size_t layer_norm_bwd_workspace_bytes(int64_t G, int64_t R, int64_t D);
 int layer_norm_bwd(const void* x, int64_t ldx, const int8_t* codes, const uint8_t* exps, const float* mean,
                    const float* rstd, const void* w, int wdtype, const void* dy, void* dx, void* dw, void* db, int64_t G,
                    int64_t R, int64_t D, int dtype, void* ws, cudaStream_t s);
@@ -102,9 +102,9 @@ int flb_layer_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b,
   return layer_norm_fwd(x, ldx, w, b, wdtype, y, mean, rstd, codes, exps, G, R, D, dtype, eps, as_stream(stream));
 }
 
-size_t flb_layer_norm_bwd_workspace_bytes(int64_t G, int64_t R, int64_t D, int dtype) {
+size_t flb_layer_norm_bwd_workspace_bytes(int64_t G, int64_t R, int64_t D) {
   if (G < 1 || R < 1 || D < 1 || D > 16384) return 0;
-  return layer_norm_bwd_workspace_bytes(G, R, D, dtype);
+  return layer_norm_bwd_workspace_bytes(G, R, D);
 }
 
 int flb_layer_norm_bwd(const void* x, int64_t ldx, const int8_t* codes, const uint8_t* exps, const float* mean,
@@ -130,7 +130,7 @@ int flb_layer_norm_bwd(const void* x, int64_t ldx, const int8_t* codes, const ui
   const size_t es = (size_t)dtype_size(dtype);
   if (off(x, es) || off(dy, es) || off(dx, es) || off(mean, 4) || off(rstd, 4))
     return fail(FLB_ERR_ALIGN, "layer_norm_bwd: pointers must be aligned to their element size");
-  const size_t need = dw ? layer_norm_bwd_workspace_bytes(G, R, D, dtype) : 0;
+  const size_t need = dw ? layer_norm_bwd_workspace_bytes(G, R, D) : 0;
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(FLB_ERR_WORKSPACE, "layer_norm_bwd: workspace smaller than flb_layer_norm_bwd_workspace_bytes()");
   if (off(workspace, 16)) return fail(FLB_ERR_ALIGN, "layer_norm_bwd: workspace must be 16-byte aligned");

@@ -178,7 +178,7 @@ std::tuple<Tensor, Opt, Opt> norm_backward(const Opt& x_, const Tensor& rstd, co
   if (given(like) && want_params) {
     dw = at::empty(like->sizes(), like->options());
     db = at::empty(like->sizes(), like->options());
-    need = flb_layer_norm_bwd_workspace_bytes(G, R, D, dt);
+    need = flb_layer_norm_bwd_workspace_bytes(G, R, D);
     if (need) ws = buffer(need, dy);
   }
   check(flb_layer_norm_bwd(ptr(x), ldx, (const int8_t*)ptr(codes), (const uint8_t*)ptr(exps), (const float*)ptr(mean),

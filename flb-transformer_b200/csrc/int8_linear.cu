@@ -46,6 +46,8 @@ struct Int8Args {
   bool pairs;         // 16-bit outputs two channels at a time
   int k_blocks;       // of kStep
   int n_tiles, tiles, splits;
+  int group;          // many tokens: tiles of tokens that go through all channels together
+  bool stream_out;    // and the output leaves L2 before the operands do
   int32_t* parts;     // [tiles][splits][NT][128], splits > 1
   uint32_t* counts;   // [tiles], zero
   uint32_t* error;
@@ -317,8 +319,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 
 constexpr int kTokens = 128;    // a tile's tokens
 constexpr int kStaged = 4096;   // bytes a warp hands to one TMA store: 32 tokens of 128 bytes
-constexpr int kGroup = 16;      // tiles of tokens that go through all channels together, so that few operand
-                                // tiles are in use at a time
 
 template <int NC> constexpr int many_stage_bytes() { return (kTokens + NC) * kStep; }
 template <int NC> constexpr int many_stages() { return NC == 256 ? 3 : 4; }
@@ -327,9 +327,9 @@ template <int NC> constexpr int many_smem() {
   return many_stages<NC>() * many_stage_bytes<NC>() + kEpilogue / 32 * (2 * kStaged + NC / 2 * 8) + 1024;
 }
 
-__device__ __forceinline__ void tma_store_2d(const void* tmap, const void* src, int c0, int c1) {
-  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(tmap), "r"(smem_u32(src)), "r"(c0),
-               "r"(c1)
+__device__ __forceinline__ void tma_store_2d(const void* tmap, const void* src, int c0, int c1, uint64_t policy) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group.L2::cache_hint [%0, {%2, %3}], [%1], %4;" ::"l"(tmap),
+               "r"(smem_u32(src)), "r"(c0), "r"(c1), "l"(policy)
                : "memory");
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
@@ -364,9 +364,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   const uint32_t tmem = tmem_base;
   const int m_tiles = a.tiles / a.n_tiles;
   auto place = [&](int tile, int& m0, int& n0) {
-    const int g = tile / (kGroup * a.n_tiles), in = tile - g * kGroup * a.n_tiles;
-    const int rows = min(kGroup, m_tiles - g * kGroup);
-    m0 = (g * kGroup + in % rows) * kTokens;
+    // a.group tiles of tokens go through all channels together
+    const int g = tile / (a.group * a.n_tiles), in = tile - g * a.group * a.n_tiles;
+    const int rows = min(a.group, m_tiles - g * a.group);
+    m0 = (g * a.group + in % rows) * kTokens;
     n0 = in / rows * NC;
   };
 
@@ -434,6 +435,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     float* sw = reinterpret_cast<float*>(ring + (size_t)S * kBytes + (size_t)(kEpilogue / 32) * (2 * kStaged)) + (warp - 2) * 2 * COLS;
     float* sb = sw + COLS;
     uint32_t local = 0, limit = kWaitLimit, stores = 0;
+    uint64_t policy;
+    if (a.stream_out) asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+    else asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
     wait_predecessor();
     for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ++local) {
       const uint32_t b = local & 1;
@@ -504,7 +508,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           // a store that starts outside the output is left out; one that ends outside is cut there
           if (lane == 0) {
             const int c = n0 + (i / kPer) * kPer * 32;
-            if (c < a.N && m0 + q * 32 < a.M) tma_store_2d(&tm_out, tile_at, c, m0 + q * 32);
+            if (c < a.N && m0 + q * 32 < a.M) tma_store_2d(&tm_out, tile_at, c, m0 + q * 32, policy);
             else asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
           ++stores;
@@ -520,6 +524,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     tmem_dealloc(tmem, 2 * NC);
   }
 }
+
+// Orders of the tiles, of 126 MB of L2. A weight that stays there is best gone through once for each tile of tokens: the
+// blocks then write whole rows of the output (16384 x 768 x 32000: 415 us at either order with the output's default
+// policy, 374 against 402 with an output too large for L2 leaving it first). A larger one would come from
+// memory each time: 16 tiles of tokens at once (8192 x 4096 x 32000, 131 MB: 779 us against 1183).
+constexpr int64_t kWeightInL2 = 48 << 20;
+constexpr size_t kOutputInL2 = 64 << 20;
 
 // Which kernel, its tile's other side (NT or NC), and parts of a tile's K range.
 struct GemmShape {
@@ -651,7 +662,7 @@ int int8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, 
   if ((st = code_map(&tx, x_codes, M, ldc, K, g.many ? kTokens : g.width)) != FLB_OK) return st;
   const Int8Args a{x_scale, w_scale, bias, bias_dtype == FLB_F32, out, M, N,
                    N % 2 == 0 && reinterpret_cast<uintptr_t>(out) % 4 == 0, (int)((K + kStep - 1) / kStep), g.n_tiles, g.tiles,
-                   g.splits, reinterpret_cast<int32_t*>(p + l.parts), reinterpret_cast<uint32_t*>(p + l.counts),
+                   g.splits, N * K <= kWeightInL2 ? 1 : 16, (size_t)M * N * dtype_size(dtype) > kOutputInL2, reinterpret_cast<int32_t*>(p + l.parts), reinterpret_cast<uint32_t*>(p + l.counts),
                    reinterpret_cast<uint32_t*>(p)};
   switch (dtype) {
     case FLB_F32: st = launch_t<float>(g, tw, tx, a, x != nullptr, s); break;

@@ -34,17 +34,29 @@ template <typename T> __device__ __forceinline__ float2 gate_of(float z) {
   return z >= 0.f ? make_float2(r, e * r) : make_float2(e * r, r);
 }
 
-// The warp's chunks, one after the other; the body gets the row, the chunk's first element and the lane.
-template <bool FLAT, typename F> __device__ __forceinline__ void for_chunks(const KeptArgs& a, F&& body) {
+// The warp's chunks, two at a time so that twice the loads are under way; load(row, base, lane) gives what
+// finish(row, base, lane, loaded) goes on with, base the chunk's first element in the row.
+template <bool FLAT, typename L, typename F> __device__ __forceinline__ void for_chunks(const KeptArgs& a, L&& load, F&& finish) {
   const int lane = threadIdx.x & 31;
   const int64_t n = (int64_t)gridDim.x * (kThreads / 32);
-  for (int64_t i = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); i < a.chunks; i += n) {
-    if constexpr (FLAT) {
-      body(i, 0, lane);
-    } else {
-      const int64_t row = a.chunks <= 0xffffffffll ? (uint32_t)i / (uint32_t)a.per_row : i / a.per_row;
-      body(row, (int)(i - row * a.per_row) * 256, lane);
+  auto place = [&](int64_t i, int64_t& row, int& base) {
+    row = i, base = 0;
+    if constexpr (!FLAT) {
+      row = a.chunks <= 0xffffffffll ? (uint32_t)i / (uint32_t)a.per_row : i / a.per_row;
+      base = (int)(i - row * a.per_row) * 256;
     }
+  };
+  for (int64_t i = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); i < a.chunks; i += 2 * n) {
+    int64_t r0, r1;
+    int b0, b1;
+    place(i, r0, b0);
+    place(i + n, r1, b1);
+    const bool two = i + n < a.chunks;
+    auto x0 = load(r0, b0, lane);
+    decltype(x0) x1;
+    if (two) x1 = load(r1, b1, lane);
+    finish(r0, b0, lane, x0);
+    if (two) finish(r1, b1, lane, x1);
   }
 }
 
@@ -62,10 +74,13 @@ template <int FORM> constexpr bool kVec = FORM != 1;
 template <typename T, int FORM> __global__ void __launch_bounds__(kThreads) pack_kernel(const KeptArgs a) {
   constexpr bool VEC = kVec<FORM>;
   const int D = FORM == 2 ? 256 : a.D;
-  for_chunks<FORM == 2>(a, [&](int64_t row, int base, int lane) {
+  auto load = [&](int64_t row, int base, int lane) {
     Raw8<T> r;
-    F2 v[4];
     load_raw<T, VEC>(r, reinterpret_cast<const T*>(a.x) + row * D, base, lane, D);
+    return r;
+  };
+  for_chunks<FORM == 2>(a, load, [&](int64_t row, int base, int lane, const Raw8<T>& r) {
+    F2 v[4];
     to_float<T>(r, v);
     keep_raw<T, VEC>(r, v, a.cx, a.ex, row, base, lane, D);
   });
@@ -74,9 +89,12 @@ template <typename T, int FORM> __global__ void __launch_bounds__(kThreads) pack
 template <typename T, int FORM> __global__ void __launch_bounds__(kThreads) unpack_kernel(const KeptArgs a) {
   constexpr bool VEC = kVec<FORM>;
   const int D = FORM == 2 ? 256 : a.D;
-  for_chunks<FORM == 2>(a, [&](int64_t row, int base, int lane) {
+  auto load = [&](int64_t row, int base, int lane) {
+    return load_kept<VEC>(a.cx + row * code_pitch(D), a.ex + row * blocks_of(D), base, lane, D);
+  };
+  for_chunks<FORM == 2>(a, load, [&](int64_t row, int base, int lane, const Kept8& k) {
     F2 v[4];
-    kept_to_float<VEC>(load_kept<VEC>(a.cx + row * code_pitch(D), a.ex + row * blocks_of(D), base, lane, D), v);
+    kept_to_float<VEC>(k, v);
     if constexpr (std::is_same<T, __half>::value) {
       // a magnitude near the type's largest can be kept as 65536: back to the largest (a NaN stays one)
 #pragma unroll
@@ -92,16 +110,22 @@ template <typename T, int FORM> __global__ void __launch_bounds__(kThreads) unpa
 template <typename T, int FORM, bool KEEP> __global__ void __launch_bounds__(kThreads) gate_fwd_kernel(const KeptArgs a) {
   constexpr bool VEC = kVec<FORM>;
   const int D = FORM == 2 ? 256 : a.D;
-  for_chunks<FORM == 2>(a, [&](int64_t row, int base, int lane) {
-    Raw8<T> rx, rz;
+  struct Both {
+    Raw8<T> x, z;
+  };
+  auto load = [&](int64_t row, int base, int lane) {
+    Both r;
+    load_raw<T, VEC>(r.x, reinterpret_cast<const T*>(a.x) + row * D, base, lane, D);
+    load_raw<T, VEC>(r.z, reinterpret_cast<const T*>(a.z) + row * D, base, lane, D);
+    return r;
+  };
+  for_chunks<FORM == 2>(a, load, [&](int64_t row, int base, int lane, const Both& r) {
     F2 x[4], z[4];
-    load_raw<T, VEC>(rx, reinterpret_cast<const T*>(a.x) + row * D, base, lane, D);
-    load_raw<T, VEC>(rz, reinterpret_cast<const T*>(a.z) + row * D, base, lane, D);
-    to_float<T>(rx, x);
-    to_float<T>(rz, z);
+    to_float<T>(r.x, x);
+    to_float<T>(r.z, z);
     if constexpr (KEEP) {
-      keep_raw<T, VEC>(rx, x, a.cx, a.ex, row, base, lane, D);
-      keep_raw<T, VEC>(rz, z, a.cz, a.ez, row, base, lane, D);
+      keep_raw<T, VEC>(r.x, x, a.cx, a.ex, row, base, lane, D);
+      keep_raw<T, VEC>(r.z, z, a.cz, a.ez, row, base, lane, D);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -117,17 +141,31 @@ template <typename T, int FORM, bool KEEP>
 __global__ void __launch_bounds__(kThreads) gate_bwd_kernel(const KeptArgs a, const void* dy_) {
   constexpr bool VEC = kVec<FORM>;
   const int D = FORM == 2 ? 256 : a.D;
-  for_chunks<FORM == 2>(a, [&](int64_t row, int base, int lane) {
-    F2 x[4], z[4], dy[4], dz[4];
-    load8<T, VEC>(dy, reinterpret_cast<const T*>(dy_) + row * D, base, lane, D);
+  struct All {
+    Raw8<T> dy, x, z;
+    Kept8 kx, kz;
+  };
+  auto load = [&](int64_t row, int base, int lane) {
+    All r;
+    load_raw<T, VEC>(r.dy, reinterpret_cast<const T*>(dy_) + row * D, base, lane, D);
     if constexpr (KEEP) {
-      const Kept8 kx = load_kept<VEC>(a.cx + row * code_pitch(D), a.ex + row * blocks_of(D), base, lane, D);
-      const Kept8 kz = load_kept<VEC>(a.cz + row * code_pitch(D), a.ez + row * blocks_of(D), base, lane, D);
-      kept_to_float<VEC>(kx, x);
-      kept_to_float<VEC>(kz, z);
+      r.kx = load_kept<VEC>(a.cx + row * code_pitch(D), a.ex + row * blocks_of(D), base, lane, D);
+      r.kz = load_kept<VEC>(a.cz + row * code_pitch(D), a.ez + row * blocks_of(D), base, lane, D);
     } else {
-      load8<T, VEC>(x, reinterpret_cast<const T*>(a.x) + row * D, base, lane, D);
-      load8<T, VEC>(z, reinterpret_cast<const T*>(a.z) + row * D, base, lane, D);
+      load_raw<T, VEC>(r.x, reinterpret_cast<const T*>(a.x) + row * D, base, lane, D);
+      load_raw<T, VEC>(r.z, reinterpret_cast<const T*>(a.z) + row * D, base, lane, D);
+    }
+    return r;
+  };
+  for_chunks<FORM == 2>(a, load, [&](int64_t row, int base, int lane, const All& r) {
+    F2 x[4], z[4], dy[4], dz[4];
+    to_float<T>(r.dy, dy);
+    if constexpr (KEEP) {
+      kept_to_float<VEC>(r.kx, x);
+      kept_to_float<VEC>(r.kz, z);
+    } else {
+      to_float<T>(r.x, x);
+      to_float<T>(r.z, z);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

@@ -3,7 +3,7 @@
 //
 //   dx = (gw - mean(gw) - h mean(gw h)) / sigma,   dw = sum over rows of dy h,   db = sum over rows of dy
 //
-// Bound by memory: dy and h are read once, dx is written once. A warp (D <= 1024) or block walks over rows
+// Bound by memory: dy and h are read once, dx is written once. A warp (D <= 512) or block walks over rows
 // a fixed distance apart, the next rows on their way to shared memory meanwhile, and adds up dw and db of
 // the columns that its threads own in float32 registers. A block's sums go to its own row of a
 // workspace, which a second kernel adds up in a fixed order: no atomics, the same bits every time. With
@@ -37,61 +37,11 @@ template <typename T> __device__ __forceinline__ void store_param(void* p, bool 
   if (f32) reinterpret_cast<float*>(p)[i] = v; else st(reinterpret_cast<T*>(p) + i, v);
 }
 
-// Copies of the rows ahead, in shared memory. A thread copies, and later reads, only its own elements, so
-// its own wait for its copies is all the synchronisation there is. 16-bit rows that do not start on 16
-// bytes have no such copies (the smallest is 4 bytes): they are loaded when their turn comes.
-template <typename T, bool VEC> constexpr bool kCopies = VEC || sizeof(T) == 4;
-
-__device__ __forceinline__ uint32_t shared_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool there) {
-  // with no source bytes the destination is filled with zeros
-  if constexpr (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(there ? BYTES : 0) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-// One chunk's eight elements of this thread: slots [word group][thread], so that a warp's accesses are contiguous
-template <typename T, bool VEC>
-__device__ __forceinline__ void copy8(uint8_t* slot, const T* row, int base, int lane, int D) {
-  const uint32_t at = shared_addr(slot);
-  if constexpr (VEC) {
-    const int p = base + lane * 8;
-    const uint8_t* src = reinterpret_cast<const uint8_t*>(row + (p < D ? p : 0));
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-      copy_async<16>(at + (i * blockDim.x + threadIdx.x) * 16, src + 16 * i, p < D);
-  } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int p = base + j * 32 + lane;
-      copy_async<4>(at + (j * blockDim.x + threadIdx.x) * 4, row + (p < D ? p : 0), p < D);
-    }
-  }
-}
-template <typename T, bool VEC> __device__ __forceinline__ void copied8(const uint8_t* slot, F2 (&v)[4]) {
-  Raw8<T> r;
-  if constexpr (VEC) {
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
-      const uint4 u = reinterpret_cast<const uint4*>(slot)[i * blockDim.x + threadIdx.x];
-      r.w[4 * i] = u.x, r.w[4 * i + 1] = u.y, r.w[4 * i + 2] = u.z, r.w[4 * i + 3] = u.w;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) r.w[j % (sizeof(T) * 2)] = reinterpret_cast<const uint32_t*>(slot)[j * blockDim.x + threadIdx.x];
-  }
-  to_float<T>(r, v);
-}
-
 // Rows held at a time: three with 16-bit elements, two with float32; in the widest form, whose block is a
 // whole SM's, two and one.
 template <typename T, bool WIDE> constexpr int kStages = (sizeof(T) == 4 ? 2 : 3) - (WIDE ? 1 : 0);
 constexpr int kWarps = 4;  // of a block whose warps have a row each
-// such blocks on an SM: by the ring with float32, by the sums' registers with four chunks a thread
-template <typename T, int CH> constexpr int kBlocksPerSm = sizeof(T) == 4 || CH == 4 ? 3 : 4;
+constexpr int kBlocksPerSm = 4;  // such blocks on an SM
 
 // Bytes a thread's chunk takes in the ring
 template <typename T, bool VEC, bool KEPT> constexpr int chunk_bytes() {
@@ -99,20 +49,24 @@ template <typename T, bool VEC, bool KEPT> constexpr int chunk_bytes() {
   return KEPT ? elems + (VEC ? 8 : 0) : 2 * elems;
 }
 
-// MODE 0: a warp a row (D <= 1024), 1: a block a row (D <= 8192), 2: a block of up to 1024 threads (D <= 16384)
+// MODE 0: a warp a row (D <= 512), 1: a block a row (D <= 8192), 2: a block of up to 1024 threads (D <= 16384)
 template <typename T, bool VEC, int MODE, int CH, bool KEPT>
-__global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 1024, MODE == 0 ? kBlocksPerSm<T, CH> : 1)
+__global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 1024, MODE == 0 ? kBlocksPerSm : 1)
     ln_bwd_kernel(const BwdArgs a) {
   constexpr bool WARP = MODE == 0;
   constexpr int S = kStages<T, MODE == 2>, CB = chunk_bytes<T, VEC, KEPT>();
   constexpr bool COPY_DY = kCopies<T, VEC>, COPY_X = !KEPT && COPY_DY, COPY_CODES = KEPT && VEC;
   extern __shared__ __align__(16) uint8_t ring[];  // [S][CH][x or codes | dy][threads]; at the end [2][D] floats
-  __shared__ float2 slot[WARP ? 1 : 2][32];
+  __shared__ __align__(16) float2 slot[WARP ? 1 : 2][32];  // zero for warps that the block does not have
   let_successor_start();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if constexpr (!WARP) {
+    if (warp == 0) slot[0][lane] = slot[1][lane] = make_float2(0.f, 0.f);
+    __syncthreads();
+  }
   const int64_t group = blockIdx.y;
   const int D = a.D;
-  const int first = WARP ? 0 : warp * 256, step = WARP ? 256 : (int)blockDim.x * 8;
+  const int first = WARP ? 0 : warp * 256 * CH;
   const int64_t stride = WARP ? (int64_t)gridDim.x * kWarps : gridDim.x;
   const int64_t row0 = WARP ? (int64_t)blockIdx.x * kWarps + warp : blockIdx.x;
   const float inv_d = 1.f / D;
@@ -126,7 +80,7 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
     if (r < a.R) {
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
-        const int base = first + c * step;
+        const int base = first + c * 256;
         if constexpr (COPY_DY) copy8<T, VEC>(part_of(stage, c, true), dy_row(r), base, lane, D);
         if constexpr (COPY_X) copy8<T, VEC>(part_of(stage, c, false), x_row(r), base, lane, D);
         if constexpr (COPY_CODES) {
@@ -144,6 +98,19 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
 #pragma unroll
     for (int i = 0; i < 4; ++i) dw[c][i] = db[c][i] = f2(0.f);
 
+  F2 w[CH][4];  // the group's weight
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    if (!a.w) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[c][i] = f2(1.f);
+    } else if (a.w32) {
+      load8<float, VEC>(w[c], reinterpret_cast<const float*>(a.w) + group * D, first + c * 256, lane, D);
+    } else {
+      load8<T, VEC>(w[c], reinterpret_cast<const T*>(a.w) + group * D, first + c * 256, lane, D);
+    }
+  }
+
   // what is not copied: the row's statistics, its blocks' exponents, and the rows without copies
   float mean = 0.f, rstd = 0.f;
   uint32_t exps[CH];
@@ -153,7 +120,7 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
     rstd = __ldg(a.rstd + rr);
     if constexpr (KEPT) {
 #pragma unroll
-      for (int c = 0; c < CH; ++c) exps[c] = load_exps<VEC>(a.exps + rr * blocks_of(D), first + c * step, lane, D);
+      for (int c = 0; c < CH; ++c) exps[c] = load_exps<VEC>(a.exps + rr * blocks_of(D), first + c * 256, lane, D);
     }
   };
 
@@ -168,7 +135,7 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
     Raw8<T> rx[CH], rdy[CH];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int base = first + c * step;
+      const int base = first + c * 256;
       if constexpr (KEPT) rk[c].e = exps[c];
       if constexpr (KEPT && !COPY_CODES) rk[c].c = load_codes<VEC>(code_row(row), base, lane, D);
       if constexpr (!KEPT && !COPY_X) load_raw<T, VEC>(rx[c], x_row(row), base, lane, D);
@@ -176,10 +143,9 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
     }
     if (row + stride < a.R) fetch_small(row + stride);
     copies_wait<S - 1>();
-    // chunk c of x (or the kept h), dy and the weight; read again after the sums, which costs less than the
+    // chunk c of x (or the kept h) and dy; read again after the sums, which costs less than the
     // registers to hold them
-    auto values = [&](int c, F2 (&x)[4], F2 (&dy)[4], F2 (&w)[4]) {
-      const int base = first + c * step;
+    auto values = [&](int c, F2 (&x)[4], F2 (&dy)[4]) {
       if constexpr (COPY_DY) copied8<T, VEC>(part_of(stage, c, true), dy); else to_float<T>(rdy[c], dy);
       if constexpr (KEPT) {
         Kept8 k = rk[c];
@@ -188,25 +154,17 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
       } else {
         if constexpr (COPY_X) copied8<T, VEC>(part_of(stage, c, false), x); else to_float<T>(rx[c], x);
       }
-      if (!a.w) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = f2(1.f);
-      } else if (a.w32) {
-        load8<float, VEC>(w, reinterpret_cast<const float*>(a.w) + group * D, base, lane, D);
-      } else {
-        load8<T, VEC>(w, reinterpret_cast<const T*>(a.w) + group * D, base, lane, D);
-      }
     };
     // h = x h1 + h0
     const float h1 = KEPT ? 1.f : rs, h0 = KEPT ? 0.f : -m * rs;
     F2 t1 = f2(0.f), t2 = f2(0.f);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      F2 x[4], dy[4], w[4];
-      values(c, x, dy, w);
+      F2 x[4], dy[4];
+      values(c, x, dy);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {  // dy is zero beyond D
-        const F2 h = KEPT ? x[i] : fma2(x[i], f2(h1), f2(h0)), gw = mul2(dy[i], w[i]);
+        const F2 h = KEPT ? x[i] : fma2(x[i], f2(h1), f2(h0)), gw = mul2(dy[i], w[c][i]);
         dw[c][i] = fma2(dy[i], h, dw[c][i]);
         db[c][i] = add2(db[c][i], dy[i]);
         t1 = add2(t1, gw);
@@ -220,10 +178,10 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
       if (lane == 0) slot[turn][warp] = make_float2(s1, s2);
       __syncthreads();
       s1 = s2 = 0.f;
-      for (int i = 0; i < (int)(blockDim.x >> 5); ++i) {
-        const float2 t = slot[turn][i];
-        s1 += t.x;
-        s2 += t.y;
+      for (int i = 0; i < (int)(blockDim.x >> 5); i += 2) {
+        const float4 t = *reinterpret_cast<const float4*>(&slot[turn][i]);
+        s1 += t.x + t.z;
+        s2 += t.y + t.w;
       }
       turn ^= 1;
     }
@@ -234,11 +192,11 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
     T* dx = reinterpret_cast<T*>(a.dx) + (group * a.R + row) * D;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      F2 x[4], dy[4], w[4];
-      values(c, x, dy, w);
+      F2 x[4], dy[4];
+      values(c, x, dy);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = fma2(mul2(f2(rs), w[i]), dy[i], fma2(x[i], f2(c1), f2(c0)));
-      store8<T, VEC>(dx, x, first + c * step, lane, D);
+      for (int i = 0; i < 4; ++i) x[i] = fma2(mul2(f2(rs), w[c][i]), dy[i], fma2(x[i], f2(c1), f2(c0)));
+      store8<T, VEC>(dx, x, first + c * 256, lane, D);
     }
     stage = stage + 1 == S ? 0 : stage + 1;
   }
@@ -268,7 +226,7 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
         to_scalars(db[c], vb);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int p = Chunk<VEC>::at(first + c * step, lane, j);
+          const int p = Chunk<VEC>::at(first + c * 256, lane, j);
           if (p < D) {
             sm[p] = (t ? sm[p] : 0.f) + vw[j];
             sm[D + p] = (t ? sm[D + p] : 0.f) + vb[j];
@@ -286,7 +244,7 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
       to_scalars(db[c], vb);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int p = Chunk<VEC>::at(first + c * step, lane, j);
+        const int p = Chunk<VEC>::at(first + c * 256, lane, j);
         if (p < D) out(p, vw[j], vb[j]);
       }
     }
@@ -315,18 +273,18 @@ __global__ void __launch_bounds__(1024) ln_sum_kernel(const float* __restrict__ 
   if (tx == 0 && out < D) store_param<T>(which ? db : dw, w32, group * D + out, v);
 }
 
-// Threads a row, and blocks a group: enough to fill the SMs (kBlocksPerSm, or 512 threads on each), but at least two rows a warp or block, and one block where that leaves it
+// Threads a row, and blocks a group: enough to fill the SMs (512 threads on each), but at least two rows a warp or block, and one block where that leaves it
 // four rows a warp at most.
 struct BwdShape {
   int mode, threads;
   int64_t blocks;
 };
-BwdShape bwd_shape(int64_t G, int64_t R, int64_t D, int dtype) {
+BwdShape bwd_shape(int64_t G, int64_t R, int64_t D) {
   BwdShape p;
-  p.mode = D <= 1024 ? 0 : D <= 8192 ? 1 : 2;
+  p.mode = D <= 512 ? 0 : D <= 8192 ? 1 : 2;
   p.threads = p.mode == 0 ? 32 * kWarps : 32 * (int)((D + 511) / 512);
   const int64_t at_once = p.mode == 0 ? kWarps : 1;
-  const int per_sm = p.mode == 0 ? (dtype == FLB_F32 || D > 768 ? 3 : 4) : std::max(1, 512 / p.threads);
+  const int per_sm = p.mode == 0 ? kBlocksPerSm : std::max(1, 512 / p.threads);
   const int64_t room = std::max<int64_t>(1, (int64_t)num_sms() * per_sm / G);
   p.blocks = R <= 4 * at_once ? 1 : std::min<int64_t>(room, (R + 2 * at_once - 1) / (2 * at_once));
   return p;
@@ -344,17 +302,12 @@ int launch_mode(const BwdArgs& a, const BwdShape& p, int64_t G, cudaStream_t s) 
 }
 
 template <typename T, bool VEC, bool KEPT>
-int launch_bwd(const BwdArgs& a, int64_t G, int dtype, cudaStream_t s) {
+int launch_bwd(const BwdArgs& a, int64_t G, cudaStream_t s) {
   const int D = a.D;
-  const BwdShape p = bwd_shape(G, a.R, D, dtype);
+  const BwdShape p = bwd_shape(G, a.R, D);
   int st;
   if (p.mode == 0) {
-    switch ((D + 255) / 256) {
-      case 1: st = launch_mode<T, VEC, 0, 1, KEPT>(a, p, G, s); break;
-      case 2: st = launch_mode<T, VEC, 0, 2, KEPT>(a, p, G, s); break;
-      case 3: st = launch_mode<T, VEC, 0, 3, KEPT>(a, p, G, s); break;
-      default: st = launch_mode<T, VEC, 0, 4, KEPT>(a, p, G, s); break;
-    }
+    st = D <= 256 ? launch_mode<T, VEC, 0, 1, KEPT>(a, p, G, s) : launch_mode<T, VEC, 0, 2, KEPT>(a, p, G, s);
   } else if (p.mode == 1) {
     st = launch_mode<T, VEC, 1, 2, KEPT>(a, p, G, s);
   } else {
@@ -373,16 +326,16 @@ int launch_bwd(const BwdArgs& a, int64_t G, int dtype, cudaStream_t s) {
 
 bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-template <typename T> int dispatch_bwd(const BwdArgs& a, int64_t G, int dtype, cudaStream_t s) {
+template <typename T> int dispatch_bwd(const BwdArgs& a, int64_t G, cudaStream_t s) {
   const bool vec = a.D % 8 == 0 && on16(a.x) && a.ldx * sizeof(T) % 16 == 0 && on16(a.codes) && on16(a.w) && on16(a.dy) && on16(a.dx);
-  if (a.codes) return vec ? launch_bwd<T, true, true>(a, G, dtype, s) : launch_bwd<T, false, true>(a, G, dtype, s);
-  return vec ? launch_bwd<T, true, false>(a, G, dtype, s) : launch_bwd<T, false, false>(a, G, dtype, s);
+  if (a.codes) return vec ? launch_bwd<T, true, true>(a, G, s) : launch_bwd<T, false, true>(a, G, s);
+  return vec ? launch_bwd<T, true, false>(a, G, s) : launch_bwd<T, false, false>(a, G, s);
 }
 
 }  // namespace
 
-size_t layer_norm_bwd_workspace_bytes(int64_t G, int64_t R, int64_t D, int dtype) {
-  const BwdShape p = bwd_shape(G, R, D, dtype);
+size_t layer_norm_bwd_workspace_bytes(int64_t G, int64_t R, int64_t D) {
+  const BwdShape p = bwd_shape(G, R, D);
   return p.blocks > 1 ? (size_t)G * p.blocks * 2 * D * sizeof(float) : 0;
 }
 
@@ -391,9 +344,9 @@ int layer_norm_bwd(const void* x, int64_t ldx, const int8_t* codes, const uint8_
                    int64_t R, int64_t D, int dtype, void* ws, cudaStream_t s) {
   const BwdArgs a{x, ldx, codes, exps, mean, rstd, w, wdtype == FLB_F32, dy, dx, dw, db, reinterpret_cast<float*>(ws), R, (int)D};
   switch (dtype) {
-    case FLB_F32: return dispatch_bwd<float>(a, G, dtype, s);
-    case FLB_F16: return dispatch_bwd<__half>(a, G, dtype, s);
-    default: return dispatch_bwd<__nv_bfloat16>(a, G, dtype, s);
+    case FLB_F32: return dispatch_bwd<float>(a, G, s);
+    case FLB_F16: return dispatch_bwd<__half>(a, G, s);
+    default: return dispatch_bwd<__nv_bfloat16>(a, G, s);
   }
 }
 

@@ -6,8 +6,9 @@
 //
 // Bound by memory: a row is read and written once. It stays in registers between its statistics and its
 // output, so the variance is the second moment about the mean itself, not a difference of large sums. A
-// warp takes a row of up to 1024 elements and needs no barrier; wider rows get a block each, 32 elements a
-// thread. The weight and bias are re-read for every row: they stay in L1.
+// warp takes a row of up to 1024 elements and needs no barrier; a wider one gets a block, 16 elements a
+// thread (32 beyond 8192). A block walks over rows a fixed distance apart, the next rows on their way to shared
+// memory meanwhile.
 #include "rows.cuh"
 
 namespace flb {
@@ -59,144 +60,205 @@ template <bool VEC> __device__ __forceinline__ void zero_beyond(F2 (&v)[4], int 
   }
 }
 
-template <typename T, bool VEC, bool WARP, int CH, bool NORM, int OUT>
-__global__ void __launch_bounds__(WARP ? 256 : 1024) row_fwd_kernel(const RowArgs a) {
-  __shared__ float slot[WARP ? 1 : 3][32];
+// Rows held at a time, the present one included: with the widest rows one
+template <int CH, int MODE> constexpr int kStages = MODE == 2 ? 1 : 2;
+constexpr int kWarps = 4;  // of a block whose warps have a row each
+template <int MODE> constexpr int kMostThreads = MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 1024;
+
+// MODE 0: a warp a row (D <= 1024), 1: a block a row (D <= 8192), 2: a block of up to 1024 threads
+template <typename T, bool VEC, int MODE, int CH, bool NORM, int OUT>
+__global__ void __launch_bounds__(kMostThreads<MODE>, 1024 / kMostThreads<MODE>) row_fwd_kernel(const RowArgs a) {
+  constexpr bool WARP = MODE == 0, COPY = kCopies<T, VEC>;
+  constexpr bool PARAMS = NORM && MODE != 2;  // the weight and bias stay in shared memory, as float32
+  constexpr int S = kStages<CH, MODE>;
+  // [CH][4][threads, or lanes of a warp's row] float4: weight and bias | [S][CH][threads] chunks of rows, with COPY
+  extern __shared__ __align__(16) uint8_t dyn[];
+  __shared__ __align__(16) float slot[WARP ? 1 : 2][3][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if constexpr (!NORM) {
     let_successor_start();
     if (blockIdx.x == 0)
       for (int64_t i = threadIdx.x; i < a.n_zero; i += blockDim.x) a.zero[i] = 0;
   }
-  const int64_t row = WARP ? (int64_t)blockIdx.x * (blockDim.x >> 5) + warp : blockIdx.x;
-  if (row >= a.rows) return;
   const int D = a.D;
-  // chunk c of this warp starts at first + c * step
-  const int first = WARP ? 0 : warp * 256, step = WARP ? 256 : (int)blockDim.x * 8;
-  const T* x = reinterpret_cast<const T*>(a.x) + row * a.ldx;
-  Raw8<T> raw[CH];  // as loaded: fewer registers for 16-bit rows, so more rows in flight
+  // chunk c of this warp starts at first + c * 256
+  const int first = WARP ? 0 : warp * 256 * CH;
+  const int64_t stride = WARP ? (int64_t)gridDim.x * (blockDim.x >> 5) : gridDim.x;
+  const int64_t row0 = WARP ? (int64_t)blockIdx.x * (blockDim.x >> 5) + warp : blockIdx.x;
+  const int64_t group = blockIdx.y, rows = a.rows_per_group;
+  const T* const x = reinterpret_cast<const T*>(a.x) + group * rows * a.ldx;
+  const int param_threads = WARP ? 32 : (int)blockDim.x, param_thread = WARP ? lane : (int)threadIdx.x;
+  float4* const params = reinterpret_cast<float4*>(dyn) + param_thread;
+  uint8_t* const ring = dyn + (PARAMS ? (size_t)CH * 64 * param_threads : 0);
+  auto chunk_at = [&](int stage, int c) { return ring + (size_t)(stage * CH + c) * 8 * sizeof(T) * blockDim.x; };
+  auto issue = [&](int64_t r, int stage) {
+    if constexpr (COPY) {
+      if (r < rows) {
 #pragma unroll
-  for (int c = 0; c < CH; ++c) load_raw<T, VEC>(raw[c], x, first + c * step, lane, D);
-  float mean = 0.f, rstd = 1.f;
-  if constexpr (NORM) {
-    F2 s = f2(0.f);
+        for (int c = 0; c < CH; ++c) copy8<T, VEC>(chunk_at(stage, c), x + r * a.ldx, first + c * 256, lane, D);
+      }
+      copies_commit();
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < S - 1; ++k) issue(row0 + k * stride, k);
+  if constexpr (!WARP) {
+    if (warp == 0)
+      for (int i = 0; i < 6; ++i) slot[i / 3][i % 3][lane] = 0.f;
+  }
+  if constexpr (PARAMS) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      F2 v[4];
-      to_float<T>(raw[c], v);
-      s = add2(s, add2(add2(v[0], v[1]), add2(v[2], v[3])));
-    }
-    mean = row_sum<WARP>(sum2(s), slot[0]) / D;
-    s = f2(0.f);
+      if (WARP && c % (int)(blockDim.x >> 5) != warp) continue;
+      F2 w[4], b[4];
+      load_param<T, VEC>(w, a.w, a.w32, 1.f, group * D, first + c * 256, lane, D);
+      load_param<T, VEC>(b, a.b, a.w32, 0.f, group * D, first + c * 256, lane, D);
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      F2 v[4];
-      to_float<T>(raw[c], v);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = add2(v[i], f2(-mean));
-      zero_beyond<VEC>(v, first + c * step, lane, D);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s = fma2(v[i], v[i], s);
-    }
-    rstd = 1.f / sqrtf(row_sum<WARP>(sum2(s), slot[WARP ? 0 : 1]) / D + a.eps);
-    if (threadIdx.x == 0 || (WARP && lane == 0)) {
-      if (a.mean) a.mean[row] = mean;
-      if (a.rstd) a.rstd[row] = rstd;
+      for (int k = 0; k < 4; ++k) {
+        const float2 lo = split(k < 2 ? w[2 * k] : b[2 * k - 4]), hi = split(k < 2 ? w[2 * k + 1] : b[2 * k - 3]);
+        params[(c * 4 + k) * param_threads] = make_float4(lo.x, lo.y, hi.x, hi.y);
+      }
     }
   }
-  const int64_t param = NORM && a.rows_per_group != a.rows ? row / a.rows_per_group * D : 0;
-  // the normalised chunk, then with the weight and bias (beyond the row: anything)
-  auto normalised = [&](int c, F2 (&v)[4]) {
-    to_float<T>(raw[c], v);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = mul2(add2(v[i], f2(-mean)), f2(rstd));
-  };
-  auto affine = [&](int c, F2 (&v)[4]) {
-    F2 w[4], b[4];
-    load_param<T, VEC>(w, a.w, a.w32, 1.f, param, first + c * step, lane, D);
-    load_param<T, VEC>(b, a.b, a.w32, 0.f, param, first + c * step, lane, D);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = fma2(v[i], w[i], b[i]);
-  };
-  if constexpr (OUT != OUT_INT8) {
+  __syncthreads();
+
+  int stage = 0, turn = 0;
+  for (int64_t r = row0; r < rows; r += stride) {
+    issue(r + (S - 1) * stride, stage == 0 ? S - 1 : stage - 1);  // where the row before this one was
+    const int64_t row = group * rows + r;
+    // the chunks' elements, and as they were loaded (for the largest magnitudes of plain rows)
+    F2 v[CH][4];
+    Raw8<T> raw[NORM ? 1 : CH];
+    if constexpr (COPY) copies_wait<S - 1>();
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int base = first + c * step;
-      F2 v[4];
-      normalised(c, v);
-      if constexpr (OUT == OUT_KEPT) {
-        if (base < D) {
-          zero_beyond<VEC>(v, base, lane, D);
-          // a row with an infinity or NaN has NaN throughout, so a block's values are all NaN or none
-          uint32_t m[VEC ? 1 : 2];
-          max_bits<VEC>(v, m);
-          keep8<VEC>(v, m, a.codes + row * code_pitch(D), a.exps + row * blocks_of(D), base, lane, D);
+      Raw8<T>& u = raw[NORM ? 0 : c];
+      if constexpr (COPY) copied_raw<T, VEC>(chunk_at(stage, c), u);
+      else load_raw<T, VEC>(u, x + r * a.ldx, first + c * 256, lane, D);
+      to_float<T>(u, v[c]);
+    }
+    if constexpr (NORM) {
+      F2 s = f2(0.f);
+#pragma unroll
+      for (int c = 0; c < CH; ++c) s = add2(s, add2(add2(v[c][0], v[c][1]), add2(v[c][2], v[c][3])));
+      const float mean = row_sum<WARP>(sum2(s), slot[turn][0]) / D;
+      s = f2(0.f);
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[c][i] = add2(v[c][i], f2(-mean));
+        zero_beyond<VEC>(v[c], first + c * 256, lane, D);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s = fma2(v[c][i], v[c][i], s);
+      }
+      const float rstd = 1.f / sqrtf(row_sum<WARP>(sum2(s), slot[turn][WARP ? 0 : 1]) / D + a.eps);
+      if (threadIdx.x == 0 || (WARP && lane == 0)) {
+        if (a.mean) a.mean[row] = mean;
+        if (a.rstd) a.rstd[row] = rstd;
+      }
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int base = first + c * 256;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[c][i] = mul2(v[c][i], f2(rstd));
+        if constexpr (OUT == OUT_KEPT) {
+          if (base < D) {
+            // a row with an infinity or NaN has NaN throughout, so a block's values are all NaN or none
+            uint32_t m[VEC ? 1 : 2];
+            max_bits<VEC>(v[c], m);
+            keep8<VEC>(v[c], m, a.codes + row * code_pitch(D), a.exps + row * blocks_of(D), base, lane, D);
+          }
+        }
+        F2 w[4], b[4];
+        if constexpr (PARAMS) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float4 u = params[(c * 4 + k) * param_threads], t = params[(c * 4 + 2 + k) * param_threads];
+            w[2 * k] = f2(u.x, u.y), w[2 * k + 1] = f2(u.z, u.w);
+            b[2 * k] = f2(t.x, t.y), b[2 * k + 1] = f2(t.z, t.w);
+          }
+        } else {
+          load_param<T, VEC>(w, a.w, a.w32, 1.f, group * D, base, lane, D);
+          load_param<T, VEC>(b, a.b, a.w32, 0.f, group * D, base, lane, D);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[c][i] = fma2(v[c][i], w[i], b[i]);
+        if constexpr (OUT != OUT_INT8) store8<T, VEC>(reinterpret_cast<T*>(a.y) + row * D, v[c], base, lane, D);
+      }
+    }
+    if constexpr (OUT == OUT_INT8) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        if constexpr (NORM) {
+          zero_beyond<VEC>(v[c], first + c * 256, lane, D);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 r = split(v[c][i]);
+            m = __vimax3_u32(m, abs_bits(r.x), abs_bits(r.y));
+          }
+        } else {
+          uint32_t h[1];
+          max_bits<T, true>(raw[c], h);
+          m = max(m, h[0]);
         }
       }
-      affine(c, v);
-      store8<T, VEC>(reinterpret_cast<T*>(a.y) + row * D, v, base, lane, D);
-    }
-  } else {
-    uint32_t m = 0;
-    F2 v[NORM ? CH : 1][4];
+      m = row_max<WARP>(m, reinterpret_cast<uint32_t*>(slot[turn][WARP ? 0 : 2]));
+      // An infinity or NaN in the row makes its scale, and so all that is computed with it, NaN. Below
+      // 2^-118 the factor 127 / a would be infinite: such a row counts as zeros.
+      const float amax = __uint_as_float(m);
+      const bool bad = m >= 0x7f800000u;
+      const float f = bad || amax < 3.0092655e-36f ? 0.f : 127.f / amax;
+      if (threadIdx.x == 0 || (WARP && lane == 0)) a.scale[row] = bad ? __uint_as_float(0x7fffffffu) : amax / 127.f;
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      if constexpr (NORM) {
-        normalised(c, v[c]);
-        affine(c, v[c]);
-        zero_beyond<VEC>(v[c], first + c * step, lane, D);
+      for (int c = 0; c < CH; ++c) {
+        uint32_t q[8];
+        float t[8];
+        to_scalars(v[c], t);
+        // product and rounding apart, each rounded as written above (as a packed pair they come out as one
+        // multiply-add, with another code now and then)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 r = split(v[c][i]);
-          m = __vimax3_u32(m, abs_bits(r.x), abs_bits(r.y));
-        }
-      } else {
-        uint32_t h[1];
-        max_bits<T, true>(raw[c], h);
-        m = max(m, h[0]);
+        for (int j = 0; j < 8; ++j) q[j] = f == 0.f ? 0u : code_of(__fmul_rn(t[j], f));
+        store_codes<VEC>(a.codes + row * code_pitch(D), q, first + c * 256, lane, D);
       }
     }
-    m = row_max<WARP>(m, reinterpret_cast<uint32_t*>(slot[WARP ? 0 : 2]));
-    // An infinity or NaN in the row makes its scale, and so all that is computed with it, NaN. Below
-    // 2^-118 the factor 127 / a would be infinite: such a row counts as zeros.
-    const float amax = __uint_as_float(m);
-    const bool bad = m >= 0x7f800000u;
-    const float f = bad || amax < 3.0092655e-36f ? 0.f : 127.f / amax;
-    if (threadIdx.x == 0 || (WARP && lane == 0)) a.scale[row] = bad ? __uint_as_float(0x7fffffffu) : amax / 127.f;
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      uint32_t q[8];
-      F2 u[4];
-      if constexpr (!NORM) to_float<T>(raw[c], u);
-      float t[8];
-      to_scalars(NORM ? v[NORM ? c : 0] : u, t);
-      // product and rounding apart, each rounded as written above (as a packed pair they come out as one
-      // multiply-add, with another code now and then)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) q[j] = f == 0.f ? 0u : code_of(__fmul_rn(t[j], f));
-      store_codes<VEC>(a.codes + row * code_pitch(D), q, first + c * step, lane, D);
-    }
+    // a warp that is a row ahead writes the other slots, and is not two ahead before every warp has passed
+    // a barrier of the row between, after reading this one's
+    if constexpr (!WARP) turn ^= 1;
+    if constexpr (S > 1) stage = stage + 1 == S ? 0 : stage + 1;
   }
 }
 
-template <typename T, bool VEC, bool NORM, int OUT>
-int launch_rows(const RowArgs& a, cudaStream_t s) {
-  const int D = a.D;
-  if (D <= 1024) {
-    // few rows: a warp a block, so that they spread over the SMs; many: eight, fewer blocks to start
-    const int warps = a.rows >= 16 * (int64_t)num_sms() ? 8 : a.rows >= 4 * (int64_t)num_sms() ? 4 : 1;
-    const dim3 grid((unsigned)((a.rows + warps - 1) / warps)), block(32 * warps);
-    switch ((D + 255) / 256) {
-      case 1: row_fwd_kernel<T, VEC, true, 1, NORM, OUT><<<grid, block, 0, s>>>(a); break;
-      case 2: row_fwd_kernel<T, VEC, true, 2, NORM, OUT><<<grid, block, 0, s>>>(a); break;
-      case 3: row_fwd_kernel<T, VEC, true, 3, NORM, OUT><<<grid, block, 0, s>>>(a); break;
-      default: row_fwd_kernel<T, VEC, true, 4, NORM, OUT><<<grid, block, 0, s>>>(a); break;
-    }
-  } else {
-    row_fwd_kernel<T, VEC, false, 4, NORM, OUT><<<(unsigned)a.rows, 32 * ((D + 1023) / 1024), 0, s>>>(a);
-  }
+template <typename T, bool VEC, int MODE, int CH, bool NORM, int OUT> int launch_mode(const RowArgs& a, int threads, cudaStream_t s) {
+  auto k = row_fwd_kernel<T, VEC, MODE, CH, NORM, OUT>;
+  const size_t ring = kCopies<T, VEC> ? (size_t)kStages<CH, MODE> * CH * 8 * sizeof(T) * threads : 0;
+  const size_t smem = ring + (NORM && MODE != 2 ? (size_t)CH * 64 * (MODE == 0 ? 32 : threads) : 0);
+  const int st = ensure_dyn_smem(reinterpret_cast<const void*>(k), (int)smem, "row kernel shared memory");
+  if (st != FLB_OK) return st;
+  // as many blocks as an SM holds (64 registers a thread, 224 KB), each with as many rows as the others
+  const int64_t at_once = MODE == 0 ? threads / 32 : 1, groups = a.rows / a.rows_per_group;
+  const int64_t units = (a.rows_per_group + at_once - 1) / at_once;
+  const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>(1024 / threads, (224 << 10) / (int64_t)(smem + 2048)));
+  const int64_t room = std::max<int64_t>(1, num_sms() * per_sm / groups);
+  k<<<dim3((unsigned)std::min(units, room), (unsigned)groups), threads, smem, s>>>(a);
   count_launches(1);
   return check_cuda(cudaGetLastError(), "row kernel launch");
+}
+
+template <typename T, bool VEC, bool NORM, int OUT> int launch_rows(const RowArgs& a, cudaStream_t s) {
+  const int D = a.D;
+  if (D <= 1024) {
+    // few rows: a warp a block, so that they spread over the SMs
+    const int threads = a.rows >= 4 * (int64_t)num_sms() ? 32 * kWarps : 32;
+    switch ((D + 255) / 256) {
+      case 1: return launch_mode<T, VEC, 0, 1, NORM, OUT>(a, threads, s);
+      case 2: return launch_mode<T, VEC, 0, 2, NORM, OUT>(a, threads, s);
+      case 3: return launch_mode<T, VEC, 0, 3, NORM, OUT>(a, threads, s);
+      default: return launch_mode<T, VEC, 0, 4, NORM, OUT>(a, threads, s);
+    }
+  }
+  if (D <= 8192) return launch_mode<T, VEC, 1, 2, NORM, OUT>(a, 32 * ((D + 511) / 512), s);
+  return launch_mode<T, VEC, 2, 4, NORM, OUT>(a, 32 * ((D + 1023) / 1024), s);
 }
 
 bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

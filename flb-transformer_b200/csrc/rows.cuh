@@ -331,17 +331,73 @@ template <bool VEC> __device__ __forceinline__ void kept_to_float(const Kept8& k
 __host__ __device__ inline int64_t code_pitch(int64_t D) { return (D + 15) & ~(int64_t)15; }
 __host__ __device__ inline int64_t blocks_of(int64_t D) { return (D + kBlock - 1) / kBlock; }
 
+// ---- rows ahead ------------------------------------------------------------------------------------
+// Copies of the rows ahead, in shared memory. A thread copies, and later reads, only its own elements, so
+// its own wait for its copies is all the synchronisation there is. 16-bit rows that do not start on 16
+// bytes have no such copies (the smallest is 4 bytes): they are loaded when their turn comes.
+template <typename T, bool VEC> constexpr bool kCopies = VEC || sizeof(T) == 4;
+
+__device__ __forceinline__ uint32_t shared_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool there) {
+  // with no source bytes the destination is filled with zeros
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(there ? BYTES : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// One chunk's eight elements of this thread: slots [word group][thread], so that a warp's accesses are contiguous
+template <typename T, bool VEC>
+__device__ __forceinline__ void copy8(uint8_t* slot, const T* row, int base, int lane, int D) {
+  const uint32_t at = shared_addr(slot);
+  if constexpr (VEC) {
+    const int p = base + lane * 8;
+    const uint8_t* src = reinterpret_cast<const uint8_t*>(row + (p < D ? p : 0));
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+      copy_async<16>(at + (i * blockDim.x + threadIdx.x) * 16, src + 16 * i, p < D);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int p = base + j * 32 + lane;
+      copy_async<4>(at + (j * blockDim.x + threadIdx.x) * 4, row + (p < D ? p : 0), p < D);
+    }
+  }
+}
+template <typename T, bool VEC> __device__ __forceinline__ void copied_raw(const uint8_t* slot, Raw8<T>& r) {
+  if constexpr (VEC) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+      const uint4 u = reinterpret_cast<const uint4*>(slot)[i * blockDim.x + threadIdx.x];
+      r.w[4 * i] = u.x, r.w[4 * i + 1] = u.y, r.w[4 * i + 2] = u.z, r.w[4 * i + 3] = u.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r.w[j % (sizeof(T) * 2)] = reinterpret_cast<const uint32_t*>(slot)[j * blockDim.x + threadIdx.x];
+  }
+}
+template <typename T, bool VEC> __device__ __forceinline__ void copied8(const uint8_t* slot, F2 (&v)[4]) {
+  Raw8<T> r;
+  copied_raw<T, VEC>(slot, r);
+  to_float<T>(r, v);
+}
+
 // ---- reductions over a row ------------------------------------------------------------------------
 // Over one warp, or over the whole block through `slot` (32 words, not used for anything else until every
 // thread has passed a later barrier). Every thread gets the result, summed in the same order each time.
+// The slots of warps that the block does not have hold zeros.
 template <bool WARP> __device__ __forceinline__ float row_sum(float v, float* slot) {
   v = warp_sum(v);
   if constexpr (!WARP) {
-    const int n = blockDim.x >> 5;
     if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = slot[0];
-    for (int i = 1; i < n; ++i) v += slot[i];
+    v = 0.f;
+    for (int i = 0; i < (int)(blockDim.x >> 5); i += 4) {
+      const float4 t = *reinterpret_cast<const float4*>(slot + i);
+      v += (t.x + t.y) + (t.z + t.w);
+    }
   }
   return v;
 }

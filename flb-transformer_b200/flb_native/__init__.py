@@ -90,7 +90,7 @@ PROTOTYPES = {
     "flb_kept_blocks": (_i64, [_i64]),
     "flb_layer_norm_fwd": (_i32, [_vp, _i64, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i64,
                                   _i64, _i32, ctypes.c_float, _vp]),
-    "flb_layer_norm_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32]),
+    "flb_layer_norm_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "flb_layer_norm_bwd": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i64,
                                   _i64, _i64, _i32, _vp, _sz, _vp]),
     "flb_pack8": (_i32, [_vp, _vp, _vp, _i64, _i64, _i32, _vp]),

@@ -416,7 +416,7 @@ int flb_layer_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b,
 /* dx in dtype; dw and db ([G, D] in wdtype, OVERWRITTEN; both or neither NULL) are summed in a fixed
  * order (the same bits every time). Either x and mean, or codes and exps. Workspace:
  * flb_layer_norm_bwd_workspace_bytes(), 16-byte aligned, asked for on the same device. */
-size_t flb_layer_norm_bwd_workspace_bytes(int64_t G, int64_t R, int64_t D, int dtype);
+size_t flb_layer_norm_bwd_workspace_bytes(int64_t G, int64_t R, int64_t D);
 int flb_layer_norm_bwd(const void* x, int64_t ldx, const int8_t* codes, const uint8_t* exps,
                        const float* mean, const float* rstd, const void* w, int wdtype, const void* dy,
                        void* dx, void* dw, void* db, int64_t G, int64_t R, int64_t D, int dtype,

@@ -60,8 +60,8 @@ def test_norm_arguments():
     assert norm_bwd(D=16385) == FLB_UNSUPPORTED and norm_bwd(dy=None) == FLB_SHAPE and norm_bwd(mean=None) == FLB_SHAPE
     assert norm_bwd(rstd=None) == FLB_SHAPE and norm_bwd(dw=16) == FLB_SHAPE and norm_bwd(dx=3) == FLB_ALIGN
     assert norm_bwd(x=None, codes=16) == FLB_SHAPE
-    need = nat.lib.flb_layer_norm_bwd_workspace_bytes(1, 4096, 768, BF16)
-    assert need > 0 and nat.lib.flb_layer_norm_bwd_workspace_bytes(1, 4, 768, BF16) == 0
+    need = nat.lib.flb_layer_norm_bwd_workspace_bytes(1, 4096, 768)
+    assert need > 0 and nat.lib.flb_layer_norm_bwd_workspace_bytes(1, 4, 768) == 0
     assert norm_bwd(dw=16, db=16, R=4096, D=768, ldx=768) == FLB_WORKSPACE
     assert norm_bwd(dw=16, db=16, R=4096, D=768, ldx=768, ws=16, n=need - 1) == FLB_WORKSPACE
     assert norm_bwd(dw=16, db=16, R=4096, D=768, ldx=768, ws=24, n=need) == FLB_ALIGN
