@@ -34,6 +34,9 @@
 
 namespace flb {
 
+int pack8(const void* x, int8_t* codes, uint8_t* exps, int64_t R, int64_t D, int dtype, cudaStream_t s);
+int unpack8(const int8_t* codes, const uint8_t* exps, void* out, int64_t R, int64_t D, int dtype, cudaStream_t s);
+
 namespace {
 
 using bf16 = __nv_bfloat16;
@@ -460,6 +463,24 @@ __host__ __device__ inline int64_t plane_offset(int p, int64_t cells, int64_t BD
   return u * cells * BD;
 }
 
+// A training step's per-cell tensors in the 8-bit kept form (flb_block_grid_saved8_bytes): per tick, in the order of the
+// ticks, the rows (of D elements) [lat_prior | tokens | z_l | z_x | q|k|v | att] of its cells, kKeptUnits rows for each
+// cell and batch row; codes of all rows, then their exponents. The forward leaves a tick's tensors on end
+// in its work buffers, and one launch keeps them; the backward's unpacking of a tick takes the place of recomputing its
+// forward stages. (The LayerNorm outputs are not kept: they come from the port grids in one launch.)
+constexpr int kKeptUnits = 18;
+
+struct Kept8Store {
+  int8_t* codes;
+  uint8_t* exps;
+};
+size_t kept8_layout(int64_t L, int64_t S, int64_t B, int64_t D, void* base, Kept8Store* k) {
+  const int64_t rows = L * S * kKeptUnits * B;
+  const size_t codes = ((size_t)rows * D + 255) & ~(size_t)255;  // D is a multiple of 16: no padding within a row
+  if (k) *k = Kept8Store{reinterpret_cast<int8_t*>(base), reinterpret_cast<uint8_t*>(base) + codes};
+  return codes + (size_t)rows * flb_kept_blocks(D);
+}
+
 constexpr size_t kBlkBlasWs = 32u << 20;
 
 struct BlockWs {
@@ -667,6 +688,12 @@ struct TickBufs {
   int64_t cs;
 };
 
+// The n cells' tensors in the order of the kept form, on end from `base` (the first of work buffers that follow each
+// other in that order)
+TickBufs on_end(bf16* ln, bf16* base, int64_t n, int64_t BD) {
+  return TickBufs{ln, base, base + n * BD, base + 4 * n * BD, base + 5 * n * BD, base + 6 * n * BD, base + 15 * n * BD, BD};
+}
+
 // stages 1-6 of a tick (everything up to the attention output)
 // the side stream and its cuBLAS handle for GEMMs off the critical chain of a tick
 struct Side {
@@ -765,13 +792,13 @@ int tick_forward(cublasHandle_t hb, const Side& side, const flb_block_weights* W
 int block_grid_fwd_ex(const flb_block_weights* W, const void* x, void* grids, int64_t L,
                       int64_t S, int64_t B, int64_t D, int64_t H, float eps, void* ws,
                       size_t ws_bytes, cudaStream_t s, int path, int drop_cta, int drop_bar,
-                      uint32_t spin_limit, void* saved) {
+                      uint32_t spin_limit, void* saved, void* saved8) {
   // the persistent forward only on request: at the end-to-end shape (12 layers x 1024
   // positions, d_model 768, batch 16) it measured 111 ms per forward against 80 ms tick by tick
   const bool persist = persist_fits(L, S, B, D, H) && path == FLB_BLOCK_PATH_PERSISTENT;
   if (path == FLB_BLOCK_PATH_PERSISTENT && !persist)
     return fail(FLB_ERR_UNSUPPORTED, "block_grid persistent forward: needs batch 16 and D a multiple of 128 up to 1024");
-  if (persist && saved)
+  if (persist && (saved || saved8))
     return fail(FLB_ERR_UNSUPPORTED, "block_grid: the persistent forward keeps no intermediates");
   BlockWs w;
   block_ws_layout(max_cells_per_tick(L, S), L, B, D, &w, ws);
@@ -801,6 +828,9 @@ int block_grid_fwd_ex(const flb_block_weights* W, const void* x, void* grids, in
                               dim3(128), 0, s, w.lnr, W->ln_lat_b, W->ln_fdbk_b, Li, Bi, Di);
   if (ie != cudaSuccess) return check_cuda(ie, "block_grid LayerNorm init launch");
   int launches = 1;
+  Kept8Store kept{};
+  if (saved8) kept8_layout(L, S, B, D, saved8, &kept);
+  int64_t kept_rows = 0;  // of the ticks so far
   for (int T = 0; T < ticks; ++T) {
     const Tick tk = tick_of(T, Li, Si);
     const int n = tk.n, l0 = tk.l0;
@@ -814,6 +844,7 @@ int block_grid_fwd_ex(const flb_block_weights* W, const void* x, void* grids, in
       tb = TickBufs{w.ln, at(PL_LAT), at(PL_TOK), at(PL_ZL), at(PL_ZX), at(PL_QKV), at(PL_ATT),
                     (2 * S - 1) * BD};
     }
+    if (saved8) tb = on_end(w.ln, w.lat, n, BD);
     if ((st = tick_forward(hb, side, W, xb, g, port_stride, tb, T, l0, n, Li, Si, Bi, Di, Hi, eps,
                            s, w.glpf, w.lnr)) != FLB_OK)
       return st;
@@ -828,6 +859,12 @@ int block_grid_fwd_ex(const flb_block_weights* W, const void* x, void* grids, in
                                W->ln_lat_b, W->ln_fdbk_w, W->ln_fdbk_b, eps, T, l0, n, Li, Si, Bi, Di);
     if (e != cudaSuccess) return check_cuda(e, "block_grid output launch");
     launches += 4;  // own kernels: two gates, attention, output (the GEMMs are cuBLAS's)
+    if (saved8) {
+      const int64_t rows = (int64_t)n * kKeptUnits * B;
+      if ((st = pack8(tb.lat, kept.codes + kept_rows * D, kept.exps + kept_rows * flb_kept_blocks(D), rows, D, FLB_BF16, s)) != FLB_OK)
+        return st;
+      kept_rows += rows;
+    }
   }
   if (planes) {
     // the LayerNorm planes of every cell, from the port grids the ticks wrote
@@ -847,7 +884,7 @@ int block_grid_fwd(const flb_block_weights* W, const void* x, void* grids, int64
                    int64_t B, int64_t D, int64_t H, float eps, void* ws, size_t ws_bytes,
                    cudaStream_t s) {
   return block_grid_fwd_ex(W, x, grids, L, S, B, D, H, eps, ws, ws_bytes, s, FLB_BLOCK_PATH_AUTO,
-                           -1, -1, 0, nullptr);
+                           -1, -1, 0, nullptr, nullptr);
 }
 
 int block_grid_status(const void* ws, cudaStream_t s) {
@@ -1320,6 +1357,10 @@ size_t block_bwd_ws_layout(int64_t L, int64_t S, int64_t B, int64_t D, BlockBwdW
 
 }  // namespace
 
+size_t block_grid_saved8_bytes(int64_t L, int64_t S, int64_t B, int64_t D) {
+  return kept8_layout(L, S, B, D, nullptr, nullptr);
+}
+
 size_t block_grid_saved_bytes(int64_t L, int64_t S, int64_t B, int64_t D) {
   return (size_t)L * S * kSavedUnits * B * D * sizeof(bf16);
 }
@@ -1331,8 +1372,11 @@ size_t block_grid_bwd_workspace_bytes(int64_t L, int64_t S, int64_t B, int64_t D
 int block_grid_bwd(const flb_block_weights* W, const void* x, const void* grids,
                    const void* const* dgrids, float* dx, const flb_block_grads* G, int64_t L,
                    int64_t S, int64_t B, int64_t D, int64_t H, float eps, void* ws,
-                   size_t ws_bytes, cudaStream_t s, void* saved) {
-  bf16* planes = reinterpret_cast<bf16*>(saved);  // null: recompute
+                   size_t ws_bytes, cudaStream_t s, void* saved, void* saved8) {
+  bf16* planes = reinterpret_cast<bf16*>(saved);  // null: recompute, or unpack saved8
+  Kept8Store kept{};
+  if (saved8) kept8_layout(L, S, B, D, saved8, &kept);
+  int64_t kept_rows = L * S * kKeptUnits * B;  // of the ticks before the present one, once it has been unpacked
   BlockBwdWs w;
   block_bwd_ws_layout(L, S, B, D, &w, ws);
   SideStream* side;
@@ -1387,6 +1431,7 @@ int block_grid_bwd(const flb_block_weights* W, const void* x, const void* grids,
     // tick's cells lie 2S - 1 cells apart there; nothing is copied in or out), else the work
     // buffers the recomputed forward fills (cs = B x D)
     int64_t cs = BD;
+    if (saved8) w.f = on_end(w.f.ln, w.f.lat, n, BD);
     const bf16 *f_lat = w.f.lat, *f_tok = w.f.tok, *f_zl = w.f.zl, *f_zx = w.f.zx,
                *f_qkv = w.f.qkv;
     bf16 *d_o = w.d_o, *d_qkv = w.d_qkv, *d_zx = w.d_zx, *d_zl = w.d_zl, *d_lp_h = w.d_lp_h,
@@ -1406,6 +1451,14 @@ int block_grid_bwd(const flb_block_weights* W, const void* x, const void* grids,
       d_zl = at(PL_DZL);
       d_lp_h = at(PL_DLP);
       d_fp_h = at(PL_DFP);
+    } else if (saved8) {
+      const int64_t rows = (int64_t)n * kKeptUnits * B;
+      kept_rows -= rows;
+      if ((st = unpack8(kept.codes + kept_rows * D, kept.exps + kept_rows * flb_kept_blocks(D), w.f.lat, rows, D, FLB_BF16, s)) != FLB_OK)
+        return st;
+      ce = launch_pdl(blk_ln_kernel, dim3((2 * n * B + 7) / 8), dim3(256), 0, s, g + port_stride, g + 2 * port_stride, W->ln_lat_w,
+                      W->ln_lat_b, W->ln_fdbk_w, W->ln_fdbk_b, w.f.ln, T, l0, n, Li, Si, Bi, Di, eps);
+      if (ce != cudaSuccess) return check_cuda(ce, "block_grid_bwd LayerNorm launch");
     } else if ((st = tick_forward(hb, Side{side, hs}, W, xb, g, port_stride, w.f, T, l0, n, Li, Si,
                                   Bi, Di, Hi, eps, s)) != FLB_OK) {
       return st;
@@ -1507,7 +1560,8 @@ int block_grid_bwd(const flb_block_weights* W, const void* x, const void* grids,
                          Bi, Di, eps)) != cudaSuccess)
       return check_cuda(ce, "block_grid_bwd launch");
     if (!saved && (st = join()) != FLB_OK) return st;
-    launches += saved ? 5 : 9;  // own kernels: 5 backward (+ 4 of the recomputed forward)
+    // own kernels: 5 backward (+ 4 of the recomputed forward; the unpacking counts itself, + its LayerNorm)
+    launches += saved ? 5 : saved8 ? 6 : 9;
   }
   if (saved) {
     // Weight gradients: per layer, one GEMM over all of its cells (K = S x rows), from the

@@ -17,6 +17,11 @@ state_dict trained with either loads into the other:
                                aux_loss = mean(aux grid) * aux_weight; next contexts = the last
                                column of ports 1 and 2.
 
+fused_ops=True evaluates the blocks' norms and gates with kernels.layer_norm and kernels.sigmoid_gate
+instead of torch's (the parameters' names and shapes are the same); keep8=True (with fused_ops) has
+them keep what their backward reads in 8 bits. Where the engine runs its native whole-grid kernels
+(bf16 autocast), neither is consulted: engine.native_flb_save says there what is kept.
+
 The dropout modules exist for state compatibility and run where the reference runs them (the
 attention layer's own dropout is not applied there either).
 """
@@ -25,14 +30,16 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
-from kernels.additive_attention import fused_additive_attention
+from kernels import FusedLayerNorm, fused_additive_attention, sigmoid_gate
 from wavefront.wavefront_api import WavefrontConfig
 from wavefront.wavefront_engine import WavefrontEngine
 
 
 class FLBAttentionLayer(nn.Module):
-    def __init__(self, hidden_dim: int, num_heads: int = 8, dropout: float = 0.1):
+    def __init__(self, hidden_dim: int, num_heads: int = 8, dropout: float = 0.1,
+                 fused_ops: bool = False, keep8: bool = False):
         super().__init__()
+        self.fused_ops, self.keep8 = fused_ops, keep8
         if hidden_dim % num_heads:
             raise ValueError(f"hidden_dim {hidden_dim} is not divisible by {num_heads} heads")
         self.hidden_dim, self.num_heads = hidden_dim, num_heads
@@ -46,10 +53,16 @@ class FLBAttentionLayer(nn.Module):
         self.W_o = nn.Linear(hidden_dim, hidden_dim, bias=False)
         self.dropout = nn.Dropout(dropout)
 
+    def gate(self, token, z):
+        if not self.fused_ops:
+            return token * torch.sigmoid(z)
+        dtype = torch.promote_types(token.dtype, z.dtype)
+        return sigmoid_gate(token.to(dtype), z.to(dtype), keep8=self.keep8)
+
     def forward(self, x_token, lat_token, fdbk_token):
         n, _, dim = x_token.shape                      # each token [n, 1, dim]
-        lat_ref = lat_token * torch.sigmoid(self.linear_gate_L(fdbk_token))
-        x_ref = x_token * torch.sigmoid(self.linear_gate_X(lat_ref))
+        lat_ref = self.gate(lat_token, self.linear_gate_L(fdbk_token))
+        x_ref = self.gate(x_token, self.linear_gate_X(lat_ref))
         seq = torch.cat([x_ref, lat_ref, fdbk_token], dim=1)       # [n, 3, dim]
 
         def heads(t):                                  # [n, 3, dim] -> [n, H, 3, dim/H]
@@ -65,13 +78,20 @@ class FLBBlock(nn.Module):
     """FLB_Block (models/FLB_Model.py:64-96). The reference fixes 8 attention heads (:73);
     num_heads (default 8) makes the head count a constructor argument."""
 
-    def __init__(self, hidden_dim: int, dropout: float = 0.1, num_heads: int = 8):
+    def __init__(self, hidden_dim: int, dropout: float = 0.1, num_heads: int = 8,
+                 fused_ops: bool = False, keep8: bool = False):
         super().__init__()
-        self.norm_lat = nn.LayerNorm(hidden_dim)
-        self.norm_fdbk = nn.LayerNorm(hidden_dim)
+        if keep8 and not fused_ops:
+            raise ValueError("keep8 needs fused_ops")
+
+        def norm():
+            return FusedLayerNorm(hidden_dim, keep8=keep8) if fused_ops else nn.LayerNorm(hidden_dim)
+
+        self.norm_lat, self.norm_fdbk = norm(), norm()
         self.proj_lateral = nn.Linear(hidden_dim, hidden_dim, bias=False)
         self.proj_feedback = nn.Linear(hidden_dim, hidden_dim, bias=False)
-        self.flb_attention = FLBAttentionLayer(hidden_dim, num_heads=num_heads, dropout=dropout)
+        self.flb_attention = FLBAttentionLayer(hidden_dim, num_heads=num_heads, dropout=dropout,
+                                               fused_ops=fused_ops, keep8=keep8)
 
     def forward(self, x_input, prev_lat, prev_fdbk):
         b, cells, dim = x_input.shape
@@ -90,7 +110,8 @@ FLB_DEPENDENCIES = [((-1, 0), 0), ((0, -1), 1), ((1, -1), 2)]
 class FLBTransformer(nn.Module):
     def __init__(self, vocab_size: int, hidden_dim: int = 256, num_layers: int = 6,
                  seq_len: int = 128, batch_size: int = 32, dropout: float = 0.1,
-                 aux_weight: float = 0.05, num_heads: int = 8):
+                 aux_weight: float = 0.05, num_heads: int = 8, fused_ops: bool = False,
+                 keep8: bool = False):
         super().__init__()
         self.aux_weight = aux_weight
         self.embedding = nn.Embedding(vocab_size, hidden_dim)
@@ -98,28 +119,29 @@ class FLBTransformer(nn.Module):
         self.out_dropout = nn.Dropout(dropout)
         self.config = WavefrontConfig(grid_shape=(num_layers, seq_len), batch_size=batch_size,
                                       dim=hidden_dim, dependencies=FLB_DEPENDENCIES, num_ports=4)
-        self.layers = nn.ModuleList([FLBBlock(hidden_dim, dropout, num_heads)
+        self.layers = nn.ModuleList([FLBBlock(hidden_dim, dropout, num_heads, fused_ops, keep8)
                                      for _ in range(num_layers)])
         self.engine = WavefrontEngine(self.config, self.layers)
         self.head = nn.Linear(hidden_dim, vocab_size)
 
-    def grids_to_outputs(self, grids):
+    def grids_to_outputs(self, grids, head=None):
         """(logits [batch, seq, vocab], aux_loss, (next_lat, next_fdbk)) from the engine's four
-        port grids [cells, batch, dim]."""
+        port grids [cells, batch, dim]. `head` optionally replaces self.head."""
         L, S = self.config.grid_shape
         B, D = self.config.batch_size, self.config.dim
         y, lat, fdbk, aux = (g.view(L, S, B, D) for g in grids)
         top = self.out_dropout(y[-1].transpose(0, 1))               # [batch, seq, dim]
-        logits = self.head(top)
+        logits = (head or self.head)(top)
         aux_loss = aux.mean() * self.aux_weight
         return logits, aux_loss, (lat[:, -1], fdbk[:, -1])
 
-    def forward(self, tokens, context=None, engine=None):
+    def forward(self, tokens, context=None, engine=None, head=None):
         """tokens [batch, seq_len] int64. `engine` optionally replaces self.engine (for example
-        a GraphedWavefrontEngine captured from it)."""
+        a GraphedWavefrontEngine captured from it), `head` self.head (for example its
+        kernels.Int8Linear, for inference)."""
         x = self.emb_dropout(self.embedding(tokens))
         states = {}
         if context is not None:
             states = {1: context[0], 2: context[1]}
         grids = (engine or self.engine)(x, states)
-        return self.grids_to_outputs(grids)
+        return self.grids_to_outputs(grids, head)

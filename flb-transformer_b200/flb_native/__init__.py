@@ -63,6 +63,12 @@ PROTOTYPES = {
     "flb_block_grid_bwd_saved": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64,
                                         _i64, _i64, _i64, ctypes.c_float, _vp, _sz, _vp, _sz,
                                         _vp]),
+    "flb_block_grid_saved8_bytes": (_sz, [_i64, _i64, _i64, _i64]),
+    "flb_block_grid_fwd_save8": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
+                                        ctypes.c_float, _vp, _sz, _vp, _sz, _vp]),
+    "flb_block_grid_bwd_saved8": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64,
+                                         _i64, _i64, _i64, ctypes.c_float, _vp, _sz, _vp, _sz,
+                                         _vp]),
     "flb_block_grid_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
     "flb_block_grid_bwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
                                   _i64, _i64, ctypes.c_float, _vp, _sz, _vp]),

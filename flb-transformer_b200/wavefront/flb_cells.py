@@ -15,12 +15,15 @@ training forward keeps every cell's intermediates (flb_block_grid_fwd_save) so t
 restores them instead of recomputing its ticks' forward stages, and keeps the gradients that
 meet the weights beside them to form every weight gradient in a few large GEMMs at its end;
 engine.native_flb_save = False trades that memory (L * S * 36 * batch * d_model bf16) for the
-recompute and per-tick weight-gradient GEMMs.
+recompute and per-tick weight-gradient GEMMs, and engine.native_flb_save = "int8" keeps them in the 8-bit
+form of kernels.pack8 instead (L * S * 18 * batch * d_model bytes, a quarter of that memory), which the
+backward unpacks tick by tick in the recompute's place: its gradients carry that form's rounding.
 """
 from __future__ import annotations
 
 import ctypes
 import math
+from typing import NamedTuple
 
 import torch
 
@@ -105,26 +108,36 @@ class BlockWeightStacks:
         self.eps = float(layers[0].norm_lat.eps)
 
 
-def saved_buffer(engine, device) -> torch.Tensor | None:
-    """The engine's buffer for a training forward's per-cell intermediates
-    (flb_block_grid_saved_bytes), or None when engine.native_flb_save is False (the backward
-    then recomputes each tick's forward stages). One buffer per engine, like its static grids:
-    a forward overwrites what the previous one kept."""
-    if not getattr(engine, "native_flb_save", True):
+class Saved8(NamedTuple):
+    """A buffer of intermediates in 8 bits (flb_block_grid_saved8_bytes)."""
+    buffer: torch.Tensor
+
+
+def saved_buffer(engine, device) -> torch.Tensor | Saved8 | None:
+    """The engine's buffer for a training forward's per-cell intermediates: bf16
+    (flb_block_grid_saved_bytes), or a Saved8 when engine.native_flb_save is "int8", or None when
+    it is False (the backward then recomputes each tick's forward stages). One buffer per engine
+    and kind, like its static grids: a forward overwrites what the previous one kept."""
+    kind = getattr(engine, "native_flb_save", True)
+    if isinstance(kind, str) and kind != "int8":
+        raise ValueError(f"engine.native_flb_save must be True, False or 'int8', not {kind!r}")
+    if not kind:
         return None
     cfg = engine.config
     L, S = cfg.grid_shape
-    nbytes = nat.lib.flb_block_grid_saved_bytes(L, S, cfg.batch_size, cfg.dim)
+    size, key = ((nat.lib.flb_block_grid_saved8_bytes, "flb_saved8") if kind == "int8" else
+                 (nat.lib.flb_block_grid_saved_bytes, "flb_saved"))
+    nbytes = size(L, S, cfg.batch_size, cfg.dim)
     ws = engine.graph_workspace
-    buf = ws.get("flb_saved")
+    buf = ws.get(key)
     if buf is None or buf.numel() != nbytes or buf.device != torch.device(device):
         buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        ws["flb_saved"] = buf
-    return buf
+        ws[key] = buf
+    return Saved8(buf) if kind == "int8" else buf
 
 
 def native_flb_forward(engine, static_x: torch.Tensor, grids: torch.Tensor, weights=None,
-                       saved: torch.Tensor | None = None) -> None:
+                       saved: torch.Tensor | Saved8 | None = None) -> None:
     """Evaluate every cell of the engine's grid into `grids` ([ports, cells + L, batch, dim],
     bf16) from static_x ([batch, seq, dim], bf16), with the layers' current weights. With
     `saved` (saved_buffer) the cells' intermediates are kept for native_flb_backward."""
@@ -135,6 +148,12 @@ def native_flb_forward(engine, static_x: torch.Tensor, grids: torch.Tensor, weig
     ws_bytes = nat.lib.flb_block_grid_workspace_bytes(L, S, B, D)
     ws = nat.workspace(ws_bytes, grids.device)
     wptr = ctypes.cast(ctypes.pointer(w.struct), ctypes.c_void_p)
+    if isinstance(saved, Saved8):
+        buf = saved.buffer
+        nat.check(nat.lib.flb_block_grid_fwd_save8(
+            wptr, static_x.data_ptr(), grids.data_ptr(), L, S, B, D, w.heads, w.eps, nat.ptr(ws),
+            ws_bytes, buf.data_ptr(), buf.numel(), nat.stream_of(grids)), "flb_block_grid_fwd_save8")
+        return
     if saved is not None:
         nat.check(nat.lib.flb_block_grid_fwd_save(
             wptr, static_x.data_ptr(), grids.data_ptr(), L, S, B, D, w.heads, w.eps, nat.ptr(ws),
@@ -194,9 +213,9 @@ class FLBGridFunction(torch.autograd.Function):
         return (None, dx.to(dtype).reshape(shape), *flb_param_grads(ctx.engine, gstacks))
 
 
-def native_flb_backward(engine, w, grad_grids, saved: torch.Tensor | None = None):
-    """flb_block_grid_bwd over the engine's saved grids (flb_block_grid_bwd_saved with the
-    forward's intermediates when `saved` holds them): (fp32 gradient stacks keyed like the
+def native_flb_backward(engine, w, grad_grids, saved: torch.Tensor | Saved8 | None = None):
+    """flb_block_grid_bwd over the engine's saved grids (flb_block_grid_bwd_saved or _saved8 with
+    the forward's intermediates when `saved` holds them): (fp32 gradient stacks keyed like the
     weight stacks, dx float32 [batch, seq, dim])."""
     cfg = engine.config
     L, S = cfg.grid_shape
@@ -213,7 +232,10 @@ def native_flb_backward(engine, w, grad_grids, saved: torch.Tensor | None = None
             ws["static_stacked_grids"].data_ptr(), *[nat.ptr(g) for g in dg], dx.data_ptr(),
             ctypes.cast(ctypes.pointer(gstruct), ctypes.c_void_p), L, S, B, D, w.heads, w.eps,
             nat.ptr(wsb), ws_bytes)
-    if saved is not None:
+    if isinstance(saved, Saved8):
+        nat.check(nat.lib.flb_block_grid_bwd_saved8(*args, saved.buffer.data_ptr(), saved.buffer.numel(),
+                                                    nat.stream_of(dx)), "flb_block_grid_bwd_saved8")
+    elif saved is not None:
         nat.check(nat.lib.flb_block_grid_bwd_saved(*args, saved.data_ptr(), saved.numel(),
                                                    nat.stream_of(dx)), "flb_block_grid_bwd_saved")
     else:

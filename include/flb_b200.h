@@ -379,6 +379,23 @@ int flb_block_grid_bwd_saved(const flb_block_weights* weights, const void* x, co
                              float ln_eps, void* workspace, size_t workspace_bytes,
                              void* saved, size_t saved_bytes, void* stream);
 
+/* The same pair with the intermediates kept in 8 bits (the kept form below; no reference counterpart): 18 rows of D for
+ * each cell and batch row, about L * S * 18 * batch * D bytes against flb_block_grid_saved_bytes()'s 72. The forward's
+ * outputs are flb_block_grid_fwd's; the backward unpacks a tick's intermediates where flb_block_grid_bwd recomputes
+ * them, so its gradients carry the kept form's rounding. The buffer is 16-byte aligned and is only read by the
+ * backward. */
+size_t flb_block_grid_saved8_bytes(int64_t L, int64_t S, int64_t batch, int64_t D);
+int flb_block_grid_fwd_save8(const flb_block_weights* weights, const void* x, void* grids, int64_t L,
+                             int64_t S, int64_t batch, int64_t D, int64_t heads, float ln_eps,
+                             void* workspace, size_t workspace_bytes, void* saved8,
+                             size_t saved8_bytes, void* stream);
+int flb_block_grid_bwd_saved8(const flb_block_weights* weights, const void* x, const void* grids,
+                              const void* dgrid0, const void* dgrid1, const void* dgrid2,
+                              const void* dgrid3, float* dx, const flb_block_grads* grads,
+                              int64_t L, int64_t S, int64_t batch, int64_t D, int64_t heads,
+                              float ln_eps, void* workspace, size_t workspace_bytes,
+                              const void* saved8, size_t saved8_bytes, void* stream);
+
 /* Failure-detection check of the grid kernels' bounded dependency waits (no reference
  * counterpart). Runs flb_grid_fwd with the flag of cell (drop_row, drop_col) never released and
  * the flag-wait bound lowered to spin_limit polls: the cells waiting on it give up, record the
