@@ -150,29 +150,28 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      // the weight was written before the kernel that this one may overlap started; the tokens' codes by
-      // that kernel, so the first ring of weight tiles is on its way before the wait
-      bool ok = true, waited = false;
-      uint32_t it = 0;
+      // The weight was written before the kernel that this one may overlap started; the tokens' codes by that
+      // kernel, so a first ring of weight tiles, of the first units' steps, is on its way before the wait.
+      bool ok = true;
+      uint32_t it = 0, early = 0;
+      for (int u = blockIdx.x; u < units && early < (uint32_t)S; u += gridDim.x) {
+        int k0, k1;
+        k_range(u % a.splits, k0, k1);
+        for (int k = k0; k < k1 && early < (uint32_t)S; ++k, ++early) {
+          mbar_arrive_expect_tx(&full[early], kBytes);
+          tma_load_2d(ring + (size_t)early * kBytes, &tm_w, &full[early], k * kStep, (u / a.splits) % a.n_tiles * kChannels);
+        }
+      }
+      wait_predecessor();
       for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
         const int tile = u / a.splits;
         const int n0 = (tile % a.n_tiles) * kChannels, m0 = (tile / a.n_tiles) * NT;
         int k0, k1;
         k_range(u % a.splits, k0, k1);
-        int early = 0;  // stages of this unit whose weight part is already under way
-        if (!waited) {
-          early = min(k1 - k0, S);
-          for (int i = 0; i < early; ++i) {
-            mbar_arrive_expect_tx(&full[i], kBytes);
-            tma_load_2d(ring + (size_t)i * kBytes, &tm_w, &full[i], (k0 + i) * kStep, n0);
-          }
-          wait_predecessor();
-          waited = true;
-        }
         for (int k = k0; k < k1; ++k, ++it) {
           const int s = it % S;
           uint8_t* st = ring + (size_t)s * kBytes;
-          if (k - k0 >= early) {
+          if (it >= early) {
             if (it >= (uint32_t)S && !mbar_wait(&empty[s], ((it / S) & 1) ^ 1, kWaitLimit)) {
               ok = false;
               break;
@@ -188,7 +187,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         // the copies still in flight land before the block's shared memory is given up
         for (uint32_t i = it > (uint32_t)S ? it - S : 0; i < it; ++i) mbar_wait(&full[i % S], (i / S) & 1, kWaitLimit);
       }
-      if (!waited) wait_predecessor();
     }
   } else if (warp == 1) {
     if (lane == 0) {
@@ -295,7 +293,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             uint32_t v[CW];
 #pragma unroll
             for (int j = 0; j < CW; ++j) v[j] = 0;
-#pragma unroll 1
+            // the loads of several parts under way together
+#pragma unroll 4
             for (int i = 0; i < a.splits; ++i) {
 #pragma unroll
               for (int j = 0; j < CW; ++j)
@@ -654,8 +653,8 @@ int int8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, 
     float* scale = reinterpret_cast<float*>(p + l.scale);
     if ((st = int8_rows(x, ldx, codes, scale, M, K, dtype, reinterpret_cast<uint32_t*>(p), n_zero, s)) != FLB_OK) return st;
     x_codes = codes, x_scale = scale, ldc = rows::code_pitch(K);
-  } else if ((st = check_cuda(cudaMemsetAsync(p, 0, n_zero * 4, s), "int8_linear reset")) != FLB_OK) {
-    return st;
+  } else if (g.splits > 1 || check_timeout) {  // otherwise nothing reads those words
+    if ((st = check_cuda(cudaMemsetAsync(p, 0, n_zero * 4, s), "int8_linear reset")) != FLB_OK) return st;
   }
   CUtensorMap tw, tx;
   if ((st = code_map(&tw, w_codes, N, ldw, K, g.many ? g.width : kChannels)) != FLB_OK) return st;

@@ -16,6 +16,9 @@ using namespace rows;
 
 namespace {
 
+// Floats between two rows of the workspace: each starts on 16 bytes
+__host__ __device__ inline int part_pitch(int D) { return (D + 3) & ~3; }
+
 struct BwdArgs {
   const void* x;
   int64_t ldx;
@@ -27,7 +30,7 @@ struct BwdArgs {
   const void* dy;
   void* dx;
   void *dw, *db;  // final gradients (one block a group), w's type
-  float* part;    // [G][blocks][2][D] otherwise; null with both dw and db null
+  float* part;    // [G][blocks][2][part_pitch(D)] otherwise
   int64_t R;
   int D;
 };
@@ -203,14 +206,15 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
 
   if (!a.dw && !a.db) return;  // uniform over the grid
   const bool alone = gridDim.x == 1;
-  float* pw = a.part + (group * gridDim.x + blockIdx.x) * 2 * D;
+  const int pitch = part_pitch(D);
+  float* pw = a.part + (group * gridDim.x + blockIdx.x) * 2 * pitch;
   auto out = [&](int p, float vw, float vb) {
     if (alone) {
       store_param<T>(a.dw, a.w32, group * D + p, vw);
       store_param<T>(a.db, a.w32, group * D + p, vb);
     } else {
       pw[p] = vw;
-      pw[D + p] = vb;
+      pw[pitch + p] = vb;
     }
   };
   if constexpr (WARP) {
@@ -251,26 +255,36 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
   }
 }
 
-// dw and db from the blocks' sums: 32 columns a block, a warp for every 32nd workspace row.
+// dw and db from the blocks' sums: 16 columns a block, four a thread, so that a warp reads eight workspace rows
+// at a time and every load of a thread can be under way at once.
 template <typename T>
 __global__ void __launch_bounds__(1024) ln_sum_kernel(const float* __restrict__ part, void* dw, void* db, bool w32,
                                                       int blocks, int D) {
-  __shared__ float s[32][33];
+  __shared__ float s[256][17];
   wait_predecessor();
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int col = blockIdx.x * 32 + tx, which = blockIdx.z;
+  const int tx = threadIdx.x & 3, ty = threadIdx.x >> 2;
+  const int col = blockIdx.x * 16 + tx * 4, which = blockIdx.z, pitch = part_pitch(D);
   const int64_t group = blockIdx.y;
-  float v = 0.f;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   if (col < D) {
-    const float* p = part + (group * blocks * 2 + which) * D + col;
+    const float* p = part + (group * blocks * 2 + which) * pitch + col;
 #pragma unroll 8
-    for (int i = ty; i < blocks; i += 32) v += __ldg(p + (int64_t)i * 2 * D);
+    for (int i = ty; i < blocks; i += 256) {
+      const float4 t = __ldg(reinterpret_cast<const float4*>(p + (int64_t)i * 2 * pitch));
+      v.x += t.x, v.y += t.y, v.z += t.z, v.w += t.w;
+    }
   }
-  s[ty][tx] = v;
+  s[ty][tx * 4] = v.x, s[ty][tx * 4 + 1] = v.y, s[ty][tx * 4 + 2] = v.z, s[ty][tx * 4 + 3] = v.w;
   __syncthreads();
-  v = warp_sum(s[tx][ty]);  // the 32 sums of column ty
-  const int out = blockIdx.x * 32 + ty;
-  if (tx == 0 && out < D) store_param<T>(which ? db : dw, w32, group * D + out, v);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (warp < 16) {
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += s[i * 32 + lane][warp];
+    sum = warp_sum(sum);
+    const int out = blockIdx.x * 16 + warp;
+    if (lane == 0 && out < D) store_param<T>(which ? db : dw, w32, group * D + out, sum);
+  }
 }
 
 // Threads a row, and blocks a group: enough to fill the SMs (512 threads on each), but at least two rows a warp or block, and one block where that leaves it
@@ -317,7 +331,7 @@ int launch_bwd(const BwdArgs& a, int64_t G, cudaStream_t s) {
   count_launches(1);
   cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess && p.blocks > 1 && (a.dw || a.db)) {
-    e = launch_dependent(ln_sum_kernel<T>, dim3((unsigned)((D + 31) / 32), (unsigned)G, 2), dim3(1024), 0, s,
+    e = launch_dependent(ln_sum_kernel<T>, dim3((unsigned)((D + 15) / 16), (unsigned)G, 2), dim3(1024), 0, s,
                          (const float*)a.part, a.dw, a.db, a.w32, (int)p.blocks, D);
     count_launches(1);
   }
@@ -336,7 +350,7 @@ template <typename T> int dispatch_bwd(const BwdArgs& a, int64_t G, cudaStream_t
 
 size_t layer_norm_bwd_workspace_bytes(int64_t G, int64_t R, int64_t D) {
   const BwdShape p = bwd_shape(G, R, D);
-  return p.blocks > 1 ? (size_t)G * p.blocks * 2 * D * sizeof(float) : 0;
+  return p.blocks > 1 ? (size_t)G * p.blocks * 2 * part_pitch((int)D) * sizeof(float) : 0;
 }
 
 int layer_norm_bwd(const void* x, int64_t ldx, const int8_t* codes, const uint8_t* exps, const float* mean,
