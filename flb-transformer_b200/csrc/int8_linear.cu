@@ -10,12 +10,13 @@
 // workspace, and the block that counts itself last adds them up: integers, the same in any order. Bound by
 // reading the weight, of which a ring of 11 stages (NT = 16) keeps 176 KB a SM in flight. Any N and alignment.
 //
-// int8_many_kernel, for tiles enough to fill the SMs. The tokens are the M side, 128 a tile, and 256 or 128
+// int8_many_kernel, for tiles enough to fill the SMs. The tokens are the M side, 128 a block, and 256 or 128
 // channels the N side: a thread of the epilogue has a token's consecutive channels, packs them and leaves
 // them in shared memory for a TMA store. (With the other orientation a thread has one channel of many
-// tokens; pairing them up by shuffles took three times the instructions and bound the kernel: 552 us
-// against XXX for 16384 x 768 x 32000.) Bound by the tensor cores, and by the output's way to memory for
-// small K.
+// tokens; pairing them up by shuffles took three times the instructions and bound the kernel.) For long K two
+// blocks of a cluster share a tile of 256 x 256 (cta_group::2). Bound by the tensor cores: 8192 x 8192 x 8192
+// in 360 us, 3.06 POPS, 1.85 times the bf16 product's measured rate. With small K the output's way to memory
+// takes its share: 16384 x 768 x 32000 in 370 us, 2.18 POPS, of which 160 us would write the output alone.
 #include "rows.cuh"
 #include "sm100.cuh"
 #include "tma_host.cuh"
@@ -31,7 +32,7 @@ constexpr int kStep = 128;       // bytes of K a stage
 constexpr int kRing = 198 * 1024;
 constexpr int kEpilogue = 256;   // threads that read TMEM and store
 constexpr int kGemmThreads = 64 + kEpilogue;
-constexpr uint32_t kWaitLimit = 4000000u;  // polls, each of which the hardware may hold for a while
+constexpr uint32_t kWaitLimit = 1u << 20;  // polls, each of which the hardware may hold for a while
 
 template <int NT> constexpr int stage_bytes() { return (kChannels + NT) * kStep; }
 template <int NT> constexpr int stages() { return kRing / stage_bytes<NT>(); }
@@ -316,57 +317,120 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 
 // ---- many tokens ----------------------------------------------------------------------------------------
 
-constexpr int kTokens = 128;    // a tile's tokens
+constexpr int kTokens = 128;    // a block's tokens of a tile
 constexpr int kStaged = 4096;   // bytes a warp hands to one TMA store: 32 tokens of 128 bytes
-
-template <int NC> constexpr int many_stage_bytes() { return (kTokens + NC) * kStep; }
-template <int NC> constexpr int many_stages() { return NC == 256 ? 3 : 4; }
+template <bool PAIR, int NC> constexpr int many_rows() { return PAIR ? NC / 2 : NC; }  // weight rows a block loads a stage
+template <bool PAIR, int NC> constexpr int many_stage_bytes() { return (kTokens + many_rows<PAIR, NC>()) * kStep; }
+template <bool PAIR, int NC> constexpr int many_stages() { return many_rows<PAIR, NC>() == 256 ? 3 : 4; }
 // ring | two staged tiles a warp | a warp's channel scales and biases
-template <int NC> constexpr int many_smem() {
-  return many_stages<NC>() * many_stage_bytes<NC>() + kEpilogue / 32 * (2 * kStaged + NC / 2 * 8) + 1024;
+template <bool PAIR, int NC> constexpr int many_smem() {
+  return many_stages<PAIR, NC>() * many_stage_bytes<PAIR, NC>() + kEpilogue / 32 * (2 * kStaged + NC / 2 * 8) + 1024;
 }
 
 __device__ __forceinline__ void tma_store_2d(const void* tmap, const void* src, int c0, int c1, uint64_t policy) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group.L2::cache_hint [%0, {%2, %3}], [%1], %4;" ::"l"(tmap),
                "r"(smem_u32(src)), "r"(c0), "r"(c1), "l"(policy)
                : "memory");
-  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
-template <int NC, typename T>
+// Two blocks that work on one tile (PAIR) or one: the instructions that differ.
+template <bool PAIR> struct Group;
+template <> struct Group<false> {
+  static __device__ __forceinline__ void alloc(uint32_t* dst, uint32_t n) { tmem_alloc(dst, n); }
+  static __device__ __forceinline__ void relinquish() { tmem_relinquish(); }
+  static __device__ __forceinline__ void dealloc(uint32_t t, uint32_t n) { tmem_dealloc(t, n); }
+  static __device__ __forceinline__ void load(void* dst, const void* tmap, uint64_t* bar, int c0, int c1) { tma_load_2d(dst, tmap, bar, c0, c1); }
+  static __device__ __forceinline__ void mma(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) { umma_i8(d, da, db, idesc, acc); }
+  static __device__ __forceinline__ void commit(uint64_t* bar) { umma_commit(bar); }
+  static __device__ __forceinline__ void arrive_first(uint64_t* bar) { mbar_arrive(bar); }
+  static __device__ __forceinline__ void meet() { __syncthreads(); }
+};
+template <> struct Group<true> {
+  static __device__ __forceinline__ void alloc(uint32_t* dst, uint32_t n) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(n) : "memory");
+  }
+  static __device__ __forceinline__ void relinquish() { asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory"); }
+  static __device__ __forceinline__ void dealloc(uint32_t t, uint32_t n) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(t), "r"(n) : "memory");
+  }
+  // this barrier in the pair's first block
+  static __device__ __forceinline__ uint32_t first(uint64_t* bar) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(bar)));
+    return r;
+  }
+  // into this block's shared memory; the bytes count at the first block's barrier
+  static __device__ __forceinline__ void load(void* dst, const void* tmap, uint64_t* bar, int c0, int c1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
+            smem_u32(dst)),
+        "l"(tmap), "r"(first(bar)), "r"(c0), "r"(c1)
+        : "memory");
+  }
+  // issued by the first block for both: each block's tokens, the two halves of the channels
+  static __device__ __forceinline__ void mma(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(da), "l"(db), "r"(idesc), "r"(acc)
+        : "memory");
+  }
+  // arrives at this barrier in both blocks
+  static __device__ __forceinline__ void commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+                 "h"((uint16_t)3)
+                 : "memory");
+  }
+  static __device__ __forceinline__ void arrive_first(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(first(bar)) : "memory");
+  }
+  static __device__ __forceinline__ void meet() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+};
+
+// A tile is 128 tokens x NC channels, or with PAIR 256 x NC for two blocks of a cluster: each loads its own tokens
+// and half of the channels' weight rows.
+template <bool PAIR, int NC, typename T>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     int8_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
                      const __grid_constant__ CUtensorMap tm_out, const Int8Args a) {
-  constexpr int S = many_stages<NC>();
-  constexpr uint32_t kBytes = many_stage_bytes<NC>();
+  using G = Group<PAIR>;
+  constexpr int S = many_stages<PAIR, NC>(), BLOCKS = PAIR ? 2 : 1, ROWS = many_rows<PAIR, NC>();
+  constexpr uint32_t kBytes = many_stage_bytes<PAIR, NC>();
   extern __shared__ uint8_t dyn[];
   __shared__ __align__(8) uint64_t full[S], empty[S], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_base;
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int place_in_pair = PAIR ? blockIdx.x & 1 : 0, worker = blockIdx.x / BLOCKS, workers = gridDim.x / BLOCKS;
 
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&tm_w);
     tma_prefetch_desc(&tm_x);
     tma_prefetch_desc(&tm_out);
     for (int i = 0; i < S; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
-    for (int i = 0; i < 2; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], kEpilogue);
+    for (int i = 0; i < 2; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], BLOCKS * kEpilogue / 32);
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc(&tmem_base, 2 * NC);
-    tmem_relinquish();
+    G::alloc(&tmem_base, 2 * NC);
+    G::relinquish();
   }
   tc_fence_before();
-  __syncthreads();
+  __syncwarp();
+  G::meet();
   tc_fence_after();
   const uint32_t tmem = tmem_base;
   const int m_tiles = a.tiles / a.n_tiles;
+  // this block's tokens, and the tile's channels
   auto place = [&](int tile, int& m0, int& n0) {
     // a.group tiles of tokens go through all channels together
     const int g = tile / (a.group * a.n_tiles), in = tile - g * a.group * a.n_tiles;
     const int rows = min(a.group, m_tiles - g * a.group);
-    m0 = (g * a.group + in % rows) * kTokens;
+    m0 = ((g * a.group + in % rows) * BLOCKS + place_in_pair) * kTokens;
     n0 = in / rows * NC;
   };
 
@@ -375,9 +439,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       bool ok = true;
       uint32_t it = 0;
       wait_predecessor();
-      for (int tile = blockIdx.x; tile < a.tiles && ok; tile += gridDim.x) {
+      for (int tile = worker; tile < a.tiles && ok; tile += workers) {
         int m0, n0;
         place(tile, m0, n0);
+        if (PAIR) n0 += place_in_pair * ROWS;
         for (int k = 0; k < a.k_blocks; ++k, ++it) {
           const int s = it % S;
           if (it >= (uint32_t)S && !mbar_wait(&empty[s], ((it / S) & 1) ^ 1, kWaitLimit)) {
@@ -385,23 +450,31 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             break;
           }
           uint8_t* st = ring + (size_t)s * kBytes;
-          mbar_arrive_expect_tx(&full[s], kBytes);
-          tma_load_2d(st, &tm_x, &full[s], k * kStep, m0);
-          tma_load_2d(st + kTokens * kStep, &tm_w, &full[s], k * kStep, n0);
+          // the first block expects both blocks' bytes (the other's may land before: the count goes below zero)
+          if (place_in_pair == 0) mbar_arrive_expect_tx(&full[s], BLOCKS * kBytes);
+          G::load(st, &tm_x, &full[s], k * kStep, m0);
+          G::load(st + kTokens * kStep, &tm_w, &full[s], k * kStep, n0);
         }
       }
+      const uint32_t last = it > (uint32_t)S ? it - S : 0;
       if (!ok) {
         atomicExch(a.error, 1u);
-        // the copies still in flight land before the block's shared memory is given up
-        for (uint32_t i = it > (uint32_t)S ? it - S : 0; i < it; ++i) mbar_wait(&full[i % S], (i / S) & 1, kWaitLimit);
+        // the copies still in flight land before the blocks' shared memory is given up: the other block
+        // waits for this one below
+        if (place_in_pair == 0)
+          for (uint32_t i = last; i < it; ++i) mbar_wait(&full[i % S], (i / S) & 1, kWaitLimit);
+      } else if (PAIR) {
+        // the first block's arrivals at this block's barriers are all in before the block ends
+        for (uint32_t i = last; i < it; ++i)
+          if (!mbar_wait(&empty[i % S], (i / S) & 1, kWaitLimit)) atomicExch(a.error, 1u);
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = idesc_i8<NC>();
+    if (lane == 0 && place_in_pair == 0) {
+      constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(NC >> 3) << 17) | ((uint32_t)(BLOCKS * kTokens >> 4) << 24);
       uint32_t it = 0, local = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < a.tiles && ok; tile += gridDim.x, ++local) {
+      for (int tile = worker; tile < a.tiles && ok; tile += workers, ++local) {
         const uint32_t b = local & 1;
         if (local >= 2 && !mbar_wait(&acc_empty[b], ((local >> 1) & 1) ^ 1, kWaitLimit)) {
           ok = false;
@@ -419,26 +492,27 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           uint64_t da = make_smem_desc(at, 16, 1024, kSwizzle128B);
           uint64_t db = make_smem_desc(at + kTokens * kStep, 16, 1024, kSwizzle128B);
 #pragma unroll
-          for (int i = 0; i < kStep / 32; ++i, da += 2, db += 2) umma_i8(tmem + b * NC, da, db, idesc, (k > 0 || i > 0) ? 1u : 0u);
-          umma_commit(&empty[s]);
+          for (int i = 0; i < kStep / 32; ++i, da += 2, db += 2) G::mma(tmem + b * NC, da, db, idesc, (k > 0 || i > 0) ? 1u : 0u);
+          G::commit(&empty[s]);
         }
-        if (ok) umma_commit(&acc_full[b]);
+        if (ok) G::commit(&acc_full[b]);
       }
       if (!ok) atomicExch(a.error, 1u);
     }
   } else {
-    // a warp has the 32 TMEM lanes, here tokens, of its number mod 4, and half of the channels
+    // a warp has the 32 TMEM lanes, here tokens, of its number mod 4, and half of the channels. (16 warps with a quarter
+    // each and one staged tile took 423 us instead of 369 for 16384 x 768 x 32000.)
     constexpr int COLS = NC / 2, STEPS = COLS / 32, kWords = 32 * (int)sizeof(T) / 16;  // 16-byte words a lane stages a step
     const int q = warp & 3, first = (warp - 2) / 4 * COLS;
-    uint8_t* mine = ring + (size_t)S * kBytes + (size_t)(warp - 2) * (2 * kStaged);
-    float* sw = reinterpret_cast<float*>(ring + (size_t)S * kBytes + (size_t)(kEpilogue / 32) * (2 * kStaged)) + (warp - 2) * 2 * COLS;
-    float* sb = sw + COLS;
+    uint8_t* const mine = ring + (size_t)S * kBytes + (size_t)(warp - 2) * (2 * kStaged);
+    float* const sw = reinterpret_cast<float*>(ring + (size_t)S * kBytes + (size_t)(kEpilogue / 32) * (2 * kStaged)) + (warp - 2) * 2 * COLS;
+    float* const sb = sw + COLS;
     uint32_t local = 0, limit = kWaitLimit, stores = 0;
     uint64_t policy;
     if (a.stream_out) asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
     else asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
     wait_predecessor();
-    for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ++local) {
+    for (int tile = worker; tile < a.tiles; tile += workers, ++local) {
       const uint32_t b = local & 1;
       int m0, n0;
       place(tile, m0, n0);
@@ -471,11 +545,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           tmem_ld32(acc + (i + 1) * 32, v[(i + 1) & 1]);
         } else {
           tc_fence_before();
-          mbar_arrive(&acc_empty[b]);
+          __syncwarp();
+          if (lane == 0) G::arrive_first(&acc_empty[b]);
         }
         // the staged tile of 32 tokens x 128 bytes is full after one step of float32, two of 16-bit types
         constexpr int kPer = 128 / (kWords * 16);
-        uint8_t* tile_at = mine + (stores & 1) * kStaged;
+        uint8_t* const staged = mine + (stores & 1) * kStaged;
         if (i % kPer == 0) {
           // the store before the last one has read its bytes
           if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
@@ -499,7 +574,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
 #pragma unroll
         for (int j = 0; j < kWords; ++j)
-          *reinterpret_cast<uint4*>(tile_at + sw128_offset(lane, (i % kPer) * kWords + j)) =
+          *reinterpret_cast<uint4*>(staged + sw128_offset(lane, (i % kPer) * kWords + j)) =
               make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
         if (i % kPer == kPer - 1) {
           fence_async_shared();
@@ -507,8 +582,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           // a store that starts outside the output is left out; one that ends outside is cut there
           if (lane == 0) {
             const int c = n0 + (i / kPer) * kPer * 32;
-            if (c < a.N && m0 + q * 32 < a.M) tma_store_2d(&tm_out, tile_at, c, m0 + q * 32, policy);
-            else asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            if (c < a.N && m0 + q * 32 < a.M) tma_store_2d(&tm_out, staged, c, m0 + q * 32, policy);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
           ++stores;
         }
@@ -517,10 +592,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   tc_fence_before();
-  __syncthreads();
+  __syncwarp();
+  G::meet();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 2 * NC);
+    G::dealloc(tmem, 2 * NC);
   }
 }
 
@@ -533,21 +609,26 @@ constexpr size_t kOutputInL2 = 64 << 20;
 
 // Which kernel, its tile's other side (NT or NC), and parts of a tile's K range.
 struct GemmShape {
-  bool many;
+  bool many, pair = false;
   int width, n_tiles, tiles, splits;
 };
 GemmShape gemm_shape(int64_t M, int64_t N, int64_t K, bool rows_on_16) {
   GemmShape g;
   const int64_t sms = num_sms(), m_tiles = (M + kTokens - 1) / kTokens;
   auto tiles = [&](int nc) { return m_tiles * ((N + nc - 1) / nc); };
-  // The kernel for many tokens where its smaller tiles fill the SMs once over and its stores can be made; of its two
-  // widths the one whose rounds of tiles over the SMs cost least, a K step of a tile costing the rows it loads.
+  // The kernel for many tokens where its smaller tiles fill the SMs once over and its stores can be made.
   g.many = rows_on_16 && M > 64 && tiles(128) >= sms;
   if (g.many) {
+    // Pairs of blocks load a third less for each product, but start later and hand over tiles between them: for more
+    // tiles than SMs with K of 1024 on (8192 x 1024 x 8192: 58 us against 62, 8192 x 4096 x 4096: 94 against 105;
+    // 8192 x 768 x 8192: 56 against 50, 1000 x 4096 x 4096: 20.5 against 19.2).
+    g.pair = sms % 2 == 0 && K >= 1024 && tiles(256) > sms;
+    // Of a block's own tiles those whose rounds over the SMs cost least, a K step of a tile costing the rows that it
+    // loads (2931 x 768 x 2304: 12.4 us with 256 channels, 14.1 with 128; 300 x 4096 x 4096: 18.5 and 17.8).
     auto cost = [&](int nc) { return (tiles(nc) + sms - 1) / sms * (kTokens + nc); };
-    g.width = cost(256) <= cost(128) ? 256 : 128;
+    g.width = g.pair || cost(256) <= cost(128) ? 256 : 128;
     g.n_tiles = (int)((N + g.width - 1) / g.width);
-    g.tiles = (int)tiles(g.width);
+    g.tiles = (int)(g.pair ? (M + 255) / 256 * g.n_tiles : tiles(g.width));
     g.splits = 1;
     return g;
   }
@@ -579,25 +660,43 @@ GemmWs gemm_ws(const GemmShape& g, int64_t M, int64_t K, bool quantise) {
   return w;
 }
 
+// blocks: of a cluster that shares a tile. after_rows: the kernel may start while the one before it, which makes the
+// tokens' rows, drains.
 template <typename... K, typename... A>
-int launch(void (*k)(K...), int smem, const Int8Args& a, bool after_rows, cudaStream_t s, const A&... args) {
+int launch(void (*k)(K...), int blocks, int smem, const Int8Args& a, bool after_rows, cudaStream_t s, const A&... args) {
   int st = ensure_dyn_smem(reinterpret_cast<const void*>(k), smem, "int8_linear shared memory");
   if (st != FLB_OK) return st;
-  const dim3 grid((unsigned)std::min<int64_t>((int64_t)a.tiles * a.splits, num_sms()));
-  cudaError_t e;
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)std::min<int64_t>((int64_t)a.tiles * a.splits * blocks, num_sms() / blocks * blocks));
+  cfg.blockDim = dim3(kGemmThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
   if (after_rows) {
-    e = launch_dependent(k, grid, dim3(kGemmThreads), smem, s, args..., a);
-  } else {
-    k<<<grid, kGemmThreads, smem, s>>>(args..., a);
-    e = cudaGetLastError();
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
   }
+  if (blocks > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = blocks;
+    attr[cfg.numAttrs].val.clusterDim.y = 1;
+    attr[cfg.numAttrs++].val.clusterDim.z = 1;
+  }
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, k, args..., a);
   count_launches(1);
   return check_cuda(e, "int8_linear launch");
 }
 
 template <int NT, typename T>
 int launch_few(const CUtensorMap& tw, const CUtensorMap& tx, const Int8Args& a, bool after_rows, cudaStream_t s) {
-  return launch(int8_few_kernel<NT, T>, stages<NT>() * stage_bytes<NT>() + 1024, a, after_rows, s, tw, tx);
+  return launch(int8_few_kernel<NT, T>, 1, stages<NT>() * stage_bytes<NT>() + 1024, a, after_rows, s, tw, tx);
+}
+
+template <bool PAIR, int NC, typename T>
+int launch_many(const CUtensorMap& tw, const CUtensorMap& tx, const CUtensorMap& to, const Int8Args& a, bool after_rows, cudaStream_t s) {
+  return launch(int8_many_kernel<PAIR, NC, T>, PAIR ? 2 : 1, many_smem<PAIR, NC>(), a, after_rows, s, tw,
+                tx, to);
 }
 
 template <typename T>
@@ -611,8 +710,9 @@ int launch_t(const GemmShape& g, const CUtensorMap& tw, const CUtensorMap& tx, c
                                    : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     const int st = make_tmap(&to, a.out, dt, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (st != FLB_OK) return st;
-    if (g.width == 256) return launch(int8_many_kernel<256, T>, many_smem<256>(), a, after_rows, s, tw, tx, to);
-    return launch(int8_many_kernel<128, T>, many_smem<128>(), a, after_rows, s, tw, tx, to);
+    if (g.pair) return launch_many<true, 256, T>(tw, tx, to, a, after_rows, s);
+    if (g.width == 256) return launch_many<false, 256, T>(tw, tx, to, a, after_rows, s);
+    return launch_many<false, 128, T>(tw, tx, to, a, after_rows, s);
   }
   switch (g.width) {
     case 16: return launch_few<16, T>(tw, tx, a, after_rows, s);
@@ -657,7 +757,7 @@ int int8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, 
     if ((st = check_cuda(cudaMemsetAsync(p, 0, n_zero * 4, s), "int8_linear reset")) != FLB_OK) return st;
   }
   CUtensorMap tw, tx;
-  if ((st = code_map(&tw, w_codes, N, ldw, K, g.many ? g.width : kChannels)) != FLB_OK) return st;
+  if ((st = code_map(&tw, w_codes, N, ldw, K, g.many ? (g.pair ? g.width / 2 : g.width) : kChannels)) != FLB_OK) return st;
   if ((st = code_map(&tx, x_codes, M, ldc, K, g.many ? kTokens : g.width)) != FLB_OK) return st;
   const Int8Args a{x_scale, w_scale, bias, bias_dtype == FLB_F32, out, M, N,
                    N % 2 == 0 && reinterpret_cast<uintptr_t>(out) % 4 == 0, (int)((K + kStep - 1) / kStep), g.n_tiles, g.tiles,

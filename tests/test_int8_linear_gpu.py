@@ -39,11 +39,14 @@ def test_rows_exact(K, dtype):
 
 
 # tokens around the tiles' widths (16 to 256), one or two short of and over them; outputs around a tile's 128
-# channels and odd ones; K around a step's 128 and where it is split between blocks
+# channels and odd ones; K around a step's 128 and where it is split between blocks; outputs whose rows do not start on
+# 16 bytes
 SHAPES = [(1, 768, 32000), (1, 1, 1), (2, 16, 8), (15, 128, 128), (16, 4096, 4096), (17, 129, 130), (31, 1001, 257), (32, 256, 127),
           (33, 33, 129), (63, 768, 2304), (64, 16384, 64), (65, 640, 1000), (127, 2048, 384), (128, 100, 129), (129, 768, 513),
           (200, 8192, 100), (255, 768, 2304), (257, 384, 4097), (300, 1024, 16), (700, 512, 1280), (2931, 768, 2304), (5000, 64, 640),
-          (3, 32768, 40)]
+          (3, 32768, 40),
+          # two blocks a tile: a last tile with few tokens, or none, for its second block, and channels for one of them
+          (2690, 1024, 4360), (2600, 1056, 4104), (5120, 1100, 2048)]
 
 
 @pytest.mark.parametrize("M,K,N", SHAPES)
