@@ -45,6 +45,7 @@ struct Int8Args {
   void* out;          // [M, N]
   int64_t M, N;
   bool pairs;         // 16-bit outputs two channels at a time
+  bool early;         // the kernel before this one wrote no weight
   int k_blocks;       // of kStep
   int n_tiles, tiles, splits;
   int group;          // many tokens: tiles of tokens that go through all channels together
@@ -151,11 +152,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      // The weight was written before the kernel that this one may overlap started; the tokens' codes by that
-      // kernel, so a first ring of weight tiles, of the first units' steps, is on its way before the wait.
+      // Where the kernel that this one may overlap is the one that makes the tokens' codes here, the weight was
+      // written before that kernel started: a first ring of weight tiles, of the first units' steps, is on
+      // its way before the wait.
       bool ok = true;
       uint32_t it = 0, early = 0;
-      for (int u = blockIdx.x; u < units && early < (uint32_t)S; u += gridDim.x) {
+      for (int u = blockIdx.x; a.early && u < units && early < (uint32_t)S; u += gridDim.x) {
         int k0, k1;
         k_range(u % a.splits, k0, k1);
         for (int k = k0; k < k1 && early < (uint32_t)S; ++k, ++early) {
@@ -660,10 +662,9 @@ GemmWs gemm_ws(const GemmShape& g, int64_t M, int64_t K, bool quantise) {
   return w;
 }
 
-// blocks: of a cluster that shares a tile. after_rows: the kernel may start while the one before it, which makes the
-// tokens' rows, drains.
+// blocks: of a cluster that shares a tile. overlap: the kernel may start while the one before it drains.
 template <typename... K, typename... A>
-int launch(void (*k)(K...), int blocks, int smem, const Int8Args& a, bool after_rows, cudaStream_t s, const A&... args) {
+int launch(void (*k)(K...), int blocks, int smem, const Int8Args& a, bool overlap, cudaStream_t s, const A&... args) {
   int st = ensure_dyn_smem(reinterpret_cast<const void*>(k), smem, "int8_linear shared memory");
   if (st != FLB_OK) return st;
   cudaLaunchAttribute attr[2];
@@ -673,7 +674,7 @@ int launch(void (*k)(K...), int blocks, int smem, const Int8Args& a, bool after_
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cfg.attrs = attr;
-  if (after_rows) {
+  if (overlap) {
     attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
   }
@@ -689,18 +690,18 @@ int launch(void (*k)(K...), int blocks, int smem, const Int8Args& a, bool after_
 }
 
 template <int NT, typename T>
-int launch_few(const CUtensorMap& tw, const CUtensorMap& tx, const Int8Args& a, bool after_rows, cudaStream_t s) {
-  return launch(int8_few_kernel<NT, T>, 1, stages<NT>() * stage_bytes<NT>() + 1024, a, after_rows, s, tw, tx);
+int launch_few(const CUtensorMap& tw, const CUtensorMap& tx, const Int8Args& a, bool overlap, cudaStream_t s) {
+  return launch(int8_few_kernel<NT, T>, 1, stages<NT>() * stage_bytes<NT>() + 1024, a, overlap, s, tw, tx);
 }
 
 template <bool PAIR, int NC, typename T>
-int launch_many(const CUtensorMap& tw, const CUtensorMap& tx, const CUtensorMap& to, const Int8Args& a, bool after_rows, cudaStream_t s) {
-  return launch(int8_many_kernel<PAIR, NC, T>, PAIR ? 2 : 1, many_smem<PAIR, NC>(), a, after_rows, s, tw,
+int launch_many(const CUtensorMap& tw, const CUtensorMap& tx, const CUtensorMap& to, const Int8Args& a, bool overlap, cudaStream_t s) {
+  return launch(int8_many_kernel<PAIR, NC, T>, PAIR ? 2 : 1, many_smem<PAIR, NC>(), a, overlap, s, tw,
                 tx, to);
 }
 
 template <typename T>
-int launch_t(const GemmShape& g, const CUtensorMap& tw, const CUtensorMap& tx, const Int8Args& a, bool after_rows, cudaStream_t s) {
+int launch_t(const GemmShape& g, const CUtensorMap& tw, const CUtensorMap& tx, const Int8Args& a, bool overlap, cudaStream_t s) {
   if (g.many) {
     CUtensorMap to;
     const uint64_t dims[2] = {(uint64_t)a.N, (uint64_t)a.M};
@@ -710,15 +711,15 @@ int launch_t(const GemmShape& g, const CUtensorMap& tw, const CUtensorMap& tx, c
                                    : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     const int st = make_tmap(&to, a.out, dt, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (st != FLB_OK) return st;
-    if (g.pair) return launch_many<true, 256, T>(tw, tx, to, a, after_rows, s);
-    if (g.width == 256) return launch_many<false, 256, T>(tw, tx, to, a, after_rows, s);
-    return launch_many<false, 128, T>(tw, tx, to, a, after_rows, s);
+    if (g.pair) return launch_many<true, 256, T>(tw, tx, to, a, overlap, s);
+    if (g.width == 256) return launch_many<false, 256, T>(tw, tx, to, a, overlap, s);
+    return launch_many<false, 128, T>(tw, tx, to, a, overlap, s);
   }
   switch (g.width) {
-    case 16: return launch_few<16, T>(tw, tx, a, after_rows, s);
-    case 32: return launch_few<32, T>(tw, tx, a, after_rows, s);
-    case 64: return launch_few<64, T>(tw, tx, a, after_rows, s);
-    default: return launch_few<128, T>(tw, tx, a, after_rows, s);
+    case 16: return launch_few<16, T>(tw, tx, a, overlap, s);
+    case 32: return launch_few<32, T>(tw, tx, a, overlap, s);
+    case 64: return launch_few<64, T>(tw, tx, a, overlap, s);
+    default: return launch_few<128, T>(tw, tx, a, overlap, s);
   }
 }
 
@@ -746,6 +747,7 @@ int int8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, 
   const GemmWs l = gemm_ws(g, M, K, x != nullptr);
   uint8_t* p = reinterpret_cast<uint8_t*>(ws);
   const int64_t n_zero = 1 + (g.splits > 1 ? g.tiles : 0);
+  const bool reset = !x && (g.splits > 1 || check_timeout);
   int st;
   if (x) {
     // the rows' kernel clears the error word and the counts too
@@ -753,20 +755,20 @@ int int8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, 
     float* scale = reinterpret_cast<float*>(p + l.scale);
     if ((st = int8_rows(x, ldx, codes, scale, M, K, dtype, reinterpret_cast<uint32_t*>(p), n_zero, s)) != FLB_OK) return st;
     x_codes = codes, x_scale = scale, ldc = rows::code_pitch(K);
-  } else if (g.splits > 1 || check_timeout) {  // otherwise nothing reads those words
+  } else if (reset) {  // otherwise nothing reads those words
     if ((st = check_cuda(cudaMemsetAsync(p, 0, n_zero * 4, s), "int8_linear reset")) != FLB_OK) return st;
   }
   CUtensorMap tw, tx;
   if ((st = code_map(&tw, w_codes, N, ldw, K, g.many ? (g.pair ? g.width / 2 : g.width) : kChannels)) != FLB_OK) return st;
   if ((st = code_map(&tx, x_codes, M, ldc, K, g.many ? kTokens : g.width)) != FLB_OK) return st;
   const Int8Args a{x_scale, w_scale, bias, bias_dtype == FLB_F32, out, M, N,
-                   N % 2 == 0 && reinterpret_cast<uintptr_t>(out) % 4 == 0, (int)((K + kStep - 1) / kStep), g.n_tiles, g.tiles,
+                   N % 2 == 0 && reinterpret_cast<uintptr_t>(out) % 4 == 0, x != nullptr, (int)((K + kStep - 1) / kStep), g.n_tiles, g.tiles,
                    g.splits, N * K <= kWeightInL2 ? 1 : 16, (size_t)M * N * dtype_size(dtype) > kOutputInL2, reinterpret_cast<int32_t*>(p + l.parts), reinterpret_cast<uint32_t*>(p + l.counts),
                    reinterpret_cast<uint32_t*>(p)};
   switch (dtype) {
-    case FLB_F32: st = launch_t<float>(g, tw, tx, a, x != nullptr, s); break;
-    case FLB_F16: st = launch_t<__half>(g, tw, tx, a, x != nullptr, s); break;
-    default: st = launch_t<__nv_bfloat16>(g, tw, tx, a, x != nullptr, s); break;
+    case FLB_F32: st = launch_t<float>(g, tw, tx, a, !reset, s); break;
+    case FLB_F16: st = launch_t<__half>(g, tw, tx, a, !reset, s); break;
+    default: st = launch_t<__nv_bfloat16>(g, tw, tx, a, !reset, s); break;
   }
   if (st != FLB_OK || !check_timeout) return st;
   uint32_t err = 0;

@@ -75,8 +75,8 @@ __global__ void __launch_bounds__(kMostThreads<MODE>, 1024 / kMostThreads<MODE>)
   extern __shared__ __align__(16) uint8_t dyn[];
   __shared__ __align__(16) float slot[WARP ? 1 : 2][3][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if constexpr (OUT == OUT_INT8) let_successor_start();  // the product that reads the rows
   if constexpr (!NORM) {
-    let_successor_start();
     if (blockIdx.x == 0)
       for (int64_t i = threadIdx.x; i < a.n_zero; i += blockDim.x) a.zero[i] = 0;
   }
