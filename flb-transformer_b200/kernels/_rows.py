@@ -6,6 +6,12 @@ import torch
 transforms_active = torch._C._are_functorch_transforms_active
 
 
+def no_transforms(what: str) -> None:
+    """Refuses torch.func transforms where an operator has no rule for them."""
+    if transforms_active():
+        raise RuntimeError(f"{what} is not supported under torch.func transforms")
+
+
 def plain(t):
     """The tensor inside torch.func's gradient wrappers. A batched one is refused: its storage holds
     every sample of a vmap that the caller's formula knows nothing of."""

@@ -22,6 +22,7 @@ import torch.nn as nn
 
 import flb_native  # noqa: F401  (loads libflb_b200.so, or says that it is missing)
 import flb_ops
+from ._rows import no_transforms
 
 __all__ = ["Int8Rows", "quantize_int8", "int8_linear", "Int8Linear"]
 
@@ -42,18 +43,21 @@ class Int8Rows(NamedTuple):
 def quantize_int8(x: torch.Tensor) -> Int8Rows:
     """x [..., K] (float32, float16 or bfloat16) with each row of its last axis in 8-bit integers: a token's
     features, or (x a weight [out, in]) an output channel's."""
+    no_transforms("quantize_int8")
     return Int8Rows(*flb_ops.quantize_int8(x), x.dtype)
 
 
 def int8_linear(x: torch.Tensor | Int8Rows, weight: Int8Rows, bias: torch.Tensor | None = None) -> torch.Tensor:
     """x [..., K] times weight [N, K] (an Int8Rows), plus bias [N] (float32 or x's type): [..., N] in x's type."""
+    no_transforms("int8_linear")
     if isinstance(x, Int8Rows):
         return flb_ops.int8_linear(None, x.codes, x.scale, weight.codes, weight.scale, bias, x.dtype)
     return flb_ops.int8_linear(x, None, None, weight.codes, weight.scale, bias, None)
 
 
 class Int8Linear(nn.Module):
-    """A linear map whose weight is kept in 8-bit integers (buffers `codes` and `scale`)."""
+    """A linear map whose weight is kept in 8-bit integers (buffers `codes` and `scale`). For inference: its output
+    has no gradient."""
 
     def __init__(self, weight: Int8Rows, bias: torch.Tensor | None = None):
         super().__init__()

@@ -21,7 +21,7 @@ from torch.autograd.function import once_differentiable
 
 import flb_native  # noqa: F401  (loads libflb_b200.so, or says that it is missing)
 import flb_ops
-from ._rows import plain, to_front, transforms_active
+from ._rows import no_transforms, plain, to_front, transforms_active
 
 __all__ = ["Packed8", "pack8", "unpack8", "sigmoid_gate"]
 
@@ -37,11 +37,13 @@ class Packed8(NamedTuple):
 def pack8(x: torch.Tensor) -> Packed8:
     """The kept form of x (float32, float16 or bfloat16, any shape with at least one axis). Not
     differentiable: it is what an operator's forward keeps for its backward."""
+    no_transforms("pack8")
     return Packed8(*flb_ops.pack8(x.detach()), x.shape, x.dtype)
 
 
 def unpack8(p: Packed8, dtype: torch.dtype | None = None) -> torch.Tensor:
     """The tensor that p stands for, in its own type or `dtype` (float16 saturates)."""
+    no_transforms("unpack8")
     return flb_ops.unpack8(p.codes, p.exps, list(p.shape), dtype or p.dtype)
 
 

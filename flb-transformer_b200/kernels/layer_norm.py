@@ -23,7 +23,7 @@ from torch.autograd.function import once_differentiable
 
 import flb_native  # noqa: F401  (loads libflb_b200.so, or says that it is missing)
 import flb_ops
-from ._rows import plain, to_front, transforms_active
+from ._rows import no_transforms, plain, to_front, transforms_active
 from .int8_linear import Int8Rows
 
 __all__ = ["layer_norm", "layer_norm_int8", "FusedLayerNorm"]
@@ -79,6 +79,7 @@ def layer_norm_int8(x: torch.Tensor, weight: torch.Tensor | None = None, bias: t
                     eps: float = 1e-5) -> Int8Rows:
     """The rows of layer_norm's output, before their rounding to x's type, as 8-bit integers: the input that
     int8_linear reads, in one pass over x. No gradient."""
+    no_transforms("layer_norm_int8")
     return Int8Rows(*flb_ops.layer_norm_int8(x, weight, bias, eps), x.dtype)
 
 

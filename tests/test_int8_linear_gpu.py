@@ -46,7 +46,9 @@ SHAPES = [(1, 768, 32000), (1, 1, 1), (2, 16, 8), (15, 128, 128), (16, 4096, 409
           (200, 8192, 100), (255, 768, 2304), (257, 384, 4097), (300, 1024, 16), (700, 512, 1280), (2931, 768, 2304), (5000, 64, 640),
           (3, 32768, 40),
           # two blocks a tile: a last tile with few tokens, or none, for its second block, and channels for one of them
-          (2690, 1024, 4360), (2600, 1056, 4104), (5120, 1100, 2048)]
+          (2690, 1024, 4360), (2600, 1056, 4104), (5120, 1100, 2048),
+          # fewer tokens than a tile and many channels; a weight larger than L2 keeps, tokens in two groups of tiles
+          (100, 256, 19000), (2300, 32768, 1544)]
 
 
 @pytest.mark.parametrize("M,K,N", SHAPES)
@@ -197,6 +199,31 @@ def test_error_word():
         nat.check(nat.lib.flb_int8_linear(x.data_ptr(), 640, None, 0, None, w.codes.data_ptr(), 640, w.scale.data_ptr(), None, 0,
                                           out.data_ptr(), M, 300, 640, nat.BF16, ws.data_ptr(), n, 1, nat.stream_of(x)), "int8")
         assert torch.equal(out, kernels.int8_linear(x, w))
+
+
+def test_refusals():
+    import kernels
+    x = torch.zeros(4, 32, device="cuda")
+    w = kernels.quantize_int8(torch.ones(8, 32, device="cuda"))
+    for bad in (kernels.Int8Rows(w.codes[:, :16], w.scale), kernels.Int8Rows(w.codes, w.scale[:4]), kernels.Int8Rows(w.codes[0], w.scale[0]),
+                kernels.Int8Rows(w.codes[None], w.scale[None])):
+        with pytest.raises(ValueError):
+            kernels.int8_linear(x, bad)
+    for bad in (kernels.Int8Rows(w.codes.short(), w.scale), kernels.Int8Rows(w.codes, w.scale.double())):
+        with pytest.raises(TypeError):
+            kernels.int8_linear(x, bad)
+    with pytest.raises(ValueError):
+        kernels.int8_linear(x, w, torch.zeros(7, device="cuda"))
+    with pytest.raises(TypeError):
+        kernels.int8_linear(x, w, torch.zeros(8, device="cuda", dtype=BF))
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        kernels.int8_linear(x, kernels.Int8Rows(w.codes.cpu(), w.scale.cpu()))
+    with pytest.raises(TypeError):
+        kernels.quantize_int8(x.double())
+    with pytest.raises(ValueError):
+        kernels.quantize_int8(x[:, :0])
+    with pytest.raises(RuntimeError, match="UNSUPPORTED"):
+        kernels.quantize_int8(torch.zeros(1, 32769, device="cuda"))
 
 
 def test_module_and_gradients():

@@ -86,6 +86,45 @@ def test_kept_arguments():
     assert L.flb_gate_bwd(None, None, None, None, None, None, None, None, None, 0, 8, F16, None) == 0
 
 
+def int8(x=16, ldx=64, xc=None, ldc=0, xs=None, wc=16, ldw=64, ws=16, bias=None, bdt=F32, out=16, M=4, N=8, K=64, dt=BF16, work=256,
+         n=1 << 30):
+    import flb_native as nat
+    return nat.lib.flb_int8_linear(x, ldx, xc, ldc, xs, wc, ldw, ws, bias, bdt, out, M, N, K, dt, work, n, 0, None)
+
+
+def test_int8_arguments():
+    """Every refusal comes before any device work."""
+    import flb_native as nat
+    L = nat.lib
+    assert int8(dt=9) == FLB_DTYPE and int8(bias=16, bdt=F16) == FLB_DTYPE
+    assert int8(M=-1) == FLB_SHAPE and int8(N=-1) == FLB_SHAPE and int8(K=0) == FLB_SHAPE and int8(K=32769) == FLB_UNSUPPORTED
+    assert int8(M=2 ** 31) == FLB_SHAPE and int8(M=2 ** 30, N=2 ** 30) == FLB_SHAPE
+    assert int8(x=None) == FLB_SHAPE and int8(xc=16, xs=16, ldc=64) == FLB_SHAPE and int8(x=None, xc=16) == FLB_SHAPE
+    assert int8(wc=None) == FLB_SHAPE and int8(ws=None) == FLB_SHAPE and int8(out=None) == FLB_SHAPE
+    assert int8(ldx=-1) == FLB_SHAPE and int8(ldw=48) == FLB_SHAPE and int8(x=None, xc=16, xs=16, ldc=48) == FLB_SHAPE
+    assert int8(ldw=72) == FLB_ALIGN and int8(wc=8) == FLB_ALIGN and int8(x=None, xc=24, xs=16, ldc=64) == FLB_ALIGN
+    assert int8(x=17) == FLB_ALIGN and int8(out=17) == FLB_ALIGN and int8(ws=18) == FLB_ALIGN
+    assert int8(work=None) == FLB_WORKSPACE and int8(n=16) == FLB_WORKSPACE and int8(work=128) == FLB_ALIGN
+    assert int8(M=0, x=None, out=None) == 0 and int8(N=0, wc=None, ws=None) == 0
+    assert L.flb_int8_linear_workspace_bytes(4, 8, 64, 0) > L.flb_int8_linear_workspace_bytes(4, 8, 64, 1) > 0
+    assert L.flb_int8_linear_workspace_bytes(0, 8, 64, 0) == 0 and L.flb_int8_linear_workspace_bytes(4, 8, 0, 0) == 0
+    assert L.flb_int8_rows(16, 8, 16, 16, 2, 8, 5, None) == FLB_DTYPE and L.flb_int8_rows(16, 8, 24, 16, 2, 8, F32, None) == FLB_ALIGN
+    assert L.flb_int8_rows(None, 8, 16, 16, 2, 8, F32, None) == FLB_SHAPE and L.flb_int8_rows(None, 8, None, None, 0, 8, F32, None) == 0
+    assert L.flb_layer_norm_int8(16, 8, 16, None, F16, 16, 16, 1, 2, 8, BF16, 1e-5, None) == FLB_DTYPE
+    assert L.flb_layer_norm_int8(16, 8, None, None, F32, None, 16, 1, 2, 8, BF16, 1e-5, None) == FLB_SHAPE
+
+
+def test_kept_training_arguments():
+    import flb_native as nat
+    L = nat.lib
+    assert L.flb_block_grid_saved8_bytes(0, 4, 2, 64) == 0
+    b16, b8 = L.flb_block_grid_saved_bytes(4, 6, 3, 128), L.flb_block_grid_saved8_bytes(4, 6, 3, 128)
+    assert b8 <= 4 * 6 * 3 * 18 * 129 + 256 and b16 == 4 * 6 * 3 * 36 * 128 * 2
+    assert L.flb_block_grid_fwd_save8(None, 16, 16, 4, 6, 3, 64, 8, 1e-5, 16, 1 << 30, 16, 1 << 30, None) == FLB_SHAPE
+    assert L.flb_block_grid_bwd_saved8(None, 16, 16, None, None, None, None, 16, 16, 4, 6, 3, 64, 8, 1e-5, 16, 1 << 30, 16, 1 << 30,
+                                       None) == FLB_SHAPE
+
+
 def test_rows_of_views():
     """Which views the kernels take as they are, and which are copied."""
     from flb_ops import rows_of as as_rows

@@ -362,6 +362,98 @@ def test_streams_graphs_and_memory():
     assert kept <= big.numel() * (1 + 1 / 128) + 4096 * 4 + 4096, kept
 
 
+@pytest.mark.parametrize("offset", [30.0, 3000.0])
+def test_norm_far_from_zero(offset):
+    """Rows whose offset is many times their spread: the bounds grow with the offset, as the mean's rounding does."""
+    import kernels
+    for D in (200, 1001, 4096):
+        x, (w, b), dy = rows_of((33, D), F, 1, offset=offset), params((D,), F, 2), rows_of((33, D), F, 3)
+        y, tol, back = orc.layer_norm(x, w, b, 1e-5, F)
+        xs, ws, bs, dys = cuda(x, w, b, dy)
+        for t in (xs, ws, bs):
+            t.requires_grad_(True)
+        got = kernels.layer_norm(xs, ws, bs)
+        close(got, y, tol, "y")
+        for g, (v, tl), name in zip(torch.autograd.grad(got, (xs, ws, bs), dys), orc.layer_norm_backward(*back, w, dy, F, F), ("dx", "dw", "db")):
+            close(g, v, tl, name)
+
+
+def test_norm_widest():
+    import kernels
+    x, (w, b) = rows_of((5, 32768), F, 1), params((32768,), F, 2)
+    y, tol, _ = orc.layer_norm(x, w, b, 1e-5, F)
+    close(kernels.layer_norm(*cuda(x, w, b)), y, tol, "y")
+    with pytest.raises(RuntimeError, match="wider than 16384"):
+        kernels.layer_norm(torch.zeros(2, 16385, device="cuda", requires_grad=True))
+    with pytest.raises(RuntimeError, match="UNSUPPORTED"):
+        kernels.layer_norm(torch.zeros(2, 32769, device="cuda"))
+
+
+def test_frozen_leaves_and_in_place():
+    """Gradients for the input alone, the parameters alone, one of them; an input changed after the forward is
+    noticed where the backward reads it, and allowed where it does not; a second derivative is refused."""
+    import kernels
+    x, (w, b), dy = rows_of((64, 256), F, 1), params((256,), F, 2), rows_of((64, 256), F, 3)
+    _, _, back = orc.layer_norm(x, w, b, 1e-5, F)
+    want = orc.layer_norm_backward(*back, w, dy, F, F)
+    for wanted in ((0,), (1,), (2,), (1, 2), (0, 2)):
+        ts = cuda(x, w, b)
+        for i in wanted:
+            ts[i].requires_grad_(True)
+        grads = torch.autograd.grad(kernels.layer_norm(*ts), [ts[i] for i in wanted], dy.cuda())
+        for g, i in zip(grads, wanted):
+            close(g, *want[i], f"leaf {i}")
+    for keep8 in (False, True):
+        leaf = x.cuda().requires_grad_(True)
+        mid = leaf * 1
+        y = kernels.layer_norm(mid, keep8=keep8)
+        mid.zero_()
+        if keep8:
+            y.backward(dy.cuda())
+        else:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                y.backward(dy.cuda())
+        xs, zs = x.cuda().requires_grad_(True), x.cuda().requires_grad_(True)
+        for out in (kernels.layer_norm(xs, keep8=keep8), kernels.sigmoid_gate(xs, zs, keep8=keep8)):
+            (g,) = torch.autograd.grad(out.square().sum(), xs, create_graph=True)
+            with pytest.raises(RuntimeError, match="differentiable once"):
+                g.sum().backward()
+
+
+def test_refusals():
+    import kernels
+    x = torch.zeros(4, 8, device="cuda")
+    for bad in (torch.ones(9, device="cuda"), torch.ones(3, 8, device="cuda"), torch.ones(4, 1, 8, device="cuda"), torch.tensor(1.0, device="cuda")):
+        with pytest.raises(ValueError):
+            kernels.layer_norm(x, bad)
+    with pytest.raises(ValueError):
+        kernels.layer_norm(x, torch.ones(8, device="cuda"), torch.ones(4, 8, device="cuda"))
+    with pytest.raises(ValueError):
+        kernels.layer_norm(x[:, :0])
+    with pytest.raises(ValueError):
+        kernels.layer_norm(torch.tensor(1.0, device="cuda"))
+    with pytest.raises(TypeError):
+        kernels.layer_norm(x, torch.ones(8, device="cuda", dtype=BF))
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        kernels.layer_norm(x, torch.ones(8))
+    with pytest.raises(ValueError):
+        kernels.sigmoid_gate(x, x[:1])
+    with pytest.raises(TypeError):
+        kernels.sigmoid_gate(x, x.half())
+    with pytest.raises(ValueError):
+        kernels.pack8(torch.tensor(1.0, device="cuda"))
+    # transforms that have no rule
+    q = kernels.quantize_int8(x)
+    for call in (lambda t: kernels.pack8(t).codes, lambda t: kernels.quantize_int8(t).codes, lambda t: kernels.layer_norm_int8(t).codes,
+                 lambda t: kernels.int8_linear(t, q)):
+        with pytest.raises(RuntimeError, match="torch.func transforms"):
+            torch.vmap(call)(x)
+    w = torch.ones(8, device="cuda")
+    for f in (lambda t: kernels.layer_norm(t, w).sum(), lambda t: kernels.sigmoid_gate(t, t).sum()):
+        with pytest.raises(RuntimeError, match="vmap over this operator's backward"):
+            torch.vmap(torch.func.grad(f))(x)
+
+
 def test_large_offsets():
     """Rows beyond 2^31 elements."""
     import kernels
