@@ -7,8 +7,12 @@
 // int8_few_kernel, for few tokens or tiles. The weight rows are the M side of the instruction, 128 output
 // channels a tile, and the tokens its N side, NT of 16 to 128: a decoding step wastes little of a tile.
 // With fewer tiles than SMs a unit is a part of a tile's K range; the parts leave integer sums in the
-// workspace, and the block that counts itself last adds them up: integers, the same in any order. Bound by
-// reading the weight, of which a ring of 11 stages (NT = 16) keeps 176 KB a SM in flight. Any N and alignment.
+// workspace, and the block that counts itself last adds them up: integers, the same in any order. Any N and
+// alignment. Bound by its chain of latencies (launch, first copies, MMAs, sums: 16 x 4096 x 4096 10.9 us with the
+// rows' kernel, 2.6 us of it the weight's bytes).
+//
+// int8_step_kernel, the same for up to 16 tokens of x itself, whose integer rows it makes on the way: 1 x 768 x 32000
+// in 9.0 us, 3.8 us of it the weight's bytes.
 //
 // int8_many_kernel, for tiles enough to fill the SMs. The tokens are the M side, 128 a block, and 256 or 128
 // channels the N side: a thread of the epilogue has a token's consecutive channels, packs them and leaves
@@ -17,6 +21,7 @@
 // blocks of a cluster share a tile of 256 x 256 (cta_group::2). Bound by the tensor cores: 8192 x 8192 x 8192
 // in 360 us, 3.06 POPS, 1.85 times the bf16 product's measured rate. With small K the output's way to memory
 // takes its share: 16384 x 768 x 32000 in 370 us, 2.18 POPS, of which 160 us would write the output alone.
+#include <cmath>
 #include "rows.cuh"
 #include "sm100.cuh"
 #include "tma_host.cuh"
@@ -317,24 +322,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   }
 }
 
-// ---- many tokens ----------------------------------------------------------------------------------------
-
-constexpr int kTokens = 128;    // a block's tokens of a tile
-constexpr int kStaged = 4096;   // bytes a warp hands to one TMA store: 32 tokens of 128 bytes
-template <bool PAIR, int NC> constexpr int many_rows() { return PAIR ? NC / 2 : NC; }  // weight rows a block loads a stage
-template <bool PAIR, int NC> constexpr int many_stage_bytes() { return (kTokens + many_rows<PAIR, NC>()) * kStep; }
-template <bool PAIR, int NC> constexpr int many_stages() { return many_rows<PAIR, NC>() == 256 ? 3 : 4; }
-// ring | two staged tiles a warp | a warp's channel scales and biases
-template <bool PAIR, int NC> constexpr int many_smem() {
-  return many_stages<PAIR, NC>() * many_stage_bytes<PAIR, NC>() + kEpilogue / 32 * (2 * kStaged + NC / 2 * 8) + 1024;
-}
-
-__device__ __forceinline__ void tma_store_2d(const void* tmap, const void* src, int c0, int c1, uint64_t policy) {
-  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group.L2::cache_hint [%0, {%2, %3}], [%1], %4;" ::"l"(tmap),
-               "r"(smem_u32(src)), "r"(c0), "r"(c1), "l"(policy)
-               : "memory");
-}
-
 // Two blocks that work on one tile (PAIR) or one: the instructions that differ.
 template <bool PAIR> struct Group;
 template <> struct Group<false> {
@@ -392,6 +379,265 @@ template <> struct Group<true> {
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
 };
+
+// ---- a decoding step ------------------------------------------------------------------------------------
+
+// Up to 16 tokens of up to 4096 elements, straight from x: each block makes the integer rows that it needs itself, in
+// the layout of the MMA's operand, while its weight tiles are on their way: one launch instead of two. With
+// fewer tiles than SMs the blocks of a cluster, up to eight, share a tile's K range; the first one adds up their
+// sums, which the others leave in its shared memory.
+constexpr int kStepTokens = 16;
+constexpr int kStepWidest = 4096;
+constexpr int kStepStages = 6;
+constexpr int kStepTile = kChannels * kStep;
+constexpr int kMostParts = 8;
+// ring | integer rows [K / 128][16][128 bytes] | the other blocks' sums [7][16][128]
+constexpr int kStepSmem = kStepStages * kStepTile + kStepTokens * kStepWidest + (kMostParts - 1) * kStepTokens * kChannels * 4 + 1024;
+
+struct StepArgs {
+  const void* x;
+  int64_t ldx;
+  bool vec;  // rows that start on 16 bytes, a multiple of 8 wide
+  int K;
+};
+
+// Eight elements of a row from k on, zeros beyond K
+template <typename T> __device__ __forceinline__ void load_row8(rows::Raw8<T>& r, const T* row, int k, int K, bool vec) {
+  if (vec) {
+    rows::load_raw<T, true>(r, row, k, 0, K);
+  } else {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = k + j < K ? ld(row + k + j) : 0.f;
+#pragma unroll
+    for (int j = 0; j < (int)sizeof(T) * 2; ++j) {
+      if constexpr (sizeof(T) == 4) r.w[j] = __float_as_uint(v[j]);
+      else r.w[j] = rows::pack2<T>(v[2 * j], v[2 * j + 1]);
+    }
+  }
+}
+
+// A channel's sums of the tokens, scaled, with the bias, stored
+template <typename T> __device__ __forceinline__ void finish_step(const Int8Args& a, const uint32_t (&acc)[kStepTokens], const float* scale, int64_t channel) {
+  const bool there = channel < a.N;
+  float bias = 0.f;
+  if (a.bias && there)
+    bias = a.bias32 ? __ldg(reinterpret_cast<const float*>(a.bias) + channel) : ld(reinterpret_cast<const T*>(a.bias) + channel);
+  store_tokens<T, kStepTokens, false>(a, acc, scale, there ? __ldg(a.sw + channel) : 0.f, bias, 0, channel);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+    int8_step_kernel(const __grid_constant__ CUtensorMap tm_w, const StepArgs x, const Int8Args a) {
+  constexpr int S = kStepStages, NT = kStepTokens;
+  extern __shared__ uint8_t dyn[];
+  __shared__ __align__(8) uint64_t full[S], empty[S], acc_full[2], acc_empty[2], rows_ready;
+  __shared__ uint32_t tmem_base, amax[NT];
+  __shared__ __align__(16) float scale[NT], factor[NT];
+  uint8_t* const ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
+  uint8_t* const codes = ring + S * kStepTile;
+  int32_t* const sums = reinterpret_cast<int32_t*>(codes + kStepTokens * kStepWidest);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // a cluster's blocks are the parts of one tile, and work on no other
+  const int part = a.splits > 1 ? blockIdx.x % a.splits : 0, first_tile = blockIdx.x / a.splits, stride = gridDim.x / a.splits;
+  const int k0 = (int)((int64_t)a.k_blocks * part / a.splits), k1 = (int)((int64_t)a.k_blocks * (part + 1) / a.splits);
+
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tm_w);
+    for (int i = 0; i < S; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], 128);
+    mbar_init(&rows_ready, 1);
+    fence_mbar_init();
+  }
+  if (threadIdx.x >= 64 && threadIdx.x < 64 + NT) amax[threadIdx.x - 64] = 0;
+  if (warp == 1) {
+    tmem_alloc(&tmem_base, 2 * NT);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncwarp();
+  if (a.splits > 1) Group<true>::meet();  // every block of the cluster runs before its memory is written to
+  else __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base;
+  wait_predecessor();
+
+  uint32_t acc_values[NT];  // a part's sums, kept for the meeting below
+  if (warp == 0) {
+    if (lane == 0) {
+      bool ok = true;
+      uint32_t it = 0;
+      for (int tile = first_tile; tile < a.tiles && ok; tile += stride) {
+        for (int k = k0; k < k1; ++k, ++it) {
+          const int s = it % S;
+          if (it >= (uint32_t)S && !mbar_wait(&empty[s], ((it / S) & 1) ^ 1, kWaitLimit)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&full[s], kStepTile);
+          tma_load_2d(ring + s * kStepTile, &tm_w, &full[s], k * kStep, tile * kChannels);
+        }
+      }
+      if (!ok) {
+        atomicExch(a.error, 1u);
+        // the copies still in flight land before the block's shared memory is given up
+        for (uint32_t i = it > (uint32_t)S ? it - S : 0; i < it; ++i) mbar_wait(&full[i % S], (i / S) & 1, kWaitLimit);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_i8<NT>();
+      uint32_t it = 0, local = 0;
+      bool ok = mbar_wait(&rows_ready, 0, kWaitLimit);
+      for (int tile = first_tile; tile < a.tiles && ok; tile += stride, ++local) {
+        const uint32_t b = local & 1;
+        if (local >= 2 && !mbar_wait(&acc_empty[b], ((local >> 1) & 1) ^ 1, kWaitLimit)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        for (int k = k0; k < k1; ++k, ++it) {
+          const int s = it % S;
+          if (!mbar_wait(&full[s], (it / S) & 1, kWaitLimit)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          uint64_t da = make_smem_desc(smem_u32(ring + s * kStepTile), 16, 1024, kSwizzle128B);
+          uint64_t db = make_smem_desc(smem_u32(codes + (k - k0) * NT * kStep), 16, 1024, kSwizzle128B);
+#pragma unroll
+          for (int i = 0; i < kStep / 32; ++i, da += 2, db += 2) umma_i8(tmem + b * NT, da, db, idesc, (k > k0 || i > 0) ? 1u : 0u);
+          umma_commit(&empty[s]);
+        }
+        if (ok) umma_commit(&acc_full[b]);
+      }
+      if (!ok) atomicExch(a.error, 1u);
+    }
+  } else {
+    const int et = threadIdx.x - 64, M = (int)a.M;
+    const T* const xp = reinterpret_cast<const T*>(x.x);
+    // the rows' largest magnitudes: all rows' loads of a step under way together
+    uint32_t m[NT];
+#pragma unroll
+    for (int r = 0; r < NT; ++r) m[r] = 0;
+    for (int k = et * 8; k < x.K; k += kEpilogue * 8) {
+      rows::Raw8<T> v[NT];
+#pragma unroll
+      for (int r = 0; r < NT; ++r)
+        if (r < M) load_row8<T>(v[r], xp + r * x.ldx, k, x.K, x.vec);
+#pragma unroll
+      for (int r = 0; r < NT; ++r)
+        if (r < M) {
+          uint32_t h[1];
+          rows::max_bits<T, true>(v[r], h);
+          m[r] = max(m[r], h[0]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < NT; ++r)
+      if (r < M) {
+        const uint32_t v = __reduce_max_sync(0xffffffffu, m[r]);
+        if (lane == 0) atomicMax(&amax[r], v);
+      }
+    epilogue_barrier();
+    if (et < NT) scale[et] = et < M ? rows::int8_scale(amax[et]) : 0.f, factor[et] = et < M ? rows::int8_factor(amax[et]) : 0.f;
+    epilogue_barrier();
+    const int groups = (k1 - k0) * (kStep / 8), all = M * groups;  // of eight elements: a row's, all rows'
+    auto convert = [&](auto batch) {
+      constexpr int B = decltype(batch)::value;  // groups of a thread whose loads are under way together
+      for (int g0 = et; g0 < all; g0 += B * kEpilogue) {
+        rows::Raw8<T> v[B];
+        int r[B], at[B];
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+          const int g = min(g0 + i * kEpilogue, all - 1);  // the last one again, with the same result
+          r[i] = (uint32_t)g / (uint32_t)groups;
+          at[i] = (g - r[i] * groups) * 8;
+          load_row8<T>(v[i], xp + r[i] * x.ldx, k0 * kStep + at[i], x.K, x.vec);
+        }
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+          rows::F2 f[4];
+          uint32_t q[8];
+          rows::to_float<T>(v[i], f);
+          rows::int8_codes(f, factor[r[i]], q);
+          *reinterpret_cast<uint2*>(codes + (at[i] / kStep) * NT * kStep + sw128_offset(r[i], (at[i] % kStep) / 16) + at[i] % 16) =
+              make_uint2(rows::bytes4(q[0], q[1], q[2], q[3]), rows::bytes4(q[4], q[5], q[6], q[7]));
+        }
+      }
+    };
+    if (all <= kEpilogue) convert(std::integral_constant<int, 1>());
+    else convert(std::integral_constant<int, 4>());
+    fence_async_shared();
+    epilogue_barrier();
+    if (et == 0) mbar_arrive(&rows_ready);
+
+    if (warp < 6) {
+      // these four warps have the 32 TMEM lanes, here channels, of their number mod 4
+      const int q = warp & 3;
+      uint32_t local = 0, limit = kWaitLimit;
+      for (int tile = first_tile; tile < a.tiles; tile += stride, ++local) {
+        const uint32_t b = local & 1;
+        if (!mbar_wait(&acc_full[b], (local >> 1) & 1, limit)) {
+          limit = 1;  // carries on with what is there
+          if (lane == 0) atomicExch(a.error, 1u);
+        }
+        tc_fence_after();
+        tmem_ld16(tmem + b * NT + ((uint32_t)(q * 32) << 16), acc_values);
+        tmem_wait_ld();
+        tc_fence_before();
+        mbar_arrive(&acc_empty[b]);
+        const int channel = q * 32 + lane;
+        if (a.splits == 1) {
+          finish_step<T>(a, acc_values, scale, (int64_t)tile * kChannels + channel);
+        } else if (part > 0) {
+          // to the first block's shared memory
+          uint32_t to;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(smem_u32(sums + (part - 1) * NT * kChannels + channel)));
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+            if (j < M) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + j * kChannels * 4), "r"(acc_values[j]) : "memory");
+        }
+      }
+    }
+  }
+  if (a.splits > 1) {
+    __syncwarp();
+    Group<true>::meet();  // every part's sums are there
+    if (part == 0 && warp >= 2 && warp < 6) {
+      const int channel = (warp & 3) * 32 + lane;
+      for (int i = 0; i < a.splits - 1; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          if (j < a.M) acc_values[j] += (uint32_t)sums[(i * NT + j) * kChannels + channel];
+      finish_step<T>(a, acc_values, scale, (int64_t)first_tile * kChannels + channel);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 2 * NT);
+  }
+}
+
+// ---- many tokens ----------------------------------------------------------------------------------------
+
+constexpr int kTokens = 128;    // a block's tokens of a tile
+constexpr int kStaged = 4096;   // bytes a warp hands to one TMA store: 32 tokens of 128 bytes
+template <bool PAIR, int NC> constexpr int many_rows() { return PAIR ? NC / 2 : NC; }  // weight rows a block loads a stage
+template <bool PAIR, int NC> constexpr int many_stage_bytes() { return (kTokens + many_rows<PAIR, NC>()) * kStep; }
+template <bool PAIR, int NC> constexpr int many_stages() { return many_rows<PAIR, NC>() == 256 ? 3 : 4; }
+// ring | two staged tiles a warp | a warp's channel scales and biases
+template <bool PAIR, int NC> constexpr int many_smem() {
+  return many_stages<PAIR, NC>() * many_stage_bytes<PAIR, NC>() + kEpilogue / 32 * (2 * kStaged + NC / 2 * 8) + 1024;
+}
+
+__device__ __forceinline__ void tma_store_2d(const void* tmap, const void* src, int c0, int c1, uint64_t policy) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group.L2::cache_hint [%0, {%2, %3}], [%1], %4;" ::"l"(tmap),
+               "r"(smem_u32(src)), "r"(c0), "r"(c1), "l"(policy)
+               : "memory");
+}
 
 // A tile is 128 tokens x NC channels, or with PAIR 256 x NC for two blocks of a cluster: each loads its own tokens
 // and half of the channels' weight rows.
@@ -611,10 +857,10 @@ constexpr size_t kOutputInL2 = 64 << 20;
 
 // Which kernel, its tile's other side (NT or NC), and parts of a tile's K range.
 struct GemmShape {
-  bool many, pair = false;
+  bool step = false, many = false, pair = false;
   int width, n_tiles, tiles, splits;
 };
-GemmShape gemm_shape(int64_t M, int64_t N, int64_t K, bool rows_on_16) {
+GemmShape gemm_shape(int64_t M, int64_t N, int64_t K, bool rows_on_16, bool from_x) {
   GemmShape g;
   const int64_t sms = num_sms(), m_tiles = (M + kTokens - 1) / kTokens;
   auto tiles = [&](int nc) { return m_tiles * ((N + nc - 1) / nc); };
@@ -637,9 +883,18 @@ GemmShape gemm_shape(int64_t M, int64_t N, int64_t K, bool rows_on_16) {
   g.width = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
   g.n_tiles = (int)((N + kChannels - 1) / kChannels);
   g.tiles = (int)((M + g.width - 1) / g.width * g.n_tiles);
-  // fewer tiles than SMs: as many parts of K as fill them
+  // Fewer tiles than SMs: parts of K, as many as fill them, but no more than pay: of p parts each loads blocks / p steps
+  // of (128 + NT) x 128 bytes, and the last one adds up p x NT x 128 sums, 4 bytes each, so that p = sqrt(blocks (128 +
+  // NT) / (4 NT)) has the least of both (100 x 8000 x 100: 19 us with 6 parts, 101 with 63).
   const int64_t blocks = (K + kStep - 1) / kStep;
-  g.splits = (int)std::max<int64_t>(1, std::min<int64_t>(blocks, sms / g.tiles));
+  const int64_t pay = std::max<int64_t>(1, std::llround(std::sqrt((double)blocks * (kChannels + g.width) / (4.0 * g.width))));
+  g.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(blocks, pay), sms / g.tiles));
+  // A decoding step's kernel while x is small: every one of its blocks goes through all of it (1 x 768 x 32000: 9.0 us
+  // against 10.1 with a launch of its own for the rows, and 3 us less for the host; 8 x 2048 x 2048: 8.4 and 10.0;
+  // 16 x 4096 x 4096: 13.3 and 10.9; 8 x 4096 x 16000: 19.3 and 15.8).
+  g.step = from_x && M <= kStepTokens && K <= kStepWidest && M * K <= (g.tiles <= 64 ? 16384 : 8192);
+  // clusters of 2, 4 or 8 blocks, no more of them than run at once (16 of 8 did not: 1 x 2048 x 2048 took 11.7 us)
+  if (g.step) g.splits = g.splits >= 8 && g.tiles <= 8 ? 8 : g.splits >= 4 && g.tiles <= 32 ? 4 : g.splits >= 2 && g.tiles <= 64 ? 2 : 1;
   return g;
 }
 
@@ -653,23 +908,23 @@ GemmWs gemm_ws(const GemmShape& g, int64_t M, int64_t K, bool quantise) {
   w.counts = 4;
   size_t off = al(4 + (g.splits > 1 ? (size_t)g.tiles * 4 : 0));
   w.codes = off;
-  off += quantise ? al((size_t)M * rows::code_pitch(K)) : 0;
+  off += quantise && !g.step ? al((size_t)M * rows::code_pitch(K)) : 0;
   w.scale = off;
-  off += quantise ? al((size_t)M * 4) : 0;
+  off += quantise && !g.step ? al((size_t)M * 4) : 0;
   w.parts = off;
-  off += g.splits > 1 ? (size_t)g.tiles * g.splits * g.width * kChannels * 4 : 0;
+  off += g.splits > 1 && !g.step ? (size_t)g.tiles * g.splits * g.width * kChannels * 4 : 0;
   w.bytes = off;
   return w;
 }
 
-// blocks: of a cluster that shares a tile. overlap: the kernel may start while the one before it drains.
+// units: of work; blocks: of a cluster that shares one. overlap: the kernel may start while the one before it drains.
 template <typename... K, typename... A>
-int launch(void (*k)(K...), int blocks, int smem, const Int8Args& a, bool overlap, cudaStream_t s, const A&... args) {
+int launch(void (*k)(K...), int64_t units, int blocks, int smem, const Int8Args& a, bool overlap, cudaStream_t s, const A&... args) {
   int st = ensure_dyn_smem(reinterpret_cast<const void*>(k), smem, "int8_linear shared memory");
   if (st != FLB_OK) return st;
   cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)std::min<int64_t>((int64_t)a.tiles * a.splits * blocks, num_sms() / blocks * blocks));
+  cfg.gridDim = dim3((unsigned)std::min<int64_t>(units * blocks, num_sms() / blocks * blocks));
   cfg.blockDim = dim3(kGemmThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
@@ -691,12 +946,12 @@ int launch(void (*k)(K...), int blocks, int smem, const Int8Args& a, bool overla
 
 template <int NT, typename T>
 int launch_few(const CUtensorMap& tw, const CUtensorMap& tx, const Int8Args& a, bool overlap, cudaStream_t s) {
-  return launch(int8_few_kernel<NT, T>, 1, stages<NT>() * stage_bytes<NT>() + 1024, a, overlap, s, tw, tx);
+  return launch(int8_few_kernel<NT, T>, (int64_t)a.tiles * a.splits, 1, stages<NT>() * stage_bytes<NT>() + 1024, a, overlap, s, tw, tx);
 }
 
 template <bool PAIR, int NC, typename T>
 int launch_many(const CUtensorMap& tw, const CUtensorMap& tx, const CUtensorMap& to, const Int8Args& a, bool overlap, cudaStream_t s) {
-  return launch(int8_many_kernel<PAIR, NC, T>, PAIR ? 2 : 1, many_smem<PAIR, NC>(), a, overlap, s, tw,
+  return launch(int8_many_kernel<PAIR, NC, T>, a.tiles, PAIR ? 2 : 1, many_smem<PAIR, NC>(), a, overlap, s, tw,
                 tx, to);
 }
 
@@ -737,19 +992,21 @@ int int8_rows(const void* x, int64_t ldx, int8_t* codes, float* scale, int64_t R
 
 // For either kernel: which one runs also depends on where the output lies.
 size_t int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, bool quantise) {
-  return std::max(gemm_ws(gemm_shape(M, N, K, false), M, K, quantise).bytes, gemm_ws(gemm_shape(M, N, K, true), M, K, quantise).bytes);
+  return std::max(gemm_ws(gemm_shape(M, N, K, false, quantise), M, K, quantise).bytes,
+                  gemm_ws(gemm_shape(M, N, K, true, quantise), M, K, quantise).bytes);
 }
 
 int int8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, const float* x_scale, const int8_t* w_codes,
                 int64_t ldw, const float* w_scale, const void* bias, int bias_dtype, void* out, int64_t M, int64_t N,
                 int64_t K, int dtype, void* ws, int check_timeout, cudaStream_t s) {
-  const GemmShape g = gemm_shape(M, N, K, N * dtype_size(dtype) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0);
+  const GemmShape g = gemm_shape(M, N, K, N * dtype_size(dtype) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0,
+                                 x != nullptr);
   const GemmWs l = gemm_ws(g, M, K, x != nullptr);
   uint8_t* p = reinterpret_cast<uint8_t*>(ws);
   const int64_t n_zero = 1 + (g.splits > 1 ? g.tiles : 0);
-  const bool reset = !x && (g.splits > 1 || check_timeout);
+  const bool reset = g.step ? check_timeout != 0 : !x && (g.splits > 1 || check_timeout);
   int st;
-  if (x) {
+  if (x && !g.step) {
     // the rows' kernel clears the error word and the counts too
     int8_t* codes = reinterpret_cast<int8_t*>(p + l.codes);
     float* scale = reinterpret_cast<float*>(p + l.scale);
@@ -758,14 +1015,21 @@ int int8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, 
   } else if (reset) {  // otherwise nothing reads those words
     if ((st = check_cuda(cudaMemsetAsync(p, 0, n_zero * 4, s), "int8_linear reset")) != FLB_OK) return st;
   }
-  CUtensorMap tw, tx;
+  CUtensorMap tw, tx = {};
   if ((st = code_map(&tw, w_codes, N, ldw, K, g.many ? (g.pair ? g.width / 2 : g.width) : kChannels)) != FLB_OK) return st;
-  if ((st = code_map(&tx, x_codes, M, ldc, K, g.many ? kTokens : g.width)) != FLB_OK) return st;
+  if (!g.step && (st = code_map(&tx, x_codes, M, ldc, K, g.many ? kTokens : g.width)) != FLB_OK) return st;
   const Int8Args a{x_scale, w_scale, bias, bias_dtype == FLB_F32, out, M, N,
                    N % 2 == 0 && reinterpret_cast<uintptr_t>(out) % 4 == 0, x != nullptr, (int)((K + kStep - 1) / kStep), g.n_tiles, g.tiles,
                    g.splits, N * K <= kWeightInL2 ? 1 : 16, (size_t)M * N * dtype_size(dtype) > kOutputInL2, reinterpret_cast<int32_t*>(p + l.parts), reinterpret_cast<uint32_t*>(p + l.counts),
                    reinterpret_cast<uint32_t*>(p)};
-  switch (dtype) {
+  const StepArgs sa{x, ldx, K % 8 == 0 && ldx * dtype_size(dtype) % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0, (int)K};
+  if (g.step) {
+    switch (dtype) {
+      case FLB_F32: st = launch(int8_step_kernel<float>, g.tiles, g.splits, kStepSmem, a, !reset, s, tw, sa); break;
+      case FLB_F16: st = launch(int8_step_kernel<__half>, g.tiles, g.splits, kStepSmem, a, !reset, s, tw, sa); break;
+      default: st = launch(int8_step_kernel<__nv_bfloat16>, g.tiles, g.splits, kStepSmem, a, !reset, s, tw, sa); break;
+    }
+  } else switch (dtype) {
     case FLB_F32: st = launch_t<float>(g, tw, tx, a, !reset, s); break;
     case FLB_F16: st = launch_t<__half>(g, tw, tx, a, !reset, s); break;
     default: st = launch_t<__nv_bfloat16>(g, tw, tx, a, !reset, s); break;

@@ -204,21 +204,12 @@ __global__ void __launch_bounds__(kMostThreads<MODE>, 1024 / kMostThreads<MODE>)
         }
       }
       m = row_max<WARP>(m, reinterpret_cast<uint32_t*>(slot[turn][WARP ? 0 : 2]));
-      // An infinity or NaN in the row makes its scale, and so all that is computed with it, NaN. Below
-      // 2^-118 the factor 127 / a would be infinite: such a row counts as zeros.
-      const float amax = __uint_as_float(m);
-      const bool bad = m >= 0x7f800000u;
-      const float f = bad || amax < 3.0092655e-36f ? 0.f : 127.f / amax;
-      if (threadIdx.x == 0 || (WARP && lane == 0)) a.scale[row] = bad ? __uint_as_float(0x7fffffffu) : amax / 127.f;
+      const float factor = int8_factor(m);
+      if (threadIdx.x == 0 || (WARP && lane == 0)) a.scale[row] = int8_scale(m);
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         uint32_t q[8];
-        float t[8];
-        to_scalars(v[c], t);
-        // product and rounding apart, each rounded as written above (as a packed pair they come out as one
-        // multiply-add, with another code now and then)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) q[j] = f == 0.f ? 0u : code_of(__fmul_rn(t[j], f));
+        int8_codes(v[c], factor, q);
         store_codes<VEC>(a.codes + row * code_pitch(D), q, first + c * 256, lane, D);
       }
     }

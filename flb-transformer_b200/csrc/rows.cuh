@@ -205,6 +205,25 @@ __device__ __forceinline__ void codes_to_float(uint2 c, F2 (&v)[4]) {
   }
 }
 
+// A row in 8-bit integers, from the bits of its largest magnitude a: factor 127 / a, scale a / 127. An infinity or NaN in
+// the row makes its scale, and so all that is computed with it, NaN. Below 2^-118 the factor would be
+// infinite: such a row counts as zeros (factor 0).
+__device__ __forceinline__ float int8_factor(uint32_t amax_bits) {
+  const float a = __uint_as_float(amax_bits);
+  return amax_bits >= 0x7f800000u || a < 3.0092655e-36f ? 0.f : 127.f / a;
+}
+__device__ __forceinline__ float int8_scale(uint32_t amax_bits) {
+  return amax_bits >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : __uint_as_float(amax_bits) / 127.f;
+}
+// Product and rounding apart, each rounded as written (as a packed pair they come out as one multiply-add,
+// with another code now and then)
+__device__ __forceinline__ void int8_codes(const F2 (&v)[4], float factor, uint32_t (&q)[8]) {
+  float t[8];
+  to_scalars(v, t);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) q[j] = factor == 0.f ? 0u : code_of(__fmul_rn(t[j], factor));
+}
+
 // ---- the kept form --------------------------------------------------------------------------------
 // A block of 128 consecutive elements is kept as codes c of magnitude at most 127 and one byte E:
 // element = c * 2^(E - 127), E the smallest of at least 1 for which the block's largest magnitude a still

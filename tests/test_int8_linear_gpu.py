@@ -48,7 +48,9 @@ SHAPES = [(1, 768, 32000), (1, 1, 1), (2, 16, 8), (15, 128, 128), (16, 4096, 409
           # two blocks a tile: a last tile with few tokens, or none, for its second block, and channels for one of them
           (2690, 1024, 4360), (2600, 1056, 4104), (5120, 1100, 2048),
           # fewer tokens than a tile and many channels; a weight larger than L2 keeps, tokens in two groups of tiles
-          (100, 256, 19000), (2300, 32768, 1544)]
+          (100, 256, 19000), (2300, 32768, 1544),
+          # a decoding step's kernel: clusters of 8, 4, 2 and 1 blocks a tile, and K on either side of its widest
+          (16, 4096, 2048), (9, 1024, 2049), (16, 4095, 4096), (3, 2000, 8190), (7, 256, 20000), (16, 130, 64), (16, 4097, 4096)]
 
 
 @pytest.mark.parametrize("M,K,N", SHAPES)
