@@ -404,7 +404,7 @@ struct StepArgs {
 // Eight elements of a row from k on, zeros beyond K
 template <typename T> __device__ __forceinline__ void load_row8(rows::Raw8<T>& r, const T* row, int k, int K, bool vec) {
   if (vec) {
-    rows::load_raw<T, true>(r, row, k, 0, K);
+    rows::load_raw<T, rows::EIGHT>(r, row, k, 0, K);
   } else {
     float v[8];
 #pragma unroll
@@ -529,7 +529,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       for (int r = 0; r < NT; ++r)
         if (r < M) {
           uint32_t h[1];
-          rows::max_bits<T, true>(v[r], h);
+          rows::max_bits<T, rows::EIGHT>(v[r], h);
           m[r] = max(m[r], h[0]);
         }
     }

@@ -60,41 +60,41 @@ template <bool FLAT, typename L, typename F> __device__ __forceinline__ void for
   }
 }
 
-template <typename T, bool VEC>
+template <typename T, Layout L>
 __device__ __forceinline__ void keep_raw(const Raw8<T>& r, const F2 (&v)[4], int8_t* codes, uint8_t* exps, int64_t row, int base,
                                          int lane, int D) {
-  uint32_t m[VEC ? 1 : 2];
-  max_bits<T, VEC>(r, m);
-  keep8<VEC>(v, m, codes + row * code_pitch(D), exps + row * blocks_of(D), base, lane, D);
+  uint32_t m[L == EIGHT ? 1 : 2];
+  max_bits<T, L>(r, m);
+  keep8<L>(v, m, codes + row * code_pitch(D), exps + row * blocks_of(D), base, lane, D);
 }
 
 // FORM 0: rows that start on 16 bytes, a multiple of 8 wide; 1: others; 2: FLAT
-template <int FORM> constexpr bool kVec = FORM != 1;
+template <typename T, int FORM> constexpr Layout kForm = kLayout<T, FORM != 1>;
 
 template <typename T, int FORM> __global__ void __launch_bounds__(kThreads) pack_kernel(const KeptArgs a) {
-  constexpr bool VEC = kVec<FORM>;
+  constexpr Layout L = kForm<T, FORM>;
   const int D = FORM == 2 ? 256 : a.D;
   auto load = [&](int64_t row, int base, int lane) {
     Raw8<T> r;
-    load_raw<T, VEC>(r, reinterpret_cast<const T*>(a.x) + row * D, base, lane, D);
+    load_raw<T, L>(r, reinterpret_cast<const T*>(a.x) + row * D, base, lane, D);
     return r;
   };
   for_chunks<FORM == 2>(a, load, [&](int64_t row, int base, int lane, const Raw8<T>& r) {
     F2 v[4];
     to_float<T>(r, v);
-    keep_raw<T, VEC>(r, v, a.cx, a.ex, row, base, lane, D);
+    keep_raw<T, L>(r, v, a.cx, a.ex, row, base, lane, D);
   });
 }
 
 template <typename T, int FORM> __global__ void __launch_bounds__(kThreads) unpack_kernel(const KeptArgs a) {
-  constexpr bool VEC = kVec<FORM>;
+  constexpr Layout L = kForm<T, FORM>;
   const int D = FORM == 2 ? 256 : a.D;
   auto load = [&](int64_t row, int base, int lane) {
-    return load_kept<VEC>(a.cx + row * code_pitch(D), a.ex + row * blocks_of(D), base, lane, D);
+    return load_kept<L>(a.cx + row * code_pitch(D), a.ex + row * blocks_of(D), base, lane, D);
   };
   for_chunks<FORM == 2>(a, load, [&](int64_t row, int base, int lane, const Kept8& k) {
     F2 v[4];
-    kept_to_float<VEC>(k, v);
+    kept_to_float<L>(k, v);
     if constexpr (std::is_same<T, __half>::value) {
       // a magnitude near the type's largest can be kept as 65536: back to the largest (a NaN stays one)
 #pragma unroll
@@ -103,20 +103,20 @@ template <typename T, int FORM> __global__ void __launch_bounds__(kThreads) unpa
         v[i] = f2(fabsf(f.x) > 65504.f ? copysignf(65504.f, f.x) : f.x, fabsf(f.y) > 65504.f ? copysignf(65504.f, f.y) : f.y);
       }
     }
-    store8<T, VEC>(reinterpret_cast<T*>(a.y) + row * D, v, base, lane, D);
+    store8<T, L>(reinterpret_cast<T*>(a.y) + row * D, v, base, lane, D);
   });
 }
 
 template <typename T, int FORM, bool KEEP> __global__ void __launch_bounds__(kThreads) gate_fwd_kernel(const KeptArgs a) {
-  constexpr bool VEC = kVec<FORM>;
+  constexpr Layout L = kForm<T, FORM>;
   const int D = FORM == 2 ? 256 : a.D;
   struct Both {
     Raw8<T> x, z;
   };
   auto load = [&](int64_t row, int base, int lane) {
     Both r;
-    load_raw<T, VEC>(r.x, reinterpret_cast<const T*>(a.x) + row * D, base, lane, D);
-    load_raw<T, VEC>(r.z, reinterpret_cast<const T*>(a.z) + row * D, base, lane, D);
+    load_raw<T, L>(r.x, reinterpret_cast<const T*>(a.x) + row * D, base, lane, D);
+    load_raw<T, L>(r.z, reinterpret_cast<const T*>(a.z) + row * D, base, lane, D);
     return r;
   };
   for_chunks<FORM == 2>(a, load, [&](int64_t row, int base, int lane, const Both& r) {
@@ -124,22 +124,22 @@ template <typename T, int FORM, bool KEEP> __global__ void __launch_bounds__(kTh
     to_float<T>(r.x, x);
     to_float<T>(r.z, z);
     if constexpr (KEEP) {
-      keep_raw<T, VEC>(r.x, x, a.cx, a.ex, row, base, lane, D);
-      keep_raw<T, VEC>(r.z, z, a.cz, a.ez, row, base, lane, D);
+      keep_raw<T, L>(r.x, x, a.cx, a.ex, row, base, lane, D);
+      keep_raw<T, L>(r.z, z, a.cz, a.ez, row, base, lane, D);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 f = split(z[i]);
       x[i] = mul2(x[i], f2(gate_of<T>(f.x).x, gate_of<T>(f.y).x));
     }
-    store8<T, VEC>(reinterpret_cast<T*>(a.y) + row * D, x, base, lane, D);
+    store8<T, L>(reinterpret_cast<T*>(a.y) + row * D, x, base, lane, D);
   });
 }
 
 // x, z as in the forward, or their kept form; y takes dx, y2 takes dz
 template <typename T, int FORM, bool KEEP>
 __global__ void __launch_bounds__(kThreads) gate_bwd_kernel(const KeptArgs a, const void* dy_) {
-  constexpr bool VEC = kVec<FORM>;
+  constexpr Layout L = kForm<T, FORM>;
   const int D = FORM == 2 ? 256 : a.D;
   struct All {
     Raw8<T> dy, x, z;
@@ -147,13 +147,13 @@ __global__ void __launch_bounds__(kThreads) gate_bwd_kernel(const KeptArgs a, co
   };
   auto load = [&](int64_t row, int base, int lane) {
     All r;
-    load_raw<T, VEC>(r.dy, reinterpret_cast<const T*>(dy_) + row * D, base, lane, D);
+    load_raw<T, L>(r.dy, reinterpret_cast<const T*>(dy_) + row * D, base, lane, D);
     if constexpr (KEEP) {
-      r.kx = load_kept<VEC>(a.cx + row * code_pitch(D), a.ex + row * blocks_of(D), base, lane, D);
-      r.kz = load_kept<VEC>(a.cz + row * code_pitch(D), a.ez + row * blocks_of(D), base, lane, D);
+      r.kx = load_kept<L>(a.cx + row * code_pitch(D), a.ex + row * blocks_of(D), base, lane, D);
+      r.kz = load_kept<L>(a.cz + row * code_pitch(D), a.ez + row * blocks_of(D), base, lane, D);
     } else {
-      load_raw<T, VEC>(r.x, reinterpret_cast<const T*>(a.x) + row * D, base, lane, D);
-      load_raw<T, VEC>(r.z, reinterpret_cast<const T*>(a.z) + row * D, base, lane, D);
+      load_raw<T, L>(r.x, reinterpret_cast<const T*>(a.x) + row * D, base, lane, D);
+      load_raw<T, L>(r.z, reinterpret_cast<const T*>(a.z) + row * D, base, lane, D);
     }
     return r;
   };
@@ -161,8 +161,8 @@ __global__ void __launch_bounds__(kThreads) gate_bwd_kernel(const KeptArgs a, co
     F2 x[4], z[4], dy[4], dz[4];
     to_float<T>(r.dy, dy);
     if constexpr (KEEP) {
-      kept_to_float<VEC>(r.kx, x);
-      kept_to_float<VEC>(r.kz, z);
+      kept_to_float<L>(r.kx, x);
+      kept_to_float<L>(r.kz, z);
     } else {
       to_float<T>(r.x, x);
       to_float<T>(r.z, z);
@@ -174,8 +174,8 @@ __global__ void __launch_bounds__(kThreads) gate_bwd_kernel(const KeptArgs a, co
       dz[i] = mul2(mul2(dx, x[i]), f2(g.y, h.y));
       x[i] = dx;
     }
-    store8<T, VEC>(reinterpret_cast<T*>(a.y) + row * D, x, base, lane, D);
-    store8<T, VEC>(reinterpret_cast<T*>(a.y2) + row * D, dz, base, lane, D);
+    store8<T, L>(reinterpret_cast<T*>(a.y) + row * D, x, base, lane, D);
+    store8<T, L>(reinterpret_cast<T*>(a.y2) + row * D, dz, base, lane, D);
   });
 }
 

@@ -48,7 +48,7 @@ constexpr int kBlocksPerSm = 4;  // such blocks on an SM
 
 // Bytes a thread's chunk takes in the ring
 template <typename T, bool VEC, bool KEPT> constexpr int chunk_bytes() {
-  const int elems = kCopies<T, VEC> ? 8 * (int)sizeof(T) : 0;
+  const int elems = kCopies<T, kLayout<T, VEC>> ? 8 * (int)sizeof(T) : 0;
   return KEPT ? elems + (VEC ? 8 : 0) : 2 * elems;
 }
 
@@ -56,9 +56,10 @@ template <typename T, bool VEC, bool KEPT> constexpr int chunk_bytes() {
 template <typename T, bool VEC, int MODE, int CH, bool KEPT>
 __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 1024, MODE == 0 ? kBlocksPerSm : 1)
     ln_bwd_kernel(const BwdArgs a) {
+  constexpr Layout L = kLayout<T, VEC>;
   constexpr bool WARP = MODE == 0;
   constexpr int S = kStages<T, MODE == 2>, CB = chunk_bytes<T, VEC, KEPT>();
-  constexpr bool COPY_DY = kCopies<T, VEC>, COPY_X = !KEPT && COPY_DY, COPY_CODES = KEPT && VEC;
+  constexpr bool COPY_DY = kCopies<T, L>, COPY_X = !KEPT && COPY_DY, COPY_CODES = KEPT && VEC;
   extern __shared__ __align__(16) uint8_t ring[];  // [S][CH][x or codes | dy][threads]; at the end [2][D] floats
   __shared__ __align__(16) float2 slot[WARP ? 1 : 2][32];  // zero for warps that the block does not have
   let_successor_start();
@@ -84,11 +85,15 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         const int base = first + c * 256;
-        if constexpr (COPY_DY) copy8<T, VEC>(part_of(stage, c, true), dy_row(r), base, lane, D);
-        if constexpr (COPY_X) copy8<T, VEC>(part_of(stage, c, false), x_row(r), base, lane, D);
+        if constexpr (COPY_DY) copy8<T, L>(part_of(stage, c, true), dy_row(r), base, lane, D);
+        if constexpr (COPY_X) copy8<T, L>(part_of(stage, c, false), x_row(r), base, lane, D);
         if constexpr (COPY_CODES) {
-          const int p = base + lane * 8;
-          copy_async<8>(shared_addr(part_of(stage, c, false)) + threadIdx.x * 8, code_row(r) + (p < D ? p : 0), p < D);
+          const uint32_t to = shared_addr(part_of(stage, c, false)) + threadIdx.x * 8;
+#pragma unroll
+          for (int i = 0; i < (L == FOURS ? 2 : 1); ++i) {
+            const int p = Chunk<L>::at(base, lane, 4 * i);
+            copy_async<L == FOURS ? 4 : 8>(to + 4 * i, code_row(r) + (p < D ? p : 0), p < D);
+          }
         }
       }
     }
@@ -108,9 +113,9 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[c][i] = f2(1.f);
     } else if (a.w32) {
-      load8<float, VEC>(w[c], reinterpret_cast<const float*>(a.w) + group * D, first + c * 256, lane, D);
+      load8<float, L>(w[c], reinterpret_cast<const float*>(a.w) + group * D, first + c * 256, lane, D);
     } else {
-      load8<T, VEC>(w[c], reinterpret_cast<const T*>(a.w) + group * D, first + c * 256, lane, D);
+      load8<T, L>(w[c], reinterpret_cast<const T*>(a.w) + group * D, first + c * 256, lane, D);
     }
   }
 
@@ -123,7 +128,7 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
     rstd = __ldg(a.rstd + rr);
     if constexpr (KEPT) {
 #pragma unroll
-      for (int c = 0; c < CH; ++c) exps[c] = load_exps<VEC>(a.exps + rr * blocks_of(D), first + c * 256, lane, D);
+      for (int c = 0; c < CH; ++c) exps[c] = load_exps<L>(a.exps + rr * blocks_of(D), first + c * 256, lane, D);
     }
   };
 
@@ -140,22 +145,22 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
     for (int c = 0; c < CH; ++c) {
       const int base = first + c * 256;
       if constexpr (KEPT) rk[c].e = exps[c];
-      if constexpr (KEPT && !COPY_CODES) rk[c].c = load_codes<VEC>(code_row(row), base, lane, D);
-      if constexpr (!KEPT && !COPY_X) load_raw<T, VEC>(rx[c], x_row(row), base, lane, D);
-      if constexpr (!COPY_DY) load_raw<T, VEC>(rdy[c], dy_row(row), base, lane, D);
+      if constexpr (KEPT && !COPY_CODES) rk[c].c = load_codes<L>(code_row(row), base, lane, D);
+      if constexpr (!KEPT && !COPY_X) load_raw<T, L>(rx[c], x_row(row), base, lane, D);
+      if constexpr (!COPY_DY) load_raw<T, L>(rdy[c], dy_row(row), base, lane, D);
     }
     if (row + stride < a.R) fetch_small(row + stride);
     copies_wait<S - 1>();
     // chunk c of x (or the kept h) and dy; read again after the sums, which costs less than the
     // registers to hold them
     auto values = [&](int c, F2 (&x)[4], F2 (&dy)[4]) {
-      if constexpr (COPY_DY) copied8<T, VEC>(part_of(stage, c, true), dy); else to_float<T>(rdy[c], dy);
+      if constexpr (COPY_DY) copied8<T, L>(part_of(stage, c, true), dy); else to_float<T>(rdy[c], dy);
       if constexpr (KEPT) {
         Kept8 k = rk[c];
         if constexpr (COPY_CODES) k.c = reinterpret_cast<const uint2*>(part_of(stage, c, false))[threadIdx.x];
-        kept_to_float<VEC>(k, x);
+        kept_to_float<L>(k, x);
       } else {
-        if constexpr (COPY_X) copied8<T, VEC>(part_of(stage, c, false), x); else to_float<T>(rx[c], x);
+        if constexpr (COPY_X) copied8<T, L>(part_of(stage, c, false), x); else to_float<T>(rx[c], x);
       }
     };
     // h = x h1 + h0
@@ -199,7 +204,7 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
       values(c, x, dy);
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[i] = fma2(mul2(f2(rs), w[c][i]), dy[i], fma2(x[i], f2(c1), f2(c0)));
-      store8<T, VEC>(dx, x, first + c * 256, lane, D);
+      store8<T, L>(dx, x, first + c * 256, lane, D);
     }
     stage = stage + 1 == S ? 0 : stage + 1;
   }
@@ -230,7 +235,7 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
         to_scalars(db[c], vb);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int p = Chunk<VEC>::at(first + c * 256, lane, j);
+          const int p = Chunk<L>::at(first + c * 256, lane, j);
           if (p < D) {
             sm[p] = (t ? sm[p] : 0.f) + vw[j];
             sm[D + p] = (t ? sm[D + p] : 0.f) + vb[j];
@@ -248,7 +253,7 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
       to_scalars(db[c], vb);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int p = Chunk<VEC>::at(first + c * 256, lane, j);
+        const int p = Chunk<L>::at(first + c * 256, lane, j);
         if (p < D) out(p, vw[j], vb[j]);
       }
     }

@@ -37,26 +37,26 @@ struct RowArgs {
 };
 
 // `fill` where there is no such vector
-template <typename T, bool VEC>
+template <typename T, Layout L>
 __device__ __forceinline__ void load_param(F2 (&v)[4], const void* p, bool f32, float fill, int64_t off, int base,
                                            int lane, int D) {
   if (!p) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = f2(fill);
   } else if (f32) {
-    load8<float, VEC>(v, reinterpret_cast<const float*>(p) + off, base, lane, D);
+    load8<float, L>(v, reinterpret_cast<const float*>(p) + off, base, lane, D);
   } else {
-    load8<T, VEC>(v, reinterpret_cast<const T*>(p) + off, base, lane, D);
+    load8<T, L>(v, reinterpret_cast<const T*>(p) + off, base, lane, D);
   }
 }
 
 // Zeros in the place of a chunk's elements at or beyond D
-template <bool VEC> __device__ __forceinline__ void zero_beyond(F2 (&v)[4], int base, int lane, int D) {
-  if (Chunk<VEC>::has(base, lane, 7, D)) return;
+template <Layout L> __device__ __forceinline__ void zero_beyond(F2 (&v)[4], int base, int lane, int D) {
+  if (Chunk<L>::has(base, lane, 7, D)) return;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 r = split(v[i]);
-    v[i] = f2(Chunk<VEC>::has(base, lane, 2 * i, D) ? r.x : 0.f, Chunk<VEC>::has(base, lane, 2 * i + 1, D) ? r.y : 0.f);
+    v[i] = f2(Chunk<L>::has(base, lane, 2 * i, D) ? r.x : 0.f, Chunk<L>::has(base, lane, 2 * i + 1, D) ? r.y : 0.f);
   }
 }
 
@@ -68,7 +68,8 @@ template <int MODE> constexpr int kMostThreads = MODE == 0 ? 32 * kWarps : MODE 
 // MODE 0: a warp a row (D <= 1024), 1: a block a row (D <= 8192), 2: a block of up to 1024 threads
 template <typename T, bool VEC, int MODE, int CH, bool NORM, int OUT>
 __global__ void __launch_bounds__(kMostThreads<MODE>, 1024 / kMostThreads<MODE>) row_fwd_kernel(const RowArgs a) {
-  constexpr bool WARP = MODE == 0, COPY = kCopies<T, VEC>;
+  constexpr Layout L = kLayout<T, VEC>;
+  constexpr bool WARP = MODE == 0, COPY = kCopies<T, L>;
   constexpr bool PARAMS = NORM && MODE != 2;  // the weight and bias stay in shared memory, as float32
   constexpr int S = kStages<CH, MODE>;
   // [CH][4][threads, or lanes of a warp's row] float4: weight and bias | [S][CH][threads] chunks of rows, with COPY
@@ -95,7 +96,7 @@ __global__ void __launch_bounds__(kMostThreads<MODE>, 1024 / kMostThreads<MODE>)
     if constexpr (COPY) {
       if (r < rows) {
 #pragma unroll
-        for (int c = 0; c < CH; ++c) copy8<T, VEC>(chunk_at(stage, c), x + r * a.ldx, first + c * 256, lane, D);
+        for (int c = 0; c < CH; ++c) copy8<T, L>(chunk_at(stage, c), x + r * a.ldx, first + c * 256, lane, D);
       }
       copies_commit();
     }
@@ -111,8 +112,8 @@ __global__ void __launch_bounds__(kMostThreads<MODE>, 1024 / kMostThreads<MODE>)
     for (int c = 0; c < CH; ++c) {
       if (WARP && c % (int)(blockDim.x >> 5) != warp) continue;
       F2 w[4], b[4];
-      load_param<T, VEC>(w, a.w, a.w32, 1.f, group * D, first + c * 256, lane, D);
-      load_param<T, VEC>(b, a.b, a.w32, 0.f, group * D, first + c * 256, lane, D);
+      load_param<T, L>(w, a.w, a.w32, 1.f, group * D, first + c * 256, lane, D);
+      load_param<T, L>(b, a.b, a.w32, 0.f, group * D, first + c * 256, lane, D);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const float2 lo = split(k < 2 ? w[2 * k] : b[2 * k - 4]), hi = split(k < 2 ? w[2 * k + 1] : b[2 * k - 3]);
@@ -133,8 +134,8 @@ __global__ void __launch_bounds__(kMostThreads<MODE>, 1024 / kMostThreads<MODE>)
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       Raw8<T>& u = raw[NORM ? 0 : c];
-      if constexpr (COPY) copied_raw<T, VEC>(chunk_at(stage, c), u);
-      else load_raw<T, VEC>(u, x + r * a.ldx, first + c * 256, lane, D);
+      if constexpr (COPY) copied_raw<T, L>(chunk_at(stage, c), u);
+      else load_raw<T, L>(u, x + r * a.ldx, first + c * 256, lane, D);
       to_float<T>(u, v[c]);
     }
     if constexpr (NORM) {
@@ -147,7 +148,7 @@ __global__ void __launch_bounds__(kMostThreads<MODE>, 1024 / kMostThreads<MODE>)
       for (int c = 0; c < CH; ++c) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[c][i] = add2(v[c][i], f2(-mean));
-        zero_beyond<VEC>(v[c], first + c * 256, lane, D);
+        zero_beyond<L>(v[c], first + c * 256, lane, D);
 #pragma unroll
         for (int i = 0; i < 4; ++i) s = fma2(v[c][i], v[c][i], s);
       }
@@ -164,9 +165,9 @@ __global__ void __launch_bounds__(kMostThreads<MODE>, 1024 / kMostThreads<MODE>)
         if constexpr (OUT == OUT_KEPT) {
           if (base < D) {
             // a row with an infinity or NaN has NaN throughout, so a block's values are all NaN or none
-            uint32_t m[VEC ? 1 : 2];
-            max_bits<VEC>(v[c], m);
-            keep8<VEC>(v[c], m, a.codes + row * code_pitch(D), a.exps + row * blocks_of(D), base, lane, D);
+            uint32_t m[L == EIGHT ? 1 : 2];
+            max_bits<L>(v[c], m);
+            keep8<L>(v[c], m, a.codes + row * code_pitch(D), a.exps + row * blocks_of(D), base, lane, D);
           }
         }
         F2 w[4], b[4];
@@ -178,12 +179,12 @@ __global__ void __launch_bounds__(kMostThreads<MODE>, 1024 / kMostThreads<MODE>)
             b[2 * k] = f2(t.x, t.y), b[2 * k + 1] = f2(t.z, t.w);
           }
         } else {
-          load_param<T, VEC>(w, a.w, a.w32, 1.f, group * D, base, lane, D);
-          load_param<T, VEC>(b, a.b, a.w32, 0.f, group * D, base, lane, D);
+          load_param<T, L>(w, a.w, a.w32, 1.f, group * D, base, lane, D);
+          load_param<T, L>(b, a.b, a.w32, 0.f, group * D, base, lane, D);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[c][i] = fma2(v[c][i], w[i], b[i]);
-        if constexpr (OUT != OUT_INT8) store8<T, VEC>(reinterpret_cast<T*>(a.y) + row * D, v[c], base, lane, D);
+        if constexpr (OUT != OUT_INT8) store8<T, L>(reinterpret_cast<T*>(a.y) + row * D, v[c], base, lane, D);
       }
     }
     if constexpr (OUT == OUT_INT8) {
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(kMostThreads<MODE>, 1024 / kMostThreads<MODE>)
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         if constexpr (NORM) {
-          zero_beyond<VEC>(v[c], first + c * 256, lane, D);
+          zero_beyond<L>(v[c], first + c * 256, lane, D);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float2 r = split(v[c][i]);
@@ -199,7 +200,7 @@ __global__ void __launch_bounds__(kMostThreads<MODE>, 1024 / kMostThreads<MODE>)
           }
         } else {
           uint32_t h[1];
-          max_bits<T, true>(raw[c], h);
+          max_bits<T, EIGHT>(raw[c], h);
           m = max(m, h[0]);
         }
       }
@@ -210,7 +211,7 @@ __global__ void __launch_bounds__(kMostThreads<MODE>, 1024 / kMostThreads<MODE>)
       for (int c = 0; c < CH; ++c) {
         uint32_t q[8];
         int8_codes(v[c], factor, q);
-        store_codes<VEC>(a.codes + row * code_pitch(D), q, first + c * 256, lane, D);
+        store_codes<L>(a.codes + row * code_pitch(D), q, first + c * 256, lane, D);
       }
     }
     // a warp that is a row ahead writes the other slots, and is not two ahead before every warp has passed
@@ -222,7 +223,7 @@ __global__ void __launch_bounds__(kMostThreads<MODE>, 1024 / kMostThreads<MODE>)
 
 template <typename T, bool VEC, int MODE, int CH, bool NORM, int OUT> int launch_mode(const RowArgs& a, int threads, cudaStream_t s) {
   auto k = row_fwd_kernel<T, VEC, MODE, CH, NORM, OUT>;
-  const size_t ring = kCopies<T, VEC> ? (size_t)kStages<CH, MODE> * CH * 8 * sizeof(T) * threads : 0;
+  const size_t ring = kCopies<T, kLayout<T, VEC>> ? (size_t)kStages<CH, MODE> * CH * 8 * sizeof(T) * threads : 0;
   const size_t smem = ring + (NORM && MODE != 2 ? (size_t)CH * 64 * (MODE == 0 ? 32 : threads) : 0);
   const int st = ensure_dyn_smem(reinterpret_cast<const void*>(k), (int)smem, "row kernel shared memory");
   if (st != FLB_OK) return st;

@@ -8,18 +8,25 @@
 namespace flb {
 namespace rows {
 
+constexpr int kBlock = 128;  // elements of the 8-bit kept form that share an exponent
+
 // A row's threads (one warp, or a whole block) cover it in chunks of 256 consecutive elements per warp,
-// eight elements a lane. VEC (rows that start on 16 bytes, a multiple of 8 elements wide): a lane's eight
-// are consecutive, one 16-byte access for 16-bit types, two for float32. Otherwise they lie 32 apart, so
-// that a warp's scalar accesses are still one contiguous run each. Both ways a warp's chunk is two blocks
-// of 128 elements: lanes 0-15 and 16-31, or a lane's first four and last four.
-template <bool VEC> struct Chunk {
-  // element j of the chunk that starts at `base`, and whether the row of D elements has it (VEC: all eight or none)
-  static __device__ __forceinline__ bool has(int base, int lane, int j, int D) {
-    return VEC ? base + lane * 8 < D : base + j * 32 + lane < D;
-  }
+// eight elements a lane, in one of three layouts, such that each access of a warp is one contiguous run:
+//   SCALARS  elements 32 apart, one access each (rows that do not start on 16 bytes, or not a multiple of 8 wide)
+//   EIGHT    eight consecutive elements, one 16-byte access for 16-bit types
+//   FOURS    two fours 128 apart, a 16-byte access each for float32
+// Each way a warp's chunk is two blocks of 128 elements: lanes 0-15 and 16-31 (EIGHT), or a lane's first
+// four and last four.
+enum Layout { SCALARS, EIGHT, FOURS };
+template <typename T, bool VEC> constexpr Layout kLayout = !VEC ? SCALARS : sizeof(T) == 4 ? FOURS : EIGHT;
+
+template <Layout L> struct Chunk {
+  // element j of the chunk that starts at `base`, and whether the row of D elements has it
   static __device__ __forceinline__ int at(int base, int lane, int j) {
-    return VEC ? base + lane * 8 + j : base + j * 32 + lane;
+    return L == EIGHT ? base + lane * 8 + j : L == FOURS ? base + (j >> 2) * kBlock + lane * 4 + (j & 3) : base + j * 32 + lane;
+  }
+  static __device__ __forceinline__ bool has(int base, int lane, int j, int D) {
+    return at(base, lane, L == EIGHT ? 0 : L == FOURS ? j & 4 : j) < D;
   }
 };
 
@@ -80,19 +87,14 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) 
 // are apart so that a loop can hold the next row's loads in flight.
 template <typename T> struct Raw8 { uint32_t w[sizeof(T) * 2]; };
 
-template <typename T, bool VEC>
+template <typename T, Layout L>
 __device__ __forceinline__ void load_raw(Raw8<T>& r, const T* __restrict__ row, int base, int lane, int D) {
-  if constexpr (VEC) {
-    const int p = base + lane * 8;
-    if (p < D) {
+  if constexpr (L != SCALARS) {
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + p) + i);
-        r.w[4 * i] = v.x, r.w[4 * i + 1] = v.y, r.w[4 * i + 2] = v.z, r.w[4 * i + 3] = v.w;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(T) * 2; ++i) r.w[i] = 0;
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+      const int p = Chunk<L>::at(base, lane, i * 16 / (int)sizeof(T));
+      const uint4 v = p < D ? __ldg(reinterpret_cast<const uint4*>(row + p)) : make_uint4(0, 0, 0, 0);
+      r.w[4 * i] = v.x, r.w[4 * i + 1] = v.y, r.w[4 * i + 2] = v.z, r.w[4 * i + 3] = v.w;
     }
   } else {
 #pragma unroll
@@ -125,25 +127,25 @@ __device__ __forceinline__ void to_scalars(const F2 (&v)[4], float (&s)[8]) {
     s[2 * i] = f.x, s[2 * i + 1] = f.y;
   }
 }
-template <typename T, bool VEC>
+template <typename T, Layout L>
 __device__ __forceinline__ void load8(F2 (&v)[4], const T* __restrict__ row, int base, int lane, int D) {
   Raw8<T> r;
-  load_raw<T, VEC>(r, row, base, lane, D);
+  load_raw<T, L>(r, row, base, lane, D);
   to_float<T>(r, v);
 }
-template <typename T, bool VEC>
+template <typename T, Layout L>
 __device__ __forceinline__ void store8(T* __restrict__ row, const F2 (&f)[4], int base, int lane, int D) {
   float v[8];
   to_scalars(f, v);
-  if constexpr (VEC) {
-    const int p = base + lane * 8;
-    if (p >= D) return;
-    if constexpr (sizeof(T) == 4) {
-      reinterpret_cast<float4*>(row + p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4*>(row + p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      *reinterpret_cast<uint4*>(row + p) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]),
-                                                      pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+  if constexpr (L != SCALARS) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+      const int p = Chunk<L>::at(base, lane, i * 16 / (int)sizeof(T));
+      if (p >= D) return;
+      if constexpr (sizeof(T) == 4)
+        *reinterpret_cast<float4*>(row + p) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+      else
+        *reinterpret_cast<uint4*>(row + p) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
     }
   } else {
 #pragma unroll
@@ -165,11 +167,16 @@ __device__ __forceinline__ uint32_t bytes4(uint32_t a, uint32_t b, uint32_t c, u
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 // Eight codes to a row of bytes whose start is 16-byte aligned (every code array's pitch is a multiple of 16)
-template <bool VEC>
+template <Layout L>
 __device__ __forceinline__ void store_codes(int8_t* __restrict__ row, const uint32_t (&q)[8], int base, int lane, int D) {
-  if constexpr (VEC) {
+  const uint32_t lo = bytes4(q[0], q[1], q[2], q[3]), hi = bytes4(q[4], q[5], q[6], q[7]);
+  if constexpr (L == EIGHT) {
     const int p = base + lane * 8;
-    if (p < D) *reinterpret_cast<uint2*>(row + p) = make_uint2(bytes4(q[0], q[1], q[2], q[3]), bytes4(q[4], q[5], q[6], q[7]));
+    if (p < D) *reinterpret_cast<uint2*>(row + p) = make_uint2(lo, hi);
+  } else if constexpr (L == FOURS) {
+    const int p = base + lane * 4;
+    if (p < D) *reinterpret_cast<uint32_t*>(row + p) = lo;
+    if (p + kBlock < D) *reinterpret_cast<uint32_t*>(row + p + kBlock) = hi;
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -178,12 +185,16 @@ __device__ __forceinline__ void store_codes(int8_t* __restrict__ row, const uint
     }
   }
 }
-template <bool VEC>
+template <Layout L>
 __device__ __forceinline__ uint2 load_codes(const int8_t* __restrict__ row, int base, int lane, int D) {
   uint2 r = make_uint2(0, 0);
-  if constexpr (VEC) {
+  if constexpr (L == EIGHT) {
     const int p = base + lane * 8;
     if (p < D) r = __ldg(reinterpret_cast<const uint2*>(row + p));
+  } else if constexpr (L == FOURS) {
+    const int p = base + lane * 4;
+    if (p < D) r.x = __ldg(reinterpret_cast<const uint32_t*>(row + p));
+    if (p + kBlock < D) r.y = __ldg(reinterpret_cast<const uint32_t*>(row + p + kBlock));
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -232,7 +243,6 @@ __device__ __forceinline__ void int8_codes(const F2 (&v)[4], float factor, uint3
 // computing them, an element of a 16-bit type times its inverse scale is exact in float32, and what comes
 // back fits bfloat16 without a second rounding. With a unit of a / 127 instead, the rounding error would
 // be smaller by up to a factor of two.
-constexpr int kBlock = 128;
 constexpr uint32_t kBadBlock = 255;
 
 // E for the block whose largest magnitude has these bits: with a = 1.f * 2^(x - 127) (x the exponent
@@ -250,7 +260,7 @@ __device__ __forceinline__ float scale_of(uint32_t e) {  // 2^(e - 127), NaN for
 // or NaN, whose exponent field is 255, is above every number.
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-// The largest magnitude's bits among a lane's eight elements (VEC), or its first four and last four. 16-bit
+// The largest magnitude's bits among a lane's eight elements (EIGHT), or its first four and last four. 16-bit
 // types: the packed halves' as 16-bit integers first, then as the float32 they are.
 template <typename T> __device__ __forceinline__ uint32_t float_bits(uint32_t h) {
   if constexpr (std::is_same<T, __half>::value) return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
@@ -262,36 +272,36 @@ __device__ __forceinline__ uint32_t max2_u16(uint32_t a, uint32_t b) {
   return r;
 }
 __device__ __forceinline__ uint32_t max_halves(uint32_t v) { return max(v & 0xffffu, v >> 16); }
-template <typename T, bool VEC> __device__ __forceinline__ void max_bits(const Raw8<T>& r, uint32_t (&m)[VEC ? 1 : 2]) {
+template <typename T, Layout L> __device__ __forceinline__ void max_bits(const Raw8<T>& r, uint32_t (&m)[L == EIGHT ? 1 : 2]) {
   if constexpr (sizeof(T) == 4) {
     constexpr uint32_t k = 0x7fffffffu;
     const uint32_t lo = max(__vimax3_u32(r.w[0] & k, r.w[1] & k, r.w[2] & k), r.w[3] & k);
     const uint32_t hi = max(__vimax3_u32(r.w[4] & k, r.w[5] & k, r.w[6] & k), r.w[7] & k);
-    if constexpr (VEC) m[0] = max(lo, hi); else m[0] = lo, m[1] = hi;
+    if constexpr (L == EIGHT) m[0] = max(lo, hi); else m[0] = lo, m[1] = hi;
   } else {
     constexpr uint32_t k = 0x7fff7fffu;
     const uint32_t lo = max2_u16(r.w[0] & k, r.w[1] & k), hi = max2_u16(r.w[2] & k, r.w[3] & k);
-    if constexpr (VEC) m[0] = float_bits<T>(max_halves(max2_u16(lo, hi)));
+    if constexpr (L == EIGHT) m[0] = float_bits<T>(max_halves(max2_u16(lo, hi)));
     else m[0] = float_bits<T>(max_halves(lo)), m[1] = float_bits<T>(max_halves(hi));
   }
 }
 // The same of eight floats. fmaxf passes over a NaN unless all are: for values of which all or none are.
-template <bool VEC> __device__ __forceinline__ void max_bits(const F2 (&f)[4], uint32_t (&m)[VEC ? 1 : 2]) {
+template <Layout L> __device__ __forceinline__ void max_bits(const F2 (&f)[4], uint32_t (&m)[L == EIGHT ? 1 : 2]) {
   float v[8];
   to_scalars(f, v);
   const float lo = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
   const float hi = fmaxf(fmaxf(fabsf(v[4]), fabsf(v[5])), fmaxf(fabsf(v[6]), fabsf(v[7])));
-  if constexpr (VEC) m[0] = __float_as_uint(fmaxf(lo, hi)) & 0x7fffffffu;
+  if constexpr (L == EIGHT) m[0] = __float_as_uint(fmaxf(lo, hi)) & 0x7fffffffu;
   else m[0] = __float_as_uint(lo) & 0x7fffffffu, m[1] = __float_as_uint(hi) & 0x7fffffffu;
 }
 
 // Keeps a lane's eight elements (chunk at `base`), whose largest magnitudes' bits are m: codes to `crow`,
 // the two blocks' E to `erow`. All 32 lanes take part; elements at or beyond D must be zero.
-template <bool VEC>
-__device__ __forceinline__ void keep8(const F2 (&v)[4], const uint32_t (&m)[VEC ? 1 : 2], int8_t* __restrict__ crow,
+template <Layout L>
+__device__ __forceinline__ void keep8(const F2 (&v)[4], const uint32_t (&m)[L == EIGHT ? 1 : 2], int8_t* __restrict__ crow,
                                       uint8_t* __restrict__ erow, int base, int lane, int D) {
   uint32_t q[8], e[2];
-  if constexpr (VEC) {
+  if constexpr (L == EIGHT) {
     e[0] = e[1] = block_exp(__reduce_max_sync(lane < 16 ? 0xffffu : 0xffff0000u, m[0]));
     if ((lane & 15) == 0 && base + lane * 8 < D) erow[(base + lane * 8) / kBlock] = (uint8_t)e[0];
   } else {
@@ -305,7 +315,7 @@ __device__ __forceinline__ void keep8(const F2 (&v)[4], const uint32_t (&m)[VEC 
     const float f[2] = {__uint_as_float((254u - e[0]) << 23), __uint_as_float((254u - e[1]) << 23)};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 r = split(fma2(v[i], f2(f[VEC ? 0 : i / 2]), f2(kRound)));
+      const float2 r = split(fma2(v[i], f2(f[L == EIGHT ? 0 : i / 2]), f2(kRound)));
       q[2 * i] = __float_as_uint(r.x), q[2 * i + 1] = __float_as_uint(r.y);
     }
   } else {
@@ -316,11 +326,11 @@ __device__ __forceinline__ void keep8(const F2 (&v)[4], const uint32_t (&m)[VEC 
     to_scalars(v, s);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const uint32_t ej = e[VEC ? 0 : j / 4];
+      const uint32_t ej = e[L == EIGHT ? 0 : j / 4];
       q[j] = code_of(fminf(fmaxf(s[j], -top), top) * __uint_as_float((254u - (ej > 249u ? 249u : ej)) << 23));
     }
   }
-  store_codes<VEC>(crow, q, base, lane, D);
+  store_codes<L>(crow, q, base, lane, D);
 }
 
 // What a lane's eight kept elements stand for (zero at or beyond D).
@@ -328,20 +338,20 @@ struct Kept8 {
   uint2 c;
   uint32_t e;  // two bytes: the E of the lane's first four and last four elements
 };
-template <bool VEC>
+template <Layout L>
 __device__ __forceinline__ uint32_t load_exps(const uint8_t* __restrict__ erow, int base, int lane, int D) {
-  if constexpr (VEC) return base + lane * 8 < D ? __ldg(erow + (base + lane * 8) / kBlock) : 1u;
+  if constexpr (L == EIGHT) return base + lane * 8 < D ? __ldg(erow + (base + lane * 8) / kBlock) : 1u;
   uint32_t e = base < D ? __ldg(erow + base / kBlock) : 1u;
   return e | (base + kBlock < D ? (uint32_t)__ldg(erow + base / kBlock + 1) : 1u) << 8;
 }
-template <bool VEC>
+template <Layout L>
 __device__ __forceinline__ Kept8 load_kept(const int8_t* __restrict__ crow, const uint8_t* __restrict__ erow,
                                            int base, int lane, int D) {
-  return Kept8{load_codes<VEC>(crow, base, lane, D), load_exps<VEC>(erow, base, lane, D)};
+  return Kept8{load_codes<L>(crow, base, lane, D), load_exps<L>(erow, base, lane, D)};
 }
-template <bool VEC> __device__ __forceinline__ void kept_to_float(const Kept8& k, F2 (&v)[4]) {
+template <Layout L> __device__ __forceinline__ void kept_to_float(const Kept8& k, F2 (&v)[4]) {
   codes_to_float(k.c, v);
-  const float s0 = scale_of(k.e & 0xffu), s1 = VEC ? s0 : scale_of(k.e >> 8);
+  const float s0 = scale_of(k.e & 0xffu), s1 = L == EIGHT ? s0 : scale_of(k.e >> 8);
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = mul2(v[i], f2(i < 2 ? s0 : s1));
 }
@@ -354,7 +364,7 @@ __host__ __device__ inline int64_t blocks_of(int64_t D) { return (D + kBlock - 1
 // Copies of the rows ahead, in shared memory. A thread copies, and later reads, only its own elements, so
 // its own wait for its copies is all the synchronisation there is. 16-bit rows that do not start on 16
 // bytes have no such copies (the smallest is 4 bytes): they are loaded when their turn comes.
-template <typename T, bool VEC> constexpr bool kCopies = VEC || sizeof(T) == 4;
+template <typename T, Layout L> constexpr bool kCopies = L != SCALARS || sizeof(T) == 4;
 
 __device__ __forceinline__ uint32_t shared_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool there) {
@@ -368,15 +378,15 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // One chunk's eight elements of this thread: slots [word group][thread], so that a warp's accesses are contiguous
-template <typename T, bool VEC>
+template <typename T, Layout L>
 __device__ __forceinline__ void copy8(uint8_t* slot, const T* row, int base, int lane, int D) {
   const uint32_t at = shared_addr(slot);
-  if constexpr (VEC) {
-    const int p = base + lane * 8;
-    const uint8_t* src = reinterpret_cast<const uint8_t*>(row + (p < D ? p : 0));
+  if constexpr (L != SCALARS) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-      copy_async<16>(at + (i * blockDim.x + threadIdx.x) * 16, src + 16 * i, p < D);
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+      const int p = Chunk<L>::at(base, lane, i * 16 / (int)sizeof(T));
+      copy_async<16>(at + (i * blockDim.x + threadIdx.x) * 16, row + (p < D ? p : 0), p < D);
+    }
   } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -385,8 +395,8 @@ __device__ __forceinline__ void copy8(uint8_t* slot, const T* row, int base, int
     }
   }
 }
-template <typename T, bool VEC> __device__ __forceinline__ void copied_raw(const uint8_t* slot, Raw8<T>& r) {
-  if constexpr (VEC) {
+template <typename T, Layout L> __device__ __forceinline__ void copied_raw(const uint8_t* slot, Raw8<T>& r) {
+  if constexpr (L != SCALARS) {
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
       const uint4 u = reinterpret_cast<const uint4*>(slot)[i * blockDim.x + threadIdx.x];
@@ -397,9 +407,9 @@ template <typename T, bool VEC> __device__ __forceinline__ void copied_raw(const
     for (int j = 0; j < 8; ++j) r.w[j % (sizeof(T) * 2)] = reinterpret_cast<const uint32_t*>(slot)[j * blockDim.x + threadIdx.x];
   }
 }
-template <typename T, bool VEC> __device__ __forceinline__ void copied8(const uint8_t* slot, F2 (&v)[4]) {
+template <typename T, Layout L> __device__ __forceinline__ void copied8(const uint8_t* slot, F2 (&v)[4]) {
   Raw8<T> r;
-  copied_raw<T, VEC>(slot, r);
+  copied_raw<T, L>(slot, r);
   to_float<T>(r, v);
 }
 
