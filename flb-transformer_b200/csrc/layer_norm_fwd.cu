@@ -8,7 +8,9 @@
 // output, so the variance is the second moment about the mean itself, not a difference of large sums. A
 // warp takes a row of up to 1024 elements and needs no barrier; a wider one gets a block, 16 elements a
 // thread (32 beyond 8192). A block walks over rows a fixed distance apart, the next rows on their way to shared
-// memory meanwhile.
+// memory meanwhile, the weight and bias there as float32 (in registers they cost a third of the warps: 129 us
+// against 105 for 32768 x 4096 bfloat16, which is 5.1 TB/s of reads and writes; re-read and converted for each
+// row 136).
 #include "rows.cuh"
 
 namespace flb {
@@ -69,10 +71,10 @@ template <int MODE> constexpr int kMostThreads = MODE == 0 ? 32 * kWarps : MODE 
 template <typename T, bool VEC, int MODE, int CH, bool NORM, int OUT>
 __global__ void __launch_bounds__(kMostThreads<MODE>, 1024 / kMostThreads<MODE>) row_fwd_kernel(const RowArgs a) {
   constexpr Layout L = kLayout<T, VEC>;
-  constexpr bool WARP = MODE == 0, COPY = kCopies<T, L>;
+  constexpr bool WARP = MODE == 0;
   constexpr bool PARAMS = NORM && MODE != 2;  // the weight and bias stay in shared memory, as float32
   constexpr int S = kStages<CH, MODE>;
-  // [CH][4][threads, or lanes of a warp's row] float4: weight and bias | [S][CH][threads] chunks of rows, with COPY
+  // [CH][4][threads, or lanes of a warp's row] float4: weight and bias | [S][CH] chunks of rows
   extern __shared__ __align__(16) uint8_t dyn[];
   __shared__ __align__(16) float slot[WARP ? 1 : 2][3][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -91,15 +93,13 @@ __global__ void __launch_bounds__(kMostThreads<MODE>, 1024 / kMostThreads<MODE>)
   const int param_threads = WARP ? 32 : (int)blockDim.x, param_thread = WARP ? lane : (int)threadIdx.x;
   float4* const params = reinterpret_cast<float4*>(dyn) + param_thread;
   uint8_t* const ring = dyn + (PARAMS ? (size_t)CH * 64 * param_threads : 0);
-  auto chunk_at = [&](int stage, int c) { return ring + (size_t)(stage * CH + c) * 8 * sizeof(T) * blockDim.x; };
+  auto chunk_at = [&](int stage, int c) { return ring + (size_t)(stage * CH + c) * copy_bytes<T, L>(blockDim.x); };
   auto issue = [&](int64_t r, int stage) {
-    if constexpr (COPY) {
-      if (r < rows) {
+    if (r < rows) {
 #pragma unroll
-        for (int c = 0; c < CH; ++c) copy8<T, L>(chunk_at(stage, c), x + r * a.ldx, first + c * 256, lane, D);
-      }
-      copies_commit();
+      for (int c = 0; c < CH; ++c) copy8<T, L>(chunk_at(stage, c), x + r * a.ldx, first + c * 256, lane, D);
     }
+    copies_commit();
   };
 #pragma unroll
   for (int k = 0; k < S - 1; ++k) issue(row0 + k * stride, k);
@@ -125,17 +125,18 @@ __global__ void __launch_bounds__(kMostThreads<MODE>, 1024 / kMostThreads<MODE>)
 
   int stage = 0, turn = 0;
   for (int64_t r = row0; r < rows; r += stride) {
+    meet_copies<L>();
     issue(r + (S - 1) * stride, stage == 0 ? S - 1 : stage - 1);  // where the row before this one was
     const int64_t row = group * rows + r;
     // the chunks' elements, and as they were loaded (for the largest magnitudes of plain rows)
     F2 v[CH][4];
     Raw8<T> raw[NORM ? 1 : CH];
-    if constexpr (COPY) copies_wait<S - 1>();
+    copies_wait<S - 1>();
+    meet_copies<L>();
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       Raw8<T>& u = raw[NORM ? 0 : c];
-      if constexpr (COPY) copied_raw<T, L>(chunk_at(stage, c), u);
-      else load_raw<T, L>(u, x + r * a.ldx, first + c * 256, lane, D);
+      copied_raw<T, L>(chunk_at(stage, c), u, x + r * a.ldx, first + c * 256, lane, D);
       to_float<T>(u, v[c]);
     }
     if constexpr (NORM) {
@@ -223,7 +224,7 @@ __global__ void __launch_bounds__(kMostThreads<MODE>, 1024 / kMostThreads<MODE>)
 
 template <typename T, bool VEC, int MODE, int CH, bool NORM, int OUT> int launch_mode(const RowArgs& a, int threads, cudaStream_t s) {
   auto k = row_fwd_kernel<T, VEC, MODE, CH, NORM, OUT>;
-  const size_t ring = kCopies<T, kLayout<T, VEC>> ? (size_t)kStages<CH, MODE> * CH * 8 * sizeof(T) * threads : 0;
+  const size_t ring = (size_t)kStages<CH, MODE> * CH * copy_bytes<T, kLayout<T, VEC>>(threads);
   const size_t smem = ring + (NORM && MODE != 2 ? (size_t)CH * 64 * (MODE == 0 ? 32 : threads) : 0);
   const int st = ensure_dyn_smem(reinterpret_cast<const void*>(k), (int)smem, "row kernel shared memory");
   if (st != FLB_OK) return st;

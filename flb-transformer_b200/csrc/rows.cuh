@@ -199,7 +199,7 @@ __device__ __forceinline__ uint2 load_codes(const int8_t* __restrict__ row, int 
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int p = base + j * 32 + lane;
-      const uint32_t v = p < D ? (uint32_t)(uint8_t)__ldg(row + p) : 0u;
+      const uint32_t v = p < D ? (uint32_t)(uint8_t)row[p] : 0u;
       if (j < 4) r.x |= v << (8 * j); else r.y |= v << (8 * (j - 4));
     }
   }
@@ -361,11 +361,12 @@ __host__ __device__ inline int64_t code_pitch(int64_t D) { return (D + 15) & ~(i
 __host__ __device__ inline int64_t blocks_of(int64_t D) { return (D + kBlock - 1) / kBlock; }
 
 // ---- rows ahead ------------------------------------------------------------------------------------
-// Copies of the rows ahead, in shared memory. A thread copies, and later reads, only its own elements, so
-// its own wait for its copies is all the synchronisation there is. 16-bit rows that do not start on 16
-// bytes have no such copies (the smallest is 4 bytes): they are loaded when their turn comes.
-template <typename T, Layout L> constexpr bool kCopies = L != SCALARS || sizeof(T) == 4;
-
+// Copies of the rows ahead, in shared memory, in pieces of 16 bytes. In the layouts of whole 16-byte accesses a
+// thread copies, and later reads, only its own elements, so its own wait for its copies is all the
+// synchronisation there is. Rows that do not start on 16 bytes (SCALARS) are copied from the 16 bytes that their
+// chunk starts in to those that it ends in, by the warp that reads them: it meets after the wait, and
+// before the place is copied to again. (A norm's forward over 16383 x 1001 float32 takes 26 us so, 30 with copies
+// of 4 bytes; over 16384 x 4095 bfloat16 81 us, 100 with the row loaded when its turn comes.)
 __device__ __forceinline__ uint32_t shared_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool there) {
   // with no source bytes the destination is filled with zeros
@@ -377,25 +378,37 @@ template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t dst, co
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// One chunk's eight elements of this thread: slots [word group][thread], so that a warp's accesses are contiguous
+// Bytes of a chunk of each of a block's warps. In the layouts of whole accesses: [word group][thread], so that a
+// warp's accesses are contiguous.
+template <typename T, Layout L> __host__ __device__ constexpr int copy_bytes(int threads) {
+  return L != SCALARS ? 8 * (int)sizeof(T) * threads : (256 * (int)sizeof(T) + 16) * (threads / 32);
+}
 template <typename T, Layout L>
 __device__ __forceinline__ void copy8(uint8_t* slot, const T* row, int base, int lane, int D) {
-  const uint32_t at = shared_addr(slot);
   if constexpr (L != SCALARS) {
+    const uint32_t at = shared_addr(slot);
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
       const int p = Chunk<L>::at(base, lane, i * 16 / (int)sizeof(T));
       copy_async<16>(at + (i * blockDim.x + threadIdx.x) * 16, row + (p < D ? p : 0), p < D);
     }
-  } else if constexpr (sizeof(T) == 4) {
+  } else {
+    constexpr int kPieces = 256 * (int)sizeof(T) / 16 + 1;
+    const uint32_t at = shared_addr(slot) + (threadIdx.x >> 5) * (256 * (int)sizeof(T) + 16);
+    const uintptr_t from = reinterpret_cast<uintptr_t>(row + base) & ~(uintptr_t)15, end = reinterpret_cast<uintptr_t>(row + D);
+    if (base < D) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int p = base + j * 32 + lane;
-      copy_async<4>(at + (j * blockDim.x + threadIdx.x) * 4, row + (p < D ? p : 0), p < D);
+      for (int i = 0; i < (kPieces + 31) / 32; ++i) {
+        // a piece that holds an element of the row; what else it holds is not read
+        const int n = i * 32 + lane;
+        const uintptr_t src = from + 16 * (uintptr_t)n;
+        if (n < kPieces && src < end) copy_async<16>(at + 16 * n, reinterpret_cast<const void*>(src), true);
+      }
     }
   }
 }
-template <typename T, Layout L> __device__ __forceinline__ void copied_raw(const uint8_t* slot, Raw8<T>& r) {
+template <typename T, Layout L>
+__device__ __forceinline__ void copied_raw(const uint8_t* slot, Raw8<T>& r, const T* row, int base, int lane, int D) {
   if constexpr (L != SCALARS) {
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
@@ -403,14 +416,47 @@ template <typename T, Layout L> __device__ __forceinline__ void copied_raw(const
       r.w[4 * i] = u.x, r.w[4 * i + 1] = u.y, r.w[4 * i + 2] = u.z, r.w[4 * i + 3] = u.w;
     }
   } else {
+    const uint8_t* mine = slot + (threadIdx.x >> 5) * (256 * (int)sizeof(T) + 16) + (reinterpret_cast<uintptr_t>(row + base) & 15u);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) r.w[j % (sizeof(T) * 2)] = reinterpret_cast<const uint32_t*>(slot)[j * blockDim.x + threadIdx.x];
+    for (int j = 0; j < 8; ++j) {
+      const bool has = base + j * 32 + lane < D;
+      if constexpr (sizeof(T) == 4) {
+        r.w[j] = has ? reinterpret_cast<const uint32_t*>(mine)[j * 32 + lane] : 0u;
+      } else {
+        const uint32_t v = has ? (uint32_t)reinterpret_cast<const uint16_t*>(mine)[j * 32 + lane] : 0u;
+        if (j & 1) r.w[j / 2] |= v << 16; else r.w[j / 2] = v;
+      }
+    }
   }
 }
-template <typename T, Layout L> __device__ __forceinline__ void copied8(const uint8_t* slot, F2 (&v)[4]) {
+template <typename T, Layout L>
+__device__ __forceinline__ void copied8(const uint8_t* slot, F2 (&v)[4], const T* row, int base, int lane, int D) {
   Raw8<T> r;
-  copied_raw<T, L>(slot, r);
+  copied_raw<T, L>(slot, r, row, base, lane, D);
   to_float<T>(r, v);
+}
+// The same for codes, 8 bytes a thread; their rows start on 16 bytes in every layout.
+template <Layout L>
+__device__ __forceinline__ void copy_codes(uint8_t* slot, const int8_t* row, int base, int lane, int D) {
+  const uint32_t at = shared_addr(slot);
+  if constexpr (L == SCALARS) {
+    const int p = base + lane * 16;
+    if (lane < 16 && p < D) copy_async<16>(at + (threadIdx.x >> 5) * 256 + lane * 16, row + p, true);
+  } else {
+#pragma unroll
+    for (int i = 0; i < (L == FOURS ? 2 : 1); ++i) {
+      const int p = Chunk<L>::at(base, lane, 4 * i);
+      copy_async<L == FOURS ? 4 : 8>(at + threadIdx.x * 8 + 4 * i, row + (p < D ? p : 0), p < D);
+    }
+  }
+}
+template <Layout L> __device__ __forceinline__ uint2 copied_codes(const uint8_t* slot, int base, int lane, int D) {
+  if constexpr (L != SCALARS) return reinterpret_cast<const uint2*>(slot)[threadIdx.x];
+  return load_codes<L>(reinterpret_cast<const int8_t*>(slot) + (threadIdx.x >> 5) * 256 - base, base, lane, D);
+}
+// Where a warp reads what all of its lanes have copied
+template <Layout L> __device__ __forceinline__ void meet_copies() {
+  if constexpr (L == SCALARS) __syncwarp();
 }
 
 // ---- reductions over a row ------------------------------------------------------------------------
