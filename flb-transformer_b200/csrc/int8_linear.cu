@@ -2,7 +2,7 @@
 //
 // tcgen05.mma kind::i8, 32-bit integer accumulators in TMEM (exact for K <= 32768: K 127^2 < 2^31). One block
 // a SM, persistent over units of work. Warp 0 loads by TMA into a ring, warp 1 issues the MMAs, warps 2-9 read
-// TMEM (two accumulators, so that a tile's epilogue runs beside the next one's MMAs). Two kernels:
+// TMEM (two accumulators, so that a tile's epilogue runs beside the next one's MMAs). Three kernels:
 //
 // int8_few_kernel, for few tokens or tiles. The weight rows are the M side of the instruction, 128 output
 // channels a tile, and the tokens its N side, NT of 16 to 128: a decoding step wastes little of a tile.
@@ -1018,10 +1018,16 @@ int int8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, 
   CUtensorMap tw, tx = {};
   if ((st = code_map(&tw, w_codes, N, ldw, K, g.many ? (g.pair ? g.width / 2 : g.width) : kChannels)) != FLB_OK) return st;
   if (!g.step && (st = code_map(&tx, x_codes, M, ldc, K, g.many ? kTokens : g.width)) != FLB_OK) return st;
-  const Int8Args a{x_scale, w_scale, bias, bias_dtype == FLB_F32, out, M, N,
-                   N % 2 == 0 && reinterpret_cast<uintptr_t>(out) % 4 == 0, x != nullptr, (int)((K + kStep - 1) / kStep), g.n_tiles, g.tiles,
-                   g.splits, N * K <= kWeightInL2 ? 1 : 16, (size_t)M * N * dtype_size(dtype) > kOutputInL2, reinterpret_cast<int32_t*>(p + l.parts), reinterpret_cast<uint32_t*>(p + l.counts),
-                   reinterpret_cast<uint32_t*>(p)};
+  Int8Args a = {};
+  a.sx = x_scale, a.sw = w_scale, a.bias = bias, a.bias32 = bias_dtype == FLB_F32;
+  a.out = out, a.M = M, a.N = N;
+  a.pairs = N % 2 == 0 && reinterpret_cast<uintptr_t>(out) % 4 == 0;
+  a.early = x != nullptr;
+  a.k_blocks = (int)((K + kStep - 1) / kStep), a.n_tiles = g.n_tiles, a.tiles = g.tiles, a.splits = g.splits;
+  a.group = N * K <= kWeightInL2 ? 1 : 16;
+  a.stream_out = (size_t)M * N * dtype_size(dtype) > kOutputInL2;
+  a.parts = reinterpret_cast<int32_t*>(p + l.parts), a.counts = reinterpret_cast<uint32_t*>(p + l.counts);
+  a.error = reinterpret_cast<uint32_t*>(p);
   const StepArgs sa{x, ldx, K % 8 == 0 && ldx * dtype_size(dtype) % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0, (int)K};
   if (g.step) {
     switch (dtype) {
