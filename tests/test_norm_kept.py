@@ -106,7 +106,8 @@ def test_int8_arguments():
     assert int8(x=17) == FLB_ALIGN and int8(out=17) == FLB_ALIGN and int8(ws=18) == FLB_ALIGN
     assert int8(work=None) == FLB_WORKSPACE and int8(n=16) == FLB_WORKSPACE and int8(work=128) == FLB_ALIGN
     assert int8(M=0, x=None, out=None) == 0 and int8(N=0, wc=None, ws=None) == 0
-    assert L.flb_int8_linear_workspace_bytes(4, 8, 64, 0) > L.flb_int8_linear_workspace_bytes(4, 8, 64, 1) > 0
+    assert L.flb_int8_linear_workspace_bytes(400, 8, 64, 0) > L.flb_int8_linear_workspace_bytes(400, 8, 64, 1) > 0
+    assert L.flb_int8_linear_workspace_bytes(4, 8, 64, 0) > 0
     assert L.flb_int8_linear_workspace_bytes(0, 8, 64, 0) == 0 and L.flb_int8_linear_workspace_bytes(4, 8, 0, 0) == 0
     assert L.flb_int8_rows(16, 8, 16, 16, 2, 8, 5, None) == FLB_DTYPE and L.flb_int8_rows(16, 8, 24, 16, 2, 8, F32, None) == FLB_ALIGN
     assert L.flb_int8_rows(None, 8, 16, 16, 2, 8, F32, None) == FLB_SHAPE and L.flb_int8_rows(None, 8, None, None, 0, 8, F32, None) == 0
