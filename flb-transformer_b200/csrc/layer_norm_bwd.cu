@@ -148,8 +148,8 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
       if constexpr (KEPT) kept_to_float<L>(Kept8{copied_codes<L>(part_of(stage, c, false), base, lane, D), e[c]}, x);
       else copied8<T, L>(part_of(stage, c, false), x, x_row(row), base, lane, D);
     };
-    // h = x h1 + h0
-    const float h1 = KEPT ? 1.f : rs, h0 = KEPT ? 0.f : -m * rs;
+    // h = (x - m) h1, the difference first, as in the forward: exact where x is near the mean
+    const float h1 = KEPT ? 1.f : rs;
     F2 t1 = f2(0.f), t2 = f2(0.f);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
       values(c, x, dy);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {  // dy is zero beyond D
-        const F2 h = KEPT ? x[i] : fma2(x[i], f2(h1), f2(h0)), gw = mul2(dy[i], w[c][i]);
+        const F2 h = KEPT ? x[i] : mul2(add2(x[i], f2(-m)), f2(h1)), gw = mul2(dy[i], w[c][i]);
         dw[c][i] = fma2(dy[i], h, dw[c][i]);
         db[c][i] = add2(db[c][i], dy[i]);
         t1 = add2(t1, gw);
@@ -178,17 +178,18 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
       }
       turn ^= 1;
     }
-    // dx = rs (dy w - s1 - h s2) = rs w dy + x c1 + c0
+    // dx = rs (dy w - s1 - h s2) = rs w dy + (x - m) c1 + c0
     s1 *= inv_d;
     s2 *= inv_d;
-    const float c1 = -rs * s2 * h1, c0 = -rs * fmaf(s2, h0, s1);
+    const float c1 = -rs * s2 * h1, c0 = -rs * s1;
     T* dx = reinterpret_cast<T*>(a.dx) + (group * a.R + row) * D;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       F2 x[4], dy[4];
       values(c, x, dy);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = fma2(mul2(f2(rs), w[c][i]), dy[i], fma2(x[i], f2(c1), f2(c0)));
+      for (int i = 0; i < 4; ++i)
+        x[i] = fma2(mul2(f2(rs), w[c][i]), dy[i], fma2(KEPT ? x[i] : add2(x[i], f2(-m)), f2(c1), f2(c0)));
       store8<T, L>(dx, x, first + c * 256, lane, D);
     }
     stage = stage + 1 == S ? 0 : stage + 1;

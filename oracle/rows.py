@@ -80,7 +80,8 @@ def layer_norm_backward(h, rs, dh, w, dy, dtype, wdtype, keep8=False, groups=Non
     d2 = U * (SUM + 4) * (gw * h).abs().mean(-1, keepdim=True) + (gw.abs() * dh).mean(-1, keepdim=True)
     dx = rs * (gw - s1 - h * s2)
     rel = U * (SUM + 20)
-    tol = rs * (d1 + h.abs() * d2 + s2.abs() * dh + 4 * U * (gw.abs() + s1.abs() + (h * s2).abs())) + rel * dx.abs()
+    # (h + dh)(s2 + d2) - h s2, and the roundings of the three terms
+    tol = rs * (d1 + (h.abs() + dh) * d2 + s2.abs() * dh + 4 * U * (gw.abs() + s1.abs() + (h * s2).abs())) + rel * dx.abs()
     # 1/sigma carries the error of the centred values' second moment
     tol = tol * (1 + 1e-3) + half_step(dtype) * dx.abs() + floor_of(dtype)
     shape = groups or (dy.shape[-1],)
