@@ -377,7 +377,7 @@ __host__ __device__ inline int64_t blocks_of(int64_t D) { return (D + kBlock - 1
 // synchronisation there is. Rows that do not start on 16 bytes (SCALARS) are copied from the 16 bytes that their
 // chunk starts in to those that it ends in, by the warp that reads them: it meets after the wait, and
 // before the place is copied to again. (A norm's forward over 16383 x 1001 float32 takes 26 us so, 30 with copies
-// of 4 bytes; over 16384 x 4095 bfloat16 81 us, 100 with the row loaded when its turn comes.)
+// of 4 bytes; over 16384 x 4095 bfloat16 79 us, 100 with the row loaded when its turn comes.)
 __device__ __forceinline__ uint32_t shared_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool there) {
   // with no source bytes the destination is filled with zeros
