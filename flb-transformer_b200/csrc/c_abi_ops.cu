@@ -19,7 +19,7 @@ int int8_rows(const void* x, int64_t ldx, int8_t* codes, float* scale, int64_t R
 size_t int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, bool quantise);
 int int8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, const float* x_scale, const int8_t* w_codes,
                 int64_t ldw, const float* w_scale, const void* bias, int bias_dtype, void* out, int64_t M, int64_t N,
-                int64_t K, int dtype, void* ws, int check_timeout, cudaStream_t s);
+                int64_t K, int dtype, void* ws, int check_timeout, int drop, uint32_t limit, cudaStream_t s);
 int pack8(const void* x, int8_t* codes, uint8_t* exps, int64_t R, int64_t D, int dtype, cudaStream_t s);
 int unpack8(const int8_t* codes, const uint8_t* exps, void* out, int64_t R, int64_t D, int dtype, cudaStream_t s);
 int gate_fwd(const void* x, const void* z, void* y, int8_t* cx, uint8_t* ex, int8_t* cz, uint8_t* ez, int64_t R,
@@ -75,6 +75,33 @@ int check_product(int64_t M, int64_t N, int64_t K) {
   if (M > INT32_MAX - 1024 || N > INT32_MAX - 1024 || (M > 0 && N > ((int64_t)1 << 44) / M))
     return fail(FLB_ERR_SHAPE, "int8_linear: too many rows");
   return FLB_OK;
+}
+
+int int8_linear_checked(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, const float* x_scale, const int8_t* w_codes,
+                        int64_t ldw, const float* w_scale, const void* bias, int bias_dtype, void* out, int64_t M, int64_t N,
+                        int64_t K, int dtype, void* workspace, size_t workspace_bytes, int check_timeout, int drop, uint32_t limit,
+                        void* stream) {
+  if (dtype_size(dtype) == 0) return fail(FLB_ERR_DTYPE, "int8_linear: dtype must be f32, f16 or bf16");
+  if (bias && bias_dtype != FLB_F32 && bias_dtype != dtype)
+    return fail(FLB_ERR_DTYPE, "int8_linear: the bias must be float32 or of the output's dtype");
+  int st = check_product(M, N, K);
+  if (st != FLB_OK) return st;
+  if (M == 0 || N == 0) return FLB_OK;
+  if (!x == !x_codes || !x_codes != !x_scale) return fail(FLB_ERR_SHAPE, "int8_linear: either x, or x_codes and x_scale");
+  if (!w_codes || !w_scale || !out) return fail(FLB_ERR_SHAPE, "int8_linear: null weight or out");
+  if (x ? ldx < 0 : ldc < K) return fail(FLB_ERR_SHAPE, "int8_linear: bad row pitch of x");
+  if (ldw < K) return fail(FLB_ERR_SHAPE, "int8_linear: bad row pitch of the weight");
+  if (off(w_codes, 16) || ldw % 16 || (x_codes && (off(x_codes, 16) || ldc % 16)))
+    return fail(FLB_ERR_ALIGN, "int8_linear: codes must start every row on 16 bytes");
+  const size_t es = (size_t)dtype_size(dtype);
+  if (off(x, es) || off(out, es) || off(w_scale, 4) || off(x_scale, 4) || off(bias, bias ? (size_t)dtype_size(bias_dtype) : 1))
+    return fail(FLB_ERR_ALIGN, "int8_linear: pointers must be aligned to their element size");
+  const size_t need = int8_linear_workspace_bytes(M, N, K, x != nullptr);
+  if (!workspace || workspace_bytes < need)
+    return fail(FLB_ERR_WORKSPACE, "int8_linear: workspace smaller than flb_int8_linear_workspace_bytes()");
+  if (off(workspace, 256)) return fail(FLB_ERR_ALIGN, "int8_linear: workspace must be 256-byte aligned");
+  return int8_linear(x, ldx, x_codes, ldc, x_scale, w_codes, ldw, w_scale, bias, bias_dtype, out, M, N, K, dtype, workspace,
+                     check_timeout, drop, limit, as_stream(stream));
 }
 
 }  // namespace
@@ -167,27 +194,18 @@ int flb_int8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t l
                     const int8_t* w_codes, int64_t ldw, const float* w_scale, const void* bias, int bias_dtype, void* out,
                     int64_t M, int64_t N, int64_t K, int dtype, void* workspace, size_t workspace_bytes, int check_timeout,
                     void* stream) {
-  if (dtype_size(dtype) == 0) return fail(FLB_ERR_DTYPE, "int8_linear: dtype must be f32, f16 or bf16");
-  if (bias && bias_dtype != FLB_F32 && bias_dtype != dtype)
-    return fail(FLB_ERR_DTYPE, "int8_linear: the bias must be float32 or of the output's dtype");
-  int st = check_product(M, N, K);
-  if (st != FLB_OK) return st;
-  if (M == 0 || N == 0) return FLB_OK;
-  if (!x == !x_codes || !x_codes != !x_scale) return fail(FLB_ERR_SHAPE, "int8_linear: either x, or x_codes and x_scale");
-  if (!w_codes || !w_scale || !out) return fail(FLB_ERR_SHAPE, "int8_linear: null weight or out");
-  if (x ? ldx < 0 : ldc < K) return fail(FLB_ERR_SHAPE, "int8_linear: bad row pitch of x");
-  if (ldw < K) return fail(FLB_ERR_SHAPE, "int8_linear: bad row pitch of the weight");
-  if (off(w_codes, 16) || ldw % 16 || (x_codes && (off(x_codes, 16) || ldc % 16)))
-    return fail(FLB_ERR_ALIGN, "int8_linear: codes must start every row on 16 bytes");
-  const size_t es = (size_t)dtype_size(dtype);
-  if (off(x, es) || off(out, es) || off(w_scale, 4) || off(x_scale, 4) || off(bias, bias ? (size_t)dtype_size(bias_dtype) : 1))
-    return fail(FLB_ERR_ALIGN, "int8_linear: pointers must be aligned to their element size");
-  const size_t need = int8_linear_workspace_bytes(M, N, K, x != nullptr);
-  if (!workspace || workspace_bytes < need)
-    return fail(FLB_ERR_WORKSPACE, "int8_linear: workspace smaller than flb_int8_linear_workspace_bytes()");
-  if (off(workspace, 256)) return fail(FLB_ERR_ALIGN, "int8_linear: workspace must be 256-byte aligned");
-  return int8_linear(x, ldx, x_codes, ldc, x_scale, w_codes, ldw, w_scale, bias, bias_dtype, out, M, N, K, dtype, workspace,
-                     check_timeout, as_stream(stream));
+  return int8_linear_checked(x, ldx, x_codes, ldc, x_scale, w_codes, ldw, w_scale, bias, bias_dtype, out, M, N, K, dtype, workspace,
+                             workspace_bytes, check_timeout, -1, 0, stream);
+}
+
+int flb_int8_linear_wait_test(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, const float* x_scale,
+                              const int8_t* w_codes, int64_t ldw, const float* w_scale, const void* bias, int bias_dtype, void* out,
+                              int64_t M, int64_t N, int64_t K, int dtype, void* workspace, size_t workspace_bytes, int check_timeout,
+                              int64_t drop_step, uint32_t spin_limit, void* stream) {
+  if (drop_step < -1 || drop_step > INT32_MAX || spin_limit < 1)
+    return fail(FLB_ERR_SHAPE, "int8_linear wait test: drop_step >= -1 and spin_limit >= 1 required");
+  return int8_linear_checked(x, ldx, x_codes, ldc, x_scale, w_codes, ldw, w_scale, bias, bias_dtype, out, M, N, K, dtype, workspace,
+                             workspace_bytes, check_timeout, (int)drop_step, spin_limit, stream);
 }
 
 int flb_pack8(const void* x, int8_t* codes, uint8_t* exps, int64_t R, int64_t D, int dtype, void* stream) {

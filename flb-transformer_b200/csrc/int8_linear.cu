@@ -38,6 +38,10 @@ constexpr int kRing = 198 * 1024;
 constexpr int kEpilogue = 256;   // threads that read TMEM and store
 constexpr int kGemmThreads = 64 + kEpilogue;
 constexpr uint32_t kWaitLimit = 1u << 20;  // polls, each of which the hardware may hold for a while
+// A wait that gives up leaves wrong numbers behind it, but nothing in flight: every kernel's loader waits for its last copies and
+// the thread that issues MMAs for its own (the barrier `drain`), with this limit, before the block gives up its shared
+// memory and TMEM.
+constexpr uint32_t kDrainLimit = 1u << 20;
 
 template <int NT> constexpr int stage_bytes() { return (kChannels + NT) * kStep; }
 template <int NT> constexpr int stages() { return kRing / stage_bytes<NT>(); }
@@ -58,7 +62,16 @@ struct Int8Args {
   int32_t* parts;     // [tiles][splits][NT][128], splits > 1
   uint32_t* counts;   // [tiles], zero
   uint32_t* error;
+  uint32_t limit;     // polls of a wait (kWaitLimit)
+  int drop;           // a step that the first block, or pair, never loads (a test of the waits), or -1
 };
+
+// One thread's MMAs so far are done when this returns, or the limit has run out. issued: there are any.
+__device__ __forceinline__ void drain_mma(uint64_t* drain, bool issued, uint32_t* error) {
+  if (!issued) return;
+  umma_commit(drain);
+  if (!mbar_wait(drain, 0, kDrainLimit)) atomicExch(error, 1u);
+}
 
 // signed 8-bit operands, both K-major, 32-bit integer accumulators
 template <int NT> constexpr uint32_t idesc_i8() {
@@ -127,7 +140,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   constexpr int S = stages<NT>();
   constexpr uint32_t kBytes = stage_bytes<NT>();
   extern __shared__ uint8_t dyn[];
-  __shared__ __align__(8) uint64_t full[S], empty[S], acc_full[2], acc_empty[2];
+  __shared__ __align__(8) uint64_t full[S], empty[S], acc_full[2], acc_empty[2], drain;
   __shared__ uint32_t tmem_base, last_flag;
   __shared__ __align__(16) float scales[kEpilogue / 32][NT > 64 ? NT / 2 : 32];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
@@ -138,6 +151,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     tma_prefetch_desc(&tm_x);
     for (int i = 0; i < S; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
     for (int i = 0; i < 2; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], kEpilogue);
+    mbar_init(&drain, 1);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -162,10 +176,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       // its way before the wait.
       bool ok = true;
       uint32_t it = 0, early = 0;
+      auto lost = [&](uint32_t i) { return blockIdx.x == 0 && (int)i == a.drop; };
       for (int u = blockIdx.x; a.early && u < units && early < (uint32_t)S; u += gridDim.x) {
         int k0, k1;
         k_range(u % a.splits, k0, k1);
         for (int k = k0; k < k1 && early < (uint32_t)S; ++k, ++early) {
+          if (lost(early)) continue;
           mbar_arrive_expect_tx(&full[early], kBytes);
           tma_load_2d(ring + (size_t)early * kBytes, &tm_w, &full[early], k * kStep, (u / a.splits) % a.n_tiles * kChannels);
         }
@@ -179,22 +195,22 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         for (int k = k0; k < k1; ++k, ++it) {
           const int s = it % S;
           uint8_t* st = ring + (size_t)s * kBytes;
+          if (it >= early && it >= (uint32_t)S && !mbar_wait(&empty[s], ((it / S) & 1) ^ 1, a.limit)) {
+            ok = false;
+            break;
+          }
+          if (lost(it)) continue;
           if (it >= early) {
-            if (it >= (uint32_t)S && !mbar_wait(&empty[s], ((it / S) & 1) ^ 1, kWaitLimit)) {
-              ok = false;
-              break;
-            }
             mbar_arrive_expect_tx(&full[s], kBytes);
             tma_load_2d(st, &tm_w, &full[s], k * kStep, n0);
           }
           tma_load_2d(st + kChannels * kStep, &tm_x, &full[s], k * kStep, m0);
         }
       }
-      if (!ok) {
-        atomicExch(a.error, 1u);
-        // the copies still in flight land before the block's shared memory is given up
-        for (uint32_t i = it > (uint32_t)S ? it - S : 0; i < it; ++i) mbar_wait(&full[i % S], (i / S) & 1, kWaitLimit);
-      }
+      // (every early step is among these: their x tiles were issued without a wait)
+      for (uint32_t i = it > (uint32_t)S ? it - S : 0; i < it; ++i)
+        if (!lost(i) && !mbar_wait(&full[i % S], (i / S) & 1, kDrainLimit)) ok = false;
+      if (!ok) atomicExch(a.error, 1u);
     }
   } else if (warp == 1) {
     if (lane == 0) {
@@ -203,7 +219,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       bool ok = true;
       for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++local) {
         const uint32_t b = local & 1;
-        if (local >= 2 && !mbar_wait(&acc_empty[b], ((local >> 1) & 1) ^ 1, kWaitLimit)) {
+        if (local >= 2 && !mbar_wait(&acc_empty[b], ((local >> 1) & 1) ^ 1, a.limit)) {
           ok = false;
           break;
         }
@@ -212,7 +228,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         k_range(u % a.splits, k0, k1);
         for (int k = k0; k < k1; ++k, ++it) {
           const int s = it % S;
-          if (!mbar_wait(&full[s], (it / S) & 1, kWaitLimit)) {
+          if (!mbar_wait(&full[s], (it / S) & 1, a.limit)) {
             ok = false;
             break;
           }
@@ -229,6 +245,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         if (ok) umma_commit(&acc_full[b]);
       }
       if (!ok) atomicExch(a.error, 1u);
+      drain_mma(&drain, it > 0, a.error);
     }
   } else {
     // each epilogue warp has the 32 TMEM lanes, here channels, of its number mod 4, and half of the tokens
@@ -237,7 +254,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     const int q = warp & 3, first = (warp - 2) / 4 * COLS;
     const bool has_cols = first < NT;
     float* sx = scales[warp - 2];
-    uint32_t local = 0, limit = kWaitLimit;
+    uint32_t local = 0, limit = a.limit;
     wait_predecessor();
     for (int u = blockIdx.x; u < units; u += gridDim.x, ++local) {
       const uint32_t b = local & 1;
@@ -331,6 +348,7 @@ template <> struct Group<false> {
   static __device__ __forceinline__ void load(void* dst, const void* tmap, uint64_t* bar, int c0, int c1) { tma_load_2d(dst, tmap, bar, c0, c1); }
   static __device__ __forceinline__ void mma(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) { umma_i8(d, da, db, idesc, acc); }
   static __device__ __forceinline__ void commit(uint64_t* bar) { umma_commit(bar); }
+  static __device__ __forceinline__ void arrive_all(uint64_t* bar) { mbar_arrive(bar); }
   static __device__ __forceinline__ void arrive_first(uint64_t* bar) { mbar_arrive(bar); }
   static __device__ __forceinline__ void meet() { __syncthreads(); }
 };
@@ -342,12 +360,13 @@ template <> struct Group<true> {
   static __device__ __forceinline__ void dealloc(uint32_t t, uint32_t n) {
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(t), "r"(n) : "memory");
   }
-  // this barrier in the pair's first block
-  static __device__ __forceinline__ uint32_t first(uint64_t* bar) {
+  // this barrier in one of the pair's blocks
+  static __device__ __forceinline__ uint32_t in_block(uint64_t* bar, int block) {
     uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(bar)));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(bar)), "r"(block));
     return r;
   }
+  static __device__ __forceinline__ uint32_t first(uint64_t* bar) { return in_block(bar, 0); }
   // into this block's shared memory; the bytes count at the first block's barrier
   static __device__ __forceinline__ void load(void* dst, const void* tmap, uint64_t* bar, int c0, int c1) {
     asm volatile(
@@ -371,9 +390,11 @@ template <> struct Group<true> {
                  "h"((uint16_t)3)
                  : "memory");
   }
-  static __device__ __forceinline__ void arrive_first(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(first(bar)) : "memory");
+  static __device__ __forceinline__ void arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
   }
+  static __device__ __forceinline__ void arrive_all(uint64_t* bar) { arrive(in_block(bar, 0)), arrive(in_block(bar, 1)); }
+  static __device__ __forceinline__ void arrive_first(uint64_t* bar) { arrive(first(bar)); }
   static __device__ __forceinline__ void meet() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -431,7 +452,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     int8_step_kernel(const __grid_constant__ CUtensorMap tm_w, const StepArgs x, const Int8Args a) {
   constexpr int S = kStepStages, NT = kStepTokens;
   extern __shared__ uint8_t dyn[];
-  __shared__ __align__(8) uint64_t full[S], empty[S], acc_full[2], acc_empty[2], rows_ready;
+  __shared__ __align__(8) uint64_t full[S], empty[S], acc_full[2], acc_empty[2], rows_ready, drain;
   __shared__ uint32_t tmem_base, amax[NT];
   __shared__ __align__(16) float scale[NT], factor[NT];
   uint8_t* const ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
@@ -446,7 +467,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     tma_prefetch_desc(&tm_w);
     for (int i = 0; i < S; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
     for (int i = 0; i < 2; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], 128);
-    mbar_init(&rows_ready, 1);
+    mbar_init(&rows_ready, 1), mbar_init(&drain, 1);
     fence_mbar_init();
   }
   if (threadIdx.x >= 64 && threadIdx.x < 64 + NT) amax[threadIdx.x - 64] = 0;
@@ -467,38 +488,38 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     if (lane == 0) {
       bool ok = true;
       uint32_t it = 0;
+      auto lost = [&](uint32_t i) { return blockIdx.x == 0 && (int)i == a.drop; };
       for (int tile = first_tile; tile < a.tiles && ok; tile += stride) {
         for (int k = k0; k < k1; ++k, ++it) {
           const int s = it % S;
-          if (it >= (uint32_t)S && !mbar_wait(&empty[s], ((it / S) & 1) ^ 1, kWaitLimit)) {
+          if (it >= (uint32_t)S && !mbar_wait(&empty[s], ((it / S) & 1) ^ 1, a.limit)) {
             ok = false;
             break;
           }
+          if (lost(it)) continue;
           mbar_arrive_expect_tx(&full[s], kStepTile);
           tma_load_2d(ring + s * kStepTile, &tm_w, &full[s], k * kStep, tile * kChannels);
         }
       }
-      if (!ok) {
-        atomicExch(a.error, 1u);
-        // the copies still in flight land before the block's shared memory is given up
-        for (uint32_t i = it > (uint32_t)S ? it - S : 0; i < it; ++i) mbar_wait(&full[i % S], (i / S) & 1, kWaitLimit);
-      }
+      for (uint32_t i = it > (uint32_t)S ? it - S : 0; i < it; ++i)
+        if (!lost(i) && !mbar_wait(&full[i % S], (i / S) & 1, kDrainLimit)) ok = false;
+      if (!ok) atomicExch(a.error, 1u);
     }
   } else if (warp == 1) {
     if (lane == 0) {
       constexpr uint32_t idesc = idesc_i8<NT>();
       uint32_t it = 0, local = 0;
-      bool ok = mbar_wait(&rows_ready, 0, kWaitLimit);
+      bool ok = mbar_wait(&rows_ready, 0, a.limit);
       for (int tile = first_tile; tile < a.tiles && ok; tile += stride, ++local) {
         const uint32_t b = local & 1;
-        if (local >= 2 && !mbar_wait(&acc_empty[b], ((local >> 1) & 1) ^ 1, kWaitLimit)) {
+        if (local >= 2 && !mbar_wait(&acc_empty[b], ((local >> 1) & 1) ^ 1, a.limit)) {
           ok = false;
           break;
         }
         tc_fence_after();
         for (int k = k0; k < k1; ++k, ++it) {
           const int s = it % S;
-          if (!mbar_wait(&full[s], (it / S) & 1, kWaitLimit)) {
+          if (!mbar_wait(&full[s], (it / S) & 1, a.limit)) {
             ok = false;
             break;
           }
@@ -512,6 +533,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         if (ok) umma_commit(&acc_full[b]);
       }
       if (!ok) atomicExch(a.error, 1u);
+      drain_mma(&drain, it > 0, a.error);
     }
   } else {
     const int et = threadIdx.x - 64, M = (int)a.M;
@@ -575,7 +597,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     if (warp < 6) {
       // these four warps have the 32 TMEM lanes, here channels, of their number mod 4
       const int q = warp & 3;
-      uint32_t local = 0, limit = kWaitLimit;
+      uint32_t local = 0, limit = a.limit;
       for (int tile = first_tile; tile < a.tiles; tile += stride, ++local) {
         const uint32_t b = local & 1;
         if (!mbar_wait(&acc_full[b], (local >> 1) & 1, limit)) {
@@ -649,7 +671,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   constexpr int S = many_stages<PAIR, NC>(), BLOCKS = PAIR ? 2 : 1, ROWS = many_rows<PAIR, NC>();
   constexpr uint32_t kBytes = many_stage_bytes<PAIR, NC>();
   extern __shared__ uint8_t dyn[];
-  __shared__ __align__(8) uint64_t full[S], empty[S], acc_full[2], acc_empty[2];
+  // other_done: in the first block, the second one's loader has issued its last load
+  __shared__ __align__(8) uint64_t full[S], empty[S], acc_full[2], acc_empty[2], drain, other_done;
   __shared__ uint32_t tmem_base;
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -661,6 +684,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     tma_prefetch_desc(&tm_out);
     for (int i = 0; i < S; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
     for (int i = 0; i < 2; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], BLOCKS * kEpilogue / 32);
+    mbar_init(&drain, 1), mbar_init(&other_done, 1);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -686,6 +710,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     if (lane == 0) {
       bool ok = true;
       uint32_t it = 0;
+      auto lost = [&](uint32_t i) { return worker == 0 && (int)i == a.drop; };
       wait_predecessor();
       for (int tile = worker; tile < a.tiles && ok; tile += workers) {
         int m0, n0;
@@ -693,10 +718,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         if (PAIR) n0 += place_in_pair * ROWS;
         for (int k = 0; k < a.k_blocks; ++k, ++it) {
           const int s = it % S;
-          if (it >= (uint32_t)S && !mbar_wait(&empty[s], ((it / S) & 1) ^ 1, kWaitLimit)) {
+          if (it >= (uint32_t)S && !mbar_wait(&empty[s], ((it / S) & 1) ^ 1, a.limit)) {
             ok = false;
             break;
           }
+          if (lost(it)) continue;
           uint8_t* st = ring + (size_t)s * kBytes;
           // the first block expects both blocks' bytes (the other's may land before: the count goes below zero)
           if (place_in_pair == 0) mbar_arrive_expect_tx(&full[s], BLOCKS * kBytes);
@@ -705,17 +731,35 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
       }
       const uint32_t last = it > (uint32_t)S ? it - S : 0;
-      if (!ok) {
-        atomicExch(a.error, 1u);
-        // the copies still in flight land before the blocks' shared memory is given up: the other block
-        // waits for this one below
-        if (place_in_pair == 0)
-          for (uint32_t i = last; i < it; ++i) mbar_wait(&full[i % S], (i / S) & 1, kWaitLimit);
-      } else if (PAIR) {
-        // the first block's arrivals at this block's barriers are all in before the block ends
-        for (uint32_t i = last; i < it; ++i)
-          if (!mbar_wait(&empty[i % S], (i / S) & 1, kWaitLimit)) atomicExch(a.error, 1u);
+      const bool complete = ok;
+      if (place_in_pair == 0) {
+        // both blocks' copies count here: the other block waits for this one at the end
+        uint32_t landed = 0;  // of the ring's stages
+        for (uint32_t i = last; i < it; ++i) {
+          if (lost(i)) continue;
+          if (mbar_wait(&full[i % S], (i / S) & 1, kDrainLimit)) landed |= 1u << (i % S);
+          else ok = false;
+        }
+        if (PAIR && !complete && mbar_wait(&other_done, 0, kDrainLimit)) {
+          // The other block's wait may have seen what this one's gave up on: its copies for up to a ring of further steps
+          // come down on barriers where nothing expects them yet. (It issued none where the last one there has not landed.)
+          for (uint32_t i = it; i < it + S; ++i) {
+            if (!(landed >> (i % S) & 1)) continue;
+            mbar_arrive_expect_tx(&full[i % S], kBytes);
+            mbar_wait(&full[i % S], (i / S) & 1, kDrainLimit >> 6);  // runs out where it issued none
+          }
+        }
+      } else {
+        G::arrive_first(&other_done);
       }
+      if (PAIR) {
+        // the first block's arrivals at this block's barriers are all in before the block ends
+        if (complete)
+          for (uint32_t i = last; i < it; ++i)
+            if (!lost(i) && !mbar_wait(&empty[i % S], (i / S) & 1, a.limit)) ok = false;
+        if (place_in_pair == 1 && !mbar_wait(&drain, 0, kDrainLimit)) ok = false;
+      }
+      if (!ok) atomicExch(a.error, 1u);
     }
   } else if (warp == 1) {
     if (lane == 0 && place_in_pair == 0) {
@@ -724,14 +768,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       bool ok = true;
       for (int tile = worker; tile < a.tiles && ok; tile += workers, ++local) {
         const uint32_t b = local & 1;
-        if (local >= 2 && !mbar_wait(&acc_empty[b], ((local >> 1) & 1) ^ 1, kWaitLimit)) {
+        if (local >= 2 && !mbar_wait(&acc_empty[b], ((local >> 1) & 1) ^ 1, a.limit)) {
           ok = false;
           break;
         }
         tc_fence_after();
         for (int k = 0; k < a.k_blocks; ++k, ++it) {
           const int s = it % S;
-          if (!mbar_wait(&full[s], (it / S) & 1, kWaitLimit)) {
+          if (!mbar_wait(&full[s], (it / S) & 1, a.limit)) {
             ok = false;
             break;
           }
@@ -745,6 +789,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
         if (ok) G::commit(&acc_full[b]);
       }
+      if (it > 0) G::commit(&drain);
+      else G::arrive_all(&drain);
+      if (!mbar_wait(&drain, 0, kDrainLimit)) ok = false;
       if (!ok) atomicExch(a.error, 1u);
     }
   } else {
@@ -755,7 +802,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     uint8_t* const mine = ring + (size_t)S * kBytes + (size_t)(warp - 2) * (2 * kStaged);
     float* const sw = reinterpret_cast<float*>(ring + (size_t)S * kBytes + (size_t)(kEpilogue / 32) * (2 * kStaged)) + (warp - 2) * 2 * COLS;
     float* const sb = sw + COLS;
-    uint32_t local = 0, limit = kWaitLimit, stores = 0;
+    uint32_t local = 0, limit = a.limit, stores = 0;
     uint64_t policy;
     if (a.stream_out) asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
     else asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
@@ -998,7 +1045,7 @@ size_t int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, bool quantis
 
 int int8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, const float* x_scale, const int8_t* w_codes,
                 int64_t ldw, const float* w_scale, const void* bias, int bias_dtype, void* out, int64_t M, int64_t N,
-                int64_t K, int dtype, void* ws, int check_timeout, cudaStream_t s) {
+                int64_t K, int dtype, void* ws, int check_timeout, int drop, uint32_t limit, cudaStream_t s) {
   const GemmShape g = gemm_shape(M, N, K, N * dtype_size(dtype) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0,
                                  x != nullptr);
   const GemmWs l = gemm_ws(g, M, K, x != nullptr);
@@ -1028,6 +1075,7 @@ int int8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, 
   a.stream_out = (size_t)M * N * dtype_size(dtype) > kOutputInL2;
   a.parts = reinterpret_cast<int32_t*>(p + l.parts), a.counts = reinterpret_cast<uint32_t*>(p + l.counts);
   a.error = reinterpret_cast<uint32_t*>(p);
+  a.limit = limit ? limit : kWaitLimit, a.drop = drop;
   const StepArgs sa{x, ldx, K % 8 == 0 && ldx * dtype_size(dtype) % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0, (int)K};
   if (g.step) {
     switch (dtype) {

@@ -109,6 +109,8 @@ PROTOTYPES = {
     "flb_int8_linear_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32]),
     "flb_int8_linear": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i32, _vp, _i64, _i64,
                                _i64, _i32, _vp, _sz, _i32, _vp]),
+    "flb_int8_linear_wait_test": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i32, _vp, _i64, _i64,
+                                         _i64, _i32, _vp, _sz, _i32, _i64, ctypes.c_uint32, _vp]),
     "flb_microbench": (_i32, [_i32, _vp, _dblp]),
     "flb_selftest_umma": (_i32, [_i32, _i32, _vp, _vp, _vp, _vp, _vp]),
 }

@@ -477,6 +477,16 @@ int flb_int8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t l
                     const int8_t* w_codes, int64_t ldw, const float* w_scale, const void* bias,
                     int bias_dtype, void* out, int64_t M, int64_t N, int64_t K, int dtype, void* workspace,
                     size_t workspace_bytes, int check_timeout, void* stream);
+/* Failure-detection check of the product's bounded waits. flb_int8_linear with its waits' limit lowered to spin_limit polls,
+ * and with step drop_step (128 bytes of K of a tile, counted along a block's own work) of the first block, or pair of
+ * blocks, never loaded; -1: every step is loaded. What waits for the step gives up, everything in flight lands, and with
+ * check_timeout the call returns FLB_ERR_TIMEOUT; out is then undefined and the context stays usable. No GPU fault is
+ * involved. */
+int flb_int8_linear_wait_test(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, const float* x_scale,
+                              const int8_t* w_codes, int64_t ldw, const float* w_scale, const void* bias, int bias_dtype,
+                              void* out, int64_t M, int64_t N, int64_t K, int dtype, void* workspace,
+                              size_t workspace_bytes, int check_timeout, int64_t drop_step, uint32_t spin_limit,
+                              void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Measurement helpers (used by bench.py for the roofline denominators).

@@ -1,0 +1,62 @@
+"""The 8-bit product's bounded waits on a B200: a wait that gives up is reported, and leaves a context that works."""
+import time
+
+import pytest
+import torch
+
+from test_norm_kept_gpu import rows_of
+
+pytestmark = pytest.mark.gpu
+
+BF = torch.bfloat16
+TIMEOUT = 4  # FLB_ERR_TIMEOUT
+LIMIT = 1 << 14  # polls: some milliseconds at most, where a wait of a product is some microseconds
+
+
+def product(x, w, out, step, limit=LIMIT, check=1):
+    """flb_int8_linear_wait_test of x (Int8Rows, or a tensor) and w into out."""
+    import flb_native as nat
+    rows = not isinstance(x, torch.Tensor)
+    (M, K), N = (x.codes if rows else x).shape, w.codes.shape[0]
+    n = nat.lib.flb_int8_linear_workspace_bytes(M, N, K, int(rows))
+    ws = nat.workspace(n, out.device)
+    what = (None, 0, x.codes.data_ptr(), x.codes.stride(0), x.scale.data_ptr()) if rows else (x.data_ptr(), K, None, 0, None)
+    return nat.lib.flb_int8_linear_wait_test(*what, w.codes.data_ptr(), w.codes.stride(0), w.scale.data_ptr(), None, 0, out.data_ptr(),
+                                             M, N, K, nat.BF16, ws.data_ptr(), n, check, step, limit, nat.stream_of(out))
+
+
+# the kernel for few tokens (K whole, and in parts), one block a tile, two blocks a tile; steps in the first ring and after it
+CASES = [(40, 2048, 20000, 2), (40, 2048, 20000, 20), (100, 4096, 1000, 1), (2931, 768, 2304, 0), (2931, 768, 2304, 5),
+         (2931, 768, 2304, 7), (5120, 1104, 2048, 0), (5120, 1104, 2048, 3), (5120, 1104, 2048, 11)]
+
+
+def dropped(x, w, step):
+    import flb_native as nat
+    import kernels
+    M, N = (x if isinstance(x, torch.Tensor) else x.codes).shape[0], w.codes.shape[0]
+    want = kernels.int8_linear(x, w)
+    out = torch.empty(M, N, dtype=BF, device="cuda")
+    assert product(x, w, out, -1) == 0 and torch.equal(out, want)
+    start = time.perf_counter()
+    assert product(x, w, out, step) == TIMEOUT and b"gave up" in nat.lib.flb_last_error()
+    took = time.perf_counter() - start
+    torch.cuda.synchronize()
+    assert took < 5, took  # every wait ended at its limit
+    for _ in range(3):
+        assert product(x, w, out, -1) == 0 and torch.equal(out, want)
+
+
+@pytest.mark.parametrize("M,K,N,step", CASES)
+def test_a_lost_step_is_reported(M, K, N, step):
+    import kernels
+    x = kernels.quantize_int8(rows_of((M, K), BF, 1).cuda())
+    w = kernels.quantize_int8(rows_of((N, K), BF, 2).cuda())
+    dropped(x, w, step)
+
+
+# the decoding step's kernel: one block a tile (several tiles each), clusters of two, four and eight
+@pytest.mark.parametrize("M,K,N,step", [(1, 768, 32000, 3), (2, 768, 32000, 8), (3, 2000, 8190, 2), (7, 2048, 1000, 1), (4, 4096, 1000, 3)])
+def test_a_lost_step_of_a_decoding_step_is_reported(M, K, N, step):
+    import kernels
+    x = rows_of((M, K), BF, 1).cuda()
+    dropped(x, kernels.quantize_int8(rows_of((N, K), BF, 2).cuda()), step)
