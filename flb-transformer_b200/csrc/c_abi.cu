@@ -114,6 +114,7 @@ int grid_fwd_static(const void* W_l, const void* W_t, const float* bias, const v
                     void* h_out, int64_t R, int64_t C, int64_t B, int64_t H, int64_t G,
                     int check_timeout, cudaStream_t s);
 int microbench(int kind, void* scratch, double* ops_per_s);
+int late_copy(const void* src, void* dst, int64_t bytes, int64_t delay_us, cudaStream_t s);
 int umma_selftest(int variant, int n, const void* A, const void* B, float* D, int* err,
                   cudaStream_t s);
 
@@ -528,6 +529,10 @@ int flb_selftest_umma(int variant, int n, const void* A, const void* B, float* D
                       void* stream) {
   if (!A || !B || !D || !err) return fail(FLB_ERR_SHAPE, "selftest_umma: null pointer");
   return umma_selftest(variant, n, A, B, D, err, as_stream(stream));
+}
+
+int flb_selftest_late_copy(const void* src, void* dst, int64_t bytes, int64_t delay_us, void* stream) {
+  return late_copy(src, dst, bytes, delay_us, as_stream(stream));
 }
 
 }  // extern "C"

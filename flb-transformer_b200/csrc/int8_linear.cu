@@ -37,7 +37,7 @@ constexpr int kStep = 128;       // bytes of K a stage
 constexpr int kRing = 198 * 1024;
 constexpr int kEpilogue = 256;   // threads that read TMEM and store
 constexpr int kGemmThreads = 64 + kEpilogue;
-constexpr uint32_t kWaitLimit = 1u << 20;  // polls, each of which the hardware may hold for a while
+constexpr uint32_t kWaitLimit = 1u << 20;  // polls, each held for about 4 us by the hardware: 4 s
 // A wait that gives up leaves wrong numbers behind it, but nothing in flight: every kernel's loader waits for its last copies and
 // the thread that issues MMAs for its own (the barrier `drain`), with this limit, before the block gives up its shared
 // memory and TMEM.
@@ -217,6 +217,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       constexpr uint32_t idesc = idesc_i8<NT>();
       uint32_t it = 0, local = 0;
       bool ok = true;
+      // every warp waits for the predecessor before its first bounded wait: the polls are not spent on what that one has left
+      wait_predecessor();
       for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++local) {
         const uint32_t b = local & 1;
         if (local >= 2 && !mbar_wait(&acc_empty[b], ((local >> 1) & 1) ^ 1, a.limit)) {
@@ -766,6 +768,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(NC >> 3) << 17) | ((uint32_t)(BLOCKS * kTokens >> 4) << 24);
       uint32_t it = 0, local = 0;
       bool ok = true;
+      wait_predecessor();
       for (int tile = worker; tile < a.tiles && ok; tile += workers, ++local) {
         const uint32_t b = local & 1;
         if (local >= 2 && !mbar_wait(&acc_empty[b], ((local >> 1) & 1) ^ 1, a.limit)) {

@@ -97,7 +97,28 @@ umma_selftest_kernel(const __nv_bfloat16* __restrict__ A, const __grid_constant_
   if (warp == 0) tmem_dealloc(tmem, 128);
 }
 
+// dst = src once delay_ns have passed (or the iterations run out), the next kernel of the stream free to start meanwhile.
+__global__ void __launch_bounds__(256) late_copy_kernel(const uint4* src, uint4* dst, int64_t n, uint64_t delay_ns) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  uint64_t start, now;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(start)::"memory");
+  for (int i = 0; i < (1 << 20); ++i) {
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now)::"memory");
+    if (now - start >= delay_ns) break;
+    __nanosleep(200);
+  }
+  for (int64_t i = threadIdx.x; i < n; i += blockDim.x) dst[i] = src[i];
+}
+
 }  // namespace
+
+int late_copy(const void* src, void* dst, int64_t bytes, int64_t delay_us, cudaStream_t s) {
+  if (bytes < 0 || bytes % 16 || delay_us < 0 || delay_us > 100000 || !src || !dst)
+    return fail(FLB_ERR_SHAPE, "late_copy: a multiple of 16 bytes, and a delay of 0 to 100000 us");
+  if (((uintptr_t)src | (uintptr_t)dst) & 15u) return fail(FLB_ERR_ALIGN, "late_copy: pointers must be 16-byte aligned");
+  late_copy_kernel<<<1, 256, 0, s>>>((const uint4*)src, (uint4*)dst, bytes / 16, (uint64_t)delay_us * 1000);
+  return check_cuda(cudaGetLastError(), "late_copy launch");
+}
 
 int umma_selftest(int variant, int n, const void* A, const void* B, float* D, int* err,
                   cudaStream_t s) {

@@ -113,6 +113,7 @@ PROTOTYPES = {
                                          _i64, _i32, _vp, _sz, _i32, _i64, ctypes.c_uint32, _vp]),
     "flb_microbench": (_i32, [_i32, _vp, _dblp]),
     "flb_selftest_umma": (_i32, [_i32, _i32, _vp, _vp, _vp, _vp, _vp]),
+    "flb_selftest_late_copy": (_i32, [_vp, _vp, _i64, _i64, _vp]),
 }
 
 

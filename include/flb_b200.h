@@ -509,6 +509,10 @@ int flb_microbench(int kind, void* scratch, double* ops_per_s);
 int flb_selftest_umma(int variant, int n, const void* A, const void* B, float* D, int* err,
                       void* stream);
 
+/* Test of programmatic dependent launch: dst = src (a multiple of 16 bytes, 16-byte aligned) by one block that lets its
+ * successor in the stream start at once and copies after delay_us (at most 100000). */
+int flb_selftest_late_copy(const void* src, void* dst, int64_t bytes, int64_t delay_us, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

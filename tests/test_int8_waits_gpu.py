@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 
 BF = torch.bfloat16
 TIMEOUT = 4  # FLB_ERR_TIMEOUT
-LIMIT = 1 << 14  # polls: some milliseconds at most, where a wait of a product is some microseconds
+LIMIT = 1 << 14  # polls of about 4 us, where a wait of a product is some microseconds
 
 
 def product(x, w, out, step, limit=LIMIT, check=1):
@@ -60,3 +60,35 @@ def test_a_lost_step_of_a_decoding_step_is_reported(M, K, N, step):
     import kernels
     x = rows_of((M, K), BF, 1).cuda()
     dropped(x, kernels.quantize_int8(rows_of((N, K), BF, 2).cuda()), step)
+
+
+def late(rows, delay_us):
+    """Rows whose codes and scales are copied into place after the delay, by kernels that let their successor start."""
+    import flb_native as nat
+    import kernels
+    M, pitch = rows.codes.shape[0], rows.codes.stride(0)
+    buffer = torch.zeros(M * pitch + 4 * M + 16, dtype=torch.uint8, device="cuda")
+    source = torch.cat([rows.codes.as_strided((M * pitch,), (1,)).view(torch.uint8), rows.scale.view(torch.uint8)])
+    n = source.numel() // 16 * 16
+    buffer[n:source.numel()].copy_(source[n:])
+    torch.cuda.synchronize()
+    codes = buffer[:M * pitch].view(torch.int8).view(M, pitch)[:, :rows.codes.shape[1]]
+    out = kernels.Int8Rows(codes, buffer[M * pitch:M * pitch + 4 * M].view(torch.float32), rows.dtype)
+    assert nat.lib.flb_selftest_late_copy(source.data_ptr(), buffer.data_ptr(), n, delay_us, nat.stream_of(buffer)) == 0
+    return out, source
+
+
+@pytest.mark.parametrize("M,K,N", [(40, 256, 20000), (300, 64, 17000), (2931, 768, 2304), (5120, 1104, 2048)])
+def test_a_late_predecessor_is_waited_for(M, K, N):
+    """The kernel that makes the rows lets the product start and takes far longer than a wait's limit: the limit is for the
+    product's own steps."""
+    import kernels
+    x, w = (kernels.quantize_int8(rows_of((n, K), BF, n).cuda()) for n in (M, N))
+    want = kernels.int8_linear(x, w)
+    out = torch.empty_like(want)
+    for delay in (0, 50000):
+        rows, source = late(x, delay)
+        assert product(rows, w, out, -1, limit=1 << 10, check=0) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), delay
+        out.zero_()
