@@ -17,11 +17,10 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 import flb_native  # noqa: F401  (loads libflb_b200.so, or says that it is missing)
 import flb_ops
-from ._rows import no_transforms, plain, to_front, transforms_active
+from ._rows import backward_of, no_transforms, to_front, transforms_active
 
 __all__ = ["Packed8", "pack8", "unpack8", "sigmoid_gate"]
 
@@ -52,18 +51,19 @@ class _GateFunc(torch.autograd.Function):
 
     @staticmethod
     def forward(x, z, keep8):
-        return tuple(flb_ops.gate_forward(x, z, keep8))
+        # with keep8 an empty tensor last, which tells the levels of torch.func that the kept forms (integers) depend on x and z
+        return (*flb_ops.gate_forward(x, z, keep8), *([x.new_empty(0)] if keep8 else []))
 
     @staticmethod
     def setup_context(ctx, inputs, output):
         x, z, keep8 = inputs
-        ctx.mark_non_differentiable(*output[1:])
+        ctx.mark_non_differentiable(*output[1:-1])
+        ctx.set_materialize_grads(False)
         ctx.save_for_backward(*(output[1:] if keep8 else (x, z)))
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, *_):
-        return *flb_ops.gate_backward([plain(t) for t in ctx.saved_tensors], plain(dy)), None
+        return *backward_of(lambda dy, *kept: flb_ops.gate_backward(list(kept[:4]), dy), dy, *ctx.saved_tensors), None
 
     @staticmethod
     def vmap(info, in_dims, x, z, keep8):

@@ -19,11 +19,10 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 import flb_native  # noqa: F401  (loads libflb_b200.so, or says that it is missing)
 import flb_ops
-from ._rows import no_transforms, plain, to_front, transforms_active
+from ._rows import backward_of, no_transforms, to_front, transforms_active
 from .int8_linear import Int8Rows
 
 __all__ = ["layer_norm", "layer_norm_int8", "FusedLayerNorm"]
@@ -39,15 +38,18 @@ class _LayerNormFunc(torch.autograd.Function):
     @staticmethod
     def setup_context(ctx, inputs, output):
         x, weight, bias, _, ctx.keep8 = inputs
-        ctx.mark_non_differentiable(*output[1:])
+        # 1/sigma is not marked: with keep8 it alone tells the levels of torch.func that what the backward reads depends on x
+        ctx.mark_non_differentiable(*output[2:])
+        ctx.set_materialize_grads(False)
         ctx.save_for_backward(None if ctx.keep8 else x, weight, bias, *output[1:])
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, *_):
-        x, weight, bias, rstd, *kept = (plain(t) for t in ctx.saved_tensors)
+        x, weight, bias, rstd, *kept = ctx.saved_tensors
         mean, codes, exps = (None, *kept) if ctx.keep8 else (kept[0], None, None)
-        return *flb_ops.norm_backward(x, rstd, mean, codes, exps, weight, bias, plain(dy), True), None, None
+        dx, *params = backward_of(flb_ops.norm_backward, x, rstd, mean, codes, exps, weight, bias, dy, True)
+        dw = params.pop(0) if weight is not None else None
+        return dx, dw, params.pop(0) if bias is not None else None, None, None
 
     @staticmethod
     def vmap(info, in_dims, x, weight, bias, eps, keep8):
