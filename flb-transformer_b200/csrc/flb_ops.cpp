@@ -4,6 +4,7 @@
 // machine, nearly all of it the interpreter's. The Python packages keep the operators' names, their
 // documentation and their torch.func rules. There is no CPU path.
 #include <torch/extension.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -40,6 +41,13 @@ void same_device(const Tensor& x, const Opt& t) {
   TORCH_CHECK_VALUE(t->device() == x.device(), "tensors on different devices: ", x.device(), " and ", t->device());
 }
 bool given(const Opt& t) { return t && t->defined(); }
+
+// The operators have no forward-mode derivative: an input with a tangent would lose it without a word. (A tangent does not set
+// requires_grad.)
+void no_tangent(const Opt& t, const char* what) {
+  TORCH_CHECK(!given(t) || !c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t->_fw_grad(0).defined(), what,
+              " has no forward-mode derivative");
+}
 void* ptr(const Opt& t) { return given(t) ? t->data_ptr() : nullptr; }
 void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 void check(int st, const char* what) {
@@ -217,6 +225,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
 bool wants_grad(const Opt& t) { return given(t) && t->requires_grad(); }
 
 Tensor layer_norm(const Tensor& x, const Opt& weight, const Opt& bias, double eps, bool keep8) {
+  for (const Opt& t : {Opt(x), weight, bias}) no_tangent(t, "layer_norm");
   if (c10::GradMode::is_enabled() && (x.requires_grad() || wants_grad(weight) || wants_grad(bias)))
     return LayerNormFn::apply(x, weight, bias, eps, keep8);
   return std::get<0>(norm_forward(x, weight, bias, eps, false, false));
@@ -317,6 +326,7 @@ struct GateFn : torch::autograd::Function<GateFn> {
 };
 
 Tensor sigmoid_gate(const Tensor& x, const Tensor& z, bool keep8) {
+  for (const Opt& t : {Opt(x), Opt(z)}) no_tangent(t, "sigmoid_gate");
   if (c10::GradMode::is_enabled() && (x.requires_grad() || z.requires_grad())) return GateFn::apply(x, z, keep8);
   return gate_forward(x, z, false)[0];
 }
@@ -325,6 +335,7 @@ Tensor sigmoid_gate(const Tensor& x, const Tensor& z, bool keep8) {
 
 void no_gradient(const Opt& t, const char* what) {
   TORCH_CHECK(!(c10::GradMode::is_enabled() && wants_grad(t)), what, " has no gradient: call it under torch.no_grad()");
+  no_tangent(t, what);
 }
 
 // codes [.., D] over rows that start every 16 bytes, and a scale each
@@ -338,9 +349,9 @@ std::pair<Tensor, Tensor> int8_buffers(const Tensor& x) {
 }
 
 std::pair<Tensor, Tensor> quantize_int8(const Tensor& x_) {
+  no_gradient(x_, "quantize_int8");
   const int dt = dtype_of(x_, "x");
   need_cuda(x_);
-  no_gradient(x_, "quantize_int8");
   TORCH_CHECK_VALUE(last_axis(x_, "x") >= 1, "x must have a last axis of at least one element");
   const c10::cuda::CUDAGuard guard(x_.device());
   auto [x, ldx] = rows_of(x_);
@@ -351,8 +362,8 @@ std::pair<Tensor, Tensor> quantize_int8(const Tensor& x_) {
 }
 
 std::pair<Tensor, Tensor> layer_norm_int8(const Tensor& x_, const Opt& weight, const Opt& bias, double eps) {
-  const NormSizes n = check_norm(x_, weight, bias);
   for (const Opt& t : {Opt(x_), weight, bias}) no_gradient(t, "layer_norm_int8");
+  const NormSizes n = check_norm(x_, weight, bias);
   const c10::cuda::CUDAGuard guard(x_.device());
   auto [x, ldx] = rows_of(x_);
   const Opt w = contiguous(weight), b = contiguous(bias);
@@ -383,13 +394,12 @@ std::tuple<Tensor, int64_t> code_rows(const Tensor& codes, const Tensor& scale, 
 // x, or x_codes and x_scale with the output's type
 Tensor int8_linear(const Opt& x_, const Opt& x_codes, const Opt& x_scale, const Tensor& w_codes, const Tensor& w_scale,
                    const Opt& bias_, std::optional<at::ScalarType> type) {
+  for (const Opt& t : {x_, bias_}) no_gradient(t, "int8_linear");
   const Tensor& in = given(x_) ? *x_ : *x_codes;
   const at::ScalarType dtype = given(x_) ? in.scalar_type() : type.value_or(at::kBFloat16);
   const int dt = dtype_of(dtype, "x");
   need_cuda(in);
   for (const Opt& t : {Opt(w_codes), Opt(w_scale), x_scale, bias_}) same_device(in, t);
-  no_gradient(x_, "int8_linear");
-  no_gradient(bias_, "int8_linear");
   const int64_t K = last_axis(in, "x"), M = rows_in(in);
   TORCH_CHECK_VALUE(w_codes.dim() == 2 && w_codes.size(1) == K && K >= 1, "a weight of shape ", w_codes.sizes(), " for x of shape ",
                     in.sizes());

@@ -1,4 +1,7 @@
 """More refusals of the row operators and 8-bit products, and what their modules do without a kernel (no GPU)."""
+import pytest
+import torch
+from torch.autograd import forward_ad
 
 
 def test_wait_test_arguments():
@@ -7,3 +10,30 @@ def test_wait_test_arguments():
     assert nat.lib.flb_selftest_late_copy(16, 24, 16, 0, None) == 3
     assert nat.lib.flb_int8_linear_wait_test(16, 64, None, 0, None, 16, 64, 16, None, 0, 16, 4, 8, 64, 2, 256, 1 << 30, 1, -2, 1, None) == 1
     assert nat.lib.flb_int8_linear_wait_test(16, 64, None, 0, None, 16, 64, 16, None, 0, 16, 4, 8, 64, 2, 256, 1 << 30, 1, 0, 0, None) == 1
+
+
+def int8_rows(n=4, K=8, requires_grad=False):
+    import kernels
+    return kernels.Int8Rows(torch.ones(n, K, dtype=torch.int8), torch.ones(n, requires_grad=requires_grad), torch.float32)
+
+
+def calls():
+    """Every operator that reads floating-point tensors, as functions of one of them (the others have no derivative)."""
+    import kernels
+    x, w = torch.ones(2, 8), torch.ones(8)
+    return [kernels.layer_norm, lambda t: kernels.layer_norm(x, t[0]), lambda t: kernels.layer_norm(x, None, t[0]),
+            lambda t: kernels.layer_norm(t, w, w, keep8=True), lambda t: kernels.sigmoid_gate(t, x), lambda t: kernels.sigmoid_gate(x, t),
+            kernels.layer_norm_int8, lambda t: kernels.layer_norm_int8(x, t[0]), kernels.quantize_int8,
+            lambda t: kernels.int8_linear(t, int8_rows()), lambda t: kernels.int8_linear(x, int8_rows(2), t[:, 0])]
+
+
+def test_tangents_are_refused():
+    for call in calls():
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(torch.ones(2, 8), torch.ones(2, 8))
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                    call(dual)
+            # without its tangent the call goes on to the check of its device
+            with pytest.raises(RuntimeError, match="CUDA tensors only"):
+                call(forward_ad.unpack_dual(dual).primal)
