@@ -394,7 +394,7 @@ std::tuple<Tensor, int64_t> code_rows(const Tensor& codes, const Tensor& scale, 
 // x, or x_codes and x_scale with the output's type
 Tensor int8_linear(const Opt& x_, const Opt& x_codes, const Opt& x_scale, const Tensor& w_codes, const Tensor& w_scale,
                    const Opt& bias_, std::optional<at::ScalarType> type) {
-  for (const Opt& t : {x_, bias_}) no_gradient(t, "int8_linear");
+  for (const Opt& t : {x_, x_scale, Opt(w_scale), bias_}) no_gradient(t, "int8_linear");
   const Tensor& in = given(x_) ? *x_ : *x_codes;
   const at::ScalarType dtype = given(x_) ? in.scalar_type() : type.value_or(at::kBFloat16);
   const int dt = dtype_of(dtype, "x");

@@ -37,3 +37,14 @@ def test_tangents_are_refused():
             # without its tangent the call goes on to the check of its device
             with pytest.raises(RuntimeError, match="CUDA tensors only"):
                 call(forward_ad.unpack_dual(dual).primal)
+
+
+def test_scales_that_want_a_gradient_are_refused():
+    """The scales of integer rows are inputs of the product like any other."""
+    import kernels
+    x, wants = torch.ones(2, 8), int8_rows(requires_grad=True)
+    for call in (lambda: kernels.int8_linear(x, wants), lambda: kernels.int8_linear(wants, int8_rows())):
+        with pytest.raises(RuntimeError, match="has no gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA tensors only"):
+            call()
