@@ -100,6 +100,12 @@ int int8_linear_checked(const void* x, int64_t ldx, const int8_t* x_codes, int64
   if (!workspace || workspace_bytes < need)
     return fail(FLB_ERR_WORKSPACE, "int8_linear: workspace smaller than flb_int8_linear_workspace_bytes()");
   if (off(workspace, 256)) return fail(FLB_ERR_ALIGN, "int8_linear: workspace must be 256-byte aligned");
+  if (check_timeout) {
+    cudaStreamCaptureStatus capture;
+    if ((st = check_cuda(cudaStreamIsCapturing(as_stream(stream), &capture), "int8_linear capture status")) != FLB_OK) return st;
+    if (capture != cudaStreamCaptureStatusNone)
+      return fail(FLB_ERR_UNSUPPORTED, "int8_linear: check_timeout waits for the product, which a stream capture does not allow");
+  }
   return int8_linear(x, ldx, x_codes, ldc, x_scale, w_codes, ldw, w_scale, bias, bias_dtype, out, M, N, K, dtype, workspace,
                      check_timeout, drop, limit, as_stream(stream));
 }

@@ -393,7 +393,7 @@ std::tuple<Tensor, int64_t> code_rows(const Tensor& codes, const Tensor& scale, 
 
 // x, or x_codes and x_scale with the output's type
 Tensor int8_linear(const Opt& x_, const Opt& x_codes, const Opt& x_scale, const Tensor& w_codes, const Tensor& w_scale,
-                   const Opt& bias_, std::optional<at::ScalarType> type) {
+                   const Opt& bias_, std::optional<at::ScalarType> type, bool check_timeout) {
   for (const Opt& t : {x_, x_scale, Opt(w_scale), bias_}) no_gradient(t, "int8_linear");
   const Tensor& in = given(x_) ? *x_ : *x_codes;
   const at::ScalarType dtype = given(x_) ? in.scalar_type() : type.value_or(at::kBFloat16);
@@ -431,7 +431,7 @@ Tensor int8_linear(const Opt& x_, const Opt& x_codes, const Opt& x_scale, const 
   const size_t need = flb_int8_linear_workspace_bytes(M, N, K, given(x) ? 0 : 1);
   Tensor ws = buffer(need, in);
   check(flb_int8_linear(ptr(x), ldx, (const int8_t*)ptr(xc), ldc, (const float*)ptr(xs), (const int8_t*)wc.data_ptr(), ldw,
-                        (const float*)ws_.data_ptr(), ptr(b), bdt, out.data_ptr(), M, N, K, dt, ws.data_ptr(), need, 0, stream_of(in)),
+                        (const float*)ws_.data_ptr(), ptr(b), bdt, out.data_ptr(), M, N, K, dt, ws.data_ptr(), need, check_timeout ? 1 : 0, stream_of(in)),
         "flb_int8_linear");
   return out;
 }
@@ -456,10 +456,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("sigmoid_gate", &sigmoid_gate, off);
   m.def("quantize_int8", &quantize_int8, off);
   m.def("layer_norm_int8", &layer_norm_int8, off);
-  m.def("int8_linear", [](const Opt& x, const Opt& xc, const Opt& xs, const Tensor& wc, const Tensor& ws, const Opt& bias, py::object dtype) {
+  m.def("int8_linear", [](const Opt& x, const Opt& xc, const Opt& xs, const Tensor& wc, const Tensor& ws, const Opt& bias, py::object dtype,
+                          bool check_timeout) {
     std::optional<at::ScalarType> t;
     if (!dtype.is_none()) t = torch::python::detail::py_object_to_dtype(dtype);
     py::gil_scoped_release release;
-    return int8_linear(x, xc, xs, wc, ws, bias, t);
+    return int8_linear(x, xc, xs, wc, ws, bias, t, check_timeout);
   });
 }

@@ -1,7 +1,7 @@
 """Linear maps in 8-bit integers with a scale for each token and each output channel, on B200 (sm_100a).
 
     quantize_int8(x) -> Int8Rows
-    int8_linear(x, weight, bias=None) -> x @ weight.T + bias
+    int8_linear(x, weight, bias=None, check_timeout=False) -> x @ weight.T + bias
     Int8Linear.from_linear(linear)                       a module with its weight so quantised
 
 A row v is codes round(v * 127 / max|v|) and the scale max|v| / 127; int8_linear makes its input's rows so on the
@@ -9,6 +9,9 @@ way (or takes them as Int8Rows, as layer_norm_int8 returns them), adds products 
 integers, without rounding, and multiplies by the two scales. A row that holds an infinity or NaN gives
 NaN in all its outputs; one whose largest magnitude is below 2^-118 counts as zeros. Rows of up to 32768
 elements. No gradients: inference only.
+
+The kernels' waits for their own copies and products are bounded (4 s). check_timeout waits for the product and raises a
+RuntimeError if one of them gave up, where the output is wrong; without it the call returns at once and nothing is said.
 
 The kernels are in libflb_b200.so (flb_int8_rows, flb_int8_linear: tcgen05 kind::i8), called through
 flb_ops; CUDA tensors only.
@@ -47,35 +50,38 @@ def quantize_int8(x: torch.Tensor) -> Int8Rows:
     return Int8Rows(*flb_ops.quantize_int8(x), x.dtype)
 
 
-def int8_linear(x: torch.Tensor | Int8Rows, weight: Int8Rows, bias: torch.Tensor | None = None) -> torch.Tensor:
-    """x [..., K] times weight [N, K] (an Int8Rows), plus bias [N] (float32 or x's type): [..., N] in x's type."""
+def int8_linear(x: torch.Tensor | Int8Rows, weight: Int8Rows, bias: torch.Tensor | None = None,
+                check_timeout: bool = False) -> torch.Tensor:
+    """x [..., K] times weight [N, K] (an Int8Rows), plus bias [N] (float32 or x's type): [..., N] in x's type.
+    check_timeout: see the module's text; not while a CUDA graph is captured."""
     no_transforms("int8_linear")
     if isinstance(x, Int8Rows):
-        return flb_ops.int8_linear(None, x.codes, x.scale, weight.codes, weight.scale, bias, x.dtype)
-    return flb_ops.int8_linear(x, None, None, weight.codes, weight.scale, bias, None)
+        return flb_ops.int8_linear(None, x.codes, x.scale, weight.codes, weight.scale, bias, x.dtype, check_timeout)
+    return flb_ops.int8_linear(x, None, None, weight.codes, weight.scale, bias, None, check_timeout)
 
 
 class Int8Linear(nn.Module):
     """A linear map whose weight is kept in 8-bit integers (buffers `codes` and `scale`). For inference: its output
-    has no gradient."""
+    has no gradient. check_timeout as in int8_linear."""
 
-    def __init__(self, weight: Int8Rows, bias: torch.Tensor | None = None):
+    def __init__(self, weight: Int8Rows, bias: torch.Tensor | None = None, check_timeout: bool = False):
         super().__init__()
+        self.check_timeout = check_timeout
         self.out_features, self.in_features = weight.codes.shape
         self.register_buffer("codes", weight.codes)
         self.register_buffer("scale", weight.scale)
         self.register_buffer("bias", bias)
 
     @classmethod
-    def from_linear(cls, linear: nn.Linear) -> "Int8Linear":
+    def from_linear(cls, linear: nn.Linear, check_timeout: bool = False) -> "Int8Linear":
         """The map of an nn.Linear on a CUDA device, with its weight as it is now."""
         with torch.no_grad():
             bias = None if linear.bias is None else linear.bias.detach().clone()
-            return cls(quantize_int8(linear.weight), bias)
+            return cls(quantize_int8(linear.weight), bias, check_timeout)
 
     @torch.no_grad()
     def forward(self, x: torch.Tensor | Int8Rows) -> torch.Tensor:
         bias = self.bias
         if bias is not None and bias.dtype not in (torch.float32, x.dtype):
             bias = bias.float()
-        return int8_linear(x, Int8Rows(self.codes, self.scale), bias)
+        return int8_linear(x, Int8Rows(self.codes, self.scale), bias, self.check_timeout)

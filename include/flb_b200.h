@@ -471,7 +471,8 @@ int flb_layer_norm_int8(const void* x, int64_t ldx, const void* w, const void* b
  * on the way. W: codes [N, K] (pitch ldw >= K, a multiple of 16, 16-byte aligned) and scale [N]. bias: [N],
  * float32 or dtype, or NULL. K <= 32768. Workspace: flb_int8_linear_workspace_bytes(), 256-byte
  * aligned, asked for on the same device; calls that may overlap on the GPU need one each.
- * check_timeout != 0: reads the kernel's error word back (synchronises `stream`). */
+ * check_timeout != 0: reads the kernel's error word back (synchronises `stream`; refused while it is being captured). Without
+ * it nobody hears of a wait that gave up, and out is then wrong. */
 size_t flb_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int x_is_codes);
 int flb_int8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, const float* x_scale,
                     const int8_t* w_codes, int64_t ldw, const float* w_scale, const void* bias,

@@ -92,3 +92,23 @@ def test_a_late_predecessor_is_waited_for(M, K, N):
         torch.cuda.synchronize()
         assert torch.equal(out, want), delay
         out.zero_()
+
+
+def test_check_timeout_from_python():
+    """The checked call gives the unchecked one's output, and is refused while a graph is captured, which goes on."""
+    import kernels
+    w = kernels.quantize_int8(rows_of((300, 640), BF, 1).cuda())
+    for M in (1, 64, 600):
+        x = rows_of((M, 640), BF, M).cuda()
+        want = kernels.int8_linear(x, w)
+        assert torch.equal(kernels.int8_linear(x, w, check_timeout=True), want)
+        assert torch.equal(kernels.int8_linear(kernels.quantize_int8(x), w, check_timeout=True), want)
+        assert torch.equal(kernels.Int8Linear(w, check_timeout=True)(x), want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="stream capture"):
+            kernels.int8_linear(x, w, check_timeout=True)
+        got = kernels.int8_linear(x, w)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)

@@ -48,3 +48,29 @@ def test_scales_that_want_a_gradient_are_refused():
             call()
         with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA tensors only"):
             call()
+
+
+def test_check_timeout_reaches_the_kernel(monkeypatch):
+    import sys
+    import kernels
+
+    class Ops:
+        calls = []
+
+        @staticmethod
+        def int8_linear(*args):
+            Ops.calls.append(args[-1])
+
+        @staticmethod
+        def quantize_int8(w):
+            return int8_rows()[:2]
+
+    monkeypatch.setattr(sys.modules["kernels.int8_linear"], "flb_ops", Ops)
+    x, linear = torch.ones(2, 8), torch.nn.Linear(8, 4)
+    for check in (True, False):
+        kernels.int8_linear(x, int8_rows(), check_timeout=check)
+        kernels.int8_linear(int8_rows(), int8_rows(), None, check)
+        kernels.Int8Linear(int8_rows(), check_timeout=check)(x)
+        kernels.Int8Linear.from_linear(linear, check)(int8_rows())
+        assert Ops.calls == [check] * 4
+        Ops.calls.clear()
