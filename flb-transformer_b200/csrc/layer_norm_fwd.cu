@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(kMostThreads<MODE>, 1024 / kMostThreads<MODE>)
         for (int i = 0; i < 4; ++i) v[c][i] = mul2(v[c][i], f2(rstd));
         if constexpr (OUT == OUT_KEPT) {
           if (base < D) {
-            // a row with an infinity or NaN has NaN throughout, so a block's values are all NaN or none
+            // a row with an infinity or NaN, or whose sum is one, has NaN throughout
             uint32_t m[L == EIGHT ? 1 : 2];
             max_bits<L>(v[c], m);
             keep8<L>(v[c], m, a.codes + row * code_pitch(D), a.exps + row * blocks_of(D), base, lane, D);

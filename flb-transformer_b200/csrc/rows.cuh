@@ -296,14 +296,22 @@ template <typename T, Layout L> __device__ __forceinline__ void max_bits(const R
     else m[0] = float_bits<T>(max_halves(lo)), m[1] = float_bits<T>(max_halves(hi));
   }
 }
-// The same of eight floats. fmaxf passes over a NaN unless all are: for values of which all or none are.
+// The same of eight floats. A NaN among them gives a NaN's bits, also beside the zeros beyond a row's end.
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 template <Layout L> __device__ __forceinline__ void max_bits(const F2 (&f)[4], uint32_t (&m)[L == EIGHT ? 1 : 2]) {
   float v[8];
   to_scalars(f, v);
-  const float lo = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
-  const float hi = fmaxf(fmaxf(fabsf(v[4]), fabsf(v[5])), fmaxf(fabsf(v[6]), fabsf(v[7])));
-  if constexpr (L == EIGHT) m[0] = __float_as_uint(fmaxf(lo, hi)) & 0x7fffffffu;
-  else m[0] = __float_as_uint(lo) & 0x7fffffffu, m[1] = __float_as_uint(hi) & 0x7fffffffu;
+  const float lo = max3_abs(max3_abs(v[0], v[1], v[2]), v[3], 0.f);
+  if constexpr (L == EIGHT) {
+    m[0] = abs_bits(max3_abs(max3_abs(lo, v[4], v[5]), v[6], v[7]));
+  } else {
+    m[0] = abs_bits(lo);
+    m[1] = abs_bits(max3_abs(max3_abs(v[4], v[5], v[6]), v[7], 0.f));
+  }
 }
 
 // Keeps a lane's eight elements (chunk at `base`), whose largest magnitudes' bits are m: codes to `crow`,
