@@ -480,7 +480,7 @@ int flb_int8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t l
                     size_t workspace_bytes, int check_timeout, void* stream);
 /* Failure-detection check of the product's bounded waits. flb_int8_linear with its waits' limit lowered to spin_limit polls,
  * and with step drop_step (128 bytes of K of a tile, counted along a block's own work) of the first block, or pair of
- * blocks, never loaded; -1: every step is loaded. What waits for the step gives up, everything in flight lands, and with
+ * blocks, never reported as loaded; -1: every step is. What waits for the step gives up, everything in flight lands, and with
  * check_timeout the call returns FLB_ERR_TIMEOUT; out is then undefined and the context stays usable. No GPU fault is
  * involved. */
 int flb_int8_linear_wait_test(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, const float* x_scale,
