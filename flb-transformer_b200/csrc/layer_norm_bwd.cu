@@ -148,7 +148,8 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
       if constexpr (KEPT) kept_to_float<L>(Kept8{copied_codes<L>(part_of(stage, c, false), base, lane, D), e[c]}, x);
       else copied8<T, L>(part_of(stage, c, false), x, x_row(row), base, lane, D);
     };
-    // h = (x - m) h1, the difference first, as in the forward: exact where x is near the mean
+    // h = (x - m) h1, the difference first, as in the forward: exact where x is near the mean. Beyond D, dy and x are zero, and the
+    // mean counts as zero too: over a small sigma it can be infinite (a row of 2^110 throughout, eps 1e-12), and 0 h NaN then.
     const float h1 = KEPT ? 1.f : rs;
     F2 t1 = f2(0.f), t2 = f2(0.f);
 #pragma unroll
@@ -156,12 +157,30 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
       F2 x[4], dy[4];
       values(c, x, dy);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {  // dy is zero beyond D
-        const F2 h = KEPT ? x[i] : mul2(add2(x[i], f2(-m)), f2(h1)), gw = mul2(dy[i], w[c][i]);
+      for (int i = 0; i < 4; ++i) {
+        const F2 minus = f2(L == SCALARS || Chunk<L>::has(first + c * 256, lane, 2 * i, D) ? -m : 0.f);
+        const F2 h = KEPT ? x[i] : mul2(add2(x[i], minus), f2(h1)), gw = mul2(dy[i], w[c][i]);
         dw[c][i] = fma2(dy[i], h, dw[c][i]);
         db[c][i] = add2(db[c][i], dy[i]);
         t1 = add2(t1, gw);
         t2 = fma2(gw, h, t2);
+      }
+    }
+    if constexpr (!KEPT && L == SCALARS) {
+      // Scalars have that place element by element, and a choice at each in every row took 45.6 us instead of 41.7 for 16383 x 1001
+      // float32 and 139 instead of 118 for 16384 x 4095 bfloat16: the sum again, without those places, where it matters.
+      if (isinf(m * h1)) {
+        t2 = f2(0.f);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          F2 x[4], dy[4];
+          values(c, x, dy);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = add2(x[i], f2(-m));
+          zero_beyond<L>(x, first + c * 256, lane, D);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) t2 = fma2(mul2(dy[i], w[c][i]), mul2(x[i], f2(h1)), t2);
+        }
       }
     }
     float s1 = warp_sum(sum2(t1)), s2 = warp_sum(sum2(t2));

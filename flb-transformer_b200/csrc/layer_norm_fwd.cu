@@ -52,16 +52,6 @@ __device__ __forceinline__ void load_param(F2 (&v)[4], const void* p, bool f32, 
   }
 }
 
-// Zeros in the place of a chunk's elements at or beyond D
-template <Layout L> __device__ __forceinline__ void zero_beyond(F2 (&v)[4], int base, int lane, int D) {
-  if (Chunk<L>::has(base, lane, 7, D)) return;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 r = split(v[i]);
-    v[i] = f2(Chunk<L>::has(base, lane, 2 * i, D) ? r.x : 0.f, Chunk<L>::has(base, lane, 2 * i + 1, D) ? r.y : 0.f);
-  }
-}
-
 // Rows held at a time, the present one included: with the widest rows one
 template <int CH, int MODE> constexpr int kStages = MODE == 2 ? 1 : 2;
 constexpr int kWarps = 4;  // of a block whose warps have a row each

@@ -166,6 +166,16 @@ __device__ __forceinline__ void store8(T* __restrict__ row, const F2 (&f)[4], in
   }
 }
 
+// Zeros in the place of a chunk's elements at or beyond D
+template <Layout L> __device__ __forceinline__ void zero_beyond(F2 (&v)[4], int base, int lane, int D) {
+  if (Chunk<L>::has(base, lane, 7, D)) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 r = split(v[i]);
+    v[i] = f2(Chunk<L>::has(base, lane, 2 * i, D) ? r.x : 0.f, Chunk<L>::has(base, lane, 2 * i + 1, D) ? r.y : 0.f);
+  }
+}
+
 // ---- 8-bit integers -----------------------------------------------------------------------------
 // A float of magnitude at most 127 plus 1.5 * 2^23 is that float rounded to the nearest integer (ties to
 // even), whose two's complement is in the low byte of the sum's bits.

@@ -1,4 +1,4 @@
-"""Rows near the ends of float32's range."""
+"""Rows near the ends of float32's range: LayerNorm and its kept form, the kept form's errors, integer products."""
 import pytest
 import torch
 
@@ -11,6 +11,27 @@ BF, H, F = torch.bfloat16, torch.float16, torch.float32
 
 # widths that leave lanes of a warp's last chunk empty, or none; in every mode and layout
 WIDTHS = [20, 24, 256, 300, 600, 1001, 2056, 8200]
+
+
+@pytest.mark.parametrize("D", WIDTHS)
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_norm_of_large_constant_rows(D, dtype):
+    """Rows of 2^110 throughout: sums and mean are exact, h is zero and 1/sigma is 1 / sqrt(eps), a million here. A lane beyond
+    the row must not count as an element of value zero, whose h would be infinite."""
+    import kernels
+    x = torch.full((5, D), 2.0 ** 110).to(dtype)
+    x[3] = rows_of((D,), dtype, 3)
+    (w, b), dy, eps = params((D,), F, 1), rows_of((5, D), dtype, 2), 1e-12
+    leaves = [t.requires_grad_(True) for t in cuda(x, w, b)]
+    y = kernels.layer_norm(*leaves, eps=eps)
+    got = torch.autograd.grad(y, leaves, dy.cuda())
+    _, _, (h, rs, dh) = orc.layer_norm(x, w, b, eps, dtype)
+    flat = [0, 1, 2, 4]
+    h, dh = h.clone(), dh.clone()
+    assert not h[flat].any()
+    dh[flat] = 0  # exact
+    for g, (v, tol), name in zip(got, orc.layer_norm_backward(h, rs, dh, w, dy, dtype, F), ("dx", "dw", "db")):
+        close(g, v, tol, name)
 
 
 @pytest.mark.parametrize("D", WIDTHS)
