@@ -101,6 +101,14 @@ __device__ __forceinline__ void load_cols(uint32_t taddr, uint32_t (&r)[16]) { t
 
 __device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
+// Sum times a token's scale, times a channel's: of an integer of up to 2^29 the first product passes float32 for scales from 2^99
+// on, also where the second would bring it back. For such tokens the channel's scale comes first.
+constexpr float kLargeScale = 0x1p96f;
+__device__ __forceinline__ float scaled(uint32_t sum, float sx, float sw, float bias) {
+  const bool large = fabsf(sx) > kLargeScale;
+  return fmaf(__int2float_rn((int)sum) * (large ? sw : sx), large ? sx : sw, bias);
+}
+
 // One channel's values of CW tokens from token t0 on: scaled, with the bias, stored. FULL: the tile is
 // inside the output.
 template <typename T, int CW, bool FULL>
@@ -112,10 +120,10 @@ __device__ __forceinline__ void store_tokens(const Int8Args& a, const uint32_t (
 #pragma unroll
   for (int j = 0; j < CW; j += 4) {
     const float4 s = *reinterpret_cast<const float4*>(sx + j);
-    v[j] = fmaf(__int2float_rn((int)acc[j]) * s.x, sw, bias);
-    v[j + 1] = fmaf(__int2float_rn((int)acc[j + 1]) * s.y, sw, bias);
-    v[j + 2] = fmaf(__int2float_rn((int)acc[j + 2]) * s.z, sw, bias);
-    v[j + 3] = fmaf(__int2float_rn((int)acc[j + 3]) * s.w, sw, bias);
+    v[j] = scaled(acc[j], s.x, sw, bias);
+    v[j + 1] = scaled(acc[j + 1], s.y, sw, bias);
+    v[j + 2] = scaled(acc[j + 2], s.z, sw, bias);
+    v[j + 3] = scaled(acc[j + 3], s.w, sw, bias);
   }
   if (sizeof(T) == 2 && a.pairs) {
     // two channels a store: an even lane takes both channels of an even token, its neighbour of the odd one
@@ -827,7 +835,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       n0 += first;
       const int token = m0 + q * 32 + lane;
       const float sx = token < a.M ? __ldg(a.sx + token) : 0.f;
-      __syncwarp();
+      const bool any_large = __any_sync(0xffffffffu, fabsf(sx) > kLargeScale);
 #pragma unroll
       for (int c = 0; c < COLS; c += 32) {
         const int64_t n = n0 + c + lane;
@@ -865,19 +873,30 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           __syncwarp();
         }
         uint32_t w[kWords * 4];
-#pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          const float4 s = *reinterpret_cast<const float4*>(sw + i * 32 + j), t = *reinterpret_cast<const float4*>(sb + i * 32 + j);
-          const rows::F2 x = rows::f2(sx);
-          const rows::F2 lo = rows::fma2(rows::mul2(rows::f2(__int2float_rn((int)v[i & 1][j]), __int2float_rn((int)v[i & 1][j + 1])), x),
-                                         rows::f2(s.x, s.y), rows::f2(t.x, t.y));
-          const rows::F2 hi = rows::fma2(rows::mul2(rows::f2(__int2float_rn((int)v[i & 1][j + 2]), __int2float_rn((int)v[i & 1][j + 3])), x),
-                                         rows::f2(s.z, s.w), rows::f2(t.z, t.w));
-          const float2 p = rows::split(lo), r = rows::split(hi);
+        auto put = [&](int j, float2 p, float2 r) {
           if constexpr (sizeof(T) == 4) {
             w[j] = __float_as_uint(p.x), w[j + 1] = __float_as_uint(p.y), w[j + 2] = __float_as_uint(r.x), w[j + 3] = __float_as_uint(r.y);
           } else {
             w[j / 2] = rows::pack2<T>(p.x, p.y), w[j / 2 + 1] = rows::pack2<T>(r.x, r.y);
+          }
+        };
+        if (!any_large) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float4 s = *reinterpret_cast<const float4*>(sw + i * 32 + j), t = *reinterpret_cast<const float4*>(sb + i * 32 + j);
+            const rows::F2 x = rows::f2(sx);
+            const rows::F2 lo = rows::fma2(rows::mul2(rows::f2(__int2float_rn((int)v[i & 1][j]), __int2float_rn((int)v[i & 1][j + 1])), x),
+                                           rows::f2(s.x, s.y), rows::f2(t.x, t.y));
+            const rows::F2 hi = rows::fma2(rows::mul2(rows::f2(__int2float_rn((int)v[i & 1][j + 2]), __int2float_rn((int)v[i & 1][j + 3])), x),
+                                           rows::f2(s.z, s.w), rows::f2(t.z, t.w));
+            put(j, rows::split(lo), rows::split(hi));
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float4 s = *reinterpret_cast<const float4*>(sw + i * 32 + j), t = *reinterpret_cast<const float4*>(sb + i * 32 + j);
+            put(j, make_float2(scaled(v[i & 1][j], sx, s.x, t.x), scaled(v[i & 1][j + 1], sx, s.y, t.y)),
+                make_float2(scaled(v[i & 1][j + 2], sx, s.z, t.z), scaled(v[i & 1][j + 3], sx, s.w, t.w)));
           }
         }
 #pragma unroll

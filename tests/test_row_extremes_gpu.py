@@ -52,3 +52,24 @@ def test_norm_of_rows_whose_sum_overflows(D, dtype):
         (dx,) = torch.autograd.grad(y, xs, dy.cuda())
         for t in (y, dx):
             assert torch.isnan(t[[1, 4]]).all() and torch.isfinite(t[fine]).all(), keep8
+
+
+# the kernels of a decoding step (alone, in clusters), of few tokens (whole and partial tiles, K in parts), of many tokens,
+# and of two blocks a tile
+@pytest.mark.parametrize("M,K,N", [(1, 768, 32000), (3, 2048, 300), (20, 256, 20000), (20, 4096, 300), (300, 64, 17000), (2931, 768, 2304),
+                                   (2600, 1056, 4104)])
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_products_of_large_rows(M, K, N, dtype):
+    """An integer sum times a token's scale alone can pass float32 where the output does not."""
+    import kernels
+    x = rows_of((M, K), F, 1)
+    x[::2] *= 3e36
+    x = x.to(dtype)
+    wt = kernels.quantize_int8((rows_of((N, K), F, 2) * 1e-6).cuda())
+    bias = params((N,), dtype, 3)[1]
+    want, tol = orc.int8_product(*orc.int8_rows(x), wt.codes.cpu(), wt.scale.cpu(), bias, dtype)
+    assert want.abs().max() < 1e35
+    rows = kernels.quantize_int8(x.cuda())
+    assert rows.scale.max() > 1e35
+    close(kernels.int8_linear(x.cuda(), wt, bias.cuda()), want, tol, "from x")
+    close(kernels.int8_linear(rows, wt, bias.cuda()), want, tol, "from rows")
