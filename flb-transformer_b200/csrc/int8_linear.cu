@@ -66,6 +66,11 @@ struct Int8Args {
   int drop;           // a step whose copies the first block, or pair, waits for in vain (a test of the waits), or -1
 };
 
+// A bounded wait whose first poll is not behind the limit, an argument: 8192 x 4096 x 4096 in 93 us, 96 with it in front
+__device__ __forceinline__ bool step_wait(uint64_t* bar, uint32_t phase, uint32_t limit) {
+  return mbar_try_wait(bar, phase) || mbar_wait(bar, phase, limit);
+}
+
 // One thread's MMAs so far are done when this returns, or the limit has run out. issued: there are any.
 __device__ __forceinline__ void drain_mma(uint64_t* drain, bool issued, uint32_t* error) {
   if (issued) umma_commit(drain);
@@ -213,7 +218,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           const int s = it % S;
           uint8_t* st = ring + (size_t)s * kBytes;
           if (it >= early) {
-            if (it >= (uint32_t)S && !mbar_wait(&empty[s], ((it / S) & 1) ^ 1, a.limit)) {
+            if (it >= (uint32_t)S && !step_wait(&empty[s], ((it / S) & 1) ^ 1, a.limit)) {
               ok = false;
               break;
             }
@@ -239,7 +244,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       wait_predecessor();
       for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++local) {
         const uint32_t b = local & 1;
-        if (local >= 2 && !mbar_wait(&acc_empty[b], ((local >> 1) & 1) ^ 1, a.limit)) {
+        if (local >= 2 && !step_wait(&acc_empty[b], ((local >> 1) & 1) ^ 1, a.limit)) {
           ok = false;
           break;
         }
@@ -248,7 +253,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         k_range(u % a.splits, k0, k1);
         for (int k = k0; k < k1; ++k, ++it) {
           const int s = it % S;
-          if (!mbar_wait(&full[s], (it / S) & 1, a.limit)) {
+          if (!step_wait(&full[s], (it / S) & 1, a.limit)) {
             ok = false;
             break;
           }
@@ -291,7 +296,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       for (int c = 0; c < COLS; c += 32)
         if (c + lane < COLS) sx[c + lane] = m0 + c + lane < a.M ? __ldg(a.sx + m0 + c + lane) : 0.f;
       __syncwarp();
-      if (!mbar_wait(&acc_full[b], (local >> 1) & 1, limit)) {
+      if (!step_wait(&acc_full[b], (local >> 1) & 1, limit)) {
         // carries on with what is there, so that the warps meet at every barrier below
         limit = 1;
         if (lane == 0) atomicExch(a.error, 1u);
@@ -512,7 +517,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       for (int tile = first_tile; tile < a.tiles && ok; tile += stride) {
         for (int k = k0; k < k1; ++k, ++it) {
           const int s = it % S;
-          if (it >= (uint32_t)S && !mbar_wait(&empty[s], ((it / S) & 1) ^ 1, a.limit)) {
+          if (it >= (uint32_t)S && !step_wait(&empty[s], ((it / S) & 1) ^ 1, a.limit)) {
             ok = false;
             break;
           }
@@ -530,17 +535,17 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     if (lane == 0) {
       constexpr uint32_t idesc = idesc_i8<NT>();
       uint32_t it = 0, local = 0;
-      bool ok = mbar_wait(&rows_ready, 0, a.limit);
+      bool ok = step_wait(&rows_ready, 0, a.limit);
       for (int tile = first_tile; tile < a.tiles && ok; tile += stride, ++local) {
         const uint32_t b = local & 1;
-        if (local >= 2 && !mbar_wait(&acc_empty[b], ((local >> 1) & 1) ^ 1, a.limit)) {
+        if (local >= 2 && !step_wait(&acc_empty[b], ((local >> 1) & 1) ^ 1, a.limit)) {
           ok = false;
           break;
         }
         tc_fence_after();
         for (int k = k0; k < k1; ++k, ++it) {
           const int s = it % S;
-          if (!mbar_wait(&full[s], (it / S) & 1, a.limit)) {
+          if (!step_wait(&full[s], (it / S) & 1, a.limit)) {
             ok = false;
             break;
           }
@@ -621,7 +626,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       uint32_t local = 0, limit = a.limit;
       for (int tile = first_tile; tile < a.tiles; tile += stride, ++local) {
         const uint32_t b = local & 1;
-        if (!mbar_wait(&acc_full[b], (local >> 1) & 1, limit)) {
+        if (!step_wait(&acc_full[b], (local >> 1) & 1, limit)) {
           limit = 1;  // carries on with what is there
           if (lane == 0) atomicExch(a.error, 1u);
         }
@@ -739,7 +744,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         if (PAIR) n0 += place_in_pair * ROWS;
         for (int k = 0; k < a.k_blocks; ++k, ++it) {
           const int s = it % S;
-          if (it >= (uint32_t)S && !mbar_wait(&empty[s], ((it / S) & 1) ^ 1, a.limit)) {
+          if (it >= (uint32_t)S && !step_wait(&empty[s], ((it / S) & 1) ^ 1, a.limit)) {
             ok = false;
             break;
           }
@@ -776,7 +781,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         // the first block's arrivals at this block's barriers are all in before the block ends
         if (complete)
           for (uint32_t i = last; i < it; ++i)
-            if (!mbar_wait(&empty[i % S], (i / S) & 1, a.limit)) ok = false;
+            if (!step_wait(&empty[i % S], (i / S) & 1, a.limit)) ok = false;
         if (place_in_pair == 1 && !mbar_wait(&drain, 0, kDrainLimit)) ok = false;
       }
       if (!ok) atomicExch(a.error, 1u);
@@ -789,14 +794,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       wait_predecessor();
       for (int tile = worker; tile < a.tiles && ok; tile += workers, ++local) {
         const uint32_t b = local & 1;
-        if (local >= 2 && !mbar_wait(&acc_empty[b], ((local >> 1) & 1) ^ 1, a.limit)) {
+        if (local >= 2 && !step_wait(&acc_empty[b], ((local >> 1) & 1) ^ 1, a.limit)) {
           ok = false;
           break;
         }
         tc_fence_after();
         for (int k = 0; k < a.k_blocks; ++k, ++it) {
           const int s = it % S;
-          if (!mbar_wait(&full[s], (it / S) & 1, a.limit)) {
+          if (!step_wait(&full[s], (it / S) & 1, a.limit)) {
             ok = false;
             break;
           }
@@ -846,7 +851,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         sb[c + lane] = bias;
       }
       __syncwarp();
-      if (!mbar_wait(&acc_full[b], (local >> 1) & 1, limit)) {
+      if (!step_wait(&acc_full[b], (local >> 1) & 1, limit)) {
         limit = 1;  // carries on with what is there
         if (lane == 0) atomicExch(a.error, 1u);
       }
