@@ -61,8 +61,8 @@ def int8_linear(x: torch.Tensor | Int8Rows, weight: Int8Rows, bias: torch.Tensor
 
 
 class Int8Linear(nn.Module):
-    """A linear map whose weight is kept in 8-bit integers (buffers `codes` and `scale`). For inference: its output
-    has no gradient. check_timeout as in int8_linear."""
+    """A linear map whose weight is kept in 8-bit integers (buffers `codes` and `scale`, which keep their types when the module
+    is cast). For inference: its output has no gradient. check_timeout as in int8_linear."""
 
     def __init__(self, weight: Int8Rows, bias: torch.Tensor | None = None, check_timeout: bool = False):
         super().__init__()
@@ -78,6 +78,16 @@ class Int8Linear(nn.Module):
         with torch.no_grad():
             bias = None if linear.bias is None else linear.bias.detach().clone()
             return cls(quantize_int8(linear.weight), bias, check_timeout)
+
+    def _apply(self, fn, recurse=True):
+        # a cast of the model is not for the codes and scales: they follow to its device alone
+        kept = {"codes": self.codes, "scale": self.scale}
+        super()._apply(fn, recurse)
+        for name, t in kept.items():
+            moved = getattr(self, name)
+            if moved.dtype != t.dtype:
+                setattr(self, name, t.to(moved.device))
+        return self
 
     @torch.no_grad()
     def forward(self, x: torch.Tensor | Int8Rows) -> torch.Tensor:

@@ -1,4 +1,5 @@
-"""More refusals of the row operators and 8-bit products, and what their modules do without a kernel (no GPU)."""
+"""More refusals of the row operators and 8-bit products, and what their modules do without a kernel (no GPU,
+but for the test that is marked)."""
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -74,3 +75,33 @@ def test_check_timeout_reaches_the_kernel(monkeypatch):
         kernels.Int8Linear.from_linear(linear, check)(int8_rows())
         assert Ops.calls == [check] * 4
         Ops.calls.clear()
+
+
+CASTS = [lambda m: m.to(torch.bfloat16), lambda m: m.half(), lambda m: m.double(), lambda m: m.bfloat16().float(),
+         lambda m: m.type(torch.float16)]
+
+
+@pytest.mark.parametrize("cast", CASTS)
+def test_a_cast_of_the_module_keeps_the_integers_and_scales(cast):
+    import kernels
+    rows = kernels.Int8Rows(torch.arange(-16, 16, dtype=torch.int8).reshape(4, 8), torch.rand(4) + 1 / 3)
+    m = torch.nn.Sequential(kernels.Int8Linear(rows, torch.ones(4)), torch.nn.Linear(4, 4))
+    want = [t.clone() for t in rows[:2]]
+    assert cast(m) is m
+    for got, t in zip((m[0].codes, m[0].scale), want):
+        assert got.dtype == t.dtype and torch.equal(got, t)
+    assert m[0].bias.dtype == m[1].weight.dtype and set(m[0].state_dict()) == {"codes", "scale", "bias"}
+    m[0].to("meta")
+    assert m[0].scale.device.type == m[0].codes.device.type == "meta" and m[0].scale.dtype == torch.float32
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cast", CASTS)
+def test_a_cast_module_gives_the_same(cast):
+    import kernels
+    linear = torch.nn.Linear(96, 40)
+    x = torch.randn(7, 96, device="cuda")
+    m = torch.nn.Sequential(kernels.Int8Linear.from_linear(linear.cuda()))
+    m[0].bias = None
+    want = m(x)
+    assert torch.equal(cast(m)(x), want) and torch.equal(m.cpu().cuda()(x), want)
