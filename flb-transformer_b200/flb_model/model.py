@@ -131,7 +131,7 @@ class FLBTransformer(nn.Module):
         B, D = self.config.batch_size, self.config.dim
         y, lat, fdbk, aux = (g.view(L, S, B, D) for g in grids)
         top = self.out_dropout(y[-1].transpose(0, 1))               # [batch, seq, dim]
-        logits = (head or self.head)(top)
+        logits = (self.head if head is None else head)(top)
         aux_loss = aux.mean() * self.aux_weight
         return logits, aux_loss, (lat[:, -1], fdbk[:, -1])
 

@@ -105,3 +105,13 @@ def test_a_cast_module_gives_the_same(cast):
     m[0].bias = None
     want = m(x)
     assert torch.equal(cast(m)(x), want) and torch.equal(m.cpu().cuda()(x), want)
+
+
+def test_a_head_without_modules_is_a_head():
+    """FLBTransformer takes a head that is given, also an empty nn.Sequential, whose length is zero."""
+    from flb_model import FLBTransformer
+    m = FLBTransformer(11, hidden_dim=8, num_layers=2, seq_len=3, batch_size=2, num_heads=2).eval()
+    grids = [torch.randn(6, 2, 8) for _ in range(4)]
+    top = grids[0].view(2, 3, 2, 8)[-1].transpose(0, 1)
+    assert torch.equal(m.grids_to_outputs(grids, torch.nn.Sequential())[0], top)
+    assert torch.equal(m.grids_to_outputs(grids)[0], m.head(top))
