@@ -287,14 +287,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       const int64_t n0 = (int64_t)(tile % a.n_tiles) * kChannels, m0 = (int64_t)(tile / a.n_tiles) * NT + first;
       const int64_t channel = n0 + q * 32 + lane;
       const bool there = channel < a.N, full_tile = n0 + kChannels <= a.N && m0 + COLS <= a.M;
-      const float sw = there ? __ldg(a.sw + channel) : 0.f;
+      const float sw = there ? ld(a.sw + channel) : 0.f;
       float bias = 0.f;
       if (a.bias && there)
-        bias = a.bias32 ? __ldg(reinterpret_cast<const float*>(a.bias) + channel) : ld(reinterpret_cast<const T*>(a.bias) + channel);
+        bias = a.bias32 ? ld(reinterpret_cast<const float*>(a.bias) + channel) : ld(reinterpret_cast<const T*>(a.bias) + channel);
       __syncwarp();
 #pragma unroll
       for (int c = 0; c < COLS; c += 32)
-        if (c + lane < COLS) sx[c + lane] = m0 + c + lane < a.M ? __ldg(a.sx + m0 + c + lane) : 0.f;
+        if (c + lane < COLS) sx[c + lane] = m0 + c + lane < a.M ? ld(a.sx + m0 + c + lane) : 0.f;
       __syncwarp();
       if (!step_wait(&acc_full[b], (local >> 1) & 1, limit)) {
         // carries on with what is there, so that the warps meet at every barrier below
@@ -447,10 +447,15 @@ struct StepArgs {
   int K;
 };
 
-// Eight elements of a row from k on, zeros beyond K
+// Eight elements of a row from k on, zeros beyond K. By ordinary loads, as everything here that a predecessor may have
+// written: this kernel may start beside it, and the read-only path is for what does not change while a kernel runs.
 template <typename T> __device__ __forceinline__ void load_row8(rows::Raw8<T>& r, const T* row, int k, int K, bool vec) {
   if (vec) {
-    rows::load_raw<T, rows::EIGHT>(r, row, k, 0, K);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+      const uint4 v = k < K ? reinterpret_cast<const uint4*>(row + k)[i] : make_uint4(0, 0, 0, 0);
+      r.w[4 * i] = v.x, r.w[4 * i + 1] = v.y, r.w[4 * i + 2] = v.z, r.w[4 * i + 3] = v.w;
+    }
   } else {
     float v[8];
 #pragma unroll
@@ -468,8 +473,8 @@ template <typename T> __device__ __forceinline__ void finish_step(const Int8Args
   const bool there = channel < a.N;
   float bias = 0.f;
   if (a.bias && there)
-    bias = a.bias32 ? __ldg(reinterpret_cast<const float*>(a.bias) + channel) : ld(reinterpret_cast<const T*>(a.bias) + channel);
-  store_tokens<T, kStepTokens, false>(a, acc, scale, there ? __ldg(a.sw + channel) : 0.f, bias, 0, channel);
+    bias = a.bias32 ? ld(reinterpret_cast<const float*>(a.bias) + channel) : ld(reinterpret_cast<const T*>(a.bias) + channel);
+  store_tokens<T, kStepTokens, false>(a, acc, scale, there ? ld(a.sw + channel) : 0.f, bias, 0, channel);
 }
 
 template <typename T>
@@ -839,17 +844,21 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       place(tile, m0, n0);
       n0 += first;
       const int token = m0 + q * 32 + lane;
-      const float sx = token < a.M ? __ldg(a.sx + token) : 0.f;
+      const float sx = token < a.M ? ld(a.sx + token) : 0.f;
       const bool any_large = __any_sync(0xffffffffu, fabsf(sx) > kLargeScale);
+      // all loads before the first store, which they might otherwise have to wait for
+      float channel_scale[COLS / 32], channel_bias[COLS / 32];
 #pragma unroll
-      for (int c = 0; c < COLS; c += 32) {
-        const int64_t n = n0 + c + lane;
+      for (int c = 0; c < COLS / 32; ++c) {
+        const int64_t n = n0 + c * 32 + lane;
         const bool there = n < a.N;
-        sw[c + lane] = there ? __ldg(a.sw + n) : 0.f;
-        float bias = 0.f;
-        if (a.bias && there) bias = a.bias32 ? __ldg(reinterpret_cast<const float*>(a.bias) + n) : ld(reinterpret_cast<const T*>(a.bias) + n);
-        sb[c + lane] = bias;
+        channel_scale[c] = there ? ld(a.sw + n) : 0.f;
+        channel_bias[c] = 0.f;
+        if (a.bias && there) channel_bias[c] = a.bias32 ? ld(reinterpret_cast<const float*>(a.bias) + n) : ld(reinterpret_cast<const T*>(a.bias) + n);
       }
+      __syncwarp();
+#pragma unroll
+      for (int c = 0; c < COLS / 32; ++c) sw[c * 32 + lane] = channel_scale[c], sb[c * 32 + lane] = channel_bias[c];
       __syncwarp();
       if (!step_wait(&acc_full[b], (local >> 1) & 1, limit)) {
         limit = 1;  // carries on with what is there

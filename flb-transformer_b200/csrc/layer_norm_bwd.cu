@@ -266,9 +266,10 @@ __global__ void __launch_bounds__(MODE == 0 ? 32 * kWarps : MODE == 1 ? 512 : 10
 }
 
 // dw and db from the blocks' sums: 16 columns a block, four a thread, so that a warp reads eight workspace rows
-// at a time and every load of a thread can be under way at once.
+// at a time and every load of a thread can be under way at once. Ordinary loads: the kernel may start beside the one that
+// writes the workspace, and the read-only path is for what does not change while a kernel runs.
 template <typename T>
-__global__ void __launch_bounds__(1024) ln_sum_kernel(const float* __restrict__ part, void* dw, void* db, bool w32,
+__global__ void __launch_bounds__(1024) ln_sum_kernel(const float* part, void* dw, void* db, bool w32,
                                                       int blocks, int D) {
   __shared__ float s[256][17];
   wait_predecessor();
@@ -280,7 +281,7 @@ __global__ void __launch_bounds__(1024) ln_sum_kernel(const float* __restrict__ 
     const float* p = part + (group * blocks * 2 + which) * pitch + col;
 #pragma unroll 8
     for (int i = ty; i < blocks; i += 256) {
-      const float4 t = __ldg(reinterpret_cast<const float4*>(p + (int64_t)i * 2 * pitch));
+      const float4 t = *reinterpret_cast<const float4*>(p + (int64_t)i * 2 * pitch);
       v.x += t.x, v.y += t.y, v.z += t.z, v.w += t.w;
     }
   }

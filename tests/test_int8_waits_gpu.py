@@ -112,3 +112,49 @@ def test_check_timeout_from_python():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("M,K,N", [(40, 256, 20000), (2931, 768, 2304), (5120, 1104, 2048), (1, 768, 32000)])
+def test_everything_a_late_predecessor_writes_is_read_after_it(M, K, N):
+    """Scales, bias and a decoding step's x, written beside the product's start to where other values were read before."""
+    import flb_native as nat
+    import kernels
+    x, wt = rows_of((M, K), BF, 1).cuda(), kernels.quantize_int8(rows_of((N, K), BF, 2).cuda())
+    rows = kernels.quantize_int8(x)
+    old = torch.cat([t.float().view(torch.uint8).reshape(-1) for t in (rows.scale, wt.scale, torch.zeros(N, device="cuda"))] +
+                    [x.view(torch.uint8).reshape(-1)])
+    new = old.clone()
+    sizes = [4 * M, 4 * N, 4 * N, 2 * M * K]
+
+    def parts(buffer):
+        sx, sw, bias, xs = buffer[:sum(sizes)].split(sizes)
+        return sx.view(torch.float32), sw.view(torch.float32), bias.view(torch.float32), xs.view(BF).view(M, K)
+
+    pad = torch.zeros(-sum(sizes) % 16, dtype=torch.uint8, device="cuda")
+    old, new = torch.cat([old, pad]), torch.cat([new, pad])
+    for t, f in zip(parts(new), (2.0, 0.5, None, None)):
+        t.mul_(f) if f else t.copy_(torch.randn(t.shape, device="cuda"))
+    both = [b for b in (old, new)]
+    step = M <= 16
+    n = nat.lib.flb_int8_linear_workspace_bytes(M, N, K, int(not step))
+    ws = nat.workspace(n, x.device)
+    out = torch.empty(M, N, dtype=BF, device="cuda")
+    buffer = old.clone()
+
+    def call(buffer):
+        sx, sw, bias, xs = parts(buffer)
+        what = (xs.data_ptr(), K, None, 0, None) if step else (None, 0, rows.codes.data_ptr(), rows.codes.stride(0), sx.data_ptr())
+        assert nat.lib.flb_int8_linear(*what, wt.codes.data_ptr(), wt.codes.stride(0), sw.data_ptr(), bias.data_ptr(), nat.F32,
+                                       out.data_ptr(), M, N, K, nat.BF16, ws.data_ptr(), n, 0, nat.stream_of(out)) == 0
+
+    want = []
+    for b in both:
+        call(b)
+        want.append(out.clone())
+    assert not torch.equal(*want)
+    for i in range(10):
+        call(buffer)  # what is there now has been read
+        assert nat.lib.flb_selftest_late_copy(both[i % 2].data_ptr(), buffer.data_ptr(), buffer.numel(), 100, nat.stream_of(out)) == 0
+        call(buffer)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[i % 2]), i
