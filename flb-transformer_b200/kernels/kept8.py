@@ -6,8 +6,11 @@
 The kept form holds blocks of 128 consecutive elements of the last axis as integers of at most 127 in
 magnitude times a power of two, the smallest for which the block's largest magnitude still rounds to at
 most 127: an element is off by at most 1/127 of its block's largest magnitude (half a unit of between
-1/127.5 and 1/63.5 of it). A block that holds an infinity or NaN comes back as NaN. It takes
-1 + 1/128 bytes an element (the rows of codes padded to 16 bytes).
+1/127.5 and 1/63.5 of it). That holds for largest magnitudes from 63.5 * 2^-126 to 63.5 * 2^122 (7.5e-37 to
+3.38e38). Below, the unit stays 2^-126: an element is off by at most 2^-127, and a block of less than that
+comes back as zeros. Above, where float32 does not hold a code of 64, it is 63: off by at most 1/63 of the
+largest magnitude. A block that holds an infinity or NaN comes back as NaN. It takes 1 + 1/128 bytes an
+element (the rows of codes padded to 16 bytes).
 
 The kernels are in libflb_b200.so (flb_pack8, flb_unpack8, flb_gate_fwd, flb_gate_bwd), called through
 flb_ops; CUDA tensors only.

@@ -54,6 +54,25 @@ def test_norm_of_rows_whose_sum_overflows(D, dtype):
             assert torch.isnan(t[[1, 4]]).all() and torch.isfinite(t[fine]).all(), keep8
 
 
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_kept_errors_over_the_range(dtype):
+    """What the kept form is off by: 1/127 of the block's largest magnitude between the ends of the range, 2^-127 below
+    them, and one unit in 63 where the largest magnitude would round to 64 * 2^122, which float32 does not hold."""
+    import kernels
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(400, 128, generator=g, dtype=torch.float64)
+    x = x / x.abs().amax(-1, keepdim=True) * torch.exp2(torch.linspace(-140, 128, 400, dtype=torch.float64)[:, None])
+    x = torch.cat([x, torch.full((1, 128), torch.finfo(dtype).max, dtype=torch.float64)])
+    x = x.clamp(-torch.finfo(dtype).max, torch.finfo(dtype).max).to(dtype)
+    got = kernels.unpack8(kernels.pack8(x.cuda()), F).cpu().double()
+    x = x.double()
+    top = x.abs().amax(-1, keepdim=True)
+    bound = torch.maximum(top / 127, torch.full_like(top, 2.0 ** -127))
+    bound = torch.where(top >= 63.5 * 2.0 ** 122, top / 63, bound)
+    assert ((got - x).abs() <= bound).all()
+    assert not got[top[:, 0] < 2.0 ** -127].any()
+
+
 # the kernels of a decoding step (alone, in clusters), of few tokens (whole and partial tiles, K in parts), of many tokens,
 # and of two blocks a tile
 @pytest.mark.parametrize("M,K,N", [(1, 768, 32000), (3, 2048, 300), (20, 256, 20000), (20, 4096, 300), (300, 64, 17000), (2931, 768, 2304),
