@@ -8,19 +8,21 @@
 // channels a tile, and the tokens its N side, NT of 16 to 128: a decoding step wastes little of a tile.
 // With fewer tiles than SMs a unit is a part of a tile's K range; the parts leave integer sums in the
 // workspace, and the block that counts itself last adds them up: integers, the same in any order. Any N and
-// alignment. Bound by its chain of latencies (launch, first copies, MMAs, sums: 16 x 4096 x 4096 10.9 us with the
+// alignment. Bound by its chain of latencies (launch, first copies, MMAs, sums: 16 x 4096 x 4096 10.7 us with the
 // rows' kernel, 2.6 us of it the weight's bytes).
 //
 // int8_step_kernel, the same for up to 16 tokens of x itself, whose integer rows it makes on the way: 1 x 768 x 32000
-// in 9.0 us, 3.8 us of it the weight's bytes.
+// in 8.4 us, 3.8 us of it the weight's bytes.
 //
 // int8_many_kernel, for tiles enough to fill the SMs. The tokens are the M side, 128 a block, and 256 or 128
 // channels the N side: a thread of the epilogue has a token's consecutive channels, packs them and leaves
 // them in shared memory for a TMA store. (With the other orientation a thread has one channel of many
 // tokens; pairing them up by shuffles took three times the instructions and bound the kernel.) For long K two
-// blocks of a cluster share a tile of 256 x 256 (cta_group::2). Bound by the tensor cores: 8192 x 8192 x 8192
-// in 360 us, 3.06 POPS, 1.85 times the bf16 product's measured rate. With small K the output's way to memory
-// takes its share: 16384 x 768 x 32000 in 370 us, 2.18 POPS, of which 160 us would write the output alone.
+// blocks of a cluster share a tile of 256 x 256 (cta_group::2). Bound by the tensor cores, and over seconds by the power that
+// they draw (995 W, the SMs at 1430 to 1490 MHz then): 8192 x 8192 x 8192 in 349 us in a short run and 404 in a long
+// one, 3.15 and 2.72 POPS, 1.9 times the bf16 product's measured rates for each. With small K the output's way to memory takes
+// its share: 16384 x 768 x 32000 in 397 and 461 us, 2.03 and 1.75 POPS, of which 160 us would write the output alone.
+// Times below are of short runs / of runs of seconds where there are two.
 #include <cmath>
 #include "rows.cuh"
 #include "sm100.cuh"
@@ -827,7 +829,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     }
   } else {
     // a warp has the 32 TMEM lanes, here tokens, of its number mod 4, and half of the channels. (16 warps with a quarter
-    // each and one staged tile took 423 us instead of 369 for 16384 x 768 x 32000.)
+    // each and one staged tile took 423 us instead of 369, in short runs, for 16384 x 768 x 32000.)
     constexpr int COLS = NC / 2, STEPS = COLS / 32, kWords = 32 * (int)sizeof(T) / 16;  // 16-byte words a lane stages a step
     const int q = warp & 3, first = (warp - 2) / 4 * COLS;
     uint8_t* const mine = ring + (size_t)S * kBytes + (size_t)(warp - 2) * (2 * kStaged);
@@ -942,9 +944,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 }
 
 // Orders of the tiles, of 126 MB of L2. A weight that stays there is best gone through once for each tile of tokens: the
-// blocks then write whole rows of the output (16384 x 768 x 32000: 415 us at either order with the output's default
-// policy, 374 against 402 with an output too large for L2 leaving it first). A larger one would come from
-// memory each time: 16 tiles of tokens at once (8192 x 4096 x 32000, 131 MB: 779 us against 1183).
+// blocks then write whole rows of the output (16384 x 768 x 32000: 398 / 463 us, with 16 tiles of tokens at once 419 / 475; an
+// output too large for L2 leaves it first, with the default policy 436 / 496). A larger one would come from
+// memory each time: 16 tiles of tokens at once (8192 x 4096 x 32000, 131 MB: 712 / 823 us against 857 / 1073).
 constexpr int64_t kWeightInL2 = 48 << 20;
 constexpr size_t kOutputInL2 = 64 << 20;
 
@@ -961,11 +963,11 @@ GemmShape gemm_shape(int64_t M, int64_t N, int64_t K, bool rows_on_16, bool from
   g.many = rows_on_16 && M > 64 && tiles(128) >= sms;
   if (g.many) {
     // Pairs of blocks load a third less for each product, but start later and hand over tiles between them: for more
-    // tiles than SMs with K of 1024 on (8192 x 1024 x 8192: 58 us against 62, 8192 x 4096 x 4096: 94 against 105;
-    // 8192 x 768 x 8192: 56 against 50, 1000 x 4096 x 4096: 20.5 against 19.2).
+    // tiles than SMs with K of 1024 on (8192 x 1024 x 8192: 58 / 69 us against 63 / 74, 8192 x 4096 x 4096: 93 / 107 against
+    // 106 / 120; 8192 x 768 x 8192: 53 / 62 against 51 / 60, 1000 x 4096 x 4096: 17.6 / 16.9 against 16.8 / 17.0).
     g.pair = sms % 2 == 0 && K >= 1024 && tiles(256) > sms;
     // Of a block's own tiles those whose rounds over the SMs cost least, a K step of a tile costing the rows that it
-    // loads (2931 x 768 x 2304: 12.4 us with 256 channels, 14.1 with 128; 300 x 4096 x 4096: 18.5 and 17.8).
+    // loads (2931 x 768 x 2304: 10.1 us with 256 channels, 11.6 with 128; 300 x 4096 x 4096: 15.4 and 15.3).
     auto cost = [&](int nc) { return (tiles(nc) + sms - 1) / sms * (kTokens + nc); };
     g.width = g.pair || cost(256) <= cost(128) ? 256 : 128;
     g.n_tiles = (int)((N + g.width - 1) / g.width);
@@ -982,9 +984,9 @@ GemmShape gemm_shape(int64_t M, int64_t N, int64_t K, bool rows_on_16, bool from
   const int64_t blocks = (K + kStep - 1) / kStep;
   const int64_t pay = std::max<int64_t>(1, std::llround(std::sqrt((double)blocks * (kChannels + g.width) / (4.0 * g.width))));
   g.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(blocks, pay), sms / g.tiles));
-  // A decoding step's kernel while x is small: every one of its blocks goes through all of it (1 x 768 x 32000: 9.0 us
-  // against 10.1 with a launch of its own for the rows, and 3 us less for the host; 8 x 2048 x 2048: 8.4 and 10.0;
-  // 16 x 4096 x 4096: 13.3 and 10.9; 8 x 4096 x 16000: 19.3 and 15.8).
+  // A decoding step's kernel while x is small: every one of its blocks goes through all of it (1 x 768 x 32000: 8.4 us
+  // against 10.1 with a launch of its own for the rows, and 3 us less for the host; 8 x 2048 x 2048: 8.0 and 8.9;
+  // 16 x 4096 x 4096: 12.7 and 10.8; 8 x 4096 x 16000: 18.4 and 15.9).
   g.step = from_x && M <= kStepTokens && K <= kStepWidest && M * K <= (g.tiles <= 64 ? 16384 : 8192);
   // clusters of 2, 4 or 8 blocks, no more of them than run at once (16 of 8 did not: 1 x 2048 x 2048 took 11.7 us)
   if (g.step) g.splits = g.splits >= 8 && g.tiles <= 8 ? 8 : g.splits >= 4 && g.tiles <= 32 ? 4 : g.splits >= 2 && g.tiles <= 64 ? 2 : 1;

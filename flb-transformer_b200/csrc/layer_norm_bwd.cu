@@ -7,7 +7,7 @@
 // a fixed distance apart, the next rows on their way to shared memory meanwhile, and adds up dw and db of
 // the columns that its threads own in float32 registers. A block's sums go to its own row of a
 // workspace, which a second kernel adds up in a fixed order: no atomics, the same bits every time. With
-// one block a group (few rows) the block writes dw and db itself. 32768 x 4096 bfloat16: 152 us, 5.3 TB/s, of which
+// one block a group (few rows) the block writes dw and db itself. 32768 x 4096 bfloat16: 151 us, 5.3 TB/s, of which
 // the second kernel takes 5; what is left is the warps' waits for one another once a row.
 #include "rows.cuh"
 

@@ -19,8 +19,9 @@ state_dict trained with either loads into the other:
 
 fused_ops=True evaluates the blocks' norms and gates with kernels.layer_norm and kernels.sigmoid_gate
 instead of torch's (the parameters' names and shapes are the same); keep8=True (with fused_ops) has
-them keep what their backward reads in 8 bits. Where the engine runs its native whole-grid kernels
-(bf16 autocast), neither is consulted: engine.native_flb_save says there what is kept.
+them keep what their backward reads in 8 bits. The per-tick path is not faster for it: its host time
+rises, and captured as CUDA graphs the two are within a few percent. Where the engine runs its native
+whole-grid kernels (bf16 autocast), neither is consulted: engine.native_flb_save says there what is kept.
 
 The dropout modules exist for state compatibility and run where the reference runs them (the
 attention layer's own dropout is not applied there either).

@@ -8,9 +8,11 @@
 
 x: float32, float16 or bfloat16, [..., D] with D <= 32768 (16384 where a gradient is wanted). weight and
 bias: float32 or x's type, [D], or [G, D] for x [G, ..., D]: one weight for each index of x's first
-axis. y has x's type; statistics and the gradient's sums are in float32, and the gradient of the weight
-is summed in a fixed order. With keep8 the backward reads h from 8 bits (kernels.kept8's kept form) instead
-of x from its own: about half the memory kept, and the same y.
+axis (at most 65535 of them; a vmap over weights makes such groups). y has x's type, also under autocast,
+where nn.LayerNorm's is float32. Statistics and the gradient's sums are in float32: a row whose sum overflows
+there is NaN, and where its squares do, h is zero. The gradient of the weight is summed in a fixed order. With
+keep8 the backward reads h from 8 bits (kernels.kept8's kept form) instead of x from its own: about half the
+memory kept, and the same y.
 
 The kernels are in libflb_b200.so (flb_layer_norm_fwd, flb_layer_norm_bwd), called through flb_ops;
 CUDA tensors only.
