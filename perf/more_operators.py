@@ -409,8 +409,8 @@ def _exact_round(x, noise, below, unsigned):
     size = x.abs()
     top = size.amax(1, keepdim=True)
     top = torch.where(top > 0, (torch.frexp(top.float())[1].double() - 1).clamp(min=below - 126), below - 126.0)
-    e = torch.frexp(size)[1].double() - 1
-    r = torch.floor(torch.ldexp(size, 3 - e) + noise / 65536) * torch.exp2(e - 3)
+    part, e = torch.frexp(size)
+    r = torch.floor(16 * part + noise / 65536) * torch.exp2(e.double() - 4)
     least = torch.exp2(top - below) * 1.125
     r = torch.where(r < least, least if unsigned else 0.0, r)
     return torch.where(size > 0, torch.copysign(r, x), 0.0)
