@@ -215,7 +215,6 @@ def _noise(blocks, step):
     i = torch.cat([torch.arange(b * _BLOCK, device="cuda") for b in blocks]).view(-1, _BLOCK)
     i = (i * 0x9E3779B9 + step * 0x6A09E667 + _SEED) & 0xffffffff
     i = ((i ^ (i >> 16)) * 0xBB67AE85) & 0xffffffff
-    i = ((i ^ (i >> 13)) * 0x6A09E667) & 0xffffffff
     return i ^ (i >> 16)
 
 
