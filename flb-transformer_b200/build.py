@@ -40,6 +40,9 @@ CU_SOURCES = [
     "layer_norm_bwd.cu",
     "kept8.cu",
     "int8_linear.cu",
+    "c_abi_head.cu",
+    "sample.cu",
+    "adamw.cu",
     "microbench.cu",
     "umma_selftest.cu",
 ]

@@ -436,6 +436,135 @@ Tensor int8_linear(const Opt& x_, const Opt& x_codes, const Opt& x_scale, const 
   return out;
 }
 
+// ---- a token from logits ------------------------------------------------------------------------------------
+
+// A setting for each row, or none.
+Opt row_setting(const Opt& t, const Tensor& logits, at::ScalarType type, const char* name) {
+  if (!given(t)) return Opt();
+  same_device(logits, t);
+  TORCH_CHECK_TYPE(t->scalar_type() == type, name, " must be a number or a tensor of ", type, ", not of ", t->scalar_type());
+  TORCH_CHECK_VALUE(t->sizes() == logits.sizes().slice(0, logits.dim() - 1), name, " of shape ", t->sizes(), " for logits of shape ",
+                    logits.sizes());
+  return t->contiguous();
+}
+
+Tensor sample(const Tensor& logits_, const Tensor& u_, const Opt& temperature_, double temperature_all, const Opt& top_k_, int64_t top_k_all,
+              const Opt& top_p_, double top_p_all, const Opt& min_p_, double min_p_all) {
+  const int dt = dtype_of(logits_, "logits");
+  need_cuda(logits_);
+  TORCH_CHECK_VALUE(last_axis(logits_, "logits") >= 1, "logits must have a last axis of at least one element");
+  const bool u64 = u_.scalar_type() == at::kDouble;
+  const c10::cuda::CUDAGuard guard(logits_.device());
+  const Opt u = row_setting(u_, logits_, u64 ? at::kDouble : at::kFloat, "u");
+  const Opt temperature = row_setting(temperature_, logits_, at::kFloat, "temperature"), top_k = row_setting(top_k_, logits_, at::kLong, "top_k");
+  const Opt top_p = row_setting(top_p_, logits_, at::kFloat, "top_p"), min_p = row_setting(min_p_, logits_, at::kFloat, "min_p");
+  auto [x, ld] = rows_of(logits_);
+  Tensor token = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kLong));
+  check(flb_sample(x.data_ptr(), ld, ptr(u), u64, token.data_ptr<int64_t>(), rows_in(x), x.size(-1), dt, (const float*)ptr(temperature),
+                   temperature_all, (const int64_t*)ptr(top_k), top_k_all, (const float*)ptr(top_p), top_p_all, (const float*)ptr(min_p),
+                   min_p_all, stream_of(x)),
+        "flb_sample");
+  return token;
+}
+
+// ---- AdamW ----------------------------------------------------------------------------------------------------
+
+// Elements in memory's order, one after the other: what a kernel that goes by addresses needs.
+void need_dense(const Tensor& t, const char* name) {
+  TORCH_CHECK_VALUE(t.is_non_overlapping_and_dense(), "AdamW: ", name, " of shape ", t.sizes(), " and strides ", t.strides(),
+                    " has gaps or shares elements");
+}
+void need_codes(const Tensor& codes, const Tensor& exps, const Tensor& p) {
+  const int64_t blocks = (p.numel() + 127) / 128;
+  TORCH_CHECK_VALUE(codes.scalar_type() == at::kByte && exps.scalar_type() == at::kByte && codes.numel() == blocks * 128 &&
+                        exps.numel() == blocks && codes.is_contiguous() && exps.is_contiguous(),
+                    "AdamW: a moment's codes and exponents are not those of a parameter of shape ", p.sizes());
+  same_device(p, codes);
+  same_device(p, exps);
+}
+bool same_layout(const Tensor& a, const Tensor& b) { return a.sizes() == b.sizes() && (a.numel() <= 1 || a.strides() == b.strides()); }
+
+void adamw(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& ms, const std::vector<Tensor>& vs,
+           const std::vector<Tensor>& steps, const std::vector<Tensor>& m_exps, const std::vector<Tensor>& v_exps, int64_t bits, double lr,
+           const Opt& lr_device, double b1, double b2, double eps, double decay, uint32_t seed, const Tensor& counter) {
+  const size_t n = params.size();
+  TORCH_CHECK_VALUE(grads.size() == n && ms.size() == n && vs.size() == n && steps.size() == n &&
+                        m_exps.size() == (bits == 8 ? n : 0) && v_exps.size() == m_exps.size(),
+                    "AdamW: lists of different lengths");
+  if (n == 0) return;
+  const Tensor& first = params[0];
+  const int dt = dtype_of(first, "a parameter");
+  need_cuda(first);
+  same_device(first, counter);
+  same_device(first, lr_device);
+  const c10::cuda::CUDAGuard guard(first.device());
+  std::vector<flb_adamw_tensor> t(n);
+  std::vector<Tensor> held;  // gradients in their parameters' order, until the launch
+  for (size_t i = 0; i < n; ++i) {
+    const Tensor& p = params[i];
+    same_device(first, p);
+    need_dense(p, "a parameter");
+    TORCH_CHECK_TYPE(p.scalar_type() == first.scalar_type(), "AdamW: parameters of different types in one call");
+    Tensor g = grads[i];
+    same_device(first, g);
+    TORCH_CHECK_VALUE(g.layout() == at::kStrided, "AdamW: sparse gradients are not supported");
+    TORCH_CHECK_TYPE(g.scalar_type() == p.scalar_type(), "AdamW: a gradient of ", g.scalar_type(), " for a parameter of ", p.scalar_type());
+    TORCH_CHECK_VALUE(g.sizes() == p.sizes(), "AdamW: a gradient of shape ", g.sizes(), " for a parameter of shape ", p.sizes());
+    if (!same_layout(g, p)) {
+      g = at::empty_like(p).copy_(g);
+      held.push_back(g);
+    }
+    if (bits == 8) {
+      need_codes(ms[i], m_exps[i], p);
+      need_codes(vs[i], v_exps[i], p);
+    } else {
+      for (const Tensor* m : {&ms[i], &vs[i]}) {
+        same_device(first, *m);
+        TORCH_CHECK_VALUE(m->scalar_type() == at::kFloat && same_layout(*m, p), "AdamW: a moment is not a float32 tensor laid out as its parameter");
+      }
+    }
+    same_device(first, steps[i]);
+    TORCH_CHECK_VALUE(steps[i].scalar_type() == at::kLong && steps[i].numel() == 1, "AdamW: step must be one int64");
+    t[i] = flb_adamw_tensor{p.data_ptr(), g.data_ptr(), ms[i].data_ptr(), vs[i].data_ptr(), bits == 8 ? (uint8_t*)m_exps[i].data_ptr() : nullptr,
+                            bits == 8 ? (uint8_t*)v_exps[i].data_ptr() : nullptr, steps[i].data_ptr<int64_t>(), p.numel()};
+  }
+  check(flb_adamw(t.data(), (int64_t)n, dt, (int)bits, lr, (const float*)ptr(lr_device), b1, b2, eps, decay, seed, (uint32_t*)counter.data_ptr(),
+                  stream_of(first)),
+        "flb_adamw");
+  for (size_t i = 0; i < n; ++i) {
+    // written behind autograd's back: a graph that still needs the old values is told
+    for (const Tensor* x : {&params[i], &ms[i], &vs[i], &steps[i]}) x->unsafeGetTensorImpl()->bump_version();
+    if (bits == 8)
+      for (const Tensor* x : {&m_exps[i], &v_exps[i]}) x->unsafeGetTensorImpl()->bump_version();
+  }
+}
+
+// m and v of parameters into tensors of their shapes and layouts
+void adamw_moments(const std::vector<Tensor>& params, const std::vector<Tensor>& m_out, const std::vector<Tensor>& v_out,
+                   const std::vector<Tensor>& ms, const std::vector<Tensor>& vs, const std::vector<Tensor>& m_exps,
+                   const std::vector<Tensor>& v_exps) {
+  const size_t n = params.size();
+  if (n == 0) return;
+  need_cuda(params[0]);
+  const c10::cuda::CUDAGuard guard(params[0].device());
+  std::vector<flb_adamw_tensor> t(n);
+  for (size_t i = 0; i < n; ++i) {
+    const Tensor& p = params[i];
+    same_device(params[0], p);
+    for (const Tensor* o : {&m_out[i], &v_out[i]}) {
+      same_device(p, *o);
+      TORCH_CHECK_VALUE(o->scalar_type() == at::kFloat && same_layout(*o, p), "AdamW: moments go to float32 tensors laid out as their parameters");
+    }
+    need_codes(ms[i], m_exps[i], p);
+    need_codes(vs[i], v_exps[i], p);
+    t[i] = flb_adamw_tensor{m_out[i].data_ptr(), v_out[i].data_ptr(), ms[i].data_ptr(), vs[i].data_ptr(), (uint8_t*)m_exps[i].data_ptr(),
+                            (uint8_t*)v_exps[i].data_ptr(), nullptr, p.numel()};
+  }
+  check(flb_adamw_moments(t.data(), (int64_t)n, stream_of(params[0])), "flb_adamw_moments");
+  for (size_t i = 0; i < n; ++i)
+    for (const Tensor* x : {&m_out[i], &v_out[i]}) x->unsafeGetTensorImpl()->bump_version();
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -456,6 +585,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("sigmoid_gate", &sigmoid_gate, off);
   m.def("quantize_int8", &quantize_int8, off);
   m.def("layer_norm_int8", &layer_norm_int8, off);
+  m.def("sample", &sample, off);
+  m.def("adamw", &adamw, off);
+  m.def("adamw_moments", &adamw_moments, off);
   m.def("int8_linear", [](const Opt& x, const Opt& xc, const Opt& xs, const Tensor& wc, const Tensor& ws, const Opt& bias, py::object dtype,
                           bool check_timeout) {
     std::optional<at::ScalarType> t;

@@ -111,6 +111,11 @@ PROTOTYPES = {
                                _i64, _i32, _vp, _sz, _i32, _vp]),
     "flb_int8_linear_wait_test": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i32, _vp, _i64, _i64,
                                          _i64, _i32, _vp, _sz, _i32, _i64, ctypes.c_uint32, _vp]),
+    "flb_sample": (_i32, [_vp, _i64, _vp, _i32, _vp, _i64, _i64, _i32, _vp, ctypes.c_double, _vp, _i64, _vp, ctypes.c_double, _vp,
+                          ctypes.c_double, _vp]),
+    "flb_adamw": (_i32, [_vp, _i64, _i32, _i32, ctypes.c_double, _vp, ctypes.c_double, ctypes.c_double, ctypes.c_double,
+                         ctypes.c_double, ctypes.c_uint32, _vp, _vp]),
+    "flb_adamw_moments": (_i32, [_vp, _i64, _vp]),
     "flb_microbench": (_i32, [_i32, _vp, _dblp]),
     "flb_selftest_umma": (_i32, [_i32, _i32, _vp, _vp, _vp, _vp, _vp]),
     "flb_selftest_late_copy": (_i32, [_vp, _vp, _i64, _i64, _vp]),
@@ -122,6 +127,11 @@ class BlockWeights(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in (
         "ln_lat_w", "ln_lat_b", "ln_fdbk_w", "ln_fdbk_b", "w_prior_lat", "w_prior_fdbk",
         "w_gate_l", "b_gate_l", "w_gate_x", "b_gate_x", "w_qkv", "w_o", "v_a")]
+
+
+class AdamWTensor(ctypes.Structure):
+    """flb_adamw_tensor of include/flb_b200.h."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("p", "g", "m", "v", "m_exps", "v_exps", "step")] + [("n", ctypes.c_int64)]
 
 
 IPC_HANDLE_BYTES = 80  # FLB_IPC_HANDLE_BYTES

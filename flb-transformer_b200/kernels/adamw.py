@@ -1,0 +1,169 @@
+"""AdamW on B200 (sm_100a): one kernel for all of a model's tensors, moments in 32 or in 8 bits.
+
+    opt = AdamW(params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, seed=0)
+
+    m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
+    p = p (1 - lr weight_decay) - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps)
+
+in float32, p (float32, float16 or bfloat16) rounded once. A torch.optim.Optimizer: groups, schedulers and state dicts
+as there, and the names of its state ("step", "exp_avg", "exp_avg_sq").
+
+state_bits=8 holds the moments in 8-bit floating point, blocks of 128 elements each with a byte for the exponent of its
+largest magnitude ("exp_avg_exps", "exp_avg_sq_exps"): m with a sign, 3 bits of mantissa and the 16 binades
+around and under the block's largest, v with 3 bits of mantissa and 32 binades. 2 bytes an element instead of 8. They are
+rounded up or down at random (a mix of the element's index, the step and `seed`: the same every time), so that a
+moment that changes by less than its unit a step still follows its mean. Below the smallest code m becomes zero, and v the
+smallest code. A block with an infinity or NaN becomes NaN as a whole.
+
+Steps are counted on the device, each tensor's own (its "step", an int64), so that a captured step counts on in every replay;
+lr may be a float32 tensor on the device, which a schedule then writes between replays. The first step of a tensor makes its
+state, and is not for a capture. Steps of one optimizer must not overlap on the GPU. The kernels are in libflb_b200.so
+(flb_adamw, flb_adamw_moments), called through flb_ops; CUDA tensors only.
+"""
+from __future__ import annotations
+
+import torch
+
+import flb_native  # noqa: F401  (loads libflb_b200.so, or says that it is missing)
+import flb_ops
+
+__all__ = ["AdamW"]
+
+
+class AdamW(torch.optim.Optimizer):
+    """See the module's text."""
+
+    def __init__(self, params, lr: float | torch.Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, state_bits: int = 32, seed: int = 0):
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, seed=seed))
+
+    def add_param_group(self, param_group: dict) -> None:
+        super().add_param_group(param_group)
+        try:
+            self._check(self.param_groups[-1])
+        except Exception:
+            self.param_groups.pop()
+            raise
+
+    @staticmethod
+    def _check(group):
+        lr, (b1, b2) = group["lr"], group["betas"]
+        if isinstance(lr, torch.Tensor):
+            if lr.numel() != 1 or (lr.is_cuda and lr.dtype != torch.float32):
+                raise ValueError("lr must be a number, or a tensor of one float32")
+        elif not lr >= 0:
+            raise ValueError(f"lr must be at least 0, not {lr}")
+        if not (0 <= b1 < 1 and 0 <= b2 < 1):
+            raise ValueError(f"betas must be at least 0 and below 1, not {group['betas']}")
+        if not (group["eps"] >= 0 and group["weight_decay"] >= 0):
+            raise ValueError("eps and weight_decay must be at least 0")
+        if group["state_bits"] not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, not {group['state_bits']}")
+        if len(set(map(id, group["params"]))) != len(group["params"]):
+            raise ValueError("a parameter is in the group twice")
+        for p in group["params"]:
+            if p.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+                raise TypeError(f"parameters must be float32, float16 or bfloat16, not {p.dtype}")
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for group in self.param_groups:
+            group.setdefault("state_bits", 32)
+            group.setdefault("seed", 0)
+
+    def _counter(self, device):
+        # a word of the kernel's own on each device, zero between steps
+        counters = self.__dict__.setdefault("_counters", {})
+        if device not in counters:
+            counters[device] = torch.zeros(1, dtype=torch.int32, device=device)
+        return counters[device]
+
+    def _new_state(self, p, bits):
+        state = {"step": torch.zeros((), dtype=torch.int64, device=p.device)}
+        blocks = -(-p.numel() // 128)
+        for name in ("exp_avg", "exp_avg_sq"):
+            if bits == 8:
+                state[name] = torch.zeros(blocks, 128, dtype=torch.uint8, device=p.device)
+                state[name + "_exps"] = torch.zeros(blocks, dtype=torch.uint8, device=p.device)
+            else:
+                state[name] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+        return state
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        """One step of every parameter that has a gradient."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            bits = group["state_bits"]
+            together = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                state = self.state[p]
+                if len(state) == 0:
+                    if not p.is_cuda:
+                        raise RuntimeError(f"AdamW runs on CUDA tensors only (sm_100a kernels; no CPU path); got a parameter on {p.device}")
+                    if torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("AdamW: the first step of a parameter makes its state: take one before the capture")
+                    state.update(self._new_state(p, bits))
+                    self._counter(p.device)
+                t = together.setdefault((p.device, p.dtype), ([], [], [], [], [], [], []))
+                for of, x in zip(t, (p, p.grad, state["exp_avg"], state["exp_avg_sq"], state["step"], state.get("exp_avg_exps"),
+                                     state.get("exp_avg_sq_exps"))):
+                    of.append(x)
+            lr = group["lr"]
+            on_device = isinstance(lr, torch.Tensor) and lr.is_cuda
+            for (device, _), t in together.items():
+                exps = t[5:] if bits == 8 else ([], [])
+                flb_ops.adamw(*t[:5], *exps, bits, 0.0 if on_device else float(lr), lr.detach() if on_device else None, *group["betas"],
+                              group["eps"], group["weight_decay"], group["seed"] & 0xffffffff, self._counter(device))
+        return loss
+
+    @torch.no_grad()
+    def moments(self, out=None) -> list:
+        """(m, v) of every parameter that has taken a step, in the groups' order, as float32 tensors of its shape. Of 32 bits they are the
+        state's own; of 8 bits new ones, or those of `out`, a list of such pairs of contiguous tensors, written."""
+        params = [(p, group["state_bits"]) for group in self.param_groups for p in group["params"] if len(self.state[p])]
+        if out is not None and len(out) != len(params):
+            raise ValueError(f"{len(out)} pairs for {len(params)} parameters")
+        found, together = [], {}
+        for i, (p, bits) in enumerate(params):
+            s = self.state[p]
+            if bits == 32:
+                pair = (s["exp_avg"], s["exp_avg_sq"])
+                if out is not None:
+                    for to, x in zip(out[i], pair):
+                        to.copy_(x)
+                    pair = out[i]
+            else:
+                pair = out[i] if out is not None else tuple(torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+                                                            for _ in range(2))
+                t = together.setdefault(p.device, ([], [], [], [], [], [], []))
+                for of, x in zip(t, (p, *pair, s["exp_avg"], s["exp_avg_sq"], s["exp_avg_exps"], s["exp_avg_sq_exps"])):
+                    of.append(x)
+            found.append(pair)
+        for t in together.values():
+            flb_ops.adamw_moments(*t)
+        return found
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict: dict) -> None:
+        """As torch's, but the state keeps its types. Moments in 32 bits may come from torch.optim.AdamW."""
+        for saved in state_dict["param_groups"]:
+            for key in saved["params"]:
+                s = state_dict["state"].get(key)
+                if s and ("exp_avg_exps" in s) != (saved.get("state_bits", 32) == 8):
+                    raise ValueError("the state's moments are not of the bits that its group says")
+        super().load_state_dict(state_dict)
+        for group, saved in zip(self.param_groups, state_dict["param_groups"]):
+            self._check(group)
+            for p, key in zip(group["params"], saved["params"]):
+                if key not in state_dict["state"] or not state_dict["state"][key]:
+                    continue
+                s, mine = state_dict["state"][key], self._new_state(p, group["state_bits"])
+                for name, t in mine.items():
+                    t.copy_(torch.as_tensor(s[name]))
+                self.state[p] = mine

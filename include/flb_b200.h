@@ -4,7 +4,8 @@
  *       row softmax, out = P @ V, forward and backward;
  *   (2) the anti-diagonal wavefront engine (dependency gather, port scatter, gradient routing)
  *       and the persistent tanh grid-cell kernels;
- * and of operators beside them: LayerNorm, activations kept in 8 bits, 8-bit integer products.
+ * and of operators beside them: LayerNorm, activations kept in 8 bits, 8-bit integer and floating-point
+ * products, the choice of a token from logits, AdamW.
  *
  * Conventions shared by every entry point:
  *   - all pointers are DEVICE pointers unless stated otherwise; the library never allocates,
@@ -488,6 +489,53 @@ int flb_int8_linear_wait_test(const void* x, int64_t ldx, const int8_t* x_codes,
                               void* out, int64_t M, int64_t N, int64_t K, int dtype, void* workspace,
                               size_t workspace_bytes, int check_timeout, int64_t drop_step, uint32_t spin_limit,
                               void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * A token for each row of logits (no reference counterpart: the reference's callers take the argmax).
+ * logits [rows, V] in dtype, ld elements from row to row; u [rows]: uniform numbers in [0, 1), float32 or (u_is_f64)
+ * float64; token: int64 [rows]. temperature, top_k, top_p, min_p: NULL, or [rows]; where NULL, the number after them
+ * holds for all rows. With w_i = exp((l_i - max l) / temperature): kept are the top_k tokens of the largest logits (of
+ * equal ones those of lower index; all, where top_k is not between 1 and V), of these the shortest run from the largest on
+ * whose w sum to at least top_p of theirs (always the first; all, where top_p >= 1), of these those with
+ * w_i >= min_p. The token is the first, in the vocabulary's order, at which the sum of kept w passes u of the whole. A
+ * temperature not above 0: the largest logit, of equal ones the lowest index. A row without a logit above -inf, or
+ * with a NaN: -1. Logits of +inf share all of the probability. V <= 262144.
+ * Sums are of integers: the same token every time.
+ * ------------------------------------------------------------------------------------------ */
+int flb_sample(const void* logits, int64_t ld, const void* u, int u_is_f64, int64_t* token, int64_t rows, int64_t V, int dtype,
+               const float* temperature, double temperature_all, const int64_t* top_k, int64_t top_k_all, const float* top_p,
+               double top_p_all, const float* min_p, double min_p_all, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * AdamW over many tensors at once (no reference counterpart: its trainer uses torch's).
+ * m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+ * p = p (1 - lr weight_decay) - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps),  t = *step + 1.
+ * ------------------------------------------------------------------------------------------ */
+typedef struct flb_adamw_tensor {
+  void* p;          /* [n] in dtype, updated (flb_adamw_moments: where m goes, float32)                        */
+  const void* g;    /* [n] in dtype (flb_adamw_moments: where v goes, float32, written)                        */
+  void* m;          /* float32 [n]; or codes, uint8 [ceil(n / 128) * 128], 4-byte aligned                       */
+  void* v;          /* the same                                                                               */
+  uint8_t* m_exps;  /* NULL, or with codes uint8 [ceil(n / 128)]                                              */
+  uint8_t* v_exps;
+  int64_t* step;    /* steps taken, counted up by one                                                          */
+  int64_t n;
+} flb_adamw_tensor;
+
+/* `tensors` is a HOST array, read before the call returns; no two entries share memory. state_bits: 32, or 8: moments as
+ * codes in blocks of 128 elements, the block's byte E the biased float32 exponent of its largest magnitude (at least 15 for m
+ * and 31 for v; 255: the block holds an infinity or NaN and comes back as NaN). A code c stands for 0 where its low 7 bits
+ * (m) or all 8 (v) are 0, else for the float32 with the bits (c' + (E - 14) 8) << 20, c' those 7 bits, bit 7 its sign, or
+ * for v (c + (E - 30) 8) << 20. The new moments, in float32, are rounded by random bits: x = i 0x9E3779B9 + t 0x6A09E667 +
+ * seed, x = (x ^ x >> 16) 0xBB67AE85, x ^= x >> 16 in 32 bits, i the element's index; the upper 16 bits of x for m and the lower
+ * for v are added at bits 4 to 19 of the float32, and the lowest 20 are cut. Below the smallest code m becomes 0 and v the
+ * smallest. Codes behind the n-th element must be 0, and stay so. lr_device: NULL, or a float32 on the device in lr's place.
+ * counter: a uint32 on the device, zero before the first call, which leaves it zero; calls that may overlap need one each. Launches
+ * one kernel for up to 440 tensors. */
+int flb_adamw(const flb_adamw_tensor* tensors, int64_t count, int dtype, int state_bits, double lr, const float* lr_device,
+              double beta1, double beta2, double eps, double weight_decay, uint32_t seed, uint32_t* counter, void* stream);
+/* The values of 8-bit moments: float32 [n] each, to p and g. step is not used. */
+int flb_adamw_moments(const flb_adamw_tensor* tensors, int64_t count, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Measurement helpers (used by bench.py for the roofline denominators).
