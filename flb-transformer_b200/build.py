@@ -41,6 +41,8 @@ CU_SOURCES = [
     "kept8.cu",
     "int8_linear.cu",
     "c_abi_head.cu",
+    "fp8_rows.cu",
+    "fp8_linear.cu",
     "sample.cu",
     "adamw.cu",
     "microbench.cu",

@@ -436,6 +436,192 @@ Tensor int8_linear(const Opt& x_, const Opt& x_codes, const Opt& x_scale, const 
   return out;
 }
 
+// ---- 8-bit floating-point rows and their product ----------------------------------------------------------------
+
+// Codes of a matrix of `rows` rows of K, each row from 16 bytes on, and their powers of two
+struct Fp8 {
+  Tensor codes, exps;  // [rows, pitch], [groups of 128 rows, quads of blocks, 32, 4, 4]
+};
+Fp8 fp8_buffers(int64_t rows, int64_t K, const Tensor& like) {
+  return {at::empty({rows, flb_code_pitch(K)}, like.options().dtype(at::kFloat8_e4m3fn)),
+          at::empty({(rows + 127) / 128, (K + 511) / 512, 32, 4, 4}, like.options().dtype(at::kByte))};
+}
+
+// x's rows
+Fp8 fp8_rows(const Tensor& x_) {
+  const int dt = dtype_of(x_, "x");
+  auto [x, ldx] = rows_of(x_);
+  const int64_t K = x.size(-1), R = rows_in(x);
+  Fp8 q = fp8_buffers(R, K, x);
+  check(flb_fp8_rows(x.data_ptr(), ldx, q.codes.data_ptr(), (uint8_t*)q.exps.data_ptr(), R, K, dt, stream_of(x)), "flb_fp8_rows");
+  return q;
+}
+// x's rows and columns, and with bias_grad the columns' sums
+std::pair<Fp8, Fp8> fp8_rows2(const Tensor& x_, const Opt& bias_grad) {
+  const int dt = dtype_of(x_, "x");
+  auto [x, ldx] = rows_of(x_);
+  const int64_t C = x.size(-1), R = rows_in(x);
+  Fp8 q = fp8_buffers(R, C, x), t = fp8_buffers(C, R, x);
+  const size_t need = given(bias_grad) ? flb_fp8_rows2_workspace_bytes(R, C) : 0;
+  Tensor ws = need ? buffer(need, x) : Tensor();
+  check(flb_fp8_rows2(x.data_ptr(), ldx, q.codes.data_ptr(), (uint8_t*)q.exps.data_ptr(), t.codes.data_ptr(), (uint8_t*)t.exps.data_ptr(), ptr(bias_grad),
+                      given(bias_grad) ? dtype_of(*bias_grad, "bias") : dt, R, C, dt, need ? ws.data_ptr() : nullptr, need, stream_of(x)),
+        "flb_fp8_rows2");
+  return {q, t};
+}
+
+// The product of x [M, K], or its codes, and a weight's [N, K] codes into out
+void fp8_product(const Opt& x_, int64_t ldx, const Fp8& xq, int64_t ldc, const Fp8& w, int64_t ldw, const Opt& bias, const Tensor& out, int64_t M, int64_t N,
+                 int64_t K, bool check_timeout) {
+  if (M == 0 || N == 0) return;
+  const bool from_x = given(x_);
+  const size_t need = flb_fp8_linear_workspace_bytes(M, N, K, from_x ? 0 : 1);
+  Tensor ws = buffer(need, out);
+  check(flb_fp8_linear(ptr(x_), ldx, from_x ? nullptr : xq.codes.data_ptr(), ldc, from_x ? nullptr : (const uint8_t*)xq.exps.data_ptr(), w.codes.data_ptr(),
+                       ldw, (const uint8_t*)w.exps.data_ptr(), ptr(bias), given(bias) ? dtype_of(*bias, "bias") : FLB_F32, out.data_ptr(), M, N, K,
+                       dtype_of(out, "out"), ws.data_ptr(), need, check_timeout ? 1 : 0, stream_of(out)),
+        "flb_fp8_linear");
+}
+
+std::pair<Tensor, Tensor> quantize_fp8(const Tensor& x) {
+  no_gradient(x, "quantize_fp8");
+  dtype_of(x, "x");
+  need_cuda(x);
+  TORCH_CHECK_VALUE(last_axis(x, "x") >= 1, "x must have a last axis of at least one element");
+  const c10::cuda::CUDAGuard guard(x.device());
+  Fp8 q = fp8_rows(x);
+  std::vector<int64_t> shape = x.sizes().vec();
+  shape.back() = q.codes.size(1);
+  return {q.codes.view(shape).narrow(-1, 0, x.size(-1)), q.exps};
+}
+
+// Codes as the product takes them: rows a multiple of 16 bytes apart, the first on 16 bytes; copied so if need be.
+std::tuple<Fp8, int64_t> fp8_operand(const Tensor& codes, const Tensor& exps, const char* name) {
+  TORCH_CHECK_TYPE(codes.scalar_type() == at::kFloat8_e4m3fn && exps.scalar_type() == at::kByte, name,
+                   " must be float8_e4m3fn codes and uint8 powers of two, not ", codes.scalar_type(), " and ", exps.scalar_type());
+  TORCH_CHECK_VALUE(codes.dim() >= 1 && codes.size(-1) >= 1, name, ": codes must have a last axis of at least one element");
+  const int64_t K = codes.size(-1), R = rows_in(codes);
+  TORCH_CHECK_VALUE(exps.numel() == (int64_t)flb_fp8_exps_bytes(R, K) && exps.is_contiguous() && (exps.numel() == 0 || reinterpret_cast<uintptr_t>(exps.data_ptr()) % 16 == 0),
+                    name, ": powers of two of shape ", exps.sizes(), " are not those of codes of shape ", codes.sizes());
+  if (codes.numel() == 0) return {Fp8{codes, exps}, flb_code_pitch(K)};
+  auto [t, pitch] = rows_of(codes);
+  if (R == 1) pitch = flb_code_pitch(K);  // one row has no pitch of its own
+  if (pitch % 16 == 0 && pitch >= K && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0) return {Fp8{t, exps}, pitch};
+  Tensor padded = at::empty({R, flb_code_pitch(K)}, t.options());
+  padded.view(at::kByte).narrow(1, 0, K).copy_(t.reshape({R, K}).view(at::kByte));
+  return {Fp8{padded, exps}, flb_code_pitch(K)};
+}
+
+void check_fp8(const Tensor& in, int64_t N, int64_t K, at::IntArrayRef weight, const Opt& bias) {
+  TORCH_CHECK_VALUE(weight.size() == 2 && weight[1] == K && K >= 1, "a weight of shape ", weight, " for x of shape ", in.sizes());
+  if (!given(bias)) return;
+  same_device(in, bias);
+  dtype_of(*bias, "bias");
+  TORCH_CHECK_VALUE(bias->dim() == 1 && bias->size(0) == N, "a bias of shape ", bias->sizes(), " for ", N, " outputs");
+}
+
+// x, or its codes with the output's type; a weight that is kept as codes
+Tensor fp8_linear_kept(const Opt& x_, const Opt& x_codes, const Opt& x_exps, const Tensor& w_codes, const Tensor& w_exps, const Opt& bias_,
+                       std::optional<at::ScalarType> type, bool check_timeout) {
+  for (const Opt& t : {x_, bias_}) no_gradient(t, "fp8_linear with a weight kept in 8 bits");
+  const Tensor& in = given(x_) ? *x_ : *x_codes;
+  const at::ScalarType dtype = given(x_) ? in.scalar_type() : type.value_or(at::kBFloat16);
+  dtype_of(dtype, "x");
+  need_cuda(in);
+  for (const Opt& t : {Opt(w_codes), Opt(w_exps), x_exps}) same_device(in, t);
+  const int64_t K = last_axis(in, "x"), M = rows_in(in);
+  check_fp8(in, w_codes.dim() == 2 ? w_codes.size(0) : 0, K, w_codes.sizes(), bias_);
+  const int64_t N = w_codes.size(0);
+  const c10::cuda::CUDAGuard guard(in.device());
+  std::vector<int64_t> shape = in.sizes().vec();
+  shape.back() = N;
+  Tensor out = at::empty(shape, in.options().dtype(dtype));
+  auto [w, ldw] = fp8_operand(w_codes, w_exps, "the weight");
+  const Opt bias = contiguous(bias_);
+  if (given(x_)) {
+    auto [x, ldx] = rows_of(*x_);
+    fp8_product(x, ldx, {}, 0, w, ldw, bias, out, M, N, K, check_timeout);
+  } else {
+    auto [xq, ldc] = fp8_operand(*x_codes, *x_exps, "x");
+    fp8_product({}, 0, xq, ldc, w, ldw, bias, out, M, N, K, check_timeout);
+  }
+  return out;
+}
+
+// A training step's products. x [M, K] and the weight [N, K] are kept for the backward pass as the 8-bit columns that it sums over.
+struct Fp8LinearFn : torch::autograd::Function<Fp8LinearFn> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Opt& bias) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const c10::cuda::CUDAGuard guard(x.device());
+    const int64_t K = x.size(-1), M = rows_in(x), N = weight.size(0);
+    const bool for_dx = x.requires_grad(), for_dw = weight.requires_grad();
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = N;
+    Tensor out = at::empty(shape, x.options());
+    Fp8 xq, xt, wq, wt;
+    if (M && N) {
+      if (for_dw) std::tie(xq, xt) = fp8_rows2(x, {});
+      else xq = fp8_rows(x);
+      if (for_dx) std::tie(wq, wt) = fp8_rows2(weight, {});
+      else wq = fp8_rows(weight);
+      fp8_product({}, 0, xq, flb_code_pitch(K), wq, flb_code_pitch(K), contiguous(bias), out, M, N, K, false);
+    }
+    ctx->save_for_backward({xt.codes, xt.exps, wt.codes, wt.exps});
+    ctx->saved_data["sizes"] = std::vector<int64_t>{M, N, K};
+    ctx->saved_data["x"] = x.sizes().vec();
+    ctx->saved_data["types"] = std::vector<int64_t>{(int64_t)weight.scalar_type(), given(bias) ? (int64_t)bias->scalar_type() : -1};
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+    torch::autograd::variable_list out(3);
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      const auto s = ctx->get_saved_variables();
+      const auto sizes = ctx->saved_data["sizes"].toIntVector(), types = ctx->saved_data["types"].toIntVector();
+      const int64_t M = sizes[0], N = sizes[1], K = sizes[2];
+      const bool for_dx = ctx->needs_input_grad(0), for_dw = ctx->needs_input_grad(1), for_db = types[1] >= 0 && ctx->needs_input_grad(2);
+      const Tensor& dy = g[0];
+      const c10::cuda::CUDAGuard guard(dy.device());
+      const bool some = M && N;
+      if (for_dx) out[0] = some ? at::empty(ctx->saved_data["x"].toIntVector(), dy.options()) : at::zeros(ctx->saved_data["x"].toIntVector(), dy.options());
+      const auto w_options = dy.options().dtype((at::ScalarType)types[0]);
+      if (for_dw) out[1] = some ? at::empty({N, K}, w_options) : at::zeros({N, K}, w_options);
+      if (for_db) {
+        const auto options = dy.options().dtype((at::ScalarType)types[1]);
+        out[2] = some ? at::empty({N}, options) : at::zeros({N}, options);
+      }
+      if (some) {
+        Fp8 q, t;
+        if (for_dw || for_db) std::tie(q, t) = fp8_rows2(dy, for_db ? Opt(out[2]) : Opt());
+        else q = fp8_rows(dy);
+        if (for_dx) fp8_product({}, 0, q, flb_code_pitch(N), {s[2], s[3]}, flb_code_pitch(N), {}, out[0], M, K, N, false);
+        if (for_dw) fp8_product({}, 0, t, flb_code_pitch(M), {s[0], s[1]}, flb_code_pitch(M), {}, out[1], N, K, M, false);
+      }
+    }
+    return differentiable_once(std::move(out));
+  }
+};
+
+Tensor fp8_linear(const Tensor& x, const Tensor& weight, const Opt& bias) {
+  for (const Opt& t : {Opt(x), Opt(weight), bias}) no_tangent(t, "fp8_linear");
+  dtype_of(x, "x");
+  dtype_of(weight, "weight");
+  need_cuda(x);
+  same_device(x, weight);
+  check_fp8(x, weight.dim() == 2 ? weight.size(0) : 0, last_axis(x, "x"), weight.sizes(), bias);
+  if (c10::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || wants_grad(bias))) return Fp8LinearFn::apply(x, weight, bias);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t K = x.size(-1), M = rows_in(x), N = weight.size(0);
+  std::vector<int64_t> shape = x.sizes().vec();
+  shape.back() = N;
+  Tensor out = at::empty(shape, x.options());
+  if (M == 0 || N == 0) return out;
+  auto [rows, ldx] = rows_of(x);
+  const Fp8 wq = fp8_rows(weight);
+  fp8_product(rows, ldx, {}, 0, wq, flb_code_pitch(K), contiguous(bias), out, M, N, K, false);
+  return out;
+}
+
 // ---- a token from logits ------------------------------------------------------------------------------------
 
 // A setting for each row, or none.
@@ -585,6 +771,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("sigmoid_gate", &sigmoid_gate, off);
   m.def("quantize_int8", &quantize_int8, off);
   m.def("layer_norm_int8", &layer_norm_int8, off);
+  m.def("quantize_fp8", &quantize_fp8, off);
+  m.def("fp8_linear", &fp8_linear, off);
+  m.def("fp8_linear_kept", [](const Opt& x, const Opt& xc, const Opt& xe, const Tensor& wc, const Tensor& we, const Opt& bias, py::object dtype,
+                              bool check_timeout) {
+    std::optional<at::ScalarType> t;
+    if (!dtype.is_none()) t = torch::python::detail::py_object_to_dtype(dtype);
+    py::gil_scoped_release release;
+    return fp8_linear_kept(x, xc, xe, wc, we, bias, t, check_timeout);
+  });
   m.def("sample", &sample, off);
   m.def("adamw", &adamw, off);
   m.def("adamw_moments", &adamw_moments, off);

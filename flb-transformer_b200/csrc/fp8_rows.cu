@@ -1,0 +1,256 @@
+// Rows into 8-bit floating point (fp8.cuh), along their own axis, and a matrix along both.
+//
+// rows_kernel: each row's blocks alone, for inference. A block is 16 lanes' eight 16-bit values, or a warp's four float32.
+// tile_kernel: a training step reads x, the weight and the output's gradient each along two axes, since its three products sum
+// over three of them. A block of threads takes 128 x 128 elements, which hold a power of two's block of every row and of
+// every column, from one read of them, and leaves the second kind transposed: rows of the product that sums the other way.
+// For the gradient it adds up the columns too, in float32 and a fixed order: what the bias gets.
+// Bound by memory: 2 bytes read and 2 written an element of 16 bits.
+#include "fp8.cuh"
+
+namespace flb {
+
+namespace {
+
+using namespace fp8;
+
+// PER lanes of a warp share a row's block of 128: 16 (eight values each) or 32 (four)
+template <typename T> constexpr int kPer = sizeof(T) == 2 ? 16 : 32;
+
+template <int N> __device__ __forceinline__ uint32_t max_of(uint32_t v) {
+#pragma unroll
+  for (int o = N / 2; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// Consecutive values from column c on of a row of K, zeros beyond. VEC: rows that start on 16 bytes (8 of them at least are allowed to be read
+// where c < K only if K is a multiple of their number).
+template <typename T, bool VEC, int N> __device__ __forceinline__ void load_row(float (&v)[N], const T* row, int64_t c, int64_t K) {
+  static_assert(N * sizeof(T) == 16);
+  if constexpr (VEC) {
+    const uint4 w = c < K ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (sizeof(T) == 4) {
+        v[j] = __uint_as_float(u[j]);
+      } else {
+        const float2 f = rows::unpack2<T>(u[j]);
+        v[2 * j] = f.x, v[2 * j + 1] = f.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = c + j < K ? ld(row + c + j) : 0.f;
+  }
+}
+
+// Codes of these values to their row, whose pitch is a multiple of 16: what lies behind K (up to the pitch) may be written.
+template <int N> __device__ __forceinline__ void store_codes(int8_t* row, const float (&v)[N], float inv, int64_t c, int64_t pitch) {
+  uint32_t w[N / 4];
+#pragma unroll
+  for (int j = 0; j < N / 4; ++j) w[j] = code4(v[4 * j] * inv, v[4 * j + 1] * inv, v[4 * j + 2] * inv, v[4 * j + 3] * inv);
+  if (c >= pitch) return;
+  if constexpr (N == 8) *reinterpret_cast<uint2*>(row + c) = make_uint2(w[0], w[1]);
+  else *reinterpret_cast<uint32_t*>(row + c) = w[0];
+}
+
+template <int N> __device__ __forceinline__ uint32_t largest(const float (&v)[N]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < N; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+  return m;
+}
+
+struct RowsArgs {
+  const void* x;
+  int64_t ldx, R, K, pitch, quads;
+  int8_t* codes;
+  uint8_t* exps;
+  uint32_t* zero;  // words to clear, or null
+  int n_zero;
+};
+
+template <typename T, bool VEC> __global__ void __launch_bounds__(256) rows_kernel(const RowsArgs a) {
+  let_successor_start();
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < a.n_zero; i += 256) a.zero[i] = 0;
+  constexpr int PER = kPer<T>, N = 16 / sizeof(T);
+  const int64_t blocks = blocks_of(a.K), unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / PER;
+  const int lane = threadIdx.x % PER;
+  const int64_t row = unit / blocks, block = unit % blocks;
+  const bool there = row < a.R;
+  float v[N];
+  if (there) {
+    load_row<T, VEC>(v, reinterpret_cast<const T*>(a.x) + row * a.ldx, block * kBlock + lane * N, a.K);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = 0;
+  }
+  const int u = unit_of(max_of<PER>(largest(v)));
+  if (!there) return;
+  store_codes(a.codes + row * a.pitch, v, inverse_of(u), block * kBlock + lane * N, a.pitch);
+  if (lane == 0) a.exps[exp_at(row, block, a.quads)] = (uint8_t)u;
+}
+
+struct TileArgs {
+  const void* x;
+  int64_t ldx, R, C;
+  int64_t pitch, quads;      // of the rows' form
+  int64_t pitch_t, quads_t;  // of the columns'
+  int8_t *codes, *codes_t;
+  uint8_t *exps, *exps_t;
+  float* sums;               // null, or [tiles of rows][C]: each column's sum over a tile's rows
+};
+
+// 256 threads. As 16 or 8 rows at a time (a row's block in PER lanes), then as columns: four runs of 32 rows of 64 pairs of columns.
+template <typename T, bool VEC, bool SUM> __global__ void __launch_bounds__(256) tile_kernel(const TileArgs a) {
+  constexpr int PER = kPer<T>, N = 16 / sizeof(T), ROWS = 256 / PER, kPitch = kBlock + 16 / (int)sizeof(T);
+  extern __shared__ __align__(16) uint8_t dyn[];
+  T(*tile)[kPitch] = reinterpret_cast<T(*)[kPitch]>(dyn);
+  __shared__ uint32_t tops[4][kBlock];
+  __shared__ float parts[SUM ? 4 : 1][kBlock];
+  const unsigned across = (unsigned)blocks_of(a.C), tile_r = blockIdx.x / across, tile_c = blockIdx.x % across;
+  const int64_t r0 = (int64_t)tile_r * kBlock, c0 = (int64_t)tile_c * kBlock;
+  const int lane = threadIdx.x % PER;
+#pragma unroll 4
+  for (int i = 0; i < kBlock; i += ROWS) {
+    const int r = i + threadIdx.x / PER;
+    const int64_t row = r0 + r;
+    float v[N];
+    if (row < a.R) {
+      load_row<T, VEC>(v, reinterpret_cast<const T*>(a.x) + row * a.ldx, c0 + lane * N, a.C);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = 0;
+    }
+    uint4 w;
+    if constexpr (sizeof(T) == 4) w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    else w = make_uint4(rows::pack2<T>(v[0], v[1]), rows::pack2<T>(v[2], v[3]), rows::pack2<T>(v[4], v[5]), rows::pack2<T>(v[6], v[7]));
+    *reinterpret_cast<uint4*>(&tile[r][lane * N]) = w;
+    const int u = unit_of(max_of<PER>(largest(v)));
+    if (row < a.R) {
+      store_codes(a.codes + row * a.pitch, v, inverse_of(u), c0 + lane * N, a.pitch);
+      if (lane == 0) a.exps[exp_at(row, tile_c, a.quads)] = (uint8_t)u;
+    }
+  }
+  __syncthreads();
+  // columns 2p and 2p + 1, rows 32g to 32g + 31
+  const int p = threadIdx.x % 64, g = threadIdx.x / 64;
+  uint32_t m0 = 0, m1 = 0;
+  float s0 = 0, s1 = 0;
+#pragma unroll 8
+  for (int i = 0; i < 32; ++i) {
+    const float a0 = ld(&tile[32 * g + i][2 * p]), a1 = ld(&tile[32 * g + i][2 * p + 1]);
+    m0 = max(m0, __float_as_uint(a0) & 0x7fffffffu);
+    m1 = max(m1, __float_as_uint(a1) & 0x7fffffffu);
+    if (SUM) s0 += a0, s1 += a1;
+  }
+  tops[g][2 * p] = m0, tops[g][2 * p + 1] = m1;
+  if (SUM) parts[g][2 * p] = s0, parts[g][2 * p + 1] = s1;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int c = 2 * p + j;
+    const int64_t col = c0 + c;
+    const int u = unit_of(max(max(tops[0][c], tops[1][c]), max(tops[2][c], tops[3][c])));
+    if (col >= a.C) continue;
+    const float inv = inverse_of(u);
+    int8_t* to = a.codes_t + col * a.pitch_t + r0 + 32 * g;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int r = 32 * g + 16 * h + 4 * k;
+        w[k] = code4(ld(&tile[r][c]) * inv, ld(&tile[r + 1][c]) * inv, ld(&tile[r + 2][c]) * inv, ld(&tile[r + 3][c]) * inv);
+      }
+      if (r0 + 32 * g + 16 * h < a.pitch_t) *reinterpret_cast<uint4*>(to + 16 * h) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    if (g == 0) {
+      a.exps_t[exp_at(col, tile_r, a.quads_t)] = (uint8_t)u;
+      if (SUM) a.sums[(int64_t)tile_r * a.C + col] = (parts[0][c] + parts[1][c]) + (parts[2][c] + parts[3][c]);
+    }
+  }
+}
+
+// The tiles' sums, in order, into the bias's gradient.
+template <typename T> __global__ void __launch_bounds__(256) sums_kernel(const float* __restrict__ sums, T* __restrict__ out, int64_t tiles, int64_t C) {
+  // 32 columns a block, eight runs of tiles
+  __shared__ float part[8][32];
+  const int lane = threadIdx.x & 31, run = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane, per = (tiles + 7) / 8;
+  float s = 0;
+  if (c < C)
+    for (int64_t t = run * per; t < min(tiles, (run + 1) * per); ++t) s += sums[t * C + c];
+  part[run][lane] = s;
+  __syncthreads();
+  if (run == 0 && c < C) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) s += part[i][lane];
+    st(out + c, s);
+  }
+}
+
+bool on16(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && bytes % 16 == 0; }
+
+template <typename T> int rows_t(const RowsArgs& a, cudaStream_t s) {
+  const bool vec = on16(a.x, a.ldx * sizeof(T)) && a.K * sizeof(T) % 16 == 0;
+  const int64_t grid = (a.R * blocks_of(a.K) * kPer<T> + 255) / 256;
+  if (grid > INT32_MAX) return fail(FLB_ERR_SHAPE, "fp8_rows: too many rows");
+  if (vec) rows_kernel<T, true><<<(unsigned)grid, 256, 0, s>>>(a);
+  else rows_kernel<T, false><<<(unsigned)grid, 256, 0, s>>>(a);
+  count_launches(1);
+  return check_cuda(cudaGetLastError(), "fp8_rows launch");
+}
+
+template <typename T, bool VEC, bool SUM> int launch_tiles(const TileArgs& a, unsigned grid, cudaStream_t s) {
+  constexpr int smem = kBlock * (kBlock * (int)sizeof(T) + 16);
+  const int st = ensure_dyn_smem(reinterpret_cast<const void*>(tile_kernel<T, VEC, SUM>), smem, "fp8_rows2 shared memory");
+  if (st != FLB_OK) return st;
+  tile_kernel<T, VEC, SUM><<<grid, 256, smem, s>>>(a);
+  count_launches(1);
+  return check_cuda(cudaGetLastError(), "fp8_rows2 launch");
+}
+
+template <typename T> int tiles_t(const TileArgs& a, void* bias_grad, int bias_dtype, cudaStream_t s) {
+  const bool vec = on16(a.x, a.ldx * sizeof(T)) && a.C * sizeof(T) % 16 == 0;
+  const int64_t tiles = blocks_of(a.R) * blocks_of(a.C);
+  if (tiles > INT32_MAX) return fail(FLB_ERR_SHAPE, "fp8_rows2: too many elements");
+  int st;
+  if (a.sums) st = vec ? launch_tiles<T, true, true>(a, (unsigned)tiles, s) : launch_tiles<T, false, true>(a, (unsigned)tiles, s);
+  else st = vec ? launch_tiles<T, true, false>(a, (unsigned)tiles, s) : launch_tiles<T, false, false>(a, (unsigned)tiles, s);
+  if (st != FLB_OK || !a.sums) return st;
+  const unsigned g = (unsigned)((a.C + 31) / 32);
+  switch (bias_dtype) {
+    case FLB_F32: sums_kernel<<<g, 256, 0, s>>>(a.sums, reinterpret_cast<float*>(bias_grad), blocks_of(a.R), a.C); break;
+    case FLB_F16: sums_kernel<<<g, 256, 0, s>>>(a.sums, reinterpret_cast<__half*>(bias_grad), blocks_of(a.R), a.C); break;
+    default: sums_kernel<<<g, 256, 0, s>>>(a.sums, reinterpret_cast<__nv_bfloat16*>(bias_grad), blocks_of(a.R), a.C); break;
+  }
+  count_launches(1);
+  return check_cuda(cudaGetLastError(), "fp8_rows2 sums launch");
+}
+
+}  // namespace
+
+int fp8_rows(const void* x, int64_t ldx, int8_t* codes, uint8_t* exps, int64_t R, int64_t K, int dtype, uint32_t* zero, int n_zero,
+             cudaStream_t s) {
+  const RowsArgs a{x, ldx, R, K, rows::code_pitch(K), quads_of(K), codes, exps, zero, n_zero};
+  switch (dtype) {
+    case FLB_F32: return rows_t<float>(a, s);
+    case FLB_F16: return rows_t<__half>(a, s);
+    default: return rows_t<__nv_bfloat16>(a, s);
+  }
+}
+
+int fp8_rows2(const void* x, int64_t ldx, int8_t* codes, uint8_t* exps, int8_t* codes_t, uint8_t* exps_t, float* sums, void* bias_grad,
+              int bias_dtype, int64_t R, int64_t C, int dtype, cudaStream_t s) {
+  const TileArgs a{x, ldx, R, C, rows::code_pitch(C), quads_of(C), rows::code_pitch(R), quads_of(R), codes, codes_t, exps, exps_t, sums};
+  switch (dtype) {
+    case FLB_F32: return tiles_t<float>(a, bias_grad, bias_dtype, s);
+    case FLB_F16: return tiles_t<__half>(a, bias_grad, bias_dtype, s);
+    default: return tiles_t<__nv_bfloat16>(a, bias_grad, bias_dtype, s);
+  }
+}
+
+}  // namespace flb

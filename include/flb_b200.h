@@ -491,6 +491,31 @@ int flb_int8_linear_wait_test(const void* x, int64_t ldx, const int8_t* x_codes,
                               void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * 8-bit floating-point rows and their product (no reference counterpart).
+ * Rows [R, K] as codes, e4m3 (a sign, 4 bits of exponent, 3 of mantissa) [R, flb_code_pitch(K)], 16-byte aligned (bytes
+ * from K to the pitch are written with whatever), and exps, flb_fp8_exps_bytes(R, K) bytes, 16-byte aligned: for each
+ * block of 128 elements of a row the smallest power of two 2^(byte - 127), byte >= 0, in units of which the block's
+ * largest magnitude is at most 448; 255 where the block held an infinity or NaN: it counts as NaN. The byte of row r, block b
+ * lies at ((r / 128) ceil(blocks / 4) + b / 4) 512 + (r % 32) 16 + (r / 32 % 4) 4 + b % 4, as the tensor core reads them.
+ * ------------------------------------------------------------------------------------------ */
+size_t flb_fp8_exps_bytes(int64_t R, int64_t K);
+int flb_fp8_rows(const void* x, int64_t ldx, void* codes, uint8_t* exps, int64_t R, int64_t K, int dtype, void* stream);
+/* A matrix x [R, C] (pitch ldx elements) along both axes from one read: codes and exps of its rows, and codes_t, exps_t those of its
+ * columns, [C, R]. bias_grad: NULL, or [C] in bias_dtype: the sum of each column, in float32 and a fixed order; sums is then a
+ * workspace of flb_fp8_rows2_workspace_bytes(), 16-byte aligned. */
+size_t flb_fp8_rows2_workspace_bytes(int64_t R, int64_t C);
+int flb_fp8_rows2(const void* x, int64_t ldx, void* codes, uint8_t* exps, void* codes_t, uint8_t* exps_t, void* bias_grad,
+                  int bias_dtype, int64_t R, int64_t C, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+/* out[m, n] = sum_k X[m, k] W[n, k] + bias[n], contiguous [M, N] in dtype, in float32 (the tensor core's over 1024 of K, their sum
+ * rounded). X: codes (pitch ldc) and exps, or x [M, K] in dtype (pitch ldx elements), made into 8-bit rows on the
+ * way. W: codes [N, K] (pitch ldw) and exps. Pitches are multiples of 16, codes and exps 16-byte aligned. bias: [N] in
+ * bias_dtype, or NULL. Workspace, check_timeout: as flb_int8_linear. The same bits every time. */
+size_t flb_fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int x_is_codes);
+int flb_fp8_linear(const void* x, int64_t ldx, const void* x_codes, int64_t ldc, const uint8_t* x_exps, const void* w_codes,
+                   int64_t ldw, const uint8_t* w_exps, const void* bias, int bias_dtype, void* out, int64_t M, int64_t N,
+                   int64_t K, int dtype, void* workspace, size_t workspace_bytes, int check_timeout, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * A token for each row of logits (no reference counterpart: the reference's callers take the argmax).
  * logits [rows, V] in dtype, ld elements from row to row; u [rows]: uniform numbers in [0, 1), float32 or (u_is_f64)
  * float64; token: int64 [rows]. temperature, top_k, top_p, min_p: NULL, or [rows]; where NULL, the number after them

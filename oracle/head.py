@@ -102,3 +102,41 @@ def moments32(g, m, v, betas):
     g, m, v = (x.float() for x in (g, m, v))
     f = [torch.tensor(x, dtype=torch.float64).float() for x in (betas[0], 1 - betas[0], betas[1], 1 - betas[1])]
     return m * f[0] + g * f[1], v * f[2] + (g * g) * f[3]
+
+
+# ---- 8-bit floating point ---------------------------------------------------------------------------------------
+
+def fp8_values(x):
+    """What rows of [..., K] stand for in e4m3 with a power of two for each block of 128 (float64), and the blocks' powers of two as bytes."""
+    x = x.double()
+    K = x.shape[-1]
+    blocks = torch.nn.functional.pad(x, (0, -K % 128)).unflatten(-1, (-1, 128))
+    top = blocks.abs().amax(-1, keepdim=True)
+    fine = torch.isfinite(top)
+    byte = torch.zeros(top.shape, dtype=torch.int64)
+    for b in range(254, -1, -1):  # the smallest unit in which the largest is at most 448
+        byte = torch.where(fine & (top <= 448 * 2.0 ** (b - 127)), b, byte)
+    q = torch.where(fine, blocks, 0) / torch.exp2((byte - 127).double())
+    # to 4 significant bits, or multiples of 2^-9 below 2^-6
+    e = torch.clamp(torch.frexp(q)[1] - 4, min=-9)
+    step = torch.exp2(e.double())
+    q = torch.round(q / step) * step * torch.exp2((byte - 127).double())
+    q = torch.where(fine, q, math.nan)
+    return q.flatten(-2)[..., :K], torch.where(fine, byte, 255)[..., 0]
+
+
+def fp8_product(x, w, bias, dtype):
+    """x [M, K] times w [N, K] rows, both as their 8-bit values: float64, and how far a result of `dtype` may be.
+
+    Each step of 32 of K that the tensor core adds to an accumulator of 1024 is taken to lose at most 2^-22 of the sum S of the
+    magnitudes so far: 32 such of each accumulator's own S. Accumulators are added in float32, half a step each, and the bias; then the output's
+    own rounding."""
+    qx, qw = fp8_values(x)[0], fp8_values(w)[0]
+    y, size = qx @ qw.t(), qx.abs() @ qw.abs().t()
+    K = x.shape[1]
+    tol = size * (min(K, 1024) / 32 * 2.0 ** -22 + math.ceil(K / 1024) * EPS32)
+    if bias is not None:
+        y = y + bias.double()
+        tol = tol + EPS32 * (y.abs() + bias.double().abs())
+    info = torch.finfo(dtype)
+    return y, tol + info.eps / 2 * (y.abs() + tol) + info.smallest_normal * info.eps / 2

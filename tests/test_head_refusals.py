@@ -64,3 +64,60 @@ def test_adamw_abi():
     assert call(counter=None) == 8 and call(counter=18) == 3
     assert call(count=0) == 0
     assert nat.lib.flb_adamw_moments(None, 0, None) == 0 and nat.lib.flb_adamw_moments(None, 1, None) == 1
+
+
+def test_fp8_refusals():
+    import kernels
+    from torch.autograd import forward_ad
+    x, w = torch.zeros(2, 8), torch.zeros(4, 8)
+    rows = kernels.Fp8Rows(torch.zeros(4, 8).to(torch.float8_e4m3fn), torch.zeros(1, 1, 32, 4, 4, dtype=torch.uint8))
+    for call in (lambda: kernels.fp8_linear(x, w), lambda: kernels.fp8_linear(x, rows), lambda: kernels.quantize_fp8(x), lambda: kernels.fp8_linear(rows, rows)):
+        with pytest.raises(RuntimeError, match="CUDA tensors only"):
+            call()
+        with pytest.raises(RuntimeError, match="torch.func"):
+            torch.func.vmap(lambda t: call())(x)
+    for bad in (lambda: kernels.fp8_linear(x.double(), w), lambda: kernels.fp8_linear(x, w.double())):
+        with pytest.raises(TypeError):
+            bad()
+    with pytest.raises(ValueError):
+        kernels.fp8_linear(rows, w)
+    with pytest.raises(ValueError):
+        kernels.fp8_linear(x, w, check_timeout=True)
+    wants = torch.zeros(2, 8, requires_grad=True)
+    for call in (lambda: kernels.fp8_linear(wants, rows), lambda: kernels.fp8_linear(x, rows, torch.zeros(4, requires_grad=True)),
+                 lambda: kernels.quantize_fp8(wants)):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call()
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(torch.ones(2, 8), torch.ones(2, 8))
+        for call in (lambda: kernels.fp8_linear(dual, w), lambda: kernels.quantize_fp8(dual), lambda: kernels.fp8_linear(dual, rows)):
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                call()
+
+
+def test_fp8_abi():
+    import flb_native as nat
+    L = nat.lib
+    assert L.flb_fp8_exps_bytes(1, 1) == 512 and L.flb_fp8_exps_bytes(129, 513) == 2048 and L.flb_fp8_exps_bytes(0, 5) == 0
+
+    def rows(x=16, ldx=8, codes=16, exps=16, R=1, K=8, dtype=0):
+        return L.flb_fp8_rows(x, ldx, codes, exps, R, K, dtype, None)
+
+    assert rows(dtype=5) == 2 and rows(R=-1) == 1 and rows(K=0) == 1 and rows(K=1 << 31) == 6 and rows(R=1 << 40) == 1
+    assert rows(x=None) == 1 and rows(ldx=-1) == 1 and rows(codes=24) == 3 and rows(exps=8) == 3 and rows(x=18) == 3 and rows(R=0, x=None) == 0
+
+    def rows2(bias=None, ws=None, n=0, codes_t=16, R=3, C=5, bias_dtype=0):
+        return L.flb_fp8_rows2(16, 8, 16, 16, codes_t, 16, bias, bias_dtype, R, C, 0, ws, n, None)
+
+    assert rows2(codes_t=None) == 1 and rows2(codes_t=24) == 3 and rows2(bias=16) == 8 and rows2(bias=16, ws=16, n=19) == 8
+    assert rows2(bias=16, ws=8, n=64) == 3 and rows2(bias=16, bias_dtype=4) == 2 and rows2(R=0) == 0 and rows2(C=0) == 1
+
+    def linear(x=16, ldx=8, xc=None, ldc=0, xe=None, wc=16, ldw=16, we=16, out=16, M=4, N=8, K=8, ws=256, n=1 << 30, dtype=2, bias=None, bias_dtype=0):
+        return L.flb_fp8_linear(x, ldx, xc, ldc, xe, wc, ldw, we, bias, bias_dtype, out, M, N, K, dtype, ws, n, 0, None)
+
+    assert linear(dtype=3) == 2 and linear(bias=16, bias_dtype=9) == 2 and linear(K=0) == 1 and linear(M=-1) == 1 and linear(M=0, x=None) == 0
+    assert linear(x=None) == 1 and linear(xc=16) == 1 and linear(x=None, xc=16, ldc=16) == 1 and linear(wc=None) == 1 and linear(out=None) == 1
+    assert linear(ldw=4) == 1 and linear(ldw=24) == 3 and linear(wc=8) == 3 and linear(we=8) == 3 and linear(out=17) == 3
+    assert linear(x=None, xc=16, ldc=4, xe=16) == 1 and linear(x=None, xc=16, ldc=24, xe=16) == 3
+    assert linear(ws=None) == 8 and linear(n=100) == 8 and linear(ws=128) == 3 and linear(M=1 << 30, N=1 << 30) == 1
+    assert L.flb_fp8_linear_workspace_bytes(1 << 30, 1 << 30, 8, 0) == 0
