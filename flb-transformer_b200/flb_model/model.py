@@ -23,6 +23,9 @@ them keep what their backward reads in 8 bits. The per-tick path is not faster f
 rises, and captured as CUDA graphs the two are within a few percent. Where the engine runs its native
 whole-grid kernels (bf16 autocast), neither is consulted: engine.native_flb_save says there what is kept.
 
+fp8_head=True makes the head a kernels.Fp8Linear: its product and the two products of its gradient in
+8-bit floating point, also in training (the parameters' names and shapes are the same).
+
 The dropout modules exist for state compatibility and run where the reference runs them (the
 attention layer's own dropout is not applied there either).
 """
@@ -31,7 +34,7 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
-from kernels import FusedLayerNorm, fused_additive_attention, sigmoid_gate
+from kernels import Fp8Linear, FusedLayerNorm, fused_additive_attention, sigmoid_gate
 from wavefront.wavefront_api import WavefrontConfig
 from wavefront.wavefront_engine import WavefrontEngine
 
@@ -112,7 +115,7 @@ class FLBTransformer(nn.Module):
     def __init__(self, vocab_size: int, hidden_dim: int = 256, num_layers: int = 6,
                  seq_len: int = 128, batch_size: int = 32, dropout: float = 0.1,
                  aux_weight: float = 0.05, num_heads: int = 8, fused_ops: bool = False,
-                 keep8: bool = False):
+                 keep8: bool = False, fp8_head: bool = False):
         super().__init__()
         self.aux_weight = aux_weight
         self.embedding = nn.Embedding(vocab_size, hidden_dim)
@@ -123,7 +126,7 @@ class FLBTransformer(nn.Module):
         self.layers = nn.ModuleList([FLBBlock(hidden_dim, dropout, num_heads, fused_ops, keep8)
                                      for _ in range(num_layers)])
         self.engine = WavefrontEngine(self.config, self.layers)
-        self.head = nn.Linear(hidden_dim, vocab_size)
+        self.head = (Fp8Linear if fp8_head else nn.Linear)(hidden_dim, vocab_size)
 
     def grids_to_outputs(self, grids, head=None):
         """(logits [batch, seq, vocab], aux_loss, (next_lat, next_fdbk)) from the engine's four
