@@ -670,85 +670,154 @@ void need_codes(const Tensor& codes, const Tensor& exps, const Tensor& p) {
 }
 bool same_layout(const Tensor& a, const Tensor& b) { return a.sizes() == b.sizes() && (a.numel() <= 1 || a.strides() == b.strides()); }
 
-void adamw(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& ms, const std::vector<Tensor>& vs,
-           const std::vector<Tensor>& steps, const std::vector<Tensor>& m_exps, const std::vector<Tensor>& v_exps, int64_t bits, double lr,
-           const Opt& lr_device, double b1, double b2, double eps, double decay, uint32_t seed, const Tensor& counter) {
-  const size_t n = params.size();
-  TORCH_CHECK_VALUE(grads.size() == n && ms.size() == n && vs.size() == n && steps.size() == n &&
-                        m_exps.size() == (bits == 8 ? n : 0) && v_exps.size() == m_exps.size(),
-                    "AdamW: lists of different lengths");
-  if (n == 0) return;
-  const Tensor& first = params[0];
-  const int dt = dtype_of(first, "a parameter");
-  need_cuda(first);
-  same_device(first, counter);
-  same_device(first, lr_device);
-  const c10::cuda::CUDAGuard guard(first.device());
-  std::vector<flb_adamw_tensor> t(n);
+// The optimizer's state goes by Python objects: read here, since a loop over parameters in Python took twice the time of all checks and the launch
+// (135 us a step of 48 parameters, 50 so).
+const Tensor& tensor_of(PyObject* o, const char* name) {
+  TORCH_CHECK_TYPE(o && THPVariable_Check(o), "AdamW: a parameter's state has no tensor \"", name, "\"");
+  return THPVariable_Unpack(o);
+}
+struct Names {
+  PyObject *step, *m, *v, *m_exps, *v_exps;
+};
+const Names& names() {
+  static const Names n{PyUnicode_InternFromString("step"), PyUnicode_InternFromString("exp_avg"), PyUnicode_InternFromString("exp_avg_sq"),
+                       PyUnicode_InternFromString("exp_avg_exps"), PyUnicode_InternFromString("exp_avg_sq_exps")};
+  return n;
+}
+// state[p], borrowed; null where there is none or it is empty
+PyObject* state_of(PyObject* state, PyObject* p) {
+  PyObject* const s = PyDict_GetItemWithError(state, p);
+  if (!s && PyErr_Occurred()) throw pybind11::error_already_set();
+  return s && PyDict_Check(s) && PyDict_Size(s) > 0 ? s : nullptr;
+}
+const Tensor& get(PyObject* s, PyObject* name, const char* text) { return tensor_of(PyDict_GetItemWithError(s, name), text); }
+
+// The tensors of one device and type, one kernel's.
+struct Together {
+  at::Device device;
+  at::ScalarType type;
+  std::vector<flb_adamw_tensor> t;
   std::vector<Tensor> held;  // gradients in their parameters' order, until the launch
-  for (size_t i = 0; i < n; ++i) {
-    const Tensor& p = params[i];
-    same_device(first, p);
+  Tensor like;
+};
+
+// A step of every parameter that has a gradient. Returns those that have no state yet: then nothing has been done.
+pybind11::list adamw(pybind11::list params, pybind11::dict state, int64_t bits, double lr, const Opt& lr_device, double b1, double b2, double eps,
+                     double decay, uint32_t seed, pybind11::dict counters) {
+  pybind11::list missing;
+  std::vector<Together> all;
+  std::vector<Tensor> written;
+  for (pybind11::handle h : params) {
+    const Tensor& p = tensor_of(h.ptr(), "parameter");
+    Tensor g = p.grad();
+    if (!g.defined()) continue;
+    PyObject* const s = state_of(state.ptr(), h.ptr());
+    if (!s) {
+      missing.append(h);
+      continue;
+    }
+    if (pybind11::len(missing)) continue;
+    need_cuda(p);
+    dtype_of(p, "a parameter");
     need_dense(p, "a parameter");
-    TORCH_CHECK_TYPE(p.scalar_type() == first.scalar_type(), "AdamW: parameters of different types in one call");
-    Tensor g = grads[i];
-    same_device(first, g);
+    Together* to = nullptr;
+    for (Together& x : all)
+      if (x.device == p.device() && x.type == p.scalar_type()) to = &x;
+    if (!to) {
+      all.push_back({p.device(), p.scalar_type(), {}, {}, p});
+      to = &all.back();
+    }
+    same_device(p, g);
     TORCH_CHECK_VALUE(g.layout() == at::kStrided, "AdamW: sparse gradients are not supported");
     TORCH_CHECK_TYPE(g.scalar_type() == p.scalar_type(), "AdamW: a gradient of ", g.scalar_type(), " for a parameter of ", p.scalar_type());
     TORCH_CHECK_VALUE(g.sizes() == p.sizes(), "AdamW: a gradient of shape ", g.sizes(), " for a parameter of shape ", p.sizes());
     if (!same_layout(g, p)) {
+      const c10::cuda::CUDAGuard guard(p.device());
       g = at::empty_like(p).copy_(g);
-      held.push_back(g);
+      to->held.push_back(g);
     }
+    const Names& n = names();
+    const Tensor &step = get(s, n.step, "step"), &m = get(s, n.m, "exp_avg"), &v = get(s, n.v, "exp_avg_sq");
+    flb_adamw_tensor t{p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), nullptr, nullptr, nullptr, p.numel()};
     if (bits == 8) {
-      need_codes(ms[i], m_exps[i], p);
-      need_codes(vs[i], v_exps[i], p);
+      const Tensor &me = get(s, n.m_exps, "exp_avg_exps"), &ve = get(s, n.v_exps, "exp_avg_sq_exps");
+      need_codes(m, me, p);
+      need_codes(v, ve, p);
+      t.m_exps = (uint8_t*)me.data_ptr(), t.v_exps = (uint8_t*)ve.data_ptr();
+      written.push_back(me), written.push_back(ve);
     } else {
-      for (const Tensor* m : {&ms[i], &vs[i]}) {
-        same_device(first, *m);
-        TORCH_CHECK_VALUE(m->scalar_type() == at::kFloat && same_layout(*m, p), "AdamW: a moment is not a float32 tensor laid out as its parameter");
+      for (const Tensor* x : {&m, &v}) {
+        same_device(p, *x);
+        TORCH_CHECK_VALUE(x->scalar_type() == at::kFloat && same_layout(*x, p), "AdamW: a moment is not a float32 tensor laid out as its parameter");
       }
     }
-    same_device(first, steps[i]);
-    TORCH_CHECK_VALUE(steps[i].scalar_type() == at::kLong && steps[i].numel() == 1, "AdamW: step must be one int64");
-    t[i] = flb_adamw_tensor{p.data_ptr(), g.data_ptr(), ms[i].data_ptr(), vs[i].data_ptr(), bits == 8 ? (uint8_t*)m_exps[i].data_ptr() : nullptr,
-                            bits == 8 ? (uint8_t*)v_exps[i].data_ptr() : nullptr, steps[i].data_ptr<int64_t>(), p.numel()};
+    same_device(p, step);
+    TORCH_CHECK_VALUE(step.scalar_type() == at::kLong && step.numel() == 1, "AdamW: step must be one int64");
+    t.step = step.data_ptr<int64_t>();
+    to->t.push_back(t);
+    for (const Tensor* x : {&p, &m, &v, &step}) written.push_back(*x);
   }
-  check(flb_adamw(t.data(), (int64_t)n, dt, (int)bits, lr, (const float*)ptr(lr_device), b1, b2, eps, decay, seed, (uint32_t*)counter.data_ptr(),
-                  stream_of(first)),
-        "flb_adamw");
-  for (size_t i = 0; i < n; ++i) {
-    // written behind autograd's back: a graph that still needs the old values is told
-    for (const Tensor* x : {&params[i], &ms[i], &vs[i], &steps[i]}) x->unsafeGetTensorImpl()->bump_version();
-    if (bits == 8)
-      for (const Tensor* x : {&m_exps[i], &v_exps[i]}) x->unsafeGetTensorImpl()->bump_version();
+  if (pybind11::len(missing)) return missing;
+  for (Together& x : all) {
+    same_device(x.like, lr_device);
+    const c10::cuda::CUDAGuard guard(x.device);
+    // a word of the kernel's own on each device, zero between steps
+    const pybind11::int_ key(x.device.index());
+    if (!counters.contains(key)) counters[key] = pybind11::cast(at::zeros({1}, x.like.options().dtype(at::kInt).requires_grad(false)));
+    const Tensor counter = counters[key].cast<Tensor>();
+    check(flb_adamw(x.t.data(), (int64_t)x.t.size(), dtype_of(x.type, "a parameter"), (int)bits, lr, (const float*)ptr(lr_device), b1, b2, eps, decay, seed,
+                    (uint32_t*)counter.data_ptr(), stream_of(x.like)),
+          "flb_adamw");
   }
+  // written behind autograd's back: a graph that still needs the old values is told
+  for (const Tensor& x : written) x.unsafeGetTensorImpl()->bump_version();
+  return missing;
 }
 
-// m and v of parameters into tensors of their shapes and layouts
-void adamw_moments(const std::vector<Tensor>& params, const std::vector<Tensor>& m_out, const std::vector<Tensor>& v_out,
-                   const std::vector<Tensor>& ms, const std::vector<Tensor>& vs, const std::vector<Tensor>& m_exps,
-                   const std::vector<Tensor>& v_exps) {
-  const size_t n = params.size();
-  if (n == 0) return;
-  need_cuda(params[0]);
-  const c10::cuda::CUDAGuard guard(params[0].device());
-  std::vector<flb_adamw_tensor> t(n);
-  for (size_t i = 0; i < n; ++i) {
-    const Tensor& p = params[i];
-    same_device(params[0], p);
-    for (const Tensor* o : {&m_out[i], &v_out[i]}) {
-      same_device(p, *o);
-      TORCH_CHECK_VALUE(o->scalar_type() == at::kFloat && same_layout(*o, p), "AdamW: moments go to float32 tensors laid out as their parameters");
+// The moments of parameters that have 8-bit state, as pairs: into those of `out` from its place `at` on, or new ones.
+pybind11::list adamw_moments(pybind11::list params, pybind11::dict state, pybind11::object out, size_t at) {
+  pybind11::list found;
+  std::vector<Together> all;
+  std::vector<Tensor> written;
+  for (pybind11::handle h : params) {
+    PyObject* const s = state_of(state.ptr(), h.ptr());
+    if (!s) continue;
+    const Tensor& p = tensor_of(h.ptr(), "parameter");
+    need_cuda(p);
+    const c10::cuda::CUDAGuard guard(p.device());
+    Tensor pair[2];
+    if (out.is_none()) {
+      for (Tensor& x : pair) x = at::empty_like(p, p.options().dtype(at::kFloat).requires_grad(false));
+    } else {
+      const pybind11::object given = out[pybind11::int_(at++)];
+      for (int i = 0; i < 2; ++i) {
+        pair[i] = pybind11::object(given[pybind11::int_(i)]).cast<Tensor>();
+        same_device(p, pair[i]);
+        TORCH_CHECK_VALUE(pair[i].scalar_type() == at::kFloat && same_layout(pair[i], p), "AdamW: moments go to float32 tensors laid out as their parameters");
+      }
     }
-    need_codes(ms[i], m_exps[i], p);
-    need_codes(vs[i], v_exps[i], p);
-    t[i] = flb_adamw_tensor{m_out[i].data_ptr(), v_out[i].data_ptr(), ms[i].data_ptr(), vs[i].data_ptr(), (uint8_t*)m_exps[i].data_ptr(),
-                            (uint8_t*)v_exps[i].data_ptr(), nullptr, p.numel()};
+    const Names& n = names();
+    const Tensor &m = get(s, n.m, "exp_avg"), &v = get(s, n.v, "exp_avg_sq"), &me = get(s, n.m_exps, "exp_avg_exps"), &ve = get(s, n.v_exps, "exp_avg_sq_exps");
+    need_codes(m, me, p);
+    need_codes(v, ve, p);
+    Together* to = nullptr;
+    for (Together& x : all)
+      if (x.device == p.device()) to = &x;
+    if (!to) {
+      all.push_back({p.device(), at::kFloat, {}, {}, p});
+      to = &all.back();
+    }
+    to->t.push_back(flb_adamw_tensor{pair[0].data_ptr(), pair[1].data_ptr(), m.data_ptr(), v.data_ptr(), (uint8_t*)me.data_ptr(), (uint8_t*)ve.data_ptr(),
+                                     nullptr, p.numel()});
+    for (const Tensor& x : pair) written.push_back(x);
+    found.append(pybind11::make_tuple(pair[0], pair[1]));
   }
-  check(flb_adamw_moments(t.data(), (int64_t)n, stream_of(params[0])), "flb_adamw_moments");
-  for (size_t i = 0; i < n; ++i)
-    for (const Tensor* x : {&m_out[i], &v_out[i]}) x->unsafeGetTensorImpl()->bump_version();
+  for (Together& x : all) {
+    const c10::cuda::CUDAGuard guard(x.device);
+    check(flb_adamw_moments(x.t.data(), (int64_t)x.t.size(), stream_of(x.like)), "flb_adamw_moments");
+  }
+  for (const Tensor& x : written) x.unsafeGetTensorImpl()->bump_version();
+  return found;
 }
 
 }  // namespace
@@ -781,8 +850,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return fp8_linear_kept(x, xc, xe, wc, we, bias, t, check_timeout);
   });
   m.def("sample", &sample, off);
-  m.def("adamw", &adamw, off);
-  m.def("adamw_moments", &adamw_moments, off);
+  m.def("adamw", &adamw);
+  m.def("adamw_moments", &adamw_moments);
   m.def("int8_linear", [](const Opt& x, const Opt& xc, const Opt& xs, const Tensor& wc, const Tensor& ws, const Opt& bias, py::object dtype,
                           bool check_timeout) {
     std::optional<at::ScalarType> t;

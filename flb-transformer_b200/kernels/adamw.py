@@ -71,13 +71,6 @@ class AdamW(torch.optim.Optimizer):
             group.setdefault("state_bits", 32)
             group.setdefault("seed", 0)
 
-    def _counter(self, device):
-        # a word of the kernel's own on each device, zero between steps
-        counters = self.__dict__.setdefault("_counters", {})
-        if device not in counters:
-            counters[device] = torch.zeros(1, dtype=torch.int32, device=device)
-        return counters[device]
-
     def _new_state(self, p, bits):
         state = {"step": torch.zeros((), dtype=torch.int64, device=p.device)}
         blocks = -(-p.numel() // 128)
@@ -96,57 +89,44 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        counters = self.__dict__.setdefault("_counters", {})
         for group in self.param_groups:
-            bits = group["state_bits"]
-            together = {}
-            for p in group["params"]:
-                if p.grad is None:
-                    continue
-                state = self.state[p]
-                if len(state) == 0:
-                    if not p.is_cuda:
-                        raise RuntimeError(f"AdamW runs on CUDA tensors only (sm_100a kernels; no CPU path); got a parameter on {p.device}")
-                    if torch.cuda.is_current_stream_capturing():
-                        raise RuntimeError("AdamW: the first step of a parameter makes its state: take one before the capture")
-                    state.update(self._new_state(p, bits))
-                    self._counter(p.device)
-                t = together.setdefault((p.device, p.dtype), ([], [], [], [], [], [], []))
-                for of, x in zip(t, (p, p.grad, state["exp_avg"], state["exp_avg_sq"], state["step"], state.get("exp_avg_exps"),
-                                     state.get("exp_avg_sq_exps"))):
-                    of.append(x)
             lr = group["lr"]
             on_device = isinstance(lr, torch.Tensor) and lr.is_cuda
-            for (device, _), t in together.items():
-                exps = t[5:] if bits == 8 else ([], [])
-                flb_ops.adamw(*t[:5], *exps, bits, 0.0 if on_device else float(lr), lr.detach() if on_device else None, *group["betas"],
-                              group["eps"], group["weight_decay"], group["seed"] & 0xffffffff, self._counter(device))
+            args = (group["params"], self.state, group["state_bits"], 0.0 if on_device else float(lr), lr.detach() if on_device else None,
+                    *group["betas"], group["eps"], group["weight_decay"], group["seed"] & 0xffffffff, counters)
+            new = flb_ops.adamw(*args)
+            if new:
+                for p in new:
+                    if not p.is_cuda:
+                        raise RuntimeError(f"AdamW runs on CUDA tensors only (sm_100a kernels; no CPU path); got a parameter on {p.device}")
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("AdamW: the first step of a parameter makes its state: take one before the capture")
+                for p in new:
+                    self.state[p].update(self._new_state(p, group["state_bits"]))
+                flb_ops.adamw(*args)
         return loss
 
     @torch.no_grad()
     def moments(self, out=None) -> list:
         """(m, v) of every parameter that has taken a step, in the groups' order, as float32 tensors of its shape. Of 32 bits they are the
         state's own; of 8 bits new ones, or those of `out`, a list of such pairs of contiguous tensors, written."""
-        params = [(p, group["state_bits"]) for group in self.param_groups for p in group["params"] if len(self.state[p])]
-        if out is not None and len(out) != len(params):
-            raise ValueError(f"{len(out)} pairs for {len(params)} parameters")
-        found, together = [], {}
-        for i, (p, bits) in enumerate(params):
-            s = self.state[p]
-            if bits == 32:
-                pair = (s["exp_avg"], s["exp_avg_sq"])
+        found = []
+        if out is not None and len(out) != sum(1 for group in self.param_groups for p in group["params"] if self.state.get(p)):
+            raise ValueError("`out` does not have a pair for each parameter that has taken a step")
+        for group in self.param_groups:
+            if group["state_bits"] == 8:
+                found += flb_ops.adamw_moments(group["params"], self.state, out, len(found))
+                continue
+            for p in group["params"]:
+                if not self.state.get(p):
+                    continue
+                pair = (self.state[p]["exp_avg"], self.state[p]["exp_avg_sq"])
                 if out is not None:
-                    for to, x in zip(out[i], pair):
+                    for to, x in zip(out[len(found)], pair):
                         to.copy_(x)
-                    pair = out[i]
-            else:
-                pair = out[i] if out is not None else tuple(torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
-                                                            for _ in range(2))
-                t = together.setdefault(p.device, ([], [], [], [], [], [], []))
-                for of, x in zip(t, (p, *pair, s["exp_avg"], s["exp_avg_sq"], s["exp_avg_exps"], s["exp_avg_sq_exps"])):
-                    of.append(x)
-            found.append(pair)
-        for t in together.values():
-            flb_ops.adamw_moments(*t)
+                    pair = tuple(out[len(found)])
+                found.append(pair)
         return found
 
     @torch.no_grad()
