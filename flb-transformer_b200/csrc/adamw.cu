@@ -23,8 +23,11 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBlockElems = 128;                    // a block of 8-bit moments: a warp's four elements a lane
-constexpr int kUnroll = 4;                          // such blocks a warp has in flight
-constexpr int kChunk = kThreads / 32 * kUnroll * kBlockElems;
+// Such blocks a warp has in flight, thread blocks an SM, and elements of a tensor that a thread block takes at a time. (Moments in 8 bits with two
+// blocks in flight and four thread blocks: 391 us for 106 million float32, with four and three 365, before a chunk was several such steps.)
+constexpr int kUnroll = 4;
+template <int BITS> constexpr int kPerSm = BITS == 32 ? 2 : 3;
+constexpr int kStep = kThreads / 32 * kUnroll * kBlockElems;
 constexpr int kBelowM = 14, kBitsM = 7, kBelowV = 30, kBitsV = 8;
 
 struct Tensor {
@@ -44,6 +47,7 @@ template <int CAP> struct Table {
   Tensor t[CAP];
   uint32_t first[CAP + 1];  // chunks before each tensor
   int count;
+  int chunk;                // elements, a multiple of kStep
 };
 
 struct Args {
@@ -52,13 +56,15 @@ struct Args {
   double lr, decay;
   const float* lr_device;   // null, or in lr's place
   float eps;
+  bool flush;               // see quotient()
   uint32_t seed;
   uint32_t* counter;        // blocks done; zero between launches
+  uint32_t place;           // 2^20
 };
 
-// Four consecutive elements from i on of n, zeros beyond.
-template <typename T> __device__ __forceinline__ void load4(float (&x)[4], const T* p, int64_t i, int64_t n, bool vec) {
-  if (vec && i + 4 <= n) {
+// Four consecutive elements from i on of n, zeros beyond. FULL: all are there, on 16 bytes (8 of 16-bit types).
+template <bool FULL, typename T> __device__ __forceinline__ void load4(float (&x)[4], const T* p, int i, int n, bool vec) {
+  if (FULL || (vec && i + 4 <= n)) {
     if constexpr (sizeof(T) == 4) {
       const float4 a = *reinterpret_cast<const float4*>(p + i);
       x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
@@ -72,8 +78,8 @@ template <typename T> __device__ __forceinline__ void load4(float (&x)[4], const
     for (int j = 0; j < 4; ++j) x[j] = i + j < n ? ld(p + i + j) : 0.f;
   }
 }
-template <typename T> __device__ __forceinline__ void store4(T* p, const float (&x)[4], int64_t i, int64_t n, bool vec) {
-  if (vec && i + 4 <= n) {
+template <bool FULL, typename T> __device__ __forceinline__ void store4(T* p, const float (&x)[4], int i, int n, bool vec) {
+  if (FULL || (vec && i + 4 <= n)) {
     if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p + i) = make_float4(x[0], x[1], x[2], x[3]);
     else *reinterpret_cast<uint2*>(p + i) = make_uint2(rows::pack2<T>(x[0], x[1]), rows::pack2<T>(x[2], x[3]));
   } else {
@@ -83,129 +89,191 @@ template <typename T> __device__ __forceinline__ void store4(T* p, const float (
   }
 }
 
-// A code's float32 bits, without a sign: base = (E - below) * 8. Not for a block marked as NaN.
-template <int BITS> __device__ __forceinline__ float decode(uint32_t code, int base) {
-  const uint32_t low = code & ((1u << BITS) - 1);
-  uint32_t u = low ? (low + base) << 20 : 0u;
-  if (BITS == 7) u |= (code >> 7) << 31;
-  return __uint_as_float(u);
-}
-// size: a magnitude's bits. noise: 16 random bits, from bit 4 on.
-template <bool UNSIGNED> __device__ __forceinline__ uint32_t encode(uint32_t size, uint32_t noise, int base) {
-  // (up to the largest finite exponent)
-  const int key = (int)min((size + noise) >> 20, 254u * 8 + 7) - base;
-  if (UNSIGNED) return size ? (uint32_t)max(key, 1) : 0u;
-  return (uint32_t)max(key, 0);
+// Four codes of a block. base: (E - below) * 8 << 20, what a code's bits at their place in a float32 are short of that float32's. The 8-bit
+// forms are bound by the integer units as much as by memory, so shifts here are multiplications by arguments (place: 2^20), which run
+// beside those, and what is rare (zeros, marked blocks) is looked for four codes at a time.
+template <int BITS> __device__ __forceinline__ void decode(float (&x)[4], uint32_t codes, int e, uint32_t base, uint32_t place) {
+  const uint32_t low = BITS == 7 ? codes & 0x7f7f7f7fu : codes;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t u = __byte_perm(low, 0, 0x4440 + j) * place + base;
+    if (BITS == 7) u |= codes << (24 - 8 * j) & 0x80000000u;
+    x[j] = __uint_as_float(u);
+  }
+  if ((low - 0x01010101u) & ~low & 0x80808080u) {  // a zero among them
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (!(low >> (8 * j) & 255)) x[j] = 0.f;
+  }
+  if (e == 255) {  // the block's own, so of the whole warp
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = __uint_as_float(0x7fffffffu);
+  }
 }
 // E of a block whose largest magnitude has these bits, not below the least for which every code is a normal number
 __device__ __forceinline__ int block_exponent(uint32_t top, int below) { return max((int)(top >> 23), below + 1); }
+__device__ __forceinline__ uint32_t base_of(int e, int below) { return (uint32_t)(e - below) << 23; }
 
-__device__ __forceinline__ uint32_t mix(uint32_t i, uint32_t step_and_seed) {
-  uint32_t x = i * 0x9E3779B9u + step_and_seed;  // the golden ratio's and the roots' of 2 and 3 first digits
-  x = (x ^ (x >> 16)) * 0xBB67AE85u;
-  return x ^ (x >> 16);
+// 32 random bits for element i: products with the first digits of the golden ratio and of the root of 3. Of the result x ^ x >> 16 the
+// upper half is m's noise and the lower v's, both at bits 4 to 19.
+__device__ __forceinline__ void noise_of(uint32_t i_and_salt, uint32_t& m, uint32_t& v) {
+  const uint32_t x = (i_and_salt ^ (i_and_salt >> 16)) * 0xBB67AE85u, high = x >> 12;
+  m = high & 0xffff0u;
+  v = ((x << 4) ^ high) & 0xffff0u;
+}
+__device__ __forceinline__ uint32_t bytes_of(const uint32_t (&k)[4], int from) {
+  return __byte_perm(__byte_perm(k[0], k[1], from | (4 + from) << 4), __byte_perm(k[2], k[3], from | (4 + from) << 4), 0x5410);
+}
+constexpr uint32_t kMix = 0x9E3779B9u;
+
+// The tensor that a chunk belongs to, and its place there: from element `at` on, `left` of them.
+template <int CAP> __device__ __forceinline__ const Tensor& tensor_of(const Table<CAP>& tb, uint32_t c, int64_t& at, int& left) {
+  int lo = 0, hi = tb.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (tb.first[mid] <= c) lo = mid; else hi = mid - 1;
+  }
+  const Tensor& t = tb.t[lo];
+  at = (int64_t)(c - tb.first[lo]) * tb.chunk;
+  left = (int)min((t.n >= 0 ? t.n : -t.n) - at, (int64_t)tb.chunk);
+  return t;
+}
+
+// m / (sqrt(v) root + eps), root and quotient each within 2^-22. flush: eps is so large that it makes no difference whether v and m below float32's
+// normal numbers count as zero, which saves the operations that scale them.
+__device__ __forceinline__ float quotient(float m, float v, float root, float eps, bool flush) {
+  float s, q;
+  if (flush) {
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(v));
+    asm("div.approx.ftz.f32 %0, %1, %2;" : "=f"(q) : "f"(m), "f"(fmaf(s, root, eps)));
+  } else {
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(s) : "f"(v));
+    asm("div.approx.f32 %0, %1, %2;" : "=f"(q) : "f"(m), "f"(fmaf(s, root, eps)));
+  }
+  return q;
 }
 
 template <typename T, int BITS, int CAP>
-__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<CAP> tb, const Args a) {
+__global__ void __launch_bounds__(kThreads, kPerSm<BITS>) adamw_kernel(const __grid_constant__ Table<CAP> tb, const Args a) {
+  constexpr int U = kUnroll;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t chunks = tb.first[tb.count];
   int64_t known = -1;  // the step whose factors these are
   float keep = 0, rate = 0, root = 0;
   for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
-    int lo = 0, hi = tb.count - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (tb.first[mid] <= c) lo = mid; else hi = mid - 1;
-    }
-    const Tensor& t = tb.t[lo];
+    int64_t at;
+    int left;
+    const Tensor& t = tensor_of(tb, c, at, left);
     const bool vec = t.n >= 0;
-    const int64_t n = vec ? t.n : -t.n;
-    const int64_t from = (int64_t)(c - tb.first[lo]) * kChunk + warp * (kUnroll * kBlockElems) + lane * 4;
-    float p[kUnroll][4], g[kUnroll][4], m[kUnroll][4], v[kUnroll][4];
-    uint32_t cm[kUnroll], cv[kUnroll], exps = 0;
-    const int64_t block0 = (from - lane * 4) / kBlockElems, blocks = (n + kBlockElems - 1) / kBlockElems;
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int64_t i = from + u * kBlockElems;
-      load4(p[u], static_cast<const T*>(t.p), i, n, vec);
-      load4(g[u], static_cast<const T*>(t.g), i, n, vec);
-      if constexpr (BITS == 32) {
-        load4(m[u], static_cast<const float*>(t.m), i, n, vec);
-        load4(v[u], static_cast<const float*>(t.v), i, n, vec);
-      } else {
-        const bool there = block0 + u < blocks;
-        cm[u] = there ? static_cast<const uint32_t*>(t.m)[i / 4] : 0u;
-        cv[u] = there ? static_cast<const uint32_t*>(t.v)[i / 4] : 0u;
-      }
-    }
-    // lanes 0 to 3 have the four blocks' bytes of m, 4 to 7 those of v
-    const bool has_byte = BITS == 8 && lane < 2 * kUnroll && block0 + lane % kUnroll < blocks;
-    uint8_t* const byte = (lane < kUnroll ? t.me : t.ve) + block0 + lane % kUnroll;
-    if (has_byte) exps = *byte;
+    T* const pp = static_cast<T*>(t.p) + at;
+    const T* const pg = static_cast<const T*>(t.g) + at;
+    using State = std::conditional_t<BITS == 32, float, uint8_t>;
+    State* const pm = static_cast<State*>(t.m) + at;
+    State* const pv = static_cast<State*>(t.v) + at;
+    const int blocks = (left + kBlockElems - 1) / kBlockElems;
+    // the first U lanes have the bytes of a step's blocks of m, the next those of v
+    uint8_t* const bytes = BITS == 8 ? (lane < U ? t.me : t.ve) + at / kBlockElems + lane % U : nullptr;
     const int64_t step = *t.step + 1;
-    if (step != known) {
-      known = step;
-      const double lr = a.lr_device ? (double)*a.lr_device : a.lr;
-      keep = (float)(1.0 - lr * a.decay);
-      rate = (float)(lr / -expm1((double)step * a.log_b1));
-      root = (float)rsqrt(-expm1((double)step * a.log_b2));
-    }
-    const uint32_t salt = (uint32_t)step * 0x6A09E667u + a.seed;
-    uint32_t kept_exps = 0;
+    auto step_at = [&](int o, auto full) {
+      constexpr bool FULL = decltype(full)::value;
+      float p[U][4], g[U][4], m[U][4], v[U][4];
+      uint32_t cm[U], cv[U], exps = 0;
+      const int block0 = o / kBlockElems;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int64_t i = from + u * kBlockElems;
-      if constexpr (BITS == 8) {
-        const int em = __shfl_sync(0xffffffffu, exps, u), ev = __shfl_sync(0xffffffffu, exps, kUnroll + u);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          m[u][j] = decode<kBitsM>(cm[u] >> (8 * j) & 255, (em - kBelowM) * 8);
-          v[u][j] = decode<kBitsV>(cv[u] >> (8 * j) & 255, (ev - kBelowV) * 8);
-          if (em == 255) m[u][j] = __uint_as_float(0x7fffffffu);
-          if (ev == 255) v[u][j] = __uint_as_float(0x7fffffffu);
+      for (int u = 0; u < U; ++u) {
+        const int i = o + u * kBlockElems + lane * 4;
+        load4<FULL>(p[u], pp, i, left, vec);
+        load4<FULL>(g[u], pg, i, left, vec);
+        if constexpr (BITS == 32) {
+          load4<FULL>(m[u], pm, i, left, vec);
+          load4<FULL>(v[u], pv, i, left, vec);
+        } else {
+          const bool there = FULL || block0 + u < blocks;
+          cm[u] = there ? *reinterpret_cast<const uint32_t*>(pm + i) : 0u;
+          cv[u] = there ? *reinterpret_cast<const uint32_t*>(pv + i) : 0u;
         }
       }
-      uint32_t top_m = 0, top_v = 0;
+      const bool has_byte = BITS == 8 && lane < 2 * U && (FULL || block0 + lane % U < blocks);
+      if (has_byte) exps = bytes[block0];
+      if (step != known) {
+        known = step;
+        const double lr = a.lr_device ? (double)*a.lr_device : a.lr;
+        keep = (float)(1.0 - lr * a.decay);
+        rate = (float)(lr / expm1((double)step * a.log_b1));  // (negative)
+        root = (float)rsqrt(-expm1((double)step * a.log_b2));
+      }
+      // (the root of 2's digits)
+      const uint32_t salt = ((uint32_t)at + o + lane * 4) * kMix + (uint32_t)step * 0x6A09E667u + a.seed;
+      uint32_t kept_exps = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float gj = g[u][j];
-        m[u][j] = __fadd_rn(__fmul_rn(m[u][j], a.b1), __fmul_rn(gj, a.c1));
-        v[u][j] = __fadd_rn(__fmul_rn(v[u][j], a.b2), __fmul_rn(__fmul_rn(gj, gj), a.c2));
-        const float q = __fdividef(m[u][j], fmaf(sqrtf(v[u][j]), root, a.eps));
-        p[u][j] = fmaf(p[u][j], keep, -rate * q);
+      for (int u = 0; u < U; ++u) {
+        const int i = o + u * kBlockElems + lane * 4;
         if constexpr (BITS == 8) {
-          // places beyond the last element hold zeros, and stay zeros
-          top_m = max(top_m, __float_as_uint(m[u][j]) & 0x7fffffffu);
-          top_v = max(top_v, __float_as_uint(v[u][j]) & 0x7fffffffu);
+          const int em = __shfl_sync(0xffffffffu, exps, u), ev = __shfl_sync(0xffffffffu, exps, U + u);
+          decode<kBitsM>(m[u], cm[u], em, base_of(em, kBelowM), a.place);
+          decode<kBitsV>(v[u], cv[u], ev, base_of(ev, kBelowV), a.place);
         }
-      }
-      store4(static_cast<T*>(t.p), p[u], i, n, vec);
-      if constexpr (BITS == 32) {
-        store4(static_cast<float*>(t.m), m[u], i, n, vec);
-        store4(static_cast<float*>(t.v), v[u], i, n, vec);
-      } else {
-        top_m = __reduce_max_sync(0xffffffffu, top_m);
-        top_v = __reduce_max_sync(0xffffffffu, top_v);
-        const int em = block_exponent(top_m, kBelowM), ev = block_exponent(top_v, kBelowV);
-        uint32_t wm = 0, wv = 0;
+        uint32_t top_m = 0, top_v = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t r = mix((uint32_t)i + j, salt);
-          const uint32_t bits_m = __float_as_uint(m[u][j]);
-          const uint32_t km = encode<false>(bits_m & 0x7fffffffu, r >> 16 << 4, (em - kBelowM) * 8);
-          wm |= (km | (bits_m >> 31 && km ? 128u : 0u)) << (8 * j);
-          wv |= encode<true>(__float_as_uint(v[u][j]), (r & 0xffffu) << 4, (ev - kBelowV) * 8) << (8 * j);
+          const float gj = g[u][j];
+          m[u][j] = __fadd_rn(__fmul_rn(m[u][j], a.b1), __fmul_rn(gj, a.c1));
+          v[u][j] = __fadd_rn(__fmul_rn(v[u][j], a.b2), __fmul_rn(__fmul_rn(gj, gj), a.c2));
+          p[u][j] = fmaf(p[u][j], keep, rate * quotient(m[u][j], v[u][j], root, a.eps, a.flush));
+          if constexpr (BITS == 8) {
+            // places beyond the last element hold zeros, and stay zeros
+            top_m = max(top_m, __float_as_uint(m[u][j]) & 0x7fffffffu);
+            top_v = max(top_v, __float_as_uint(v[u][j]) & 0x7fffffffu);
+          }
         }
-        if (block0 + u < blocks) {
-          static_cast<uint32_t*>(t.m)[i / 4] = wm;
-          static_cast<uint32_t*>(t.v)[i / 4] = wv;
+        store4<FULL>(pp, p[u], i, left, vec);
+        if constexpr (BITS == 32) {
+          store4<FULL>(pm, m[u], i, left, vec);
+          store4<FULL>(pv, v[u], i, left, vec);
+        } else {
+          top_m = __reduce_max_sync(0xffffffffu, top_m);
+          top_v = __reduce_max_sync(0xffffffffu, top_v);
+          const int em = block_exponent(top_m, kBelowM), ev = block_exponent(top_v, kBelowV);
+          const uint32_t base_m = base_of(em, kBelowM), base_v = base_of(ev, kBelowV);
+          uint32_t km[4], kv[4], bits_m[4];
+          bool zero = false;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t noise_m, noise_v;
+            noise_of(salt + (uint32_t)(u * kBlockElems + j) * kMix, noise_m, noise_v);
+            bits_m[j] = __float_as_uint(m[u][j]);
+            const uint32_t size_m = bits_m[j] & 0x7fffffffu, size_v = __float_as_uint(v[u][j]);
+            km[j] = (uint32_t)max((int)(size_m + noise_m - base_m) >> 20, 0);
+            kv[j] = (uint32_t)max((int)(size_v + noise_v - base_v) >> 20, 1);
+            zero |= size_v == 0;
+          }
+          if (zero) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (v[u][j] == 0) kv[j] = 0;
+          }
+          if (max(em, ev) >= 254) {  // up to the largest finite exponent (of the whole warp)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              km[j] = min(km[j], (254u * 8 + 7) - (base_m >> 20));
+              kv[j] = min(kv[j], (254u * 8 + 7) - (base_v >> 20));
+            }
+          }
+          if (FULL || block0 + u < blocks) {
+            *reinterpret_cast<uint32_t*>(pm + i) = bytes_of(km, 0) | (bytes_of(bits_m, 3) & 0x80808080u);
+            *reinterpret_cast<uint32_t*>(pv + i) = bytes_of(kv, 0);
+          }
+          if (lane == u) kept_exps = em;
+          if (lane == U + u) kept_exps = ev;
         }
-        if (lane == u) kept_exps = em;
-        if (lane == kUnroll + u) kept_exps = ev;
       }
+      if (has_byte) bytes[block0] = (uint8_t)kept_exps;
+    };
+#pragma unroll 1
+    for (int o = warp * U * kBlockElems; o < left; o += kStep) {
+      if (vec && o + U * kBlockElems <= left) step_at(o, std::true_type());
+      else step_at(o, std::false_type());
     }
-    if (has_byte) *byte = (uint8_t)kept_exps;
   }
   // The steps count up once every block has read them: by the last block to end.
   __shared__ bool last;
@@ -216,50 +284,64 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
     for (int i = threadIdx.x; i < tb.count; i += kThreads) ++*tb.t[i].step;
 }
 
-// Codes into float32: p and g are where m and v go (either may be null).
+// Codes into float32: p and g are where m and v go.
 template <int CAP> __global__ void __launch_bounds__(kThreads) moments_kernel(const __grid_constant__ Table<CAP> tb) {
+  constexpr int U = kUnroll;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t chunks = tb.first[tb.count];
   for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
-    int lo = 0, hi = tb.count - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (tb.first[mid] <= c) lo = mid; else hi = mid - 1;
-    }
-    const Tensor& t = tb.t[lo];
+    int64_t at;
+    int left;
+    const Tensor& t = tensor_of(tb, c, at, left);
     const bool vec = t.n >= 0;
-    const int64_t n = vec ? t.n : -t.n, blocks = (n + kBlockElems - 1) / kBlockElems;
-    const int64_t from = (int64_t)(c - tb.first[lo]) * kChunk + warp * (kUnroll * kBlockElems) + lane * 4;
+    float* const to_m = static_cast<float*>(t.p) + at;
+    float* const to_v = static_cast<float*>(const_cast<void*>(t.g)) + at;
+    const uint8_t* const pm = static_cast<const uint8_t*>(t.m) + at;
+    const uint8_t* const pv = static_cast<const uint8_t*>(t.v) + at;
+    const uint8_t* const pe = (lane < U ? t.me : t.ve) + at / kBlockElems + lane % U;
+    const int blocks = (left + kBlockElems - 1) / kBlockElems;
+#pragma unroll 1
+    for (int o = warp * U * kBlockElems; o < left; o += kStep) {
+      uint32_t cm[U], cv[U], exps = 0;
+      const int block0 = o / kBlockElems;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int64_t i = from + u * kBlockElems, block = i / kBlockElems;
-      if (block >= blocks) break;
-      const uint32_t cm = static_cast<const uint32_t*>(t.m)[i / 4], cv = static_cast<const uint32_t*>(t.v)[i / 4];
-      const int em = t.me[block], ev = t.ve[block];
-      float m[4], v[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        m[j] = em == 255 ? __uint_as_float(0x7fffffffu) : decode<kBitsM>(cm >> (8 * j) & 255, (em - kBelowM) * 8);
-        v[j] = ev == 255 ? __uint_as_float(0x7fffffffu) : decode<kBitsV>(cv >> (8 * j) & 255, (ev - kBelowV) * 8);
+      for (int u = 0; u < U; ++u) {
+        const int i = o + u * kBlockElems + lane * 4;
+        const bool there = block0 + u < blocks;
+        cm[u] = there ? *reinterpret_cast<const uint32_t*>(pm + i) : 0u;
+        cv[u] = there ? *reinterpret_cast<const uint32_t*>(pv + i) : 0u;
       }
-      store4(static_cast<float*>(t.p), m, i, n, vec);
-      store4(static_cast<float*>(const_cast<void*>(t.g)), v, i, n, vec);
+      if (lane < 2 * U && block0 + lane % U < blocks) exps = pe[block0];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = o + u * kBlockElems + lane * 4, em = __shfl_sync(0xffffffffu, exps, u), ev = __shfl_sync(0xffffffffu, exps, U + u);
+        float m[4], v[4];
+        decode<kBitsM>(m, cm[u], em, base_of(em, kBelowM), 1u << 20);
+        decode<kBitsV>(v, cv[u], ev, base_of(ev, kBelowV), 1u << 20);
+        store4<false>(to_m, m, i, left, vec);
+        store4<false>(to_v, v, i, left, vec);
+      }
     }
   }
 }
 
-// Fills tables of up to CAP tensors and launches for each.
+// Fills tables of up to CAP tensors and launches for each. A chunk is one step of a thread block, or up to eight where there are enough for
+// `resident` thread blocks a few times over.
 template <int CAP, typename Launch>
-int in_tables(const flb_adamw_tensor* t, int64_t count, int elem, int state_bits, Launch&& launch) {
-  static_assert(sizeof(Table<CAP>) <= 32 * 1024, "a launch's parameters");
+int in_tables(const flb_adamw_tensor* t, int64_t count, int elem, int state_bits, int resident, Launch&& launch) {
+  static_assert(sizeof(Table<CAP>) + sizeof(Args) <= 32 * 1024 - 4, "a launch's parameters");
   Table<CAP> tb;
   auto off = [](const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) != 0; };
+  int64_t total = 0;
+  for (int64_t i = 0; i < count; ++i) total += t[i].n;
+  tb.chunk = kStep;
+  while (tb.chunk < 8 * kStep && total / tb.chunk > 8 * (int64_t)resident) tb.chunk *= 2;
   for (int64_t from = 0; from < count;) {
     tb.count = 0;
     tb.first[0] = 0;
     while (from < count && tb.count < CAP) {
       const flb_adamw_tensor& s = t[from];
-      const int64_t chunks = (s.n + kChunk - 1) / kChunk;
+      const int64_t chunks = (s.n + tb.chunk - 1) / tb.chunk;
       if (chunks > 0 && chunks + tb.first[tb.count] > INT32_MAX) break;
       ++from;
       if (chunks == 0 && !s.step) continue;
@@ -269,17 +351,15 @@ int in_tables(const flb_adamw_tensor* t, int64_t count, int elem, int state_bits
       ++tb.count;
     }
     if (tb.count == 0) continue;
-    const int st = launch(tb);
+    const int st = launch(tb, (unsigned)std::max<int64_t>(1, std::min<int64_t>(tb.first[tb.count], resident)));
     if (st != FLB_OK) return st;
   }
   return FLB_OK;
 }
 
-unsigned grid_of(uint32_t chunks, int per_sm) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>(chunks, (int64_t)num_sms() * per_sm)); }
-
 template <typename T, int BITS, int CAP> int step_tables(const flb_adamw_tensor* t, int64_t count, const Args& a, cudaStream_t s) {
-  return in_tables<CAP>(t, count, sizeof(T), BITS, [&](const Table<CAP>& tb) {
-    adamw_kernel<T, BITS, CAP><<<grid_of(tb.first[tb.count], 4), kThreads, 0, s>>>(tb, a);
+  return in_tables<CAP>(t, count, sizeof(T), BITS, num_sms() * kPerSm<BITS>, [&](const Table<CAP>& tb, unsigned grid) {
+    adamw_kernel<T, BITS, CAP><<<grid, kThreads, 0, s>>>(tb, a);
     count_launches(1);
     return check_cuda(cudaGetLastError(), "adamw launch");
   });
@@ -299,7 +379,7 @@ int adamw(const flb_adamw_tensor* t, int64_t count, int dtype, int state_bits, d
   Args a = {};
   a.b1 = (float)b1, a.c1 = (float)(1 - b1), a.b2 = (float)b2, a.c2 = (float)(1 - b2);
   a.log_b1 = log(b1), a.log_b2 = log(b2);
-  a.lr = lr, a.lr_device = lr_device, a.decay = decay, a.eps = (float)eps, a.seed = seed, a.counter = counter;
+  a.lr = lr, a.lr_device = lr_device, a.decay = decay, a.eps = (float)eps, a.flush = eps >= 1e-11, a.seed = seed, a.counter = counter, a.place = 1u << 20;
   switch (dtype) {
     case FLB_F32: return step_b<float>(t, count, state_bits, a, s);
     case FLB_F16: return step_b<__half>(t, count, state_bits, a, s);
@@ -308,9 +388,9 @@ int adamw(const flb_adamw_tensor* t, int64_t count, int dtype, int state_bits, d
 }
 
 int adamw_moments(const flb_adamw_tensor* t, int64_t count, cudaStream_t s) {
-  return in_tables<440>(t, count, 4, 8, [&](const Table<440>& tb) {
+  return in_tables<440>(t, count, 4, 8, num_sms() * 8, [&](const Table<440>& tb, unsigned grid) {
     if (tb.first[tb.count] == 0) return (int)FLB_OK;
-    moments_kernel<440><<<grid_of(tb.first[tb.count], 8), kThreads, 0, s>>>(tb);
+    moments_kernel<440><<<grid, kThreads, 0, s>>>(tb);
     count_launches(1);
     return check_cuda(cudaGetLastError(), "adamw_moments launch");
   });

@@ -55,6 +55,7 @@ struct Args {
   int k_blocks, quads;
   int n_tiles, tiles, splits;
   int group;           // tiles of tokens that go through all channels together
+  bool stream_out;     // the output leaves L2 before the operands do
   float* parts;        // [tiles][splits][NC][128], splits > 1
   uint32_t* counts;    // [tiles], zero
   uint32_t* error;
@@ -84,8 +85,9 @@ __device__ __forceinline__ void umma_fp8(uint32_t d, uint64_t da, uint64_t db, u
       "l"(da), "l"(db), "r"(desc), "r"(ea), "r"(eb), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void tma_store_2d(const void* tmap, const void* src, int c0, int c1) {
-  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(tmap), "r"(smem_u32(src)), "r"(c0), "r"(c1)
+__device__ __forceinline__ void tma_store_2d(const void* tmap, const void* src, int c0, int c1, uint64_t policy) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group.L2::cache_hint [%0, {%2, %3}], [%1], %4;" ::"l"(tmap),
+               "r"(smem_u32(src)), "r"(c0), "r"(c1), "l"(policy)
                : "memory");
 }
 template <int NC> __device__ __forceinline__ void epilogue_barrier() {
@@ -240,6 +242,9 @@ __global__ void __launch_bounds__(threads<NC>(), 1)
     float* const bias = bias_all + (warp - 2) * kCols;
     uint32_t local = 0;
     bool ok = true;
+    uint64_t policy;
+    if (a.stream_out) asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+    else asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
     wait_predecessor();
     for (int u = blockIdx.x; u < units; u += gridDim.x) {
       int m0, n0, k0, k1;
@@ -334,7 +339,7 @@ __global__ void __launch_bounds__(threads<NC>(), 1)
           fence_async_shared();
           __syncwarp();
           if (lane == 0) {  // a store that ends outside the output is cut there
-            tma_store_2d(&tm_out, staged, n0 + c, m0);
+            tma_store_2d(&tm_out, staged, n0 + c, m0, policy);
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
         } else {
@@ -435,7 +440,10 @@ int code_map(CUtensorMap* m, const int8_t* codes, int64_t rows, int64_t ld, int6
   return make_tmap(m, codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// Of 126 MB of L2: a weight that stays there is gone through once for each tile of tokens, for a larger one 16 of them go together; an output that
+// does not fit beside it leaves first.
 constexpr int64_t kWeightInL2 = 48 << 20;
+constexpr size_t kOutputInL2 = 64 << 20;
 
 }  // namespace
 
@@ -479,6 +487,7 @@ int fp8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, c
   a.early = x != nullptr;
   a.k_blocks = (int)blocks_of(K), a.quads = (int)quads_of(K), a.n_tiles = g.n_tiles, a.tiles = g.tiles, a.splits = g.splits;
   a.group = N * K <= kWeightInL2 ? 1 : 16;
+  a.stream_out = (size_t)M * N * es > kOutputInL2;
   a.parts = reinterpret_cast<float*>(p + l.parts), a.counts = reinterpret_cast<uint32_t*>(p + l.counts), a.error = reinterpret_cast<uint32_t*>(p);
   switch (dtype) {
     case FLB_F32: st = launch<float>(g.width, tx, tw, to, a, x != nullptr, s); break;

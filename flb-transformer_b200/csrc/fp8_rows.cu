@@ -23,25 +23,30 @@ template <int N> __device__ __forceinline__ uint32_t max_of(uint32_t v) {
   return v;
 }
 
-// Consecutive values from column c on of a row of K, zeros beyond. VEC: rows that start on 16 bytes (8 of them at least are allowed to be read
-// where c < K only if K is a multiple of their number).
-template <typename T, bool VEC, int N> __device__ __forceinline__ void load_row(float (&v)[N], const T* row, int64_t c, int64_t K) {
-  static_assert(N * sizeof(T) == 16);
-  if constexpr (VEC) {
-    const uint4 w = c < K ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+// 16 bytes of a row of K from column c on, zeros beyond. VEC: rows that start on 16 bytes, whole ones of them.
+template <typename T, bool VEC> __device__ __forceinline__ uint4 load_row(const T* row, int64_t c, int64_t K) {
+  constexpr int N = 16 / sizeof(T);
+  if constexpr (VEC) return c < K ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
+  uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (sizeof(T) == 4) {
-        v[j] = __uint_as_float(u[j]);
-      } else {
-        const float2 f = rows::unpack2<T>(u[j]);
-        v[2 * j] = f.x, v[2 * j + 1] = f.y;
-      }
+  for (int j = 0; j < N; ++j) {
+    if (c + j < K) {
+      if constexpr (sizeof(T) == 4) w[j & 3] = __float_as_uint(row[c + j]);
+      else w[j / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(row)[c + j] << (16 * (j & 1));
     }
-  } else {
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <typename T> __device__ __forceinline__ void unpack_row(float (&v)[16 / sizeof(T)], const uint4& w) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = c + j < K ? ld(row + c + j) : 0.f;
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (sizeof(T) == 4) {
+      v[j] = __uint_as_float(u[j]);
+    } else {
+      const float2 f = rows::unpack2<T>(u[j]);
+      v[2 * j] = f.x, v[2 * j + 1] = f.y;
+    }
   }
 }
 
@@ -81,12 +86,7 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(256) rows_kern
   const int64_t row = unit / blocks, block = unit % blocks;
   const bool there = row < a.R;
   float v[N];
-  if (there) {
-    load_row<T, VEC>(v, reinterpret_cast<const T*>(a.x) + row * a.ldx, block * kBlock + lane * N, a.K);
-  } else {
-#pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = 0;
-  }
+  unpack_row<T>(v, there ? load_row<T, VEC>(reinterpret_cast<const T*>(a.x) + row * a.ldx, block * kBlock + lane * N, a.K) : make_uint4(0, 0, 0, 0));
   const int u = unit_of(max_of<PER>(largest(v)));
   if (!there) return;
   store_codes(a.codes + row * a.pitch, v, inverse_of(u), block * kBlock + lane * N, a.pitch);
@@ -103,6 +103,8 @@ struct TileArgs {
   float* sums;               // null, or [tiles of rows][C]: each column's sum over a tile's rows
 };
 
+constexpr int kDown = 8;
+
 // 256 threads. As 16 or 8 rows at a time (a row's block in PER lanes), then as columns: four runs of 32 rows of 64 pairs of columns.
 template <typename T, bool VEC, bool SUM> __global__ void __launch_bounds__(256) tile_kernel(const TileArgs a) {
   constexpr int PER = kPer<T>, N = 16 / sizeof(T), ROWS = 256 / PER, kPitch = kBlock + 16 / (int)sizeof(T);
@@ -110,24 +112,26 @@ template <typename T, bool VEC, bool SUM> __global__ void __launch_bounds__(256)
   T(*tile)[kPitch] = reinterpret_cast<T(*)[kPitch]>(dyn);
   __shared__ uint32_t tops[4][kBlock];
   __shared__ float parts[SUM ? 4 : 1][kBlock];
-  const unsigned across = (unsigned)blocks_of(a.C), tile_r = blockIdx.x / across, tile_c = blockIdx.x % across;
+  // Eight tiles down, then the next ones across: columns of codes leave in pieces of 1 KB that blocks running together write, rows come in long ones.
+  const unsigned across = (unsigned)blocks_of(a.C), down = (unsigned)blocks_of(a.R), group = blockIdx.x / (kDown * across), in = blockIdx.x % (kDown * across);
+  const unsigned high = min((unsigned)kDown, down - group * kDown), tile_r = group * kDown + in % high, tile_c = in / high;
   const int64_t r0 = (int64_t)tile_r * kBlock, c0 = (int64_t)tile_c * kBlock;
   const int lane = threadIdx.x % PER;
-#pragma unroll 4
-  for (int i = 0; i < kBlock; i += ROWS) {
-    const int r = i + threadIdx.x / PER;
-    const int64_t row = r0 + r;
-    float v[N];
-    if (row < a.R) {
-      load_row<T, VEC>(v, reinterpret_cast<const T*>(a.x) + row * a.ldx, c0 + lane * N, a.C);
-    } else {
+  // all of the thread's loads under way together
+  uint4 raw[kBlock / ROWS];
 #pragma unroll
-      for (int j = 0; j < N; ++j) v[j] = 0;
-    }
-    uint4 w;
-    if constexpr (sizeof(T) == 4) w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-    else w = make_uint4(rows::pack2<T>(v[0], v[1]), rows::pack2<T>(v[2], v[3]), rows::pack2<T>(v[4], v[5]), rows::pack2<T>(v[6], v[7]));
-    *reinterpret_cast<uint4*>(&tile[r][lane * N]) = w;
+  for (int i = 0; i < kBlock / ROWS; ++i) {
+    const int64_t row = r0 + i * ROWS + threadIdx.x / PER;
+    raw[i] = make_uint4(0, 0, 0, 0);
+    if (row < a.R) raw[i] = load_row<T, VEC>(reinterpret_cast<const T*>(a.x) + row * a.ldx, c0 + lane * N, a.C);
+  }
+#pragma unroll
+  for (int i = 0; i < kBlock / ROWS; ++i) {
+    const int r = i * ROWS + threadIdx.x / PER;
+    const int64_t row = r0 + r;
+    *reinterpret_cast<uint4*>(&tile[r][lane * N]) = raw[i];
+    float v[N];
+    unpack_row<T>(v, raw[i]);
     const int u = unit_of(max_of<PER>(largest(v)));
     if (row < a.R) {
       store_codes(a.codes + row * a.pitch, v, inverse_of(u), c0 + lane * N, a.pitch);
@@ -135,42 +139,78 @@ template <typename T, bool VEC, bool SUM> __global__ void __launch_bounds__(256)
     }
   }
   __syncthreads();
-  // columns 2p and 2p + 1, rows 32g to 32g + 31
+  // columns 2p and 2p + 1, rows 32g to 32g + 31: 16-bit pairs are read once and stay in registers
   const int p = threadIdx.x % 64, g = threadIdx.x / 64;
-  uint32_t m0 = 0, m1 = 0;
+  using Pair = std::conditional_t<sizeof(T) == 4, float2, uint32_t>;
+  auto pair_at = [&](int i) { return *reinterpret_cast<const Pair*>(&tile[32 * g + i][2 * p]); };
+  auto values = [](const Pair& x) {
+    if constexpr (sizeof(T) == 4) return x;
+    else return rows::unpack2<T>(x);
+  };
+  Pair kept[sizeof(T) == 4 ? 1 : 32];
+  uint32_t m0 = 0, m1 = 0, both = 0;
   float s0 = 0, s1 = 0;
-#pragma unroll 8
+#pragma unroll
   for (int i = 0; i < 32; ++i) {
-    const float a0 = ld(&tile[32 * g + i][2 * p]), a1 = ld(&tile[32 * g + i][2 * p + 1]);
-    m0 = max(m0, __float_as_uint(a0) & 0x7fffffffu);
-    m1 = max(m1, __float_as_uint(a1) & 0x7fffffffu);
-    if (SUM) s0 += a0, s1 += a1;
+    const Pair x = pair_at(i);
+    if constexpr (sizeof(T) == 4) {
+      m0 = max(m0, __float_as_uint(x.x) & 0x7fffffffu);
+      m1 = max(m1, __float_as_uint(x.y) & 0x7fffffffu);
+    } else {
+      kept[i] = x;
+      both = __vmaxu2(both, x & 0x7fff7fffu);
+    }
+    if (SUM) {
+      const float2 v = values(x);
+      s0 += v.x, s1 += v.y;
+    }
+  }
+  if constexpr (sizeof(T) == 2) {
+    const float2 v = rows::unpack2<T>(both);
+    m0 = __float_as_uint(v.x), m1 = __float_as_uint(v.y);
   }
   tops[g][2 * p] = m0, tops[g][2 * p + 1] = m1;
   if (SUM) parts[g][2 * p] = s0, parts[g][2 * p + 1] = s1;
   __syncthreads();
+  const int64_t col = c0 + 2 * p;
+  int unit[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int c = 2 * p + j;
-    const int64_t col = c0 + c;
-    const int u = unit_of(max(max(tops[0][c], tops[1][c]), max(tops[2][c], tops[3][c])));
-    if (col >= a.C) continue;
-    const float inv = inverse_of(u);
-    int8_t* to = a.codes_t + col * a.pitch_t + r0 + 32 * g;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t w[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int r = 32 * g + 16 * h + 4 * k;
-        w[k] = code4(ld(&tile[r][c]) * inv, ld(&tile[r + 1][c]) * inv, ld(&tile[r + 2][c]) * inv, ld(&tile[r + 3][c]) * inv);
-      }
-      if (r0 + 32 * g + 16 * h < a.pitch_t) *reinterpret_cast<uint4*>(to + 16 * h) = make_uint4(w[0], w[1], w[2], w[3]);
+    unit[j] = unit_of(max(max(tops[0][c], tops[1][c]), max(tops[2][c], tops[3][c])));
+    if (g == 0 && col + j < a.C) {
+      a.exps_t[exp_at(col + j, tile_r, a.quads_t)] = (uint8_t)unit[j];
+      if (SUM) a.sums[(int64_t)tile_r * a.C + col + j] = (parts[0][c] + parts[1][c]) + (parts[2][c] + parts[3][c]);
     }
-    if (g == 0) {
-      a.exps_t[exp_at(col, tile_r, a.quads_t)] = (uint8_t)u;
-      if (SUM) a.sums[(int64_t)tile_r * a.C + col] = (parts[0][c] + parts[1][c]) + (parts[2][c] + parts[3][c]);
+  }
+  const float inv0 = inverse_of(unit[0]), inv1 = inverse_of(unit[1]);
+  uint32_t w0[8], w1[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    float2 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (sizeof(T) == 4) v[j] = pair_at(4 * k + j);
+      else v[j] = values(kept[4 * k + j]);
     }
+    w0[k] = code4(v[0].x * inv0, v[1].x * inv0, v[2].x * inv0, v[3].x * inv0);
+    w1[k] = code4(v[0].y * inv1, v[1].y * inv1, v[2].y * inv1, v[3].y * inv1);
+  }
+  // through shared memory, so that a column's 128 codes leave in one piece (16 bytes a thread to 32 columns: 1050 us for 16384 x 32000, so 390)
+  constexpr int kOut = kBlock + 16;
+  static_assert(kBlock * kOut <= kBlock * kPitch * (int)sizeof(T), "the codes take the elements' place");
+  __syncthreads();
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    *reinterpret_cast<uint4*>(dyn + (2 * p) * kOut + 32 * g + 16 * h) = make_uint4(w0[4 * h], w0[4 * h + 1], w0[4 * h + 2], w0[4 * h + 3]);
+    *reinterpret_cast<uint4*>(dyn + (2 * p + 1) * kOut + 32 * g + 16 * h) = make_uint4(w1[4 * h], w1[4 * h + 1], w1[4 * h + 2], w1[4 * h + 3]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = i * 32 + threadIdx.x / 8, at = threadIdx.x % 8 * 16;
+    if (c0 + c < a.C && r0 + at < a.pitch_t)
+      *reinterpret_cast<uint4*>(a.codes_t + (c0 + c) * a.pitch_t + r0 + at) = *reinterpret_cast<const uint4*>(dyn + c * kOut + at);
   }
 }
 

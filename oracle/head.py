@@ -84,7 +84,7 @@ def moment_codes(x, bits16, below, unsigned):
     c = torch.clamp((size + r * 16) >> 20, max=254 * 8 + 7) - (e - below) * 8
     c = torch.where(size == 0, 0, torch.clamp(c, min=1 if unsigned else 0))
     if not unsigned:
-        c = c + torch.where((raw >> 31 == 1) & (c > 0), 128, 0)
+        c = c + torch.where(raw >> 31 == 1, 128, 0)
     return c, e[:, 0]
 
 
