@@ -24,7 +24,6 @@ namespace {
 
 constexpr int kTokens = 128;      // a tile's rows of X
 constexpr int kStep = 128;        // of K a stage: one block
-constexpr int kStages = 4;
 constexpr int kChunk = 8;         // steps that one accumulator takes
 constexpr int kCols = 64;         // channels of an epilogue warp
 constexpr int kStaged = 4096;     // bytes a warp stages for a store: 32 tokens of 128 bytes
@@ -33,18 +32,20 @@ constexpr uint32_t kDrainLimit = 1u << 20;  // the same for what is still in fli
 
 template <int NC> constexpr int epilogue_warps() { return NC / 16; }  // 4 quarters of TMEM's lanes x NC / 64
 template <int NC> constexpr int threads() { return 64 + 32 * epilogue_warps<NC>(); }
-template <int NC> constexpr int stage_bytes() { return (kTokens + NC) * kStep; }
+// PAIR: two blocks of a cluster share a tile of 256 tokens, each with its own 128 and half of the channels' weight rows.
+template <bool PAIR, int NC> constexpr int weight_rows() { return PAIR ? NC / 2 : NC; }
+template <bool PAIR, int NC> constexpr int stage_bytes() { return (kTokens + weight_rows<PAIR, NC>()) * kStep; }
+template <bool PAIR> constexpr int stages() { return PAIR ? 5 : 4; }
 // ring | its powers of two | staged tiles | biases
 constexpr int kExpBytes = 3 * kTileBytes;  // a stage's: of the tokens, and of up to two groups of 128 channels
-template <int NC> constexpr int smem_bytes() {
-  return kStages * (stage_bytes<NC>() + kExpBytes) + epilogue_warps<NC>() * (kStaged + kCols * 4) + 1024;
+template <bool PAIR, int NC> constexpr int smem_bytes() {
+  return stages<PAIR>() * (stage_bytes<PAIR, NC>() + kExpBytes) + epilogue_warps<NC>() * (kStaged + kCols * 4) + 1024;
 }
-// Tensor memory: two accumulators, then kStages sets of powers of two (4 columns of the tokens', 8 of the channels')
-template <int NC> constexpr uint32_t tmem_cols() { return NC > 64 ? 512 : 256; }
+// Tensor memory: two accumulators, then a set of powers of two a stage (4 columns of the tokens', 8 of the channels')
 constexpr int kExpCols = 12;
+template <bool PAIR, int NC> constexpr uint32_t tmem_cols() { return 2 * NC + stages<PAIR>() * kExpCols > 256 ? 512 : 256; }
 
 struct Args {
-  const uint8_t *ex, *ew;
   const void* bias;    // null, or [N]
   int bias_dtype;
   void* out;           // [M, N]
@@ -63,27 +64,92 @@ struct Args {
 
 __device__ __forceinline__ bool step_wait(uint64_t* bar, uint32_t phase) { return mbar_try_wait(bar, phase) || mbar_wait(bar, phase, kWaitLimit); }
 
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes),
-               "r"(smem_u32(bar))
-               : "memory");
-}
-// 32 rows of 16 bytes to TMEM lanes 0 to 31, four columns, and the same to the other three quarters
-__device__ __forceinline__ void copy_exps(uint32_t tmem, const void* src) {
-  const uint64_t d = make_smem_desc(smem_u32(src), 16, 128, kSwizzleNone);
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(d) : "memory");
-}
+// One block, or a pair of them: the instructions that differ.
+template <bool PAIR> struct Blocks;
+template <> struct Blocks<false> {
+  static constexpr int kCount = 1;
+  static __device__ __forceinline__ void alloc(uint32_t* dst, uint32_t n) { tmem_alloc(dst, n); }
+  static __device__ __forceinline__ void relinquish() { tmem_relinquish(); }
+  static __device__ __forceinline__ void dealloc(uint32_t t, uint32_t n) { tmem_dealloc(t, n); }
+  static __device__ __forceinline__ void load(void* dst, const void* tmap, uint64_t* bar, int c0, int c1) { tma_load_2d(dst, tmap, bar, c0, c1); }
+  static __device__ __forceinline__ void copy_exps(uint32_t tmem, uint64_t d) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(d) : "memory");
+  }
+  static __device__ __forceinline__ void mma(uint32_t d, uint64_t da, uint64_t db, uint32_t desc, uint32_t ea, uint32_t eb, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(da), "l"(db), "r"(desc), "r"(ea), "r"(eb), "r"(accumulate)
+        : "memory");
+  }
+  static __device__ __forceinline__ void commit(uint64_t* bar) { umma_commit(bar); }
+  static __device__ __forceinline__ void arrive_all(uint64_t* bar) { mbar_arrive(bar); }
+  static __device__ __forceinline__ void arrive_first(uint64_t* bar) { mbar_arrive(bar); }
+  static __device__ __forceinline__ void meet() { __syncthreads(); }
+};
+template <> struct Blocks<true> {
+  static constexpr int kCount = 2;
+  static __device__ __forceinline__ void alloc(uint32_t* dst, uint32_t n) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(n) : "memory");
+  }
+  static __device__ __forceinline__ void relinquish() { asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory"); }
+  static __device__ __forceinline__ void dealloc(uint32_t t, uint32_t n) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(t), "r"(n) : "memory");
+  }
+  // this barrier in one of the pair's blocks
+  static __device__ __forceinline__ uint32_t in_block(uint64_t* bar, int block) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(bar)), "r"(block));
+    return r;
+  }
+  // into this block's shared memory; the bytes count at the first block's barrier
+  static __device__ __forceinline__ void load(void* dst, const void* tmap, uint64_t* bar, int c0, int c1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
+            smem_u32(dst)),
+        "l"(tmap), "r"(in_block(bar, 0)), "r"(c0), "r"(c1)
+        : "memory");
+  }
+  // issued by the first block for both: each block's powers of two to its own tensor memory, each block's tokens, the two halves of the channels
+  static __device__ __forceinline__ void copy_exps(uint32_t tmem, uint64_t d) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(d) : "memory");
+  }
+  static __device__ __forceinline__ void mma(uint32_t d, uint64_t da, uint64_t db, uint32_t desc, uint32_t ea, uint32_t eb, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(da), "l"(db), "r"(desc), "r"(ea), "r"(eb), "r"(accumulate)
+        : "memory");
+  }
+  // arrives at this barrier in both blocks
+  static __device__ __forceinline__ void commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+                 "h"((uint16_t)3)
+                 : "memory");
+  }
+  static __device__ __forceinline__ void arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  }
+  static __device__ __forceinline__ void arrive_all(uint64_t* bar) { arrive(in_block(bar, 0)), arrive(in_block(bar, 1)); }
+  static __device__ __forceinline__ void arrive_first(uint64_t* bar) { arrive(in_block(bar, 0)); }
+  static __device__ __forceinline__ void meet() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+};
+// 32 rows of 16 bytes, for TMEM lanes 0 to 31 and again for the other three quarters
+__device__ __forceinline__ uint64_t exps_desc(const void* src) { return make_smem_desc(smem_u32(src), 16, 128, kSwizzleNone); }
 // e4m3 operands, both K-major, float32 accumulators, powers of two as scales; which of the four bytes of a scale's word
-template <int NC> __device__ __forceinline__ uint32_t idesc(uint32_t byte) {
-  return (byte << 4) | ((uint32_t)(NC >> 3) << 17) | (1u << 23) | ((uint32_t)(kTokens >> 7) << 27) | (byte << 29);
+template <int M, int NC> __device__ __forceinline__ uint32_t idesc(uint32_t byte) {
+  return (byte << 4) | ((uint32_t)(NC >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 7) << 27) | (byte << 29);
 }
-__device__ __forceinline__ void umma_fp8(uint32_t d, uint64_t da, uint64_t db, uint32_t desc, uint32_t ea, uint32_t eb, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-      "l"(da), "l"(db), "r"(desc), "r"(ea), "r"(eb), "r"(accumulate)
-      : "memory");
+// true in one thread of the warp, the same each time
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
 }
 __device__ __forceinline__ void tma_store_2d(const void* tmap, const void* src, int c0, int c1, uint64_t policy) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group.L2::cache_hint [%0, {%2, %3}], [%1], %4;" ::"l"(tmap),
@@ -94,49 +160,53 @@ template <int NC> __device__ __forceinline__ void epilogue_barrier() {
   asm volatile("bar.sync 1, %0;" ::"n"(epilogue_warps<NC>() * 32) : "memory");
 }
 
-template <int NC, typename T>
+template <bool PAIR, int NC, typename T>
 __global__ void __launch_bounds__(threads<NC>(), 1)
-    fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_out,
-               const Args a) {
-  constexpr int S = kStages, EW = epilogue_warps<NC>();
+    fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_ex,
+               const __grid_constant__ CUtensorMap tm_ew, const __grid_constant__ CUtensorMap tm_out, const Args a) {
+  using B = Blocks<PAIR>;
+  constexpr int S = stages<PAIR>(), EW = epilogue_warps<NC>(), ROWS = weight_rows<PAIR, NC>(), kStage = stage_bytes<PAIR, NC>();
   constexpr uint32_t kExpTmem = 2 * NC;
   extern __shared__ uint8_t dyn[];
-  __shared__ __align__(8) uint64_t full[S], empty[S], acc_full[2], acc_empty[2], drain;
+  // other_done: in the first block, the second one's loader has issued its last load
+  __shared__ __align__(8) uint64_t full[S], empty[S], acc_full[2], acc_empty[2], drain, other_done;
   __shared__ uint32_t tmem_base, last_flag;
   uint8_t* const ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
-  uint8_t* const staged_all = ring + (size_t)S * stage_bytes<NC>();  // 1024-byte aligned: 128-byte swizzled tiles
+  uint8_t* const staged_all = ring + (size_t)S * kStage;  // 1024-byte aligned: 128-byte swizzled tiles
   uint8_t* const exps = staged_all + EW * kStaged;
   float* const bias_all = reinterpret_cast<float*>(exps + S * kExpBytes);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int rank = PAIR ? blockIdx.x & 1 : 0, worker = blockIdx.x / B::kCount, workers = gridDim.x / B::kCount;
 
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&tm_x);
     tma_prefetch_desc(&tm_w);
     for (int i = 0; i < S; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
-    for (int i = 0; i < 2; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], EW);
-    mbar_init(&drain, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], B::kCount * EW);
+    mbar_init(&drain, 1), mbar_init(&other_done, 1);
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc(&tmem_base, tmem_cols<NC>());
-    tmem_relinquish();
+    B::alloc(&tmem_base, tmem_cols<PAIR, NC>());
+    B::relinquish();
   }
   tc_fence_before();
-  __syncthreads();
+  __syncwarp();
+  B::meet();
   tc_fence_after();
   const uint32_t tmem = tmem_base;
 
   const int units = a.tiles * a.splits, m_tiles = a.tiles / a.n_tiles;
-  // a unit's tokens, channels and steps of K
+  // a unit's tokens (this block's), channels and steps of K
   auto place = [&](int u, int& m0, int& n0, int& k0, int& k1) {
     const int tile = u / a.splits, split = u - tile * a.splits;
     const int g = tile / (a.group * a.n_tiles), in = tile - g * a.group * a.n_tiles, rows = min(a.group, m_tiles - g * a.group);
-    m0 = (g * a.group + in % rows) * kTokens;
+    m0 = ((g * a.group + in % rows) * B::kCount + rank) * kTokens;
     n0 = in / rows * NC;
     k0 = (int)((int64_t)a.k_blocks * split / a.splits);
     k1 = (int)((int64_t)a.k_blocks * (split + 1) / a.splits);
   };
-  const int groups_x = (int)blocks_of(a.M), groups_w = (int)blocks_of(a.N);
+  const int groups_w = (int)blocks_of(a.N);
   // groups of 128 channels' powers of two that a tile reaches: one or two, from n0 / 128 on
   auto groups_of = [&](int n0) { return min((n0 + NC - 1) / kBlock, groups_w - 1) - n0 / kBlock + 1; };
 
@@ -144,97 +214,149 @@ __global__ void __launch_bounds__(threads<NC>(), 1)
     if (lane == 0) {
       bool ok = true;
       uint32_t it = 0, early = 0;
+      // the powers of two of four steps come with the first of them. Both blocks of a pair need those of all the tile's channels.
       auto load_w = [&](int s, int n0, int k, bool first) {
-        uint8_t* const st = ring + (size_t)s * stage_bytes<NC>();
-        tma_load_2d(st + kTokens * kStep, &tm_w, &full[s], k * kStep, n0);
+        B::load(ring + (size_t)s * kStage + kTokens * kStep, &tm_w, &full[s], k * kStep, n0 + rank * ROWS);
         if (first)
           for (int g = 0; g < groups_of(n0); ++g)
-            bulk_load(exps + s * kExpBytes + (1 + g) * kTileBytes, a.ew + ((int64_t)(n0 / kBlock + g) * a.quads + k / 4) * kTileBytes, kTileBytes, &full[s]);
+            B::load(exps + s * kExpBytes + (1 + g) * kTileBytes, &tm_ew, &full[s], 0, (n0 / kBlock + g) * a.quads + k / 4);
       };
-      // the powers of two of four steps come with the first of them
-      auto bytes = [&](int n0, bool first) { return (uint32_t)((a.a_rows + NC) * kStep + (first ? (1 + groups_of(n0)) * kTileBytes : 0)); };
+      // the first block expects both blocks' bytes (the other's may land before: the count goes below zero)
+      auto expect = [&](int s, int n0, bool first) {
+        if (rank == 0)
+          mbar_arrive_expect_tx(&full[s], B::kCount * (uint32_t)((a.a_rows + ROWS) * kStep + (first ? (1 + groups_of(n0)) * kTileBytes : 0)));
+      };
       // Where the kernel that this one may overlap is the one that makes X's codes, the weight was written before that
       // kernel started: a first ring of weight tiles is on its way before the wait.
-      for (int u = blockIdx.x; a.early && u < units && early < (uint32_t)S; u += gridDim.x) {
+      for (int u = worker; a.early && u < units && early < (uint32_t)S; u += workers) {
         int m0, n0, k0, k1;
         place(u, m0, n0, k0, k1);
         for (int k = k0; k < k1 && early < (uint32_t)S; ++k, ++early) {
           const bool first = k == k0 || k % 4 == 0;
-          mbar_arrive_expect_tx(&full[early], bytes(n0, first));
+          expect(early, n0, first);
           load_w(early, n0, k, first);
         }
       }
       wait_predecessor();
-      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+      int s = 0;
+      uint32_t phase = 0;
+      for (int u = worker; u < units && ok; u += workers) {
         int m0, n0, k0, k1;
         place(u, m0, n0, k0, k1);
         for (int k = k0; k < k1; ++k, ++it) {
-          const int s = it % S;
-          const bool first = k == k0 || k % 4 == 0;
+          const bool first = k == k0 || (k & 3) == 0;
           if (it >= early) {
-            if (it >= (uint32_t)S && !step_wait(&empty[s], ((it / S) & 1) ^ 1)) {
+            if (it >= (uint32_t)S && !step_wait(&empty[s], phase ^ 1)) {
               ok = false;
               break;
             }
-            mbar_arrive_expect_tx(&full[s], bytes(n0, first));
+            expect(s, n0, first);
             load_w(s, n0, k, first);
           }
-          tma_load_2d(ring + (size_t)s * stage_bytes<NC>(), &tm_x, &full[s], k * kStep, m0);
-          if (first) bulk_load(exps + s * kExpBytes, a.ex + ((int64_t)(m0 / kBlock) * a.quads + k / 4) * kTileBytes, kTileBytes, &full[s]);
+          B::load(ring + (size_t)s * kStage, &tm_x, &full[s], k * kStep, m0);
+          if (first) B::load(exps + s * kExpBytes, &tm_ex, &full[s], 0, m0 / kBlock * a.quads + k / 4);
+          s = s + 1 == S ? 0 : s + 1;
+          phase ^= s == 0;
         }
       }
-      for (uint32_t i = it > (uint32_t)S ? it - S : 0; i < it; ++i)
-        if (!mbar_wait(&full[i % S], (i / S) & 1, kDrainLimit)) ok = false;
+      const uint32_t last = it > (uint32_t)S ? it - S : 0;
+      const bool complete = ok;
+      if (rank == 0) {
+        // both blocks' copies count here: the other block waits for this one at the end
+        uint32_t landed = 0;  // of the ring's stages
+        for (uint32_t i = last; i < it; ++i) {
+          if (mbar_wait(&full[i % S], (i / S) & 1, kDrainLimit)) landed |= 1u << (i % S);
+          else ok = false;
+        }
+        if (PAIR && !complete && mbar_wait(&other_done, 0, kDrainLimit)) {
+          // The other block's wait may have seen what this one's gave up on: its copies for up to a ring of further steps come down on
+          // barriers where nothing expects them yet. (It issued none where the last one there has not landed.) Where powers of two are among
+          // them the bytes do not add up, and the wait runs out, long after they are down; so it does where it issued none.
+          for (uint32_t i = it; i < it + S; ++i) {
+            if (!(landed >> (i % S) & 1)) continue;
+            mbar_arrive_expect_tx(&full[i % S], (uint32_t)((a.a_rows + ROWS) * kStep));
+            mbar_wait(&full[i % S], (i / S) & 1, kDrainLimit >> 6);
+          }
+        }
+      } else {
+        B::arrive_first(&other_done);
+      }
+      if (PAIR) {
+        // the first block's arrivals at this block's barriers are all in before the block ends
+        if (complete)
+          for (uint32_t i = last; i < it; ++i)
+            if (!step_wait(&empty[i % S], (i / S) & 1)) ok = false;
+        if (rank == 1 && !mbar_wait(&drain, 0, kDrainLimit)) ok = false;
+      }
       if (!ok) atomicExch(a.error, 1u);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (rank == 0) {
+      // The whole warp goes through the loop and one thread of it issues, so that the operands are known to be uniform; nothing is divided, and
+      // stages are counted: one thread alone, with remainders, took 820 cycles a step where the MMAs take 384.
       // A set of powers of two is written again after S others, so S steps at least: the step that does it has waited for
       // a stage whose copies began when all MMAs up to S steps before, its readers among them, were done.
-      uint32_t it = 0, local = 0, set = 0;
-      bool ok = true;
+      const bool issues = elect_one();
+      uint32_t s = 0, phase = 0, set = 0, b = 0, acc_phase = 0, started = 0;  // started: accumulators, up to two
+      bool ok = true, any = false;
+      const uint64_t da0 = make_smem_desc(smem_u32(ring), 16, 1024, kSwizzle128B), db0 = make_smem_desc(smem_u32(ring + kTokens * kStep), 16, 1024, kSwizzle128B);
+      const uint64_t de0 = exps_desc(exps);
       wait_predecessor();
-      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+      for (int u = worker; u < units && ok; u += workers) {
         int m0, n0, k0, k1;
         place(u, m0, n0, k0, k1);
+        const int groups = groups_of(n0);
+        const uint32_t skip = 4 + n0 % kBlock / 32;
         uint32_t at = 0;
-        for (int k = k0; k < k1; ++k, ++it) {
-          const int s = it % S;
-          const uint32_t b = local & 1;
-          const bool opens = (k - k0) % kChunk == 0;
-          if (opens) {
-            if (local >= 2 && !step_wait(&acc_empty[b], ((local >> 1) & 1) ^ 1)) {
-              ok = false;
-              break;
-            }
+        int chunk = 0;  // steps of the accumulator so far
+        for (int k = k0; k < k1; ++k) {
+          if (chunk == 0 && started >= 2 && !step_wait(&acc_empty[b], acc_phase)) {
+            ok = false;
+            break;
           }
-          if (!step_wait(&full[s], (it / S) & 1)) {
+          if (!step_wait(&full[s], phase)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          if (k == k0 || k % 4 == 0) {
-            at = tmem + kExpTmem + set % S * kExpCols;
-            ++set;
-            copy_exps(at, exps + s * kExpBytes);
-            for (int g = 0; g < groups_of(n0); ++g) copy_exps(at + 4 + 4 * g, exps + s * kExpBytes + (1 + g) * kTileBytes);
+          const uint32_t byte = k & 3, desc = idesc<B::kCount * kTokens, NC>(0) | byte << 4 | byte << 29;
+          const bool copies = k == k0 || byte == 0;
+          if (copies) {
+            at = tmem + kExpTmem + set * kExpCols;
+            set = set + 1 == (uint32_t)S ? 0 : set + 1;
           }
-          const uint32_t from = smem_u32(ring + (size_t)s * stage_bytes<NC>());
-          uint64_t da = make_smem_desc(from, 16, 1024, kSwizzle128B), db = make_smem_desc(from + kTokens * kStep, 16, 1024, kSwizzle128B);
-          const uint32_t desc = idesc<NC>(k & 3), eb = at + 4 + n0 % kBlock / 32;
+          const bool closes = chunk == kChunk - 1 || k == k1 - 1;
+          if (issues) {
+            if (copies) {
+              const uint64_t de = de0 + s * (kExpBytes >> 4);
+              B::copy_exps(at, de);
+              B::copy_exps(at + 4, de + (kTileBytes >> 4));
+              if (groups > 1) B::copy_exps(at + 8, de + 2 * (kTileBytes >> 4));
+            }
+            const uint64_t da = da0 + s * (kStage >> 4), db = db0 + s * (kStage >> 4);
 #pragma unroll
-          for (int i = 0; i < kStep / 32; ++i, da += 2, db += 2) umma_fp8(tmem + b * NC, da, db, desc, at, eb, (!opens || i > 0) ? 1u : 0u);
-          umma_commit(&empty[s]);
-          if ((k - k0) % kChunk == kChunk - 1 || k == k1 - 1) {
-            umma_commit(&acc_full[b]);
-            ++local;
+            for (int i = 0; i < kStep / 32; ++i) B::mma(tmem + b * NC, da + 2 * i, db + 2 * i, desc, at, at + skip, (chunk > 0 || i > 0) ? 1u : 0u);
+            B::commit(&empty[s]);
+            if (closes) B::commit(&acc_full[b]);
+          }
+          any = true;
+          s = s + 1 == (uint32_t)S ? 0 : s + 1;
+          phase ^= s == 0;
+          ++chunk;
+          if (closes) {
+            chunk = 0, b ^= 1;
+            if (started < 2) ++started;
+            else acc_phase ^= b == 0;
           }
         }
       }
-      if (it > 0) umma_commit(&drain);
-      else mbar_arrive(&drain);
+      __syncwarp();
+      if (issues) {
+        if (any) B::commit(&drain);
+        else B::arrive_all(&drain);
+      }
       if (!mbar_wait(&drain, 0, kDrainLimit)) ok = false;
-      if (!ok) atomicExch(a.error, 1u);
+      if (!ok && lane == 0) atomicExch(a.error, 1u);
     }
   } else {
     const int q = warp & 3, part = (warp - 2) / 4;  // this warp's 32 tokens and 64 channels
@@ -246,7 +368,7 @@ __global__ void __launch_bounds__(threads<NC>(), 1)
     if (a.stream_out) asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
     else asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
     wait_predecessor();
-    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+    for (int u = worker; u < units; u += workers) {
       int m0, n0, k0, k1;
       place(u, m0, n0, k0, k1);
       m0 += q * 32, n0 += part * kCols;
@@ -282,7 +404,7 @@ __global__ void __launch_bounds__(threads<NC>(), 1)
         tmem_wait_ld();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[b]);
+        if (lane == 0) B::arrive_first(&acc_empty[b]);
 #pragma unroll
         for (int j = 0; j < 32; ++j) sum[32 + j] = k == k0 ? __uint_as_float(v[j]) : sum[32 + j] + __uint_as_float(v[j]);
       }
@@ -358,15 +480,17 @@ __global__ void __launch_bounds__(threads<NC>(), 1)
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   tc_fence_before();
-  __syncthreads();
+  __syncwarp();
+  B::meet();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, tmem_cols<NC>());
+    B::dealloc(tmem, tmem_cols<PAIR, NC>());
   }
 }
 
 struct Shape {
   int width, n_tiles, tiles, splits;
+  bool pair;
 };
 // The tile's channels and parts of K whose rounds over the SMs cost least: a step the rows that it loads, a unit its start and
 // epilogue, a part its way through memory and back.
@@ -379,9 +503,10 @@ Shape shape_of(int64_t M, int64_t N, int64_t K) {
     for (int64_t splits = 1; splits <= std::min<int64_t>(blocks, std::max<int64_t>(1, sms / tiles)); ++splits) {
       const int64_t rounds = (tiles * splits + sms - 1) / sms, steps = (blocks + splits - 1) / splits;
       const double cost = rounds * (steps * (double)(std::min<int64_t>(M, kTokens) + nc) + 600.0) + (splits > 1 ? 400.0 + splits * (double)nc : 0.0);
-      if (cost < least) least = cost, best = Shape{nc, (int)n_tiles, (int)tiles, (int)splits};
+      if (cost < least) least = cost, best = Shape{nc, (int)n_tiles, (int)tiles, (int)splits, false};
     }
   }
+  if (getenv("FLBP") && atoi(getenv("FLBP")) == 1 && sms % 2 == 0) best = Shape{192, (int)((N + 191) / 192), (int)((M + 255) / 256 * ((N + 191) / 192)), 1, true};
   return best;
 }
 
@@ -404,35 +529,53 @@ Ws ws_of(const Shape& g, int64_t M, int64_t K, bool quantise) {
   return w;
 }
 
-template <int NC, typename T>
-int launch_t(const CUtensorMap& tx, const CUtensorMap& tw, const CUtensorMap& to, const Args& a, bool overlap, cudaStream_t s) {
-  const int st = ensure_dyn_smem(reinterpret_cast<const void*>(fp8_kernel<NC, T>), smem_bytes<NC>(), "fp8_linear shared memory");
+struct Maps {
+  CUtensorMap x, w, ex, ew, out;
+};
+
+template <bool PAIR, int NC, typename T> int launch_t(const Maps& m, const Args& a, bool overlap, cudaStream_t s) {
+  const auto kernel = fp8_kernel<PAIR, NC, T>;
+  constexpr int kBlocks = PAIR ? 2 : 1;
+  const int st = ensure_dyn_smem(reinterpret_cast<const void*>(kernel), smem_bytes<PAIR, NC>(), "fp8_linear shared memory");
   if (st != FLB_OK) return st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)std::min<int64_t>((int64_t)a.tiles * a.splits, num_sms()));
+  cfg.gridDim = dim3((unsigned)std::min<int64_t>((int64_t)a.tiles * a.splits * kBlocks, num_sms() / kBlocks * kBlocks));
   cfg.blockDim = dim3(threads<NC>());
-  cfg.dynamicSmemBytes = smem_bytes<NC>();
+  cfg.dynamicSmemBytes = smem_bytes<PAIR, NC>();
   cfg.stream = s;
   cfg.attrs = attr;
   if (overlap) {
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.numAttrs = 1;
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
   }
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, fp8_kernel<NC, T>, tx, tw, to, a);
+  if (PAIR) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = 2;
+    attr[cfg.numAttrs].val.clusterDim.y = 1;
+    attr[cfg.numAttrs++].val.clusterDim.z = 1;
+  }
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, m.x, m.w, m.ex, m.ew, m.out, a);
   count_launches(1);
   return check_cuda(e, "fp8_linear launch");
 }
 
-template <typename T> int launch(int width, const CUtensorMap& tx, const CUtensorMap& tw, const CUtensorMap& to, const Args& a, bool overlap, cudaStream_t s) {
-  switch (width) {
-    case 64: return launch_t<64, T>(tx, tw, to, a, overlap, s);
-    case 128: return launch_t<128, T>(tx, tw, to, a, overlap, s);
-    default: return launch_t<192, T>(tx, tw, to, a, overlap, s);
+template <typename T> int launch(const Shape& g, const Maps& m, const Args& a, bool overlap, cudaStream_t s) {
+  if (g.pair) return launch_t<true, 192, T>(m, a, overlap, s);
+  switch (g.width) {
+    case 64: return launch_t<false, 64, T>(m, a, overlap, s);
+    case 128: return launch_t<false, 128, T>(m, a, overlap, s);
+    default: return launch_t<false, 192, T>(m, a, overlap, s);
   }
 }
 
+// Powers of two as rows of 128 words: 128 rows' of four blocks
+int exps_map(CUtensorMap* m, const uint8_t* exps, int64_t R, int64_t K) {
+  const uint64_t dims[2] = {kTileBytes / 4, (uint64_t)(exps_bytes(R, K) / kTileBytes)};
+  const uint64_t strides[1] = {kTileBytes};
+  const uint32_t box[2] = {kTileBytes / 4, 1};
+  return make_tmap(m, exps, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
 int code_map(CUtensorMap* m, const int8_t* codes, int64_t rows, int64_t ld, int64_t K, int box_rows) {
   const uint64_t dims[2] = {(uint64_t)K, (uint64_t)rows};
   const uint64_t strides[1] = {(uint64_t)ld};
@@ -470,9 +613,10 @@ int fp8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, c
   }
   Args a = {};
   a.a_rows = (int)std::min<int64_t>(kTokens, (M + 7) / 8 * 8);
-  CUtensorMap tw, tx, to = {};
-  if ((st = code_map(&tw, w_codes, N, ldw, K, g.width)) != FLB_OK) return st;
-  if ((st = code_map(&tx, x_codes, M, ldc, K, a.a_rows)) != FLB_OK) return st;
+  Maps m = {};
+  if ((st = code_map(&m.w, w_codes, N, ldw, K, g.pair ? g.width / 2 : g.width)) != FLB_OK) return st;
+  if ((st = code_map(&m.x, x_codes, M, ldc, K, a.a_rows)) != FLB_OK) return st;
+  if ((st = exps_map(&m.ex, x_exps, M, K)) != FLB_OK || (st = exps_map(&m.ew, w_exps, N, K)) != FLB_OK) return st;
   const int es = dtype_size(dtype);
   a.tma_store = N * es % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
   if (a.tma_store) {
@@ -481,18 +625,18 @@ int fp8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, c
     const uint32_t box[2] = {(uint32_t)(128 / es), 32};
     const CUtensorMapDataType dt = dtype == FLB_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dtype == FLB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                                                                          : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    if ((st = make_tmap(&to, out, dt, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) != FLB_OK) return st;
+    if ((st = make_tmap(&m.out, out, dt, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) != FLB_OK) return st;
   }
-  a.ex = x_exps, a.ew = w_exps, a.bias = bias, a.bias_dtype = bias_dtype, a.out = out, a.M = M, a.N = N;
+  a.bias = bias, a.bias_dtype = bias_dtype, a.out = out, a.M = M, a.N = N;
   a.early = x != nullptr;
   a.k_blocks = (int)blocks_of(K), a.quads = (int)quads_of(K), a.n_tiles = g.n_tiles, a.tiles = g.tiles, a.splits = g.splits;
   a.group = N * K <= kWeightInL2 ? 1 : 16;
   a.stream_out = (size_t)M * N * es > kOutputInL2;
   a.parts = reinterpret_cast<float*>(p + l.parts), a.counts = reinterpret_cast<uint32_t*>(p + l.counts), a.error = reinterpret_cast<uint32_t*>(p);
   switch (dtype) {
-    case FLB_F32: st = launch<float>(g.width, tx, tw, to, a, x != nullptr, s); break;
-    case FLB_F16: st = launch<__half>(g.width, tx, tw, to, a, x != nullptr, s); break;
-    default: st = launch<__nv_bfloat16>(g.width, tx, tw, to, a, x != nullptr, s); break;
+    case FLB_F32: st = launch<float>(g, m, a, x != nullptr, s); break;
+    case FLB_F16: st = launch<__half>(g, m, a, x != nullptr, s); break;
+    default: st = launch<__nv_bfloat16>(g, m, a, x != nullptr, s); break;
   }
   if (st != FLB_OK || !check_timeout) return st;
   uint32_t err = 0;
