@@ -7,9 +7,15 @@
 // K range. Warp 0 loads by TMA into a ring of four steps of 128 of K, warp 1 issues the MMAs, the others read TMEM:
 // each has 32 tokens, a lane a token, and 64 channels, in registers.
 //
+// For many tiles two blocks of a cluster share one of 256 tokens (cta_group::2) and load a third less for it.
+//
 // The tensor core cuts, and does not round, what it adds to an accumulator: over 16384 of K sums came out 6.5e-6 of
 // their size too small. So an accumulator takes 1024 of K, and the warps add up those sums in float32, rounded.
 // Two accumulators: one is read while the other is filled.
+//
+// Measured: 8192 x 8192 x 8192 in 406 us, 2.71 PFLOP/s, 1.65 times the bf16 product's measured rate: bound by what L2 gives the SMs;
+// 16384 x 768 x 32000 in 463, of which 160 would write the output alone; 1 x 768 x 32000 in 8.8 us with the weight in L2, 3.8 us of
+// it the weight's bytes from memory: a chain of latencies and a second round of tiles.
 #include <cmath>
 #include "fp8.cuh"
 #include "sm100.cuh"
@@ -211,85 +217,94 @@ __global__ void __launch_bounds__(threads<NC>(), 1)
   auto groups_of = [&](int n0) { return min((n0 + NC - 1) / kBlock, groups_w - 1) - n0 / kBlock + 1; };
 
   if (warp == 0) {
-    if (lane == 0) {
-      bool ok = true;
-      uint32_t it = 0, early = 0;
-      // the powers of two of four steps come with the first of them. Both blocks of a pair need those of all the tile's channels.
-      auto load_w = [&](int s, int n0, int k, bool first) {
-        B::load(ring + (size_t)s * kStage + kTokens * kStep, &tm_w, &full[s], k * kStep, n0 + rank * ROWS);
-        if (first)
-          for (int g = 0; g < groups_of(n0); ++g)
-            B::load(exps + s * kExpBytes + (1 + g) * kTileBytes, &tm_ew, &full[s], 0, (n0 / kBlock + g) * a.quads + k / 4);
-      };
-      // the first block expects both blocks' bytes (the other's may land before: the count goes below zero)
-      auto expect = [&](int s, int n0, bool first) {
-        if (rank == 0)
-          mbar_arrive_expect_tx(&full[s], B::kCount * (uint32_t)((a.a_rows + ROWS) * kStep + (first ? (1 + groups_of(n0)) * kTileBytes : 0)));
-      };
-      // Where the kernel that this one may overlap is the one that makes X's codes, the weight was written before that
-      // kernel started: a first ring of weight tiles is on its way before the wait.
-      for (int u = worker; a.early && u < units && early < (uint32_t)S; u += workers) {
-        int m0, n0, k0, k1;
-        place(u, m0, n0, k0, k1);
-        for (int k = k0; k < k1 && early < (uint32_t)S; ++k, ++early) {
-          const bool first = k == k0 || k % 4 == 0;
-          expect(early, n0, first);
-          load_w(early, n0, k, first);
+    // as below, the whole warp goes through the loop and one thread issues
+    const bool issues = elect_one();
+    bool ok = true;
+    uint32_t it = 0, early = 0;
+    // the powers of two of four steps come with the first of them. Both blocks of a pair need those of all the tile's channels.
+    auto load_w = [&](int s, int n0, int groups, int k, bool first) {
+      B::load(ring + s * kStage + kTokens * kStep, &tm_w, &full[s], k * kStep, n0 + rank * ROWS);
+      if (first) {
+        const int row = n0 / kBlock * a.quads + k / 4;
+        B::load(exps + s * kExpBytes + kTileBytes, &tm_ew, &full[s], 0, row);
+        if (groups > 1) B::load(exps + s * kExpBytes + 2 * kTileBytes, &tm_ew, &full[s], 0, row + a.quads);
+      }
+    };
+    // the first block expects both blocks' bytes (the other's may land before: the count goes below zero)
+    const uint32_t codes_bytes = (uint32_t)((a.a_rows + ROWS) * kStep);
+    auto expect = [&](int s, int groups, bool first) {
+      if (rank == 0) mbar_arrive_expect_tx(&full[s], B::kCount * (codes_bytes + (first ? (1 + groups) * kTileBytes : 0)));
+    };
+    // Where the kernel that this one may overlap is the one that makes X's codes, the weight was written before that
+    // kernel started: a first ring of weight tiles is on its way before the wait.
+    for (int u = worker; a.early && u < units && early < (uint32_t)S; u += workers) {
+      int m0, n0, k0, k1;
+      place(u, m0, n0, k0, k1);
+      const int groups = groups_of(n0);
+      for (int k = k0; k < k1 && early < (uint32_t)S; ++k, ++early) {
+        const bool first = k == k0 || (k & 3) == 0;
+        if (issues) {
+          expect(early, groups, first);
+          load_w(early, n0, groups, k, first);
         }
       }
-      wait_predecessor();
-      int s = 0;
-      uint32_t phase = 0;
-      for (int u = worker; u < units && ok; u += workers) {
-        int m0, n0, k0, k1;
-        place(u, m0, n0, k0, k1);
-        for (int k = k0; k < k1; ++k, ++it) {
-          const bool first = k == k0 || (k & 3) == 0;
-          if (it >= early) {
-            if (it >= (uint32_t)S && !step_wait(&empty[s], phase ^ 1)) {
-              ok = false;
-              break;
-            }
-            expect(s, n0, first);
-            load_w(s, n0, k, first);
-          }
-          B::load(ring + (size_t)s * kStage, &tm_x, &full[s], k * kStep, m0);
-          if (first) B::load(exps + s * kExpBytes, &tm_ex, &full[s], 0, m0 / kBlock * a.quads + k / 4);
-          s = s + 1 == S ? 0 : s + 1;
-          phase ^= s == 0;
-        }
-      }
-      const uint32_t last = it > (uint32_t)S ? it - S : 0;
-      const bool complete = ok;
-      if (rank == 0) {
-        // both blocks' copies count here: the other block waits for this one at the end
-        uint32_t landed = 0;  // of the ring's stages
-        for (uint32_t i = last; i < it; ++i) {
-          if (mbar_wait(&full[i % S], (i / S) & 1, kDrainLimit)) landed |= 1u << (i % S);
-          else ok = false;
-        }
-        if (PAIR && !complete && mbar_wait(&other_done, 0, kDrainLimit)) {
-          // The other block's wait may have seen what this one's gave up on: its copies for up to a ring of further steps come down on
-          // barriers where nothing expects them yet. (It issued none where the last one there has not landed.) Where powers of two are among
-          // them the bytes do not add up, and the wait runs out, long after they are down; so it does where it issued none.
-          for (uint32_t i = it; i < it + S; ++i) {
-            if (!(landed >> (i % S) & 1)) continue;
-            mbar_arrive_expect_tx(&full[i % S], (uint32_t)((a.a_rows + ROWS) * kStep));
-            mbar_wait(&full[i % S], (i / S) & 1, kDrainLimit >> 6);
-          }
-        }
-      } else {
-        B::arrive_first(&other_done);
-      }
-      if (PAIR) {
-        // the first block's arrivals at this block's barriers are all in before the block ends
-        if (complete)
-          for (uint32_t i = last; i < it; ++i)
-            if (!step_wait(&empty[i % S], (i / S) & 1)) ok = false;
-        if (rank == 1 && !mbar_wait(&drain, 0, kDrainLimit)) ok = false;
-      }
-      if (!ok) atomicExch(a.error, 1u);
     }
+    wait_predecessor();
+    int s = 0;
+    uint32_t phase = 0;
+    for (int u = worker; u < units && ok; u += workers) {
+      int m0, n0, k0, k1;
+      place(u, m0, n0, k0, k1);
+      const int groups = groups_of(n0), row_x = m0 / kBlock * a.quads;
+      for (int k = k0; k < k1; ++k, ++it) {
+        const bool first = k == k0 || (k & 3) == 0, whole = it >= early;
+        if (it >= (uint32_t)S && !step_wait(&empty[s], phase ^ 1)) {
+          ok = false;
+          break;
+        }
+        if (issues) {
+          if (whole) {
+            expect(s, groups, first);
+            load_w(s, n0, groups, k, first);
+          }
+          B::load(ring + s * kStage, &tm_x, &full[s], k * kStep, m0);
+          if (first) B::load(exps + s * kExpBytes, &tm_ex, &full[s], 0, row_x + k / 4);
+        }
+        s = s + 1 == S ? 0 : s + 1;
+        phase ^= s == 0;
+      }
+    }
+    __syncwarp();
+    const uint32_t last = it > (uint32_t)S ? it - S : 0;
+    const bool complete = ok;
+    if (rank == 0) {
+      // both blocks' copies count here: the other block waits for this one at the end
+      uint32_t landed = 0;  // of the ring's stages
+      for (uint32_t i = last; i < it; ++i) {
+        if (mbar_wait(&full[i % S], (i / S) & 1, kDrainLimit)) landed |= 1u << (i % S);
+        else ok = false;
+      }
+      if (PAIR && !complete && mbar_wait(&other_done, 0, kDrainLimit)) {
+        // The other block's wait may have seen what this one's gave up on: its copies for up to a ring of further steps come down on
+        // barriers where nothing expects them yet. (It issued none where the last one there has not landed.) Where powers of two are among
+        // them the bytes do not add up, and the wait runs out, long after they are down; so it does where it issued none.
+        for (uint32_t i = it; i < it + S; ++i) {
+          if (!(landed >> (i % S) & 1)) continue;
+          if (issues) mbar_arrive_expect_tx(&full[i % S], codes_bytes);
+          mbar_wait(&full[i % S], (i / S) & 1, kDrainLimit >> 6);
+        }
+      }
+    } else if (issues) {
+      B::arrive_first(&other_done);
+    }
+    if (PAIR) {
+      // the first block's arrivals at this block's barriers are all in before the block ends
+      if (complete)
+        for (uint32_t i = last; i < it; ++i)
+          if (!step_wait(&empty[i % S], (i / S) & 1)) ok = false;
+      if (rank == 1 && !mbar_wait(&drain, 0, kDrainLimit)) ok = false;
+    }
+    if (!ok && lane == 0) atomicExch(a.error, 1u);
   } else if (warp == 1) {
     if (rank == 0) {
       // The whole warp goes through the loop and one thread of it issues, so that the operands are known to be uniform; nothing is divided, and
@@ -492,21 +507,31 @@ struct Shape {
   int width, n_tiles, tiles, splits;
   bool pair;
 };
-// The tile's channels and parts of K whose rounds over the SMs cost least: a step the rows that it loads, a unit its start and
-// epilogue, a part its way through memory and back.
+// The tile's channels, parts of K and blocks a tile whose rounds over the SMs cost least. In units of which about 850 take a microsecond: a step 100 and
+// 0.8 for each row that it loads, a unit 600 for its start and epilogue; parts 1200 for their meeting and what they
+// write and the last one adds up; a pair's start 1000. What decides (us, the product alone, operands from memory): 1 x 768 x 32000 with 128
+// channels 11.5, 192 12.7, 64 14.3; 16 x 4096 x 4096 with 64 in two parts 12.7, whole 14.0; 500 x 8000 x 500 with 64 in four parts 13.4, 128 in
+// eight 15.5; 1003 x 769 x 517 with 64 whole 7.7, in two parts 9.7; 768 x 16384 x 768 with 128 in four parts 22.2, 192 in four 24.6; 300 x 4096 x
+// 4096 with 128 16.5, 192 in two parts 17.8; 2931 x 1001 x 2304 by pairs 14.0, by one block 15.2; 2931 x 768 x 2304 11.9 and 11.2;
+// 8192 x 4096 x 4096 by pairs 110, by one block 134.
 Shape shape_of(int64_t M, int64_t N, int64_t K) {
-  const int64_t sms = num_sms(), m_tiles = (M + kTokens - 1) / kTokens, blocks = blocks_of(K);
+  const int64_t sms = num_sms(), m_tiles = (M + kTokens - 1) / kTokens, blocks = blocks_of(K), rows = std::min<int64_t>(M, kTokens);
   Shape best = {};
   double least = INFINITY;
   for (int nc : {192, 128, 64}) {
     const int64_t n_tiles = (N + nc - 1) / nc, tiles = m_tiles * n_tiles;
     for (int64_t splits = 1; splits <= std::min<int64_t>(blocks, std::max<int64_t>(1, sms / tiles)); ++splits) {
       const int64_t rounds = (tiles * splits + sms - 1) / sms, steps = (blocks + splits - 1) / splits;
-      const double cost = rounds * (steps * (double)(std::min<int64_t>(M, kTokens) + nc) + 600.0) + (splits > 1 ? 400.0 + splits * (double)nc : 0.0);
+      double cost = rounds * (steps * (100 + 0.8 * (rows + nc)) + 600);
+      if (splits > 1) cost += 1200 + nc * ((rows + 31) / 32 / 4.0) * (16 + 5 * splits);
       if (cost < least) least = cost, best = Shape{nc, (int)n_tiles, (int)tiles, (int)splits, false};
     }
   }
-  if (getenv("FLBP") && atoi(getenv("FLBP")) == 1 && sms % 2 == 0) best = Shape{192, (int)((N + 191) / 192), (int)((M + 255) / 256 * ((N + 191) / 192)), 1, true};
+  if (sms % 2 == 0) {
+    const int64_t n_tiles = (N + 191) / 192, tiles = (M + 255) / 256 * n_tiles;
+    const double cost = (tiles + sms / 2 - 1) / (sms / 2) * (blocks * (100 + 0.8 * 224) + 600) + 1000;
+    if (cost < least) best = Shape{192, (int)n_tiles, (int)tiles, 1, true};
+  }
   return best;
 }
 
