@@ -11,7 +11,7 @@ int fp8_rows2(const void* x, int64_t ldx, int8_t* codes, uint8_t* exps, int8_t* 
 size_t fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, bool quantise);
 int fp8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, const uint8_t* x_exps, const int8_t* w_codes, int64_t ldw,
                const uint8_t* w_exps, const void* bias, int bias_dtype, void* out, int64_t M, int64_t N, int64_t K, int dtype, void* ws,
-               int check_timeout, cudaStream_t s);
+               int check_timeout, int drop, uint32_t limit, cudaStream_t s);
 int sample(const void* logits, int64_t ld, const void* u, bool u64, int64_t* token, int64_t rows, int64_t V, int dtype, const float* temperature,
            const int64_t* top_k, const float* top_p, const float* min_p, double temperature1, int64_t top_k1, double top_p1, double min_p1,
            cudaStream_t s);
@@ -48,6 +48,37 @@ int check_tensors(const char* what, const flb_adamw_tensor* t, int64_t count, si
       return fail(FLB_ERR_ALIGN, at + ": pointers must be aligned to their element size, codes to 4 bytes");
   }
   return FLB_OK;
+}
+
+int fp8_linear_checked(const void* x, int64_t ldx, const void* x_codes, int64_t ldc, const uint8_t* x_exps, const void* w_codes, int64_t ldw,
+                       const uint8_t* w_exps, const void* bias, int bias_dtype, void* out, int64_t M, int64_t N, int64_t K, int dtype,
+                       void* workspace, size_t workspace_bytes, int check_timeout, int drop, uint32_t limit, void* stream) {
+  const size_t es = (size_t)dtype_size(dtype);
+  if (es == 0 || (bias && dtype_size(bias_dtype) == 0)) return fail(FLB_ERR_DTYPE, "fp8_linear: dtype must be f32, f16 or bf16");
+  int st = check_codes("fp8_linear", M, K);
+  if (st == FLB_OK) st = check_codes("fp8_linear", N, K);
+  if (st != FLB_OK) return st;
+  if (M > 0 && N > ((int64_t)1 << 42) / M) return fail(FLB_ERR_SHAPE, "fp8_linear: too many outputs");
+  if (M == 0 || N == 0) return FLB_OK;
+  if (!x == !x_codes || !x_codes != !x_exps) return fail(FLB_ERR_SHAPE, "fp8_linear: either x, or x_codes and x_exps");
+  if (!w_codes || !w_exps || !out) return fail(FLB_ERR_SHAPE, "fp8_linear: null weight or out");
+  if (x ? ldx < 0 : ldc < K) return fail(FLB_ERR_SHAPE, "fp8_linear: bad row pitch of x");
+  if (ldw < K) return fail(FLB_ERR_SHAPE, "fp8_linear: bad row pitch of the weight");
+  if (off(w_codes, 16) || off(w_exps, 16) || ldw % 16 || (x_codes && (off(x_codes, 16) || off(x_exps, 16) || ldc % 16)))
+    return fail(FLB_ERR_ALIGN, "fp8_linear: codes must start every row on 16 bytes, and exps lie on 16");
+  if (off(x, es) || off(out, es) || off(bias, bias ? (size_t)dtype_size(bias_dtype) : 1))
+    return fail(FLB_ERR_ALIGN, "fp8_linear: pointers must be aligned to their element size");
+  if (!workspace || workspace_bytes < fp8_linear_workspace_bytes(M, N, K, x != nullptr))
+    return fail(FLB_ERR_WORKSPACE, "fp8_linear: workspace smaller than flb_fp8_linear_workspace_bytes()");
+  if (off(workspace, 256)) return fail(FLB_ERR_ALIGN, "fp8_linear: workspace must be 256-byte aligned");
+  if (check_timeout) {
+    cudaStreamCaptureStatus capture;
+    if ((st = check_cuda(cudaStreamIsCapturing(as_stream(stream), &capture), "fp8_linear capture status")) != FLB_OK) return st;
+    if (capture != cudaStreamCaptureStatusNone)
+      return fail(FLB_ERR_UNSUPPORTED, "fp8_linear: check_timeout waits for the product, which a stream capture does not allow");
+  }
+  return fp8_linear(x, ldx, static_cast<const int8_t*>(x_codes), ldc, x_exps, static_cast<const int8_t*>(w_codes), ldw, w_exps, bias, bias_dtype, out, M,
+                    N, K, dtype, workspace, check_timeout, drop, limit, as_stream(stream));
 }
 
 }  // namespace
@@ -97,32 +128,17 @@ size_t flb_fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int x_is_
 int flb_fp8_linear(const void* x, int64_t ldx, const void* x_codes, int64_t ldc, const uint8_t* x_exps, const void* w_codes,
                    int64_t ldw, const uint8_t* w_exps, const void* bias, int bias_dtype, void* out, int64_t M, int64_t N,
                    int64_t K, int dtype, void* workspace, size_t workspace_bytes, int check_timeout, void* stream) {
-  const size_t es = (size_t)dtype_size(dtype);
-  if (es == 0 || (bias && dtype_size(bias_dtype) == 0)) return fail(FLB_ERR_DTYPE, "fp8_linear: dtype must be f32, f16 or bf16");
-  int st = check_codes("fp8_linear", M, K);
-  if (st == FLB_OK) st = check_codes("fp8_linear", N, K);
-  if (st != FLB_OK) return st;
-  if (M > 0 && N > ((int64_t)1 << 42) / M) return fail(FLB_ERR_SHAPE, "fp8_linear: too many outputs");
-  if (M == 0 || N == 0) return FLB_OK;
-  if (!x == !x_codes || !x_codes != !x_exps) return fail(FLB_ERR_SHAPE, "fp8_linear: either x, or x_codes and x_exps");
-  if (!w_codes || !w_exps || !out) return fail(FLB_ERR_SHAPE, "fp8_linear: null weight or out");
-  if (x ? ldx < 0 : ldc < K) return fail(FLB_ERR_SHAPE, "fp8_linear: bad row pitch of x");
-  if (ldw < K) return fail(FLB_ERR_SHAPE, "fp8_linear: bad row pitch of the weight");
-  if (off(w_codes, 16) || off(w_exps, 16) || ldw % 16 || (x_codes && (off(x_codes, 16) || off(x_exps, 16) || ldc % 16)))
-    return fail(FLB_ERR_ALIGN, "fp8_linear: codes must start every row on 16 bytes, and exps lie on 16");
-  if (off(x, es) || off(out, es) || off(bias, bias ? (size_t)dtype_size(bias_dtype) : 1))
-    return fail(FLB_ERR_ALIGN, "fp8_linear: pointers must be aligned to their element size");
-  if (!workspace || workspace_bytes < fp8_linear_workspace_bytes(M, N, K, x != nullptr))
-    return fail(FLB_ERR_WORKSPACE, "fp8_linear: workspace smaller than flb_fp8_linear_workspace_bytes()");
-  if (off(workspace, 256)) return fail(FLB_ERR_ALIGN, "fp8_linear: workspace must be 256-byte aligned");
-  if (check_timeout) {
-    cudaStreamCaptureStatus capture;
-    if ((st = check_cuda(cudaStreamIsCapturing(as_stream(stream), &capture), "fp8_linear capture status")) != FLB_OK) return st;
-    if (capture != cudaStreamCaptureStatusNone)
-      return fail(FLB_ERR_UNSUPPORTED, "fp8_linear: check_timeout waits for the product, which a stream capture does not allow");
-  }
-  return fp8_linear(x, ldx, static_cast<const int8_t*>(x_codes), ldc, x_exps, static_cast<const int8_t*>(w_codes), ldw, w_exps, bias, bias_dtype, out, M,
-                    N, K, dtype, workspace, check_timeout, as_stream(stream));
+  return fp8_linear_checked(x, ldx, x_codes, ldc, x_exps, w_codes, ldw, w_exps, bias, bias_dtype, out, M, N, K, dtype, workspace, workspace_bytes,
+                            check_timeout, -1, 0, stream);
+}
+
+int flb_fp8_linear_wait_test(const void* x, int64_t ldx, const void* x_codes, int64_t ldc, const uint8_t* x_exps, const void* w_codes,
+                             int64_t ldw, const uint8_t* w_exps, const void* bias, int bias_dtype, void* out, int64_t M, int64_t N,
+                             int64_t K, int dtype, void* workspace, size_t workspace_bytes, int check_timeout, int64_t drop_step,
+                             uint32_t spin_limit, void* stream) {
+  if (drop_step < -1 || drop_step > INT32_MAX || spin_limit == 0) return fail(FLB_ERR_SHAPE, "fp8_linear_wait_test: bad drop_step or spin_limit");
+  return fp8_linear_checked(x, ldx, x_codes, ldc, x_exps, w_codes, ldw, w_exps, bias, bias_dtype, out, M, N, K, dtype, workspace, workspace_bytes,
+                            check_timeout, (int)drop_step, spin_limit, stream);
 }
 
 int flb_sample(const void* logits, int64_t ld, const void* u, int u_is_f64, int64_t* token, int64_t rows, int64_t V, int dtype,

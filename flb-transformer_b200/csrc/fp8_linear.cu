@@ -66,9 +66,13 @@ struct Args {
   float* parts;        // [tiles][splits][NC][128], splits > 1
   uint32_t* counts;    // [tiles], zero
   uint32_t* error;
+  uint32_t limit;      // polls of a wait (kWaitLimit)
+  int drop;            // a step whose copies the first worker waits for in vain (a test of the waits), or -1
 };
 
-__device__ __forceinline__ bool step_wait(uint64_t* bar, uint32_t phase) { return mbar_try_wait(bar, phase) || mbar_wait(bar, phase, kWaitLimit); }
+__device__ __forceinline__ bool step_wait(uint64_t* bar, uint32_t phase, uint32_t limit) { return mbar_try_wait(bar, phase) || mbar_wait(bar, phase, limit); }
+// The step `drop` expects 16 bytes more than it is sent, until the MMAs have been given up.
+constexpr uint32_t kNeverSent = 16;
 
 // One block, or a pair of them: the instructions that differ.
 template <bool PAIR> struct Blocks;
@@ -232,8 +236,10 @@ __global__ void __launch_bounds__(threads<NC>(), 1)
     };
     // the first block expects both blocks' bytes (the other's may land before: the count goes below zero)
     const uint32_t codes_bytes = (uint32_t)((a.a_rows + ROWS) * kStep);
-    auto expect = [&](int s, int groups, bool first) {
-      if (rank == 0) mbar_arrive_expect_tx(&full[s], B::kCount * (codes_bytes + (first ? (1 + groups) * kTileBytes : 0)));
+    const uint32_t drop = worker == 0 ? (uint32_t)a.drop : ~0u;
+    auto expect = [&](int s, int groups, bool first, uint32_t step) {
+      if (rank == 0)
+        mbar_arrive_expect_tx(&full[s], B::kCount * (codes_bytes + (first ? (1 + groups) * kTileBytes : 0)) + (step == drop ? kNeverSent : 0));
     };
     // Where the kernel that this one may overlap is the one that makes X's codes, the weight was written before that
     // kernel started: a first ring of weight tiles is on its way before the wait.
@@ -244,7 +250,7 @@ __global__ void __launch_bounds__(threads<NC>(), 1)
       for (int k = k0; k < k1 && early < (uint32_t)S; ++k, ++early) {
         const bool first = k == k0 || (k & 3) == 0;
         if (issues) {
-          expect(early, groups, first);
+          expect(early, groups, first, early);
           load_w(early, n0, groups, k, first);
         }
       }
@@ -258,13 +264,13 @@ __global__ void __launch_bounds__(threads<NC>(), 1)
       const int groups = groups_of(n0), row_x = m0 / kBlock * a.quads;
       for (int k = k0; k < k1; ++k, ++it) {
         const bool first = k == k0 || (k & 3) == 0, whole = it >= early;
-        if (it >= (uint32_t)S && !step_wait(&empty[s], phase ^ 1)) {
+        if (it >= (uint32_t)S && !step_wait(&empty[s], phase ^ 1, a.limit)) {
           ok = false;
           break;
         }
         if (issues) {
           if (whole) {
-            expect(s, groups, first);
+            expect(s, groups, first, it);
             load_w(s, n0, groups, k, first);
           }
           B::load(ring + s * kStage, &tm_x, &full[s], k * kStep, m0);
@@ -280,6 +286,12 @@ __global__ void __launch_bounds__(threads<NC>(), 1)
     if (rank == 0) {
       // both blocks' copies count here: the other block waits for this one at the end
       uint32_t landed = 0;  // of the ring's stages
+      if (drop >= last && drop < it) {
+        mbar_wait(&drain, 0, kDrainLimit);
+        if (issues)
+          asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&full[drop % S])), "n"(kNeverSent) : "memory");
+        __syncwarp();
+      }
       for (uint32_t i = last; i < it; ++i) {
         if (mbar_wait(&full[i % S], (i / S) & 1, kDrainLimit)) landed |= 1u << (i % S);
         else ok = false;
@@ -301,7 +313,7 @@ __global__ void __launch_bounds__(threads<NC>(), 1)
       // the first block's arrivals at this block's barriers are all in before the block ends
       if (complete)
         for (uint32_t i = last; i < it; ++i)
-          if (!step_wait(&empty[i % S], (i / S) & 1)) ok = false;
+          if (!step_wait(&empty[i % S], (i / S) & 1, a.limit)) ok = false;
       if (rank == 1 && !mbar_wait(&drain, 0, kDrainLimit)) ok = false;
     }
     if (!ok && lane == 0) atomicExch(a.error, 1u);
@@ -325,11 +337,11 @@ __global__ void __launch_bounds__(threads<NC>(), 1)
         uint32_t at = 0;
         int chunk = 0;  // steps of the accumulator so far
         for (int k = k0; k < k1; ++k) {
-          if (chunk == 0 && started >= 2 && !step_wait(&acc_empty[b], acc_phase)) {
+          if (chunk == 0 && started >= 2 && !step_wait(&acc_empty[b], acc_phase, a.limit)) {
             ok = false;
             break;
           }
-          if (!step_wait(&full[s], phase)) {
+          if (!step_wait(&full[s], phase, a.limit)) {
             ok = false;
             break;
           }
@@ -403,7 +415,7 @@ __global__ void __launch_bounds__(threads<NC>(), 1)
 #pragma unroll 1
       for (int k = k0; k < k1; k += kChunk, ++local) {
         const uint32_t b = local & 1;
-        if (ok && !step_wait(&acc_full[b], (local >> 1) & 1)) {
+        if (ok && !step_wait(&acc_full[b], (local >> 1) & 1, a.limit)) {
           ok = false;  // carries on with what is there, so that the warps meet at every barrier below
           if (lane == 0) atomicExch(a.error, 1u);
         }
@@ -621,7 +633,7 @@ size_t fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, bool quantise
 
 int fp8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, const uint8_t* x_exps, const int8_t* w_codes, int64_t ldw,
                const uint8_t* w_exps, const void* bias, int bias_dtype, void* out, int64_t M, int64_t N, int64_t K, int dtype, void* ws,
-               int check_timeout, cudaStream_t s) {
+               int check_timeout, int drop, uint32_t limit, cudaStream_t s) {
   const Shape g = shape_of(M, N, K);
   const Ws l = ws_of(g, M, K, x != nullptr);
   uint8_t* const p = reinterpret_cast<uint8_t*>(ws);
@@ -654,6 +666,7 @@ int fp8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, c
   }
   a.bias = bias, a.bias_dtype = bias_dtype, a.out = out, a.M = M, a.N = N;
   a.early = x != nullptr;
+  a.limit = limit ? limit : kWaitLimit, a.drop = drop;
   a.k_blocks = (int)blocks_of(K), a.quads = (int)quads_of(K), a.n_tiles = g.n_tiles, a.tiles = g.tiles, a.splits = g.splits;
   a.group = N * K <= kWeightInL2 ? 1 : 16;
   a.stream_out = (size_t)M * N * es > kOutputInL2;

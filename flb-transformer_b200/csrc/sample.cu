@@ -502,7 +502,7 @@ template <typename T, bool HELD> __global__ void __launch_bounds__(kThreads, 2) 
   r.per_unit = fmin(0x1.71547652b82fep+0 / fmax(temperature, 1e-290), 900 / apart);
   r.lowest = fmaxf((float)(r.max_value - 900 / r.per_unit), -FLT_MAX);
   const int64_t top_k = a.top_k ? a.top_k[row] : a.top_k1;
-  const double top_p = a.top_p ? (double)a.top_p[row] : a.top_p1, min_p = fmin(a.min_p ? (double)a.min_p[row] : a.min_p1, 1.0);
+  const double top_p = a.top_p ? (double)a.top_p[row] : a.top_p1, min_p_given = a.min_p ? (double)a.min_p[row] : a.min_p1, min_p = min_p_given >= 1 ? 1.0 : min_p_given;
   const double u = a.u64 ? reinterpret_cast<const double*>(a.u)[row] : (double)reinterpret_cast<const float*>(a.u)[row];
   const uint64_t w_least = min_p > 0 ? (uint64_t)ceil(min_p * (double)(1ull << a.frac)) : 0;
   // top_p: a token is kept while the sum before it is below p of the whole; the first one always

@@ -118,6 +118,8 @@ PROTOTYPES = {
     "flb_fp8_linear_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32]),
     "flb_fp8_linear": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _i32, _vp, _sz, _i32,
                               _vp]),
+    "flb_fp8_linear_wait_test": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _i32, _vp, _sz,
+                                        _i32, _i64, ctypes.c_uint32, _vp]),
     "flb_sample": (_i32, [_vp, _i64, _vp, _i32, _vp, _i64, _i64, _i32, _vp, ctypes.c_double, _vp, _i64, _vp, ctypes.c_double, _vp,
                           ctypes.c_double, _vp]),
     "flb_adamw": (_i32, [_vp, _i64, _i32, _i32, ctypes.c_double, _vp, ctypes.c_double, ctypes.c_double, ctypes.c_double,

@@ -7,7 +7,8 @@
 
 A block of 128 consecutive elements of a row is held as e4m3 codes (4 significant bits, magnitudes up to 448) in units
 of the smallest power of two, from 2^-127 on, in which its largest magnitude is at most 448. An element is off by at
-most 1/16 of itself, or where it is below 2^-6 units, 2^-10 units. A block that holds an infinity or NaN counts as NaN.
+most 1/16 of itself, or where it is below 2^-6 units, 2^-10 units (of float32, one above 1.93 * 2^127 counts as 2^128, an
+infinity). A block that holds an infinity or NaN counts as NaN.
 Against 8-bit integers with a scale a row (int8_linear) small elements keep their precision beside large ones, and
 an outlier costs the others of its block nothing until it is 2^15 times as large.
 

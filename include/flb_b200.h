@@ -515,6 +515,13 @@ int flb_fp8_linear(const void* x, int64_t ldx, const void* x_codes, int64_t ldc,
                    int64_t ldw, const uint8_t* w_exps, const void* bias, int bias_dtype, void* out, int64_t M, int64_t N,
                    int64_t K, int dtype, void* workspace, size_t workspace_bytes, int check_timeout, void* stream);
 
+/* Failure-detection check of the product's bounded waits, as flb_int8_linear_wait_test: step drop_step (128 of K of a tile, counted along
+ * a worker's own work) of the first block, or pair of blocks, is never reported as loaded; -1: every step is. */
+int flb_fp8_linear_wait_test(const void* x, int64_t ldx, const void* x_codes, int64_t ldc, const uint8_t* x_exps, const void* w_codes,
+                             int64_t ldw, const uint8_t* w_exps, const void* bias, int bias_dtype, void* out, int64_t M, int64_t N,
+                             int64_t K, int dtype, void* workspace, size_t workspace_bytes, int check_timeout, int64_t drop_step,
+                             uint32_t spin_limit, void* stream);
+
 /* ------------------------------------------------------------------------------------------
  * A token for each row of logits (no reference counterpart: the reference's callers take the argmax).
  * logits [rows, V] in dtype, ld elements from row to row; u [rows]: uniform numbers in [0, 1), float32 or (u_is_f64)

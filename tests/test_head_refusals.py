@@ -121,3 +121,5 @@ def test_fp8_abi():
     assert linear(x=None, xc=16, ldc=4, xe=16) == 1 and linear(x=None, xc=16, ldc=24, xe=16) == 3
     assert linear(ws=None) == 8 and linear(n=100) == 8 and linear(ws=128) == 3 and linear(M=1 << 30, N=1 << 30) == 1
     assert L.flb_fp8_linear_workspace_bytes(1 << 30, 1 << 30, 8, 0) == 0
+    for drop, limit in ((-2, 1), (0, 0), (1 << 40, 1)):
+        assert L.flb_fp8_linear_wait_test(16, 8, None, 0, None, 16, 16, 16, None, 0, 16, 4, 8, 8, 2, 256, 1 << 30, 1, drop, limit, None) == 1
