@@ -60,11 +60,15 @@ template <int N> __device__ __forceinline__ void store_codes(int8_t* row, const 
   else *reinterpret_cast<uint32_t*>(row + c) = w[0];
 }
 
-template <int N> __device__ __forceinline__ uint32_t largest(const float (&v)[N]) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int j = 0; j < N; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
-  return m;
+// The float32 bits of the largest magnitude of 16 bytes a lane and PER lanes. 16-bit values as they are, two at a time: their magnitudes' bits
+// are ordered as they are.
+template <typename T, int PER> __device__ __forceinline__ uint32_t largest(const uint4& w) {
+  if constexpr (sizeof(T) == 4) {
+    return max_of<PER>(max(max(w.x & 0x7fffffffu, w.y & 0x7fffffffu), max(w.z & 0x7fffffffu, w.w & 0x7fffffffu)));
+  } else {
+    const uint32_t two = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
+    return __float_as_uint(rows::unpack2<T>(max_of<PER>(max(two & 0xffffu, two >> 16))).x);
+  }
 }
 
 struct RowsArgs {
@@ -85,9 +89,10 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(256) rows_kern
   const int lane = threadIdx.x % PER;
   const int64_t row = unit / blocks, block = unit % blocks;
   const bool there = row < a.R;
+  const uint4 raw = there ? load_row<T, VEC>(reinterpret_cast<const T*>(a.x) + row * a.ldx, block * kBlock + lane * N, a.K) : make_uint4(0, 0, 0, 0);
   float v[N];
-  unpack_row<T>(v, there ? load_row<T, VEC>(reinterpret_cast<const T*>(a.x) + row * a.ldx, block * kBlock + lane * N, a.K) : make_uint4(0, 0, 0, 0));
-  const int u = unit_of(max_of<PER>(largest(v)));
+  unpack_row<T>(v, raw);
+  const int u = unit_of(largest<T, PER>(raw));
   if (!there) return;
   store_codes(a.codes + row * a.pitch, v, inverse_of(u), block * kBlock + lane * N, a.pitch);
   if (lane == 0) a.exps[exp_at(row, block, a.quads)] = (uint8_t)u;
@@ -106,7 +111,7 @@ struct TileArgs {
 constexpr int kDown = 8;
 
 // 256 threads. As 16 or 8 rows at a time (a row's block in PER lanes), then as columns: four runs of 32 rows of 64 pairs of columns.
-template <typename T, bool VEC, bool SUM> __global__ void __launch_bounds__(256) tile_kernel(const TileArgs a) {
+template <typename T, bool VEC, bool SUM> __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) tile_kernel(const TileArgs a) {
   constexpr int PER = kPer<T>, N = 16 / sizeof(T), ROWS = 256 / PER, kPitch = kBlock + 16 / (int)sizeof(T);
   extern __shared__ __align__(16) uint8_t dyn[];
   T(*tile)[kPitch] = reinterpret_cast<T(*)[kPitch]>(dyn);
@@ -132,7 +137,7 @@ template <typename T, bool VEC, bool SUM> __global__ void __launch_bounds__(256)
     *reinterpret_cast<uint4*>(&tile[r][lane * N]) = raw[i];
     float v[N];
     unpack_row<T>(v, raw[i]);
-    const int u = unit_of(max_of<PER>(largest(v)));
+    const int u = unit_of(largest<T, PER>(raw[i]));
     if (row < a.R) {
       store_codes(a.codes + row * a.pitch, v, inverse_of(u), c0 + lane * N, a.pitch);
       if (lane == 0) a.exps[exp_at(row, tile_c, a.quads)] = (uint8_t)u;
