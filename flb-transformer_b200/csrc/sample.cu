@@ -151,10 +151,11 @@ template <typename T, bool HELD> struct Row {
     int n[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const double y = ((double)fminf(fmaxf(v[j], lowest), FLT_MAX) - max_value) * per_unit;
-      const double t = y + 0x1.8p52;
+      // (operations that a compiler does not contract: a logit's weight has to be the same integer wherever it is computed)
+      const double y = __dmul_rn(__dadd_rn((double)fminf(fmaxf(v[j], lowest), FLT_MAX), -max_value), per_unit);
+      const double t = __dadd_rn(y, 0x1.8p52);
       n[j] = __double2loint(t) + frac;
-      f[j] = y - (t - 0x1.8p52);
+      f[j] = __dadd_rn(y, -__dadd_rn(t, -0x1.8p52));
       p[j] = kCoefficients[9];
     }
 #pragma unroll
@@ -165,7 +166,7 @@ template <typename T, bool HELD> struct Row {
     for (int j = 0; j < N; ++j) {
       const double x = __hiloint2double(__double2hiint(p[j]) + (n[j] << 20), __double2loint(p[j]));
       // rounded to an integer by the addition, below 2^52
-      w[j] = (uint64_t)__double_as_longlong(x + 0x1p52) & 0xfffffffffffffull;
+      w[j] = (uint64_t)__double_as_longlong(__dadd_rn(x, 0x1p52)) & 0xfffffffffffffull;
     }
   }
   __device__ __forceinline__ uint64_t weight(float value) const {

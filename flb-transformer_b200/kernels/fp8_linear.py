@@ -71,7 +71,7 @@ def quantize_fp8(x: torch.Tensor) -> Fp8Rows:
 
 def fp8_linear(x: torch.Tensor | Fp8Rows, weight: torch.Tensor | Fp8Rows, bias: torch.Tensor | None = None,
                check_timeout: bool = False) -> torch.Tensor:
-    """x [..., K] times weight [N, K], plus bias [N]: [..., N] in x's type. weight and bias: float32, float16 or bfloat16; the
+    """x [..., K] times weight [N, K], plus bias [N]: [..., N] in x's type, also under autocast. weight and bias: float32, float16 or bfloat16; the
     weight as a plain tensor (differentiable), or in Fp8Rows (inference; then x may be so too). See the module's text."""
     no_transforms("fp8_linear")
     if not isinstance(weight, Fp8Rows):

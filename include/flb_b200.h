@@ -502,7 +502,7 @@ size_t flb_fp8_exps_bytes(int64_t R, int64_t K);
 int flb_fp8_rows(const void* x, int64_t ldx, void* codes, uint8_t* exps, int64_t R, int64_t K, int dtype, void* stream);
 /* A matrix x [R, C] (pitch ldx elements) along both axes from one read: codes and exps of its rows, and codes_t, exps_t those of its
  * columns, [C, R]. bias_grad: NULL, or [C] in bias_dtype: the sum of each column, in float32 and a fixed order; sums is then a
- * workspace of flb_fp8_rows2_workspace_bytes(), 16-byte aligned. */
+ * workspace of flb_fp8_rows2_workspace_bytes(), 16-byte aligned. R = 0: nothing is written. */
 size_t flb_fp8_rows2_workspace_bytes(int64_t R, int64_t C);
 int flb_fp8_rows2(const void* x, int64_t ldx, void* codes, uint8_t* exps, void* codes_t, uint8_t* exps_t, void* bias_grad,
                   int bias_dtype, int64_t R, int64_t C, int dtype, void* workspace, size_t workspace_bytes, void* stream);
