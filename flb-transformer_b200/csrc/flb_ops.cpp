@@ -9,6 +9,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
+#include <algorithm>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -456,20 +457,6 @@ Fp8 fp8_rows(const Tensor& x_) {
   check(flb_fp8_rows(x.data_ptr(), ldx, q.codes.data_ptr(), (uint8_t*)q.exps.data_ptr(), R, K, dt, stream_of(x)), "flb_fp8_rows");
   return q;
 }
-// x's rows and columns, and with bias_grad the columns' sums
-std::pair<Fp8, Fp8> fp8_rows2(const Tensor& x_, const Opt& bias_grad) {
-  const int dt = dtype_of(x_, "x");
-  auto [x, ldx] = rows_of(x_);
-  const int64_t C = x.size(-1), R = rows_in(x);
-  Fp8 q = fp8_buffers(R, C, x), t = fp8_buffers(C, R, x);
-  const size_t need = given(bias_grad) ? flb_fp8_rows2_workspace_bytes(R, C) : 0;
-  Tensor ws = need ? buffer(need, x) : Tensor();
-  check(flb_fp8_rows2(x.data_ptr(), ldx, q.codes.data_ptr(), (uint8_t*)q.exps.data_ptr(), t.codes.data_ptr(), (uint8_t*)t.exps.data_ptr(), ptr(bias_grad),
-                      given(bias_grad) ? dtype_of(*bias_grad, "bias") : dt, R, C, dt, need ? ws.data_ptr() : nullptr, need, stream_of(x)),
-        "flb_fp8_rows2");
-  return {q, t};
-}
-
 // The product of x [M, K], or its codes, and a weight's [N, K] codes into out
 void fp8_product(const Opt& x_, int64_t ldx, const Fp8& xq, int64_t ldc, const Fp8& w, int64_t ldw, const Opt& bias, const Tensor& out, int64_t M, int64_t N,
                  int64_t K, bool check_timeout) {
@@ -548,6 +535,42 @@ Tensor fp8_linear_kept(const Opt& x_, const Opt& x_codes, const Opt& x_exps, con
   return out;
 }
 
+// Several arrays in one buffer: a small training step is bound by the host, and an allocation costs it a microsecond.
+struct Arena {
+  size_t bytes = 0;
+  size_t add(size_t n) {
+    const size_t at = bytes;
+    bytes += (n + 255) & ~(size_t)255;
+    return at;
+  }
+};
+struct Fp8Place {
+  size_t codes, exps;
+  Fp8Place(Arena& a, int64_t rows, int64_t K) : codes(a.add((size_t)rows * flb_code_pitch(K))), exps(a.add(flb_fp8_exps_bytes(rows, K))) {}
+};
+struct Fp8At {
+  void* codes;
+  uint8_t* exps;
+  Fp8At(void* base, const Fp8Place& p) : codes((uint8_t*)base + p.codes), exps((uint8_t*)base + p.exps) {}
+};
+void fp8_codes(const Tensor& x_, const Fp8At& q) {
+  auto [x, ldx] = rows_of(x_);
+  check(flb_fp8_rows(x.data_ptr(), ldx, q.codes, q.exps, rows_in(x), x.size(-1), dtype_of(x, "x"), stream_of(x)), "flb_fp8_rows");
+}
+// along both axes, and with bias_grad the columns' sums
+void fp8_codes2(const Tensor& x_, const Fp8At& q, const Fp8At& t, const Opt& bias_grad, void* ws, size_t need) {
+  auto [x, ldx] = rows_of(x_);
+  const int dt = dtype_of(x, "x");
+  check(flb_fp8_rows2(x.data_ptr(), ldx, q.codes, q.exps, t.codes, t.exps, ptr(bias_grad), given(bias_grad) ? dtype_of(*bias_grad, "bias") : dt, rows_in(x),
+                      x.size(-1), dt, ws, need, stream_of(x)),
+        "flb_fp8_rows2");
+}
+void fp8_codes_product(const Fp8At& x, const Fp8At& w, const Opt& bias, const Tensor& out, int64_t M, int64_t N, int64_t K, void* ws, size_t need) {
+  check(flb_fp8_linear(nullptr, 0, x.codes, flb_code_pitch(K), x.exps, w.codes, flb_code_pitch(K), w.exps, ptr(bias),
+                       given(bias) ? dtype_of(*bias, "bias") : FLB_F32, out.data_ptr(), M, N, K, dtype_of(out, "out"), ws, need, 0, stream_of(out)),
+        "flb_fp8_linear");
+}
+
 // A training step's products. x [M, K] and the weight [N, K] are kept for the backward pass as the 8-bit columns that it sums over.
 struct Fp8LinearFn : torch::autograd::Function<Fp8LinearFn> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Opt& bias) {
@@ -557,19 +580,25 @@ struct Fp8LinearFn : torch::autograd::Function<Fp8LinearFn> {
     const bool for_dx = x.requires_grad(), for_dw = weight.requires_grad();
     std::vector<int64_t> shape = x.sizes().vec();
     shape.back() = N;
-    Tensor out = at::empty(shape, x.options());
-    Fp8 xq, xt, wq, wt;
+    Tensor out = at::empty(shape, x.options()), columns;
     if (M && N) {
-      if (for_dw) std::tie(xq, xt) = fp8_rows2(x, {});
-      else xq = fp8_rows(x);
-      if (for_dx) std::tie(wq, wt) = fp8_rows2(weight, {});
-      else wq = fp8_rows(weight);
-      fp8_product({}, 0, xq, flb_code_pitch(K), wq, flb_code_pitch(K), contiguous(bias), out, M, N, K, false);
+      Arena here, kept;
+      const Fp8Place xq(here, M, K), wq(here, N, K);
+      const size_t need = flb_fp8_linear_workspace_bytes(M, N, K, 1), ws = here.add(need);
+      const Fp8Place xt(kept, for_dw ? K : 0, M), wt(kept, for_dx ? K : 0, N);
+      const Tensor t = buffer(here.bytes, x);
+      columns = buffer(kept.bytes, x);
+      uint8_t* const at = (uint8_t*)t.data_ptr();
+      void* const keep = columns.data_ptr();
+      if (for_dw) fp8_codes2(x, {at, xq}, {keep, xt}, {}, nullptr, 0);
+      else fp8_codes(x, {at, xq});
+      if (for_dx) fp8_codes2(weight, {at, wq}, {keep, wt}, {}, nullptr, 0);
+      else fp8_codes(weight, {at, wq});
+      fp8_codes_product({at, xq}, {at, wq}, contiguous(bias), out, M, N, K, at + ws, need);
     }
-    ctx->save_for_backward({xt.codes, xt.exps, wt.codes, wt.exps});
-    ctx->saved_data["sizes"] = std::vector<int64_t>{M, N, K};
+    ctx->save_for_backward({columns});
+    ctx->saved_data["sizes"] = std::vector<int64_t>{M, N, K, for_dx, for_dw, (int64_t)weight.scalar_type(), given(bias) ? (int64_t)bias->scalar_type() : -1};
     ctx->saved_data["x"] = x.sizes().vec();
-    ctx->saved_data["types"] = std::vector<int64_t>{(int64_t)weight.scalar_type(), given(bias) ? (int64_t)bias->scalar_type() : -1};
     return out;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
@@ -577,25 +606,35 @@ struct Fp8LinearFn : torch::autograd::Function<Fp8LinearFn> {
     {
       at::AutoDispatchBelowADInplaceOrView below;
       const auto s = ctx->get_saved_variables();
-      const auto sizes = ctx->saved_data["sizes"].toIntVector(), types = ctx->saved_data["types"].toIntVector();
+      const auto sizes = ctx->saved_data["sizes"].toIntVector();
       const int64_t M = sizes[0], N = sizes[1], K = sizes[2];
-      const bool for_dx = ctx->needs_input_grad(0), for_dw = ctx->needs_input_grad(1), for_db = types[1] >= 0 && ctx->needs_input_grad(2);
+      const bool for_dx = ctx->needs_input_grad(0), for_dw = ctx->needs_input_grad(1), for_db = sizes[6] >= 0 && ctx->needs_input_grad(2);
       const Tensor& dy = g[0];
       const c10::cuda::CUDAGuard guard(dy.device());
       const bool some = M && N;
-      if (for_dx) out[0] = some ? at::empty(ctx->saved_data["x"].toIntVector(), dy.options()) : at::zeros(ctx->saved_data["x"].toIntVector(), dy.options());
-      const auto w_options = dy.options().dtype((at::ScalarType)types[0]);
-      if (for_dw) out[1] = some ? at::empty({N, K}, w_options) : at::zeros({N, K}, w_options);
-      if (for_db) {
-        const auto options = dy.options().dtype((at::ScalarType)types[1]);
-        out[2] = some ? at::empty({N}, options) : at::zeros({N}, options);
-      }
+      auto grad = [&](at::IntArrayRef shape, int64_t type) {
+        const auto options = dy.options().dtype((at::ScalarType)type);
+        return some ? at::empty(shape, options) : at::zeros(shape, options);
+      };
+      if (for_dx) out[0] = grad(ctx->saved_data["x"].toIntVector(), (int64_t)dy.scalar_type());
+      if (for_dw) out[1] = grad({N, K}, sizes[5]);
+      if (for_db) out[2] = grad({N}, sizes[6]);
       if (some) {
-        Fp8 q, t;
-        if (for_dw || for_db) std::tie(q, t) = fp8_rows2(dy, for_db ? Opt(out[2]) : Opt());
-        else q = fp8_rows(dy);
-        if (for_dx) fp8_product({}, 0, q, flb_code_pitch(N), {s[2], s[3]}, flb_code_pitch(N), {}, out[0], M, K, N, false);
-        if (for_dw) fp8_product({}, 0, t, flb_code_pitch(M), {s[0], s[1]}, flb_code_pitch(M), {}, out[1], N, K, M, false);
+        // (one workspace for both products: the second starts when the first has ended)
+        Arena here, kept;
+        const Fp8Place xt(kept, sizes[4] ? K : 0, M), wt(kept, sizes[3] ? K : 0, N);
+        const bool both = for_dw || for_db;
+        const Fp8Place q(here, M, N), t(here, both ? N : 0, M);
+        const size_t sums_need = for_db ? flb_fp8_rows2_workspace_bytes(M, N) : 0, sums = here.add(sums_need);
+        const size_t dx_need = for_dx ? flb_fp8_linear_workspace_bytes(M, K, N, 1) : 0, dw_need = for_dw ? flb_fp8_linear_workspace_bytes(N, K, M, 1) : 0;
+        const size_t need = std::max(dx_need, dw_need), ws = here.add(need);
+        const Tensor held = buffer(here.bytes, dy);
+        uint8_t* const at = (uint8_t*)held.data_ptr();
+        void* const keep = s[0].data_ptr();
+        if (both) fp8_codes2(dy, {at, q}, {at, t}, for_db ? Opt(out[2]) : Opt(), at + sums, sums_need);
+        else fp8_codes(dy, {at, q});
+        if (for_dx) fp8_codes_product({at, q}, {keep, wt}, {}, out[0], M, K, N, at + ws, need);
+        if (for_dw) fp8_codes_product({at, t}, {keep, xt}, {}, out[1], N, K, M, at + ws, need);
       }
     }
     return differentiable_once(std::move(out));
