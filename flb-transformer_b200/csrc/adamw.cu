@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<BITS>) adamw_kernel(const __g
     auto step_at = [&](int o, auto full) {
       constexpr bool FULL = decltype(full)::value;
       float p[U][4], g[U][4], m[U][4], v[U][4];
-      uint32_t cm[U], cv[U], exps = 0;
+      [[maybe_unused]] uint32_t cm[U], cv[U], exps = 0;
       const int block0 = o / kBlockElems;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -203,8 +203,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm<BITS>) adamw_kernel(const __g
         root = (float)rsqrt(-expm1((double)step * a.log_b2));
       }
       // (the root of 2's digits)
-      const uint32_t salt = ((uint32_t)at + o + lane * 4) * kMix + (uint32_t)step * 0x6A09E667u + a.seed;
-      uint32_t kept_exps = 0;
+      [[maybe_unused]] const uint32_t salt = ((uint32_t)at + o + lane * 4) * kMix + (uint32_t)step * 0x6A09E667u + a.seed;
+      [[maybe_unused]] uint32_t kept_exps = 0;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int i = o + u * kBlockElems + lane * 4;
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<BITS>) adamw_kernel(const __g
           decode<kBitsM>(m[u], cm[u], em, base_of(em, kBelowM), a.place);
           decode<kBitsV>(v[u], cv[u], ev, base_of(ev, kBelowV), a.place);
         }
-        uint32_t top_m = 0, top_v = 0;
+        [[maybe_unused]] uint32_t top_m = 0, top_v = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float gj = g[u][j];

@@ -18,7 +18,7 @@
 // list, or the last one, which is open, go through digits of the logits, as integers of the same order, and of the indices instead.
 // Bound by the arithmetic of the weights, 15 float64 operations a logit (at half float32's rate) and about as many others, and
 // with few rows by barriers, 0.6 us for each of a cluster's: 1 x 32000 bf16 with top_k 50 and top_p 0.95 10.3 us, 256 rows with
-// top_p 0.9 52 us, 64 x 131071 float32 with min_p 29 us, which is 1.1 TB/s.
+// top_p 0.9 56 us, 64 x 131071 float32 with min_p 29 us, which is 1.1 TB/s.
 #include <cooperative_groups.h>
 #include <cfloat>
 #include "rows.cuh"

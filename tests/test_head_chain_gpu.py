@@ -135,3 +135,63 @@ def test_a_captured_training_step_of_the_head():
         graph.replay()
         step(b, ob)
         assert torch.equal(a.weight, b.weight) and torch.equal(a.bias, b.bias)
+
+
+def test_one_vector():
+    """x without leading axes, forward and backward."""
+    import kernels
+    x, w = torch.randn(130, device="cuda", requires_grad=True), torch.randn(70, 130, device="cuda", requires_grad=True)
+    y = kernels.fp8_linear(x, w)
+    dy = torch.randn(70, device="cuda")
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    xc, wc, dyc = (t.detach().cpu() for t in (x, w, dy))
+    assert y.shape == (70,) and dx.shape == (130,)
+    close(y[None], *orc.fp8_product(xc[None], wc, None, torch.float32))
+    close(dx[None], *orc.fp8_product(dyc[None], wc.t(), None, torch.float32))
+    close(dw, *orc.fp8_product(dyc[:, None], xc[:, None], None, torch.float32))
+
+
+def test_calls_on_two_streams_at_once():
+    """Products, choices and steps on two streams, each with what it needs of its own."""
+    import kernels
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    xs = [torch.randn(300, 640, device="cuda") for _ in range(2)]
+    ws = [kernels.quantize_fp8(torch.randn(500, 640, device="cuda")) for _ in range(2)]
+    us = [torch.rand(300, device="cuda") for _ in range(2)]
+    ps = [torch.randn(5000, device="cuda") for _ in range(2)]
+    opts = [kernels.AdamW([p], state_bits=8) for p in ps]
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    twins = [p.clone() for p in ps]
+    want = [kernels.sample(kernels.fp8_linear(x, w), u, top_p=0.7) for x, w, u in zip(xs, ws, us)]
+    for t in twins:
+        o = kernels.AdamW([t], state_bits=8)
+        t.grad = torch.ones_like(t)
+        for _ in range(20):
+            o.step()
+    torch.cuda.synchronize()
+    got = [None, None]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = kernels.sample(kernels.fp8_linear(xs[i], ws[i]), us[i], top_p=0.7)
+                opts[i].step()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(got[i], want[i]) and torch.equal(ps[i], twins[i])
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_tensors_on_another_device_than_the_current_one():
+    import kernels
+    with torch.cuda.device(0):
+        x = torch.randn(40, 200, device="cuda:1", requires_grad=True)
+        w = torch.randn(90, 200, device="cuda:1", requires_grad=True)
+        y = kernels.fp8_linear(x, w)
+        y.sum().backward()
+        token = kernels.sample(y.detach(), torch.rand(40, device="cuda:1"))
+        opt = kernels.AdamW([w])
+        opt.step()
+    assert token.device == y.device == x.grad.device == w.device
+    with pytest.raises(ValueError, match="different devices"):
+        kernels.sample(y.detach(), torch.rand(40, device="cuda:0"))
