@@ -716,11 +716,12 @@ const Tensor& tensor_of(PyObject* o, const char* name) {
   return THPVariable_Unpack(o);
 }
 struct Names {
-  PyObject *step, *m, *v, *m_exps, *v_exps;
+  PyObject *step, *m, *v, *m_exps, *v_exps, *strides;
 };
 const Names& names() {
   static const Names n{PyUnicode_InternFromString("step"), PyUnicode_InternFromString("exp_avg"), PyUnicode_InternFromString("exp_avg_sq"),
-                       PyUnicode_InternFromString("exp_avg_exps"), PyUnicode_InternFromString("exp_avg_sq_exps")};
+                       PyUnicode_InternFromString("exp_avg_exps"), PyUnicode_InternFromString("exp_avg_sq_exps"),
+                       PyUnicode_InternFromString("strides")};
   return n;
 }
 // state[p], borrowed; null where there is none or it is empty
@@ -730,6 +731,19 @@ PyObject* state_of(PyObject* state, PyObject* p) {
   return s && PyDict_Check(s) && PyDict_Size(s) > 0 ? s : nullptr;
 }
 const Tensor& get(PyObject* s, PyObject* name, const char* text) { return tensor_of(PyDict_GetItemWithError(s, name), text); }
+
+// Codes lie as their parameter did when they were made: the state of one that is not contiguous has its strides.
+void need_order(PyObject* s, const Tensor& p) {
+  PyObject* const strides = PyDict_GetItemWithError(s, names().strides);
+  if (!strides && PyErr_Occurred()) throw pybind11::error_already_set();
+  bool same = strides ? PyTuple_Check(strides) && PyTuple_GET_SIZE(strides) == p.dim() : p.is_contiguous();
+  for (int64_t i = 0; strides && same && i < p.dim(); ++i) {
+    const int64_t stride = PyLong_AsLongLong(PyTuple_GET_ITEM(strides, i));
+    if (stride == -1 && PyErr_Occurred()) throw pybind11::error_already_set();
+    same = p.size(i) == 1 || stride == p.stride(i);
+  }
+  TORCH_CHECK_VALUE(same, "AdamW: 8-bit moments are not laid out as their parameter, of shape ", p.sizes(), " and strides ", p.strides());
+}
 
 // The tensors of one device and type, one kernel's.
 struct Together {
@@ -782,6 +796,7 @@ pybind11::list adamw(pybind11::list params, pybind11::dict state, int64_t bits, 
       const Tensor &me = get(s, n.m_exps, "exp_avg_exps"), &ve = get(s, n.v_exps, "exp_avg_sq_exps");
       need_codes(m, me, p);
       need_codes(v, ve, p);
+      need_order(s, p);
       t.m_exps = (uint8_t*)me.data_ptr(), t.v_exps = (uint8_t*)ve.data_ptr();
       written.push_back(me), written.push_back(ve);
     } else {
@@ -839,6 +854,7 @@ pybind11::list adamw_moments(pybind11::list params, pybind11::dict state, pybind
     const Tensor &m = get(s, n.m, "exp_avg"), &v = get(s, n.v, "exp_avg_sq"), &me = get(s, n.m_exps, "exp_avg_exps"), &ve = get(s, n.v_exps, "exp_avg_sq_exps");
     need_codes(m, me, p);
     need_codes(v, ve, p);
+    need_order(s, p);
     Together* to = nullptr;
     for (Together& x : all)
       if (x.device == p.device()) to = &x;

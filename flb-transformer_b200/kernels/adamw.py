@@ -13,7 +13,9 @@ largest magnitude ("exp_avg_exps", "exp_avg_sq_exps"): m with a sign, 3 bits of 
 around and under the block's largest, v with 3 bits of mantissa and 32 binades. 2 bytes an element instead of 8. They are
 rounded up or down at random (a mix of the element's index, the step and `seed`: the same every time), so that a
 moment that changes by less than its unit a step still follows its mean. Below the smallest code m becomes zero, and v the
-smallest code. A block with an infinity or NaN becomes NaN as a whole.
+smallest code. A block with an infinity or NaN becomes NaN as a whole. Blocks and codes go by the parameter's memory, whose
+strides are in the state ("strides") of one that is not contiguous: a state goes into, and on with, a parameter that is laid out
+the same, and into another one is refused. (Moments in 32 bits are loaded by element.)
 
 Steps are counted on the device, each tensor's own (its "step", an int64), so that a captured step counts on in every replay;
 lr may be a float32 tensor on the device, which a schedule then writes between replays. The first step of a tensor makes its
@@ -74,6 +76,8 @@ class AdamW(torch.optim.Optimizer):
     def _new_state(self, p, bits):
         state = {"step": torch.zeros((), dtype=torch.int64, device=p.device)}
         blocks = -(-p.numel() // 128)
+        if bits == 8 and not p.is_contiguous():
+            state["strides"] = p.stride()
         for name in ("exp_avg", "exp_avg_sq"):
             if bits == 8:
                 state[name] = torch.zeros(blocks, 128, dtype=torch.uint8, device=p.device)
@@ -81,6 +85,15 @@ class AdamW(torch.optim.Optimizer):
             else:
                 state[name] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
         return state
+
+    @staticmethod
+    def _check_order(s, p):
+        """Refuses 8-bit state of a parameter that was laid out otherwise. (Axes of one element have no place in memory.)"""
+        strides = s.get("strides")
+        same = p.is_contiguous() if strides is None else len(strides) == p.dim() and all(
+            n == 1 or a == b for n, a, b in zip(p.shape, strides, p.stride()))
+        if not same:
+            raise ValueError(f"8-bit moments are not laid out as their parameter, of shape {tuple(p.shape)} and strides {p.stride()}")
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -137,6 +150,11 @@ class AdamW(torch.optim.Optimizer):
                 s = state_dict["state"].get(key)
                 if s and ("exp_avg_exps" in s) != (saved.get("state_bits", 32) == 8):
                     raise ValueError("the state's moments are not of the bits that its group says")
+        for group, saved in zip(self.param_groups, state_dict["param_groups"]):
+            for p, key in zip(group["params"], saved["params"]):
+                s = state_dict["state"].get(key)
+                if s and "exp_avg_exps" in s:
+                    self._check_order(s, p)
         super().load_state_dict(state_dict)
         for group, saved in zip(self.param_groups, state_dict["param_groups"]):
             self._check(group)
@@ -145,5 +163,6 @@ class AdamW(torch.optim.Optimizer):
                     continue
                 s, mine = state_dict["state"][key], self._new_state(p, group["state_bits"])
                 for name, t in mine.items():
-                    t.copy_(torch.as_tensor(s[name]))
+                    if isinstance(t, torch.Tensor):
+                        t.copy_(torch.as_tensor(s[name]))
                 self.state[p] = mine

@@ -1,0 +1,130 @@
+"""What AdamW's state holds and takes back: layouts, captures, dicts that are refused. On the CPU where no step is taken."""
+import copy
+
+import pytest
+import torch
+
+from oracle import head as orc
+
+
+def coded(p, seed=1):
+    """An optimizer with moments in 8 bits for p, as if it had stepped: codes and exponents at random."""
+    import kernels
+    g = torch.Generator().manual_seed(seed)
+    opt = kernels.AdamW([p], state_bits=8)
+    s = opt._new_state(p, 8)
+    for name, top in (("exp_avg", 120), ("exp_avg_sq", 249)):
+        s[name].view(-1)[:p.numel()] = torch.randint(0, top, (p.numel(),), generator=g).to(torch.uint8)
+        s[name + "_exps"].copy_(torch.randint(100, 140, s[name + "_exps"].shape, generator=g))
+    s["step"] += 3
+    opt.state[p] = s
+    return opt
+
+
+def leaf(shape, order=None, device="cpu"):
+    """A parameter of that shape; order: its axes from the outermost in memory to the innermost."""
+    order = order or tuple(range(len(shape)))
+    x = torch.randn([shape[i] for i in order], generator=torch.Generator().manual_seed(5))
+    back = [order.index(i) for i in range(len(shape))]
+    return x.to(device).permute(back).requires_grad_(True)
+
+
+LAYOUTS = [((5, 300), (1, 0), (0, 1)), ((5, 300), (0, 1), (1, 0)), ((4, 3, 50), (1, 0, 2), (0, 1, 2)), ((4, 3, 50), (2, 0, 1), (1, 0, 2)),
+           ((2, 8, 3, 3), (0, 2, 3, 1), (0, 1, 2, 3))]
+
+
+@pytest.mark.parametrize("shape,was,becomes", LAYOUTS)
+def test_codes_do_not_go_into_another_layout(shape, was, becomes):
+    """Codes lie as their parameter does: one that lies otherwise would take them for other elements."""
+    import kernels
+    saved = coded(leaf(shape, was)).state_dict()
+    p = leaf(shape, becomes)
+    opt = kernels.AdamW([p], lr=0.5, state_bits=8)
+    with pytest.raises(ValueError, match="laid out"):
+        opt.load_state_dict(saved)
+    assert not opt.state.get(p) and opt.param_groups[0]["lr"] == 0.5
+
+
+@pytest.mark.parametrize("shape,order", [((5, 300), (1, 0)), ((5, 300), (0, 1)), ((4, 3, 50), (2, 0, 1)), ((300,), (0,)), ((), ())])
+def test_codes_go_into_the_same_layout(shape, order, tmp_path):
+    import kernels
+    a = leaf(shape, order)
+    opt = coded(a)
+    torch.save(opt.state_dict(), tmp_path / "state.pt")
+    for saved in (copy.deepcopy(opt.state_dict()), torch.load(tmp_path / "state.pt", weights_only=True), copy.deepcopy(opt).state_dict()):
+        b = leaf(shape, order)
+        other = kernels.AdamW([b], state_bits=8)
+        other.load_state_dict(saved)
+        again = kernels.AdamW([leaf(shape, order)], state_bits=8)
+        again.load_state_dict(other.state_dict())
+        for o, p in ((other, b), (again, again.param_groups[0]["params"][0])):
+            assert set(o.state[p]) == set(opt.state[a])
+            for name in ("exp_avg", "exp_avg_exps", "exp_avg_sq", "exp_avg_sq_exps", "step"):
+                assert torch.equal(o.state[p][name], opt.state[a][name])
+
+
+def test_axes_of_one_element_have_no_place_in_a_layout():
+    """The strides of such axes say nothing: a column and a row of one are alike."""
+    import kernels
+    a = torch.zeros(7, 40).t().unsqueeze(1).requires_grad_(True)                       # [40, 1, 7], strides (1, 280, 40) or the like
+    b = torch.empty_strided((40, 1, 7), (1, 1, 40)).zero_().requires_grad_(True)
+    assert a.stride() != b.stride()
+    kernels.AdamW([b], state_bits=8).load_state_dict(coded(a).state_dict())
+
+
+def test_moments_of_32_bits_go_by_element():
+    import kernels
+    a, b = leaf((5, 300), (1, 0)), leaf((5, 300), (0, 1))
+    opt, other = kernels.AdamW([a]), kernels.AdamW([b])
+    opt.state[a] = opt._new_state(a, 32)
+    opt.state[a]["exp_avg"].copy_(torch.randn(5, 300))
+    other.load_state_dict(opt.state_dict())
+    assert torch.equal(other.state[b]["exp_avg"], opt.state[a]["exp_avg"]) and other.state[b]["exp_avg"].stride() == b.stride()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_parameter_that_changes_its_layout_is_refused(bits):
+    import kernels
+    p = leaf((5, 300), (0, 1), "cuda").detach().requires_grad_(True)
+    opt = kernels.AdamW([p], state_bits=bits)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    kept, was = p.data, p.detach().clone()
+    p.grad = None
+    p.data = kept.t().contiguous().t()
+    p.grad = torch.ones_like(p)
+    with pytest.raises(ValueError, match="laid out"):
+        opt.step()
+    if bits == 8:
+        with pytest.raises(ValueError, match="laid out"):
+            opt.moments()
+    assert torch.equal(p, was) and int(opt.state[p]["step"]) == 1
+    p.grad = None
+    p.data = kept
+    p.grad = torch.ones_like(p)
+    opt.step()
+    assert int(opt.state[p]["step"]) == 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", [(1, 0), (0, 1)])
+def test_a_loaded_transposed_parameter_steps_on(order):
+    """Saved, loaded and stepped: the moments by element are those of the optimizer that went on."""
+    import kernels
+    g = torch.Generator().manual_seed(2)
+    a, b = (leaf((33, 40), order, "cuda").detach().requires_grad_(True) for _ in range(2))
+    one, two = (kernels.AdamW([p], lr=0.1, state_bits=8) for p in (a, b))
+    a.grad = torch.randn(33, 40, generator=g).cuda()
+    one.step()
+    two.load_state_dict(one.state_dict())
+    b.data.copy_(a.data)
+    a.grad = torch.randn(33, 40, generator=g).cuda()
+    b.grad = a.grad.clone()
+    one.step(), two.step()
+    assert torch.equal(a, b)
+    for x, y in zip(one.moments()[0], two.moments()[0]):
+        assert torch.equal(x, y) and x.stride() == a.stride()
+    flat = a.t() if order == (1, 0) else a
+    m = orc.moment_values(one.state[a]["exp_avg"], one.state[a]["exp_avg_exps"], 14, False, a.numel()).view(flat.shape)
+    assert torch.equal(one.moments()[0][0].cpu().double(), m.t() if order == (1, 0) else m)
