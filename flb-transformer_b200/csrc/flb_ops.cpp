@@ -5,6 +5,7 @@
 // documentation and their torch.func rules. There is no CPU path.
 #include <torch/extension.h>
 #include <c10/core/AutogradState.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -812,15 +813,24 @@ pybind11::list adamw(pybind11::list params, pybind11::dict state, int64_t bits, 
     for (const Tensor* x : {&p, &m, &v, &step}) written.push_back(*x);
   }
   if (pybind11::len(missing)) return missing;
+  std::vector<Tensor> words;
   for (Together& x : all) {
     same_device(x.like, lr_device);
     const c10::cuda::CUDAGuard guard(x.device);
-    // a word of the kernel's own on each device, zero between steps
+    // A word of the kernel's own on each device, zero between steps. Not made in a capture, which would only record that it is cleared.
     const pybind11::int_ key(x.device.index());
-    if (!counters.contains(key)) counters[key] = pybind11::cast(at::zeros({1}, x.like.options().dtype(at::kInt).requires_grad(false)));
-    const Tensor counter = counters[key].cast<Tensor>();
+    if (!counters.contains(key)) {
+      TORCH_CHECK(c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None,
+                  "AdamW: the first step on a device makes a word of the kernel's there: take one before the capture");
+      counters[key] = pybind11::cast(at::zeros({1}, x.like.options().dtype(at::kInt).requires_grad(false)));
+    }
+    words.push_back(counters[key].cast<Tensor>());
+  }
+  for (size_t i = 0; i < all.size(); ++i) {
+    Together& x = all[i];
+    const c10::cuda::CUDAGuard guard(x.device);
     check(flb_adamw(x.t.data(), (int64_t)x.t.size(), dtype_of(x.type, "a parameter"), (int)bits, lr, (const float*)ptr(lr_device), b1, b2, eps, decay, seed,
-                    (uint32_t*)counter.data_ptr(), stream_of(x.like)),
+                    (uint32_t*)words[i].data_ptr(), stream_of(x.like)),
           "flb_adamw");
   }
   // written behind autograd's back: a graph that still needs the old values is told

@@ -19,7 +19,7 @@ the same, and into another one is refused. (Moments in 32 bits are loaded by ele
 
 Steps are counted on the device, each tensor's own (its "step", an int64), so that a captured step counts on in every replay;
 lr may be a float32 tensor on the device, which a schedule then writes between replays. The first step of a tensor makes its
-state, and is not for a capture. Steps of one optimizer must not overlap on the GPU. The kernels are in libflb_b200.so
+state, and is not for a capture; with state that was loaded or copied a capture may be an optimizer's first step. Steps of one optimizer must not overlap on the GPU. The kernels are in libflb_b200.so
 (flb_adamw, flb_adamw_moments), called through flb_ops; CUDA tensors only.
 """
 from __future__ import annotations
@@ -72,6 +72,11 @@ class AdamW(torch.optim.Optimizer):
         for group in self.param_groups:
             group.setdefault("state_bits", 32)
             group.setdefault("seed", 0)
+        # State that was loaded or copied may take its first step in a capture, which must not make the kernel's word on its device.
+        counters = self.__dict__.setdefault("_counters", {})
+        for p, s in self.__dict__.get("state", {}).items():
+            if s and isinstance(p, torch.Tensor) and p.is_cuda and p.device.index not in counters and not torch.cuda.is_current_stream_capturing():
+                counters[p.device.index] = torch.zeros(1, dtype=torch.int32, device=p.device)
 
     def _new_state(self, p, bits):
         state = {"step": torch.zeros((), dtype=torch.int64, device=p.device)}

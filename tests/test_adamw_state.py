@@ -128,3 +128,52 @@ def test_a_loaded_transposed_parameter_steps_on(order):
     flat = a.t() if order == (1, 0) else a
     m = orc.moment_values(one.state[a]["exp_avg"], one.state[a]["exp_avg_exps"], 14, False, a.numel()).view(flat.shape)
     assert torch.equal(one.moments()[0][0].cpu().double(), m.t() if order == (1, 0) else m)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("how", ["loaded", "copied"])
+def test_a_capture_is_the_first_step_of_loaded_state(how, bits):
+    """Captured first, then stepped eagerly before any replay, then replayed and stepped again: as many eager steps."""
+    import kernels
+    g = torch.Generator().manual_seed(3)
+    shapes = [(70000,), (129, 3)]  # more blocks than one
+    start = [torch.randn(s, generator=g).cuda().requires_grad_(True) for s in shapes]
+    first = kernels.AdamW(start, lr=0.1, state_bits=bits)
+    for p in start:
+        p.grad = torch.randn(p.shape, generator=g).cuda()
+    first.step()
+    if how == "copied":
+        opt, twin = copy.deepcopy(first), copy.deepcopy(first)
+    else:
+        opt, twin = (kernels.AdamW([p.detach().clone().requires_grad_(True) for p in start], state_bits=bits) for _ in range(2))
+        opt.load_state_dict(first.state_dict()), twin.load_state_dict(first.state_dict())
+    pairs = list(zip(opt.param_groups[0]["params"], twin.param_groups[0]["params"], start))
+    for p, q, s in pairs:
+        p.grad, q.grad = s.grad.clone(), s.grad.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for n, do in enumerate((opt.step, graph.replay, graph.replay, opt.step, graph.replay), 2):
+        do()
+        twin.step()
+        for p, q, _ in pairs:
+            assert int(opt.state[p]["step"]) == n and int(twin.state[q]["step"]) == n and torch.equal(p, q)
+    for x, y in zip(opt.moments(), twin.moments()):
+        assert torch.equal(x[0], y[0]) and torch.equal(x[1], y[1])
+
+
+@pytest.mark.gpu
+def test_a_capture_does_not_make_the_kernels_word():
+    """State put in place by hand: there is no word yet, and a capture cannot make one. The step itself is refused, and one outside goes on."""
+    import kernels
+    p = torch.zeros(500, device="cuda", requires_grad=True)
+    p.grad = torch.ones_like(p)
+    opt = kernels.AdamW([p])
+    opt.state[p] = opt._new_state(p, 32)
+    with pytest.raises(RuntimeError, match="before the capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    assert not opt._counters
+    opt.step()
+    assert int(opt.state[p]["step"]) == 1 and (p < 0).all()
