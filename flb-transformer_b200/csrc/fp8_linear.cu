@@ -431,9 +431,14 @@ __global__ void __launch_bounds__(threads<NC>(), 1)
         tmem_wait_ld();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) B::arrive_first(&acc_empty[b]);
+        // (a warp that has given up no longer stands in for one that is still reading: the MMAs then end too)
+        if (lane == 0 && ok) B::arrive_first(&acc_empty[b]);
 #pragma unroll
         for (int j = 0; j < 32; ++j) sum[32 + j] = k == k0 ? __uint_as_float(v[j]) : sum[32 + j] + __uint_as_float(v[j]);
+      }
+      if (!ok) {  // what did not come is NaN, for callers that do not wait for the error word: a training step sees it in its loss
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) sum[j] = __uint_as_float(0x7fffffffu);
       }
       if (a.splits > 1) {
         const int tile = u / a.splits, split = u % a.splits;

@@ -18,9 +18,9 @@ along the tokens; db is the plain sum of dy. x and W are kept for the backward p
 there are no gradients. Products are in float32: over 1024 of K as the tensor core adds, which cuts, and between
 those rounded. The same inputs give the same bits.
 
-The kernels' waits for their own copies and products are bounded (4 s). check_timeout (inference only) waits for the
-product and raises a RuntimeError if one of them gave up, where the output is wrong; without it the call returns at once
-and nothing is said.
+The kernels' waits for their own copies and products are bounded (4 s). Where one gave up, the outputs (or gradients) that
+it held up are NaN. check_timeout (inference only) also waits for the product and raises a RuntimeError then; without it
+the call returns at once.
 
 The kernels are in libflb_b200.so (flb_fp8_rows, flb_fp8_rows2, flb_fp8_linear: tcgen05 kind::mxf8f6f4), called through
 flb_ops; CUDA tensors only. torch.func transforms are refused.

@@ -509,7 +509,8 @@ int flb_fp8_rows2(const void* x, int64_t ldx, void* codes, uint8_t* exps, void* 
 /* out[m, n] = sum_k X[m, k] W[n, k] + bias[n], contiguous [M, N] in dtype, in float32 (the tensor core's over 1024 of K, their sum
  * rounded). X: codes (pitch ldc) and exps, or x [M, K] in dtype (pitch ldx elements), made into 8-bit rows on the
  * way. W: codes [N, K] (pitch ldw) and exps. Pitches are multiples of 16, codes and exps 16-byte aligned. bias: [N] in
- * bias_dtype, or NULL. Workspace, check_timeout: as flb_int8_linear. The same bits every time. */
+ * bias_dtype, or NULL. Workspace, check_timeout: as flb_int8_linear; outputs that a wait which gave up has held
+ * up are NaN. The same bits every time. */
 size_t flb_fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int x_is_codes);
 int flb_fp8_linear(const void* x, int64_t ldx, const void* x_codes, int64_t ldc, const uint8_t* x_exps, const void* w_codes,
                    int64_t ldw, const uint8_t* w_exps, const void* bias, int bias_dtype, void* out, int64_t M, int64_t N,
