@@ -61,6 +61,11 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("eps and weight_decay must be at least 0")
         if group["state_bits"] not in (8, 32):
             raise ValueError(f"state_bits must be 8 or 32, not {group['state_bits']}")
+        for name in ("maximize", "amsgrad"):
+            if group.get(name):
+                raise ValueError(f"AdamW has no {name}")
+        if group["weight_decay"] > 0 and not group.get("decoupled_weight_decay", True):
+            raise ValueError("AdamW's weight_decay is decoupled from the moments (decoupled_weight_decay=False)")
         if len(set(map(id, group["params"]))) != len(group["params"]):
             raise ValueError("a parameter is in the group twice")
         for p in group["params"]:
@@ -147,27 +152,41 @@ class AdamW(torch.optim.Optimizer):
                 found.append(pair)
         return found
 
+    @staticmethod
+    def _check_state(s, p, bits):
+        """Refuses state that is not a parameter's of p's shape: copied in, it could be repeated to fill it."""
+        if ("exp_avg_exps" in s) != (bits == 8):
+            raise ValueError("the state's moments are not of the bits that its group says")
+        blocks = -(-p.numel() // 128)
+        want = {"step": None}
+        for name in ("exp_avg", "exp_avg_sq"):
+            want.update({name: (blocks, 128), name + "_exps": (blocks,)} if bits == 8 else {name: tuple(p.shape)})
+        for name, shape in want.items():
+            if name not in s:
+                raise ValueError(f"the state has no {name}")
+            t = torch.as_tensor(s[name])
+            if t.numel() != 1 if shape is None else tuple(t.shape) != shape or (bits == 8 and t.dtype != torch.uint8):
+                raise ValueError(f"the state's {name}, of shape {tuple(t.shape)} and {t.dtype}, is not that of a parameter of shape {tuple(p.shape)}")
+        if bits == 8:
+            AdamW._check_order(s, p)
+
     @torch.no_grad()
     def load_state_dict(self, state_dict: dict) -> None:
-        """As torch's, but the state keeps its types. Moments in 32 bits may come from torch.optim.AdamW."""
-        for saved in state_dict["param_groups"]:
-            for key in saved["params"]:
-                s = state_dict["state"].get(key)
-                if s and ("exp_avg_exps" in s) != (saved.get("state_bits", 32) == 8):
-                    raise ValueError("the state's moments are not of the bits that its group says")
+        """As torch's, but the state keeps its types. Moments in 32 bits may come from torch.optim.AdamW. What is refused leaves the
+        optimizer as it was."""
         for group, saved in zip(self.param_groups, state_dict["param_groups"]):
+            saved = {"state_bits": 32, "seed": 0, **saved}
+            self._check({**saved, "params": group["params"]})
             for p, key in zip(group["params"], saved["params"]):
-                s = state_dict["state"].get(key)
-                if s and "exp_avg_exps" in s:
-                    self._check_order(s, p)
+                if state_dict["state"].get(key):
+                    self._check_state(state_dict["state"][key], p, saved["state_bits"])
         super().load_state_dict(state_dict)
         for group, saved in zip(self.param_groups, state_dict["param_groups"]):
-            self._check(group)
             for p, key in zip(group["params"], saved["params"]):
-                if key not in state_dict["state"] or not state_dict["state"][key]:
+                if not state_dict["state"].get(key):
                     continue
                 s, mine = state_dict["state"][key], self._new_state(p, group["state_bits"])
                 for name, t in mine.items():
                     if isinstance(t, torch.Tensor):
-                        t.copy_(torch.as_tensor(s[name]))
+                        t.copy_(torch.as_tensor(s[name]).reshape(t.shape))
                 self.state[p] = mine

@@ -177,3 +177,92 @@ def test_a_capture_does_not_make_the_kernels_word():
     assert not opt._counters
     opt.step()
     assert int(opt.state[p]["step"]) == 1 and (p < 0).all()
+
+
+def torch_dict(p, **kw):
+    """A dict of torch's optimizer after a step of a parameter like p."""
+    q = p.detach().clone().requires_grad_(True)
+    opt = torch.optim.AdamW([q], lr=0.25, **kw)
+    q.grad = torch.ones_like(q)
+    opt.step()
+    return opt.state_dict()
+
+
+def spoiled(saved, group=None, **state):
+    """The dict with other options of its group, or other entries of its state (None: without)."""
+    saved = copy.deepcopy(saved)
+    saved["param_groups"][0].update(group or {})
+    for name, value in state.items():
+        if value is None:
+            del saved["state"][0][name]
+        else:
+            saved["state"][0][name] = value
+    return saved
+
+
+def refuses(opt, saved, match):
+    """ValueError, with the optimizer as it was, its groups and its state."""
+    before = copy.deepcopy(opt.state_dict())
+    with pytest.raises(ValueError, match=match):
+        opt.load_state_dict(saved)
+    after = opt.state_dict()
+    assert after["param_groups"] == before["param_groups"] and list(after["state"]) == list(before["state"])
+    for key, s in before["state"].items():
+        assert set(s) == set(after["state"][key])
+        for name, x in s.items():
+            assert torch.equal(x, after["state"][key][name]) if isinstance(x, torch.Tensor) else x == after["state"][key][name]
+
+
+def test_options_that_there_are_not_are_refused():
+    import kernels
+    p = leaf((4, 6))
+    for opt in (kernels.AdamW([p], lr=0.5), coded(p)):
+        for kw in ({"maximize": True}, {"amsgrad": True}):
+            refuses(opt, torch_dict(p, **kw), next(iter(kw)))
+        # torch.optim.Adam's decay goes through the moments
+        refuses(opt, spoiled(torch_dict(p), {"decoupled_weight_decay": False}), "decoupled")
+    for kw in ({"maximize": True}, {"amsgrad": True}):
+        with pytest.raises(ValueError, match=next(iter(kw))):
+            kernels.AdamW([{"params": [p], **kw}])
+    opt = kernels.AdamW([p])
+    for saved in (torch_dict(p), spoiled(torch_dict(p), {"decoupled_weight_decay": False, "weight_decay": 0.0})):
+        opt.load_state_dict(saved)
+        assert opt.param_groups[0]["lr"] == 0.25 and torch.equal(opt.state[p]["exp_avg"], saved["state"][0]["exp_avg"])
+
+
+def test_values_out_of_range_are_refused():
+    import kernels
+    p = leaf((4, 6))
+    for opt in (kernels.AdamW([p], lr=0.5), coded(p)):
+        for bad, match in (({"lr": -1.0}, "lr"), ({"betas": (1.0, 0.9)}, "betas"), ({"eps": -1.0}, "eps"), ({"weight_decay": -1.0}, "weight_decay")):
+            refuses(opt, spoiled(torch_dict(p), bad), match)
+
+
+@pytest.mark.parametrize("shape", [(1,), (1, 6), (4, 1), (6, 4), (4, 6, 1), ()])
+def test_moments_of_another_shape_are_refused(shape):
+    """Also where they could be repeated to fill the parameter's."""
+    import kernels
+    p = leaf((4, 6))
+    for name in ("exp_avg", "exp_avg_sq"):
+        refuses(kernels.AdamW([p], lr=0.5), spoiled(torch_dict(p), **{name: torch.ones(shape)}), name)
+    refuses(kernels.AdamW([p]), spoiled(torch_dict(p), exp_avg=None), "exp_avg")
+    refuses(kernels.AdamW([p]), spoiled(torch_dict(p), step=torch.zeros(2)), "step")
+
+
+def test_codes_of_another_shape_or_type_are_refused():
+    p, q = leaf((4, 60)), leaf((3, 100))
+    saved = coded(q).state_dict()
+    for bad, match in (({"exp_avg": torch.ones(1, 128, dtype=torch.uint8)}, "exp_avg"), ({"exp_avg_sq": torch.ones(3, 1, dtype=torch.uint8)}, "exp_avg_sq"),
+                       ({"exp_avg_exps": torch.ones(1, dtype=torch.uint8)}, "exp_avg_exps"), ({"exp_avg_sq": torch.ones(3, 128)}, "exp_avg_sq"),
+                       ({"exp_avg_sq_exps": None}, "exp_avg_sq_exps"), ({"step": torch.zeros(3)}, "step")):
+        refuses(coded(q, 7), spoiled(saved, **bad), match)
+    refuses(coded(p), saved, "exp_avg")  # 300 elements' for 240
+
+
+def test_a_step_count_of_any_kind_is_taken():
+    import kernels
+    p = leaf((4, 6))
+    opt = kernels.AdamW([p])
+    for step in (7, 7.0, torch.tensor(7.0), torch.tensor([7])):
+        opt.load_state_dict(spoiled(torch_dict(p), step=step))
+        assert int(opt.state[p]["step"]) == 7 and opt.state[p]["step"].dtype == torch.int64 and opt.state[p]["step"].shape == ()
