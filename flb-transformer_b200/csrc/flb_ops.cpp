@@ -758,6 +758,10 @@ struct Together {
 // A step of every parameter that has a gradient. Returns those that have no state yet: then nothing has been done.
 pybind11::list adamw(pybind11::list params, pybind11::dict state, int64_t bits, double lr, const Opt& lr_device, double b1, double b2, double eps,
                      double decay, uint32_t seed, pybind11::dict counters) {
+  // (a group's lr may have been put in another's place since the optimizer was made)
+  TORCH_CHECK_VALUE(!given(lr_device) || (lr_device->scalar_type() == at::kFloat && lr_device->numel() == 1),
+                    "AdamW: lr on the device must be one float32, not ", given(lr_device) ? lr_device->numel() : 0, " of ",
+                    given(lr_device) ? lr_device->scalar_type() : at::kFloat);
   pybind11::list missing;
   std::vector<Together> all;
   std::vector<Tensor> written;

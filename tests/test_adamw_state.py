@@ -266,3 +266,29 @@ def test_a_step_count_of_any_kind_is_taken():
     for step in (7, 7.0, torch.tensor(7.0), torch.tensor([7])):
         opt.load_state_dict(spoiled(torch_dict(p), step=step))
         assert int(opt.state[p]["step"]) == 7 and opt.state[p]["step"].dtype == torch.int64 and opt.state[p]["step"].shape == ()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [lambda: torch.tensor(0.1, dtype=torch.float64), lambda: torch.tensor(0.1, dtype=torch.bfloat16), lambda: torch.zeros(0),
+                                 lambda: torch.zeros(2), lambda: torch.tensor(1)], ids=["f64", "bf16", "none", "two", "int"])
+def test_another_lr_on_the_device_is_checked(bad):
+    """The kernel reads one float32: what a schedule puts in lr's place has to be one."""
+    import kernels
+    p = torch.ones(100, device="cuda", requires_grad=True)
+    opt = kernels.AdamW([p], lr=torch.tensor(0.1, device="cuda"))
+    p.grad = torch.ones_like(p)
+    opt.step()
+    was = p.detach().clone()
+    opt.param_groups[0]["lr"] = bad().cuda()
+    with pytest.raises(ValueError, match="one float32"):
+        opt.step()
+    assert torch.equal(p, was) and int(opt.state[p]["step"]) == 1
+
+
+def test_the_lr_that_a_kernel_would_read():
+    import flb_ops
+    for bad in (torch.tensor(0.1, dtype=torch.float64), torch.zeros(0), torch.zeros(3)):
+        with pytest.raises(ValueError, match="one float32"):
+            flb_ops.adamw([], {}, 32, 0.0, bad, 0.9, 0.999, 1e-8, 0.0, 0, {})
+    for good in (None, torch.tensor(0.1), torch.tensor([0.1])):
+        assert flb_ops.adamw([], {}, 32, 0.0, good, 0.9, 0.999, 1e-8, 0.0, 0, {}) == []
