@@ -125,9 +125,14 @@ class AdamW(torch.optim.Optimizer):
                         raise RuntimeError(f"AdamW runs on CUDA tensors only (sm_100a kernels; no CPU path); got a parameter on {p.device}")
                 if torch.cuda.is_current_stream_capturing():
                     raise RuntimeError("AdamW: the first step of a parameter makes its state: take one before the capture")
-                for p in new:
-                    self.state[p].update(self._new_state(p, group["state_bits"]))
-                flb_ops.adamw(*args)
+                try:
+                    for p in new:
+                        self.state[p].update(self._new_state(p, group["state_bits"]))
+                    flb_ops.adamw(*args)
+                except Exception:
+                    for p in new:  # a step that was refused was not the first one
+                        self.state.pop(p, None)
+                    raise
         return loss
 
     @torch.no_grad()

@@ -292,3 +292,23 @@ def test_the_lr_that_a_kernel_would_read():
             flb_ops.adamw([], {}, 32, 0.0, bad, 0.9, 0.999, 1e-8, 0.0, 0, {})
     for good in (None, torch.tensor(0.1), torch.tensor([0.1])):
         assert flb_ops.adamw([], {}, 32, 0.0, good, 0.9, 0.999, 1e-8, 0.0, 0, {}) == []
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_refused_first_step_leaves_no_state(bits):
+    import kernels
+    good = torch.ones(300, device="cuda", requires_grad=True)
+    good.grad = torch.ones_like(good)
+    gaps = torch.ones(40, 8, device="cuda")[:, :3].requires_grad_(True)
+    gaps.grad = torch.ones_like(gaps)
+    sparse = torch.ones(40, 8, device="cuda", requires_grad=True)
+    sparse.grad = torch.ones(40, 8, device="cuda").to_sparse()
+    for bad, match in ((gaps, "gaps"), (sparse, "sparse")):
+        opt = kernels.AdamW([good, bad], state_bits=bits)
+        with pytest.raises(ValueError, match=match):
+            opt.step()
+        assert not opt.state and opt.moments() == [] and (good == 1).all() and (bad == 1).all()
+    sparse.grad = torch.ones_like(sparse)
+    opt.step()
+    assert [int(opt.state[p]["step"]) for p in (good, sparse)] == [1, 1] and (good < 1).all() and (sparse < 1).all()
