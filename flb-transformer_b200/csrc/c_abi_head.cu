@@ -5,7 +5,8 @@
 
 namespace flb {
 
-int fp8_rows(const void* x, int64_t ldx, int8_t* codes, uint8_t* exps, int64_t R, int64_t K, int dtype, uint32_t* zero, int n_zero, cudaStream_t s);
+int fp8_rows(const void* x, int64_t ldx, int8_t* codes, uint8_t* exps, int64_t R, int64_t K, int dtype, bool whole, uint32_t* zero, int n_zero,
+             cudaStream_t s);
 int fp8_rows2(const void* x, int64_t ldx, int8_t* codes, uint8_t* exps, int8_t* codes_t, uint8_t* exps_t, float* sums, void* bias_grad,
               int bias_dtype, int64_t R, int64_t C, int dtype, cudaStream_t s);
 size_t fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, bool quantise);
@@ -97,7 +98,7 @@ int flb_fp8_rows(const void* x, int64_t ldx, void* codes, uint8_t* exps, int64_t
   if (st != FLB_OK || R == 0) return st;
   if (!x || !codes || !exps || ldx < 0) return fail(FLB_ERR_SHAPE, "fp8_rows: null x, codes or exps, or a negative pitch");
   if (off(x, es) || off(codes, 16) || off(exps, 16)) return fail(FLB_ERR_ALIGN, "fp8_rows: codes and exps must be 16-byte aligned, x to its elements");
-  return fp8_rows(x, ldx, static_cast<int8_t*>(codes), exps, R, K, dtype, nullptr, 0, as_stream(stream));
+  return fp8_rows(x, ldx, static_cast<int8_t*>(codes), exps, R, K, dtype, true, nullptr, 0, as_stream(stream));
 }
 
 size_t flb_fp8_rows2_workspace_bytes(int64_t R, int64_t C) { return R < 1 || C < 1 ? 0 : (size_t)(fp8::blocks_of(R) * C) * 4; }

@@ -632,7 +632,8 @@ constexpr size_t kOutputInL2 = 64 << 20;
 
 }  // namespace
 
-int fp8_rows(const void* x, int64_t ldx, int8_t* codes, uint8_t* exps, int64_t R, int64_t K, int dtype, uint32_t* zero, int n_zero, cudaStream_t s);
+int fp8_rows(const void* x, int64_t ldx, int8_t* codes, uint8_t* exps, int64_t R, int64_t K, int dtype, bool whole, uint32_t* zero, int n_zero,
+             cudaStream_t s);
 
 size_t fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, bool quantise) { return ws_of(shape_of(M, N, K), M, K, quantise).bytes; }
 
@@ -648,7 +649,7 @@ int fp8_linear(const void* x, int64_t ldx, const int8_t* x_codes, int64_t ldc, c
   if (x) {
     // the rows' kernel clears the error word and the counts too
     int8_t* const codes = reinterpret_cast<int8_t*>(p + l.codes);
-    if ((st = fp8_rows(x, ldx, codes, p + l.exps, M, K, dtype, reinterpret_cast<uint32_t*>(p), n_zero, s)) != FLB_OK) return st;
+    if ((st = fp8_rows(x, ldx, codes, p + l.exps, M, K, dtype, false, reinterpret_cast<uint32_t*>(p), n_zero, s)) != FLB_OK) return st;
     x_codes = codes, x_exps = p + l.exps, ldc = rows::code_pitch(K);
   } else if (reset) {  // otherwise nothing reads those words
     if ((st = check_cuda(cudaMemsetAsync(p, 0, (size_t)n_zero * 4, s), "fp8_linear reset")) != FLB_OK) return st;

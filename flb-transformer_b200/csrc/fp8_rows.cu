@@ -76,6 +76,7 @@ struct RowsArgs {
   int64_t ldx, R, K, pitch, quads;
   int8_t* codes;
   uint8_t* exps;
+  bool whole;      // zeros in the places of exps that no block has
   uint32_t* zero;  // words to clear, or null
   int n_zero;
 };
@@ -96,6 +97,12 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(256) rows_kern
   if (!there) return;
   store_codes(a.codes + row * a.pitch, v, inverse_of(u), block * kBlock + lane * N, a.pitch);
   if (lane == 0) a.exps[exp_at(row, block, a.quads)] = (uint8_t)u;
+  if (a.whole) {
+    // the last block's threads write those behind it, to the end of its four, the last row's those of the rows to the next 128
+    const int64_t blocks_to = block == blocks - 1 ? a.quads * 4 : block + 1, rows_to = row == a.R - 1 ? blocks_of(a.R) * kBlock : row + 1;
+    for (int64_t r = row + lane; r < rows_to; r += PER)
+      for (int64_t b = r == row ? block + 1 : block; b < blocks_to; ++b) a.exps[exp_at(r, b, a.quads)] = 0;
+  }
 }
 
 struct TileArgs {
@@ -278,9 +285,9 @@ template <typename T> int tiles_t(const TileArgs& a, void* bias_grad, int bias_d
 
 }  // namespace
 
-int fp8_rows(const void* x, int64_t ldx, int8_t* codes, uint8_t* exps, int64_t R, int64_t K, int dtype, uint32_t* zero, int n_zero,
+int fp8_rows(const void* x, int64_t ldx, int8_t* codes, uint8_t* exps, int64_t R, int64_t K, int dtype, bool whole, uint32_t* zero, int n_zero,
              cudaStream_t s) {
-  const RowsArgs a{x, ldx, R, K, rows::code_pitch(K), quads_of(K), codes, exps, zero, n_zero};
+  const RowsArgs a{x, ldx, R, K, rows::code_pitch(K), quads_of(K), codes, exps, whole, zero, n_zero};
   switch (dtype) {
     case FLB_F32: return rows_t<float>(a, s);
     case FLB_F16: return rows_t<__half>(a, s);

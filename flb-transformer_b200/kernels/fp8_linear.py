@@ -41,8 +41,8 @@ __all__ = ["Fp8Rows", "quantize_fp8", "fp8_linear", "Fp8Linear", "Fp8LinearKept"
 
 class Fp8Rows(NamedTuple):
     """Rows in 8-bit floating point: codes float8_e4m3fn [..., K], exps uint8 [ceil(rows / 128), ceil(K / 512), 32, 4, 4] (of
-    row r and block b at [r // 128, b // 4, r % 32, r // 32 % 4, b % 4], with 2 ** (byte - 127) as the unit; other places
-    hold nothing), and the type they had. Codes whose rows start on 16 bytes, as quantize_fp8 lays them out, are read in
+    row r and block b at [r // 128, b // 4, r % 32, r // 32 % 4, b % 4], with 2 ** (byte - 127) as the unit; zeros in
+    other places), and the type they had. Codes whose rows start on 16 bytes, as quantize_fp8 lays them out, are read in
     place; others are copied by every call that reads them."""
     codes: torch.Tensor
     exps: torch.Tensor

@@ -496,7 +496,8 @@ int flb_int8_linear_wait_test(const void* x, int64_t ldx, const int8_t* x_codes,
  * from K to the pitch are written with whatever), and exps, flb_fp8_exps_bytes(R, K) bytes, 16-byte aligned: for each
  * block of 128 elements of a row the smallest power of two 2^(byte - 127), byte >= 0, in units of which the block's
  * largest magnitude is at most 448; 255 where the block held an infinity or NaN: it counts as NaN. The byte of row r, block b
- * lies at ((r / 128) ceil(blocks / 4) + b / 4) 512 + (r % 32) 16 + (r / 32 % 4) 4 + b % 4, as the tensor core reads them.
+ * lies at ((r / 128) ceil(blocks / 4) + b / 4) 512 + (r % 32) 16 + (r / 32 % 4) 4 + b % 4, as the tensor core reads them;
+ * flb_fp8_rows writes zeros to the places that no block has.
  * ------------------------------------------------------------------------------------------ */
 size_t flb_fp8_exps_bytes(int64_t R, int64_t K);
 int flb_fp8_rows(const void* x, int64_t ldx, void* codes, uint8_t* exps, int64_t R, int64_t K, int dtype, void* stream);
