@@ -4,7 +4,7 @@
 // tcgen05.mma kind::mxf8f6f4 with a block scale: the tensor core multiplies by the powers of two as it goes (they lie in
 // tensor memory, a byte for each row and block; the instruction's scale of 32 elements is given four times the same
 // byte). One block a SM, persistent over units of work: a tile of 128 tokens and 64, 128 or 192 channels, or a part of its
-// K range. Warp 0 loads by TMA into a ring of four steps of 128 of K, warp 1 issues the MMAs, the others read TMEM:
+// K range. Warp 0 loads by TMA into a ring of four steps of 128 of K (pairs: five), warp 1 issues the MMAs, the others read TMEM:
 // each has 32 tokens, a lane a token, and 64 channels, in registers.
 //
 // For many tiles two blocks of a cluster share one of 256 tokens (cta_group::2) and load a third less for it.
@@ -13,8 +13,9 @@
 // their size too small. So an accumulator takes 1024 of K, and the warps add up those sums in float32, rounded.
 // Two accumulators: one is read while the other is filled.
 //
-// Measured: 8192 x 8192 x 8192 in 406 us, 2.71 PFLOP/s, 1.65 times the bf16 product's measured rate: bound by what L2 gives the SMs;
-// 16384 x 768 x 32000 in 463, of which 160 would write the output alone; 1 x 768 x 32000 in 8.8 us with the weight in L2, 3.8 us of
+// Measured: 8192 x 8192 x 8192 in 406 us, 2.71 PFLOP/s, 1.65 times the bf16 product's measured rate: bound by the tensor cores, 79% busy at the 1.49 GHz
+// to which the power limit takes the clock (L2 53%). 16384 x 768 x 32000 in 463, held up by its output: a plain fill of the output's 1.05 GB
+// takes 273, this product with a K of 128 345, and each further 128 of K another 25, half of what its MMAs take. 1 x 768 x 32000 in 8.8 us with the weight in L2, 3.8 us of
 // it the weight's bytes from memory: a chain of latencies and a second round of tiles.
 #include <cmath>
 #include "fp8.cuh"

@@ -5,10 +5,12 @@
 // these the ones with w_i >= min_p. The token is the first, in the vocabulary's order, at which the sum of kept weights
 // passes u of the whole.
 //
-// Which token comes depends on sums next to a border, so they are exact: a weight is computed in float64 and held
-// as a 64-bit integer in units of 2^-F, F as large as the sum over the vocabulary allows (47 for 32000 tokens). Integer
-// sums do not depend on their order, and differ from the real ones by 2^-48 a token: one draw in 10^7 falls in between.
-// (In float32 it would be one in 200.)
+// Which token comes depends on sums next to a border: a weight is computed in float64 and held as a 64-bit integer in units of
+// 2^-F, F as large as the sum over the vocabulary allows (47 for 32000 tokens, 44 for 262144). Integer sums do not depend on their order.
+// A weight w is off by at most 4e-14 w and half a unit, so a few draws fall between a border and the real one: with this arithmetic
+// against 113 bits, normal logits of deviation 0.5 to 6 at temperatures from 0.5 to 2, at most 7e-9 of them at 32000 tokens, 1e-6 at
+// 131071 and 7e-6 at 262144 (most where one token has nearly all of the weight and the others next to none). (In float32 it
+// would be one in 200.)
 //
 // A row is worked on by a block, or by a cluster of up to eight, which holds its logits in shared memory where they fit. What is kept is
 // all up to one token in the order from the largest logit down, equal ones by index: the limit. It is found without sorting:
@@ -16,8 +18,9 @@
 // token lies, or the one at which the sum passes p; the few logits of that step (or, with a small top_k, all from the top to
 // there, and then nothing else is looked at again) go into a list, where each counts those before it. Steps too full for the
 // list, or the last one, which is open, go through digits of the logits, as integers of the same order, and of the indices instead.
-// Bound by the arithmetic of the weights, 15 float64 operations a logit (at half float32's rate) and about as many others, and
-// with few rows by barriers, 0.6 us for each of a cluster's: 1 x 32000 bf16 with top_k 50 and top_p 0.95 10.3 us, 256 rows with
+// Bound by instructions where all logits are weighed (an SM issues in 63% of the cycles of 256 rows with top_p, of which the float64 pipe, with 15
+// operations a logit, has 17%; 46% and 27% with min_p over 131071) and by what hides their latency, 1.7 blocks an SM; with few rows by
+// barriers, 0.6 us for each of a cluster's: 1 x 32000 bf16 with top_k 50 and top_p 0.95 10.3 us, 256 rows with
 // top_p 0.9 56 us, 64 x 131071 float32 with min_p 29 us, which is 1.1 TB/s.
 #include <cooperative_groups.h>
 #include <cfloat>

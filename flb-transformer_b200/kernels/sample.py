@@ -12,8 +12,9 @@ uniform number in [0, 1) a row, is all the randomness there is: the same u gives
 gives the largest logit, of equal ones the lowest index. A row whose logits are all -inf (all masked), or with a NaN
 among them, gives -1; logits of +inf share all of the probability.
 
-Weights are float64 and summed as 64-bit integers in units of 2^-47 (at 32000 tokens), so that a token next to a
-border is the one of the definition. Vocabularies of up to 262144. The kernel is in libflb_b200.so (flb_sample),
+Weights are float64 and summed as 64-bit integers in units of 2^-47 (at 32000 tokens; 2^-44 at 262144), each within
+4e-14 of itself and half a unit of the definition's: over normal logits at most 7 draws in 10^9 gave another
+token than the definition, 7 in 10^6 at 262144. Vocabularies of up to 262144. The kernel is in libflb_b200.so (flb_sample),
 called through flb_ops; CUDA tensors only.
 """
 from __future__ import annotations
