@@ -177,17 +177,15 @@ class AdamW(torch.optim.Optimizer):
         if bits == 8:
             AdamW._check_order(s, p)
 
-    @torch.no_grad()
-    def load_state_dict(self, state_dict: dict) -> None:
-        """As torch's, but the state keeps its types. Moments in 32 bits may come from torch.optim.AdamW. What is refused leaves the
-        optimizer as it was."""
+    def _check_saved(self, state_dict):
         for group, saved in zip(self.param_groups, state_dict["param_groups"]):
             saved = {"state_bits": 32, "seed": 0, **saved}
             self._check({**saved, "params": group["params"]})
             for p, key in zip(group["params"], saved["params"]):
                 if state_dict["state"].get(key):
                     self._check_state(state_dict["state"][key], p, saved["state_bits"])
-        super().load_state_dict(state_dict)
+
+    def _take_state(self, state_dict):
         for group, saved in zip(self.param_groups, state_dict["param_groups"]):
             for p, key in zip(group["params"], saved["params"]):
                 if not state_dict["state"].get(key):
@@ -197,3 +195,21 @@ class AdamW(torch.optim.Optimizer):
                     if isinstance(t, torch.Tensor):
                         t.copy_(torch.as_tensor(s[name]).reshape(t.shape))
                 self.state[p] = mine
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict: dict) -> None:
+        """As torch's, but the state keeps its types. Moments in 32 bits may come from torch.optim.AdamW. What is refused leaves the
+        optimizer as it was."""
+        final = []
+
+        # the last of the hooks before the load, which see and may replace the dict, and the first of those after it
+        def check(_, saved):
+            self._check_saved(saved)
+            final.append(saved)
+
+        hooks = [self.register_load_state_dict_pre_hook(check), self.register_load_state_dict_post_hook(lambda _: self._take_state(final[0]), prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()

@@ -312,3 +312,26 @@ def test_a_refused_first_step_leaves_no_state(bits):
     sparse.grad = torch.ones_like(sparse)
     opt.step()
     assert [int(opt.state[p]["step"]) for p in (good, sparse)] == [1, 1] and (good < 1).all() and (sparse < 1).all()
+
+
+def test_hooks_of_a_load():
+    """What a hook before the load returns is what is loaded, and checked; one after it sees the state as it stays."""
+    import kernels
+    p = leaf((4, 6))
+    saved = torch_dict(p)
+    opt, seen = kernels.AdamW([p], lr=0.5), []
+
+    def before(o, d):
+        return spoiled(d, {"lr": 0.75}, exp_avg=2 * d["state"][0]["exp_avg"])
+
+    handle = opt.register_load_state_dict_pre_hook(before)
+    opt.register_load_state_dict_post_hook(lambda o: seen.append({k: t.dtype for k, t in o.state[p].items()}))
+    for _ in range(2):
+        opt.load_state_dict(saved)
+        assert opt.param_groups[0]["lr"] == 0.75 and torch.equal(opt.state[p]["exp_avg"], 2 * saved["state"][0]["exp_avg"])
+    assert seen == [{"step": torch.int64, "exp_avg": torch.float32, "exp_avg_sq": torch.float32}] * 2
+    handle.remove()
+    opt.load_state_dict(saved)
+    assert opt.param_groups[0]["lr"] == 0.25 and torch.equal(opt.state[p]["exp_avg"], saved["state"][0]["exp_avg"])
+    opt.register_load_state_dict_pre_hook(lambda o, d: spoiled(d, {"maximize": True}))
+    refuses(opt, saved, "maximize")
